@@ -22,13 +22,16 @@ EMU_FMT_NVFP4, EMU_FMT_MXFP4 = 0, 1
 EMU_RZ, EMU_RNE = 0, 1
 EMU_OUT_F16, EMU_OUT_BF16_VIA_F16, EMU_OUT_F32 = 0, 1, 2
 EMU_DTYPE_F16, EMU_DTYPE_BF16, EMU_DTYPE_F32 = 0, 1, 2
+EMU_FP8_E4M3, EMU_FP8_E5M2 = 0, 1
+EMU_BLOCK_ROW, EMU_BLOCK_TILE = 0, 1
+EMU_KV_FP8, EMU_KV_MXFP4 = 0, 1
 ABI_VERSION = 1
 
 SYMBOLS = ("emu_abi_version", "emu_last_error", "emu_status_string", "emu_gemm", "emu_gemm_workspace_size", "emu_gemm_tc_workspace_size",
            "emu_gemm_ws", "emu_gemm_tc_path_offset", "emu_gemm_static", "emu_nvfp4_global_scales", "emu_nvfp4_amax",
            "emu_nvfp4_scales_from_amax", "emu_quant_nvfp4", "emu_quant_mxfp4",
            "emu_gemm_model", "emu_gemm_sweep", "emu_gemm_compare", "emu_gemm_batch", "emu_compare", "emu_dequant_fp4", "emu_device_status",
-           "emu_set_wait_limit", "emu_test_hold_first_ready")
+           "emu_set_wait_limit", "emu_test_hold_first_ready", "emu_quant_fp8", "emu_gemm_fp8", "emu_kv_write", "emu_kv_read")
 STATIC_SCRATCH_BYTES = 64 << 20   # EMU_STATIC_SCRATCH_BYTES
 
 
@@ -131,6 +134,15 @@ def load() -> ctypes.CDLL:
         L.emu_set_wait_limit.argtypes = [i64]
         L.emu_test_hold_first_ready.restype = i32
         L.emu_test_hold_first_ready.argtypes = [i32]
+        L.emu_quant_fp8.restype = i32
+        L.emu_quant_fp8.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+        L.emu_gemm_fp8.restype = i32
+        L.emu_gemm_fp8.argtypes = [vp, i64, i32, vp, i64, i32, vp, i64, vp, i64, i32, i64, i64, i64, i32, vp, i64, vp]
+        L.emu_kv_write.restype = i32
+        L.emu_kv_write.argtypes = [vp, vp, i32, i64, i64, i64, i64, i64, i64, i64, vp, i32, i64, vp, vp, vp, vp, vp]
+        L.emu_kv_read.restype = i32
+        L.emu_kv_read.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp, i64, i64, i64, vp, i64, i32, vp, vp,
+                                  i64, i64, vp]
         v = L.emu_abi_version()
         if v != ABI_VERSION:
             raise ImportError(f"libemugen ABI version {v}, expected {ABI_VERSION}: rebuild it")

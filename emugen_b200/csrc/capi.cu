@@ -438,14 +438,20 @@ emu_status emu_device_status(void* stream) {
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: stream");
   int code = 0;
   e = emu::take_wait_error(&code);
+  if (e == cudaSuccess && code == 0) e = emu::take_fp8_wait_error(&code);
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: error word");
   if (code == 0) return ok();
   static const char* const kSite[] = {"", "producer stage slot", "producer record slot", "MMA accumulator set",
                                       "MMA stage data", "epilogue accumulator", "epilogue records",
-                                      "producer drain", "record drain", "MMA drain"};
+                                      "producer drain", "record drain", "MMA drain",
+                                      "8-bit product: producer scale slot", "8-bit product: producer stage slot",
+                                      "8-bit product: copy drain", "8-bit product: MMA accumulator",
+                                      "8-bit product: MMA stage data", "8-bit product: MMA drain",
+                                      "8-bit product: epilogue scales", "8-bit product: epilogue accumulator"};
+  constexpr int kSites = (int)(sizeof(kSite) / sizeof(kSite[0]));
   return fail(EMU_ERR_TIMEOUT,
               "a tensor-core pipeline wait ran out (code %d: %s); outputs of the calls on this device since the "
-              "last emu_device_status are undefined", code, code > 0 && code < 10 ? kSite[code] : "unknown");
+              "last emu_device_status are undefined", code, code > 0 && code < kSites ? kSite[code] : "unknown");
 }
 
 emu_status emu_dequant_fp4(const uint8_t* q, const uint8_t* sf, int64_t rows, int64_t K, int64_t sf_cols,
@@ -465,6 +471,124 @@ emu_status emu_dequant_fp4(const uint8_t* q, const uint8_t* sf, int64_t rows, in
   return cuda_status(emu::launch_dequant(q, sf, rows, K, sf_cols, format, global_scale, out,
                                          static_cast<cudaStream_t>(stream)),
                      "emu_dequant_fp4 launch");
+}
+
+static bool float_dtype(int32_t dtype) {
+  return dtype == EMU_DTYPE_F16 || dtype == EMU_DTYPE_BF16 || dtype == EMU_DTYPE_F32;
+}
+
+emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, int32_t fp8_type,
+                         int32_t block, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, uint8_t* qt,
+                         int64_t ldqt, float* scale_t, int64_t ld_scale_t, void* stream) {
+  if (M < 0 || K < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (!float_dtype(dtype)) return fail(EMU_ERR_INVALID_ARGUMENT, "dtype must be EMU_DTYPE_F16, EMU_DTYPE_BF16 or EMU_DTYPE_F32");
+  if (fp8_type != EMU_FP8_E4M3 && fp8_type != EMU_FP8_E5M2) return fail(EMU_ERR_INVALID_ARGUMENT, "unknown fp8_type %d", fp8_type);
+  if (block != EMU_BLOCK_ROW && block != EMU_BLOCK_TILE) return fail(EMU_ERR_INVALID_ARGUMENT, "unknown block %d", block);
+  if (M == 0 || K == 0) return ok();
+  const int64_t mb = (M - 1) / 128 + 1, kb = (K - 1) / 128 + 1;
+  if (!x || (!q && !qt) || (q && !scale) || (qt && !scale_t)) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (ldx < K) return fail(EMU_ERR_INVALID_ARGUMENT, "ldx (%lld) must be at least K (%lld)", (long long)ldx, (long long)K);
+  if ((q && ldq < K) || (qt && ldqt < M)) return fail(EMU_ERR_INVALID_ARGUMENT, "code rows must hold K (transposed: M) bytes");
+  if ((q && (ldq % 16 != 0 || !aligned(q, 16))) || (qt && (ldqt % 16 != 0 || !aligned(qt, 16))))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "code rows must start on 16-byte boundaries");
+  if ((q && ld_scale < (block == EMU_BLOCK_ROW ? M : kb)) || (qt && ld_scale_t < (block == EMU_BLOCK_ROW ? K : mb)))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "scale rows too short");
+  if (mb > 0x7FFFFFFF / kb || (M - 1) / 4 + 1 > 0x7FFFFFFF / ((kb - 1) / 4 + 1))
+    return fail(EMU_ERR_UNSUPPORTED, "more than 2^31 - 1 blocks");
+  return cuda_status(emu::launch_quant_fp8(x, dtype, M, K, ldx, fp8_type, block, q, ldq, scale, ld_scale, qt, ldqt, scale_t,
+                                           ld_scale_t, static_cast<cudaStream_t>(stream)),
+                     "emu_quant_fp8 launch");
+}
+
+emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, const uint8_t* b, int64_t ldb, int32_t b_type,
+                        const float* scale_a, int64_t ld_scale_a, const float* scale_b, int64_t ld_scale_b,
+                        int32_t b_block, int64_t M, int64_t N, int64_t K, int32_t out_dtype, void* out, int64_t ldo,
+                        void* stream) {
+  if (M < 0 || N < 0 || K < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if ((a_type != EMU_FP8_E4M3 && a_type != EMU_FP8_E5M2) || (b_type != EMU_FP8_E4M3 && b_type != EMU_FP8_E5M2))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "unknown operand type (%d, %d)", a_type, b_type);
+  if (b_block != EMU_BLOCK_ROW && b_block != EMU_BLOCK_TILE) return fail(EMU_ERR_INVALID_ARGUMENT, "unknown b_block %d", b_block);
+  if (!float_dtype(out_dtype)) return fail(EMU_ERR_INVALID_ARGUMENT, "out_dtype must be EMU_DTYPE_F16, EMU_DTYPE_BF16 or EMU_DTYPE_F32");
+  if (M == 0 || N == 0) return ok();
+  if (!out) return fail(EMU_ERR_INVALID_ARGUMENT, "tensor pointers must not be NULL");
+  const int esz = out_dtype == EMU_DTYPE_F32 ? 4 : 2;
+  if (ldo < N || !aligned(out, esz)) return fail(EMU_ERR_INVALID_ARGUMENT, "ldo (%lld) must be at least N (%lld), out aligned to its elements", (long long)ldo, (long long)N);
+  if (K == 0)   // an empty sum
+    return cuda_status(cudaMemset2DAsync(out, (size_t)ldo * esz, 0, (size_t)N * esz, (size_t)M, static_cast<cudaStream_t>(stream)),
+                       "emu_gemm_fp8 memset");
+  if (!a || !b || !scale_a || !scale_b) return fail(EMU_ERR_INVALID_ARGUMENT, "tensor pointers must not be NULL");
+  if (lda < K || ldb < K) return fail(EMU_ERR_INVALID_ARGUMENT, "lda and ldb must be at least K");
+  if (!aligned(a, 16) || !aligned(b, 16) || lda % 16 != 0 || ldb % 16 != 0)
+    return fail(EMU_ERR_INVALID_ARGUMENT, "rows of a and b must start on 16-byte boundaries");
+  const int64_t m4 = (M + 3) / 4 * 4, n4 = (N + 3) / 4 * 4, kb = (K - 1) / 128 + 1;
+  if (!aligned(scale_a, 16) || ld_scale_a % 4 != 0 || ld_scale_a < m4)
+    return fail(EMU_ERR_SCALE_SHAPE, "scale_a: 16-byte aligned rows of at least M floats, a multiple of 4 apart");
+  if (b_block == EMU_BLOCK_ROW && (!aligned(scale_b, 16) || ld_scale_b % 4 != 0 || ld_scale_b < n4))
+    return fail(EMU_ERR_SCALE_SHAPE, "scale_b: 16-byte aligned rows of at least N floats, a multiple of 4 apart");
+  if (b_block == EMU_BLOCK_TILE && (!aligned(scale_b, 4) || ld_scale_b < kb))
+    return fail(EMU_ERR_SCALE_SHAPE, "scale_b: rows of at least ceil(K / 128) floats");
+  if (K > 0x7FFFFF00ll) return fail(EMU_ERR_UNSUPPORTED, "K too large");
+  if ((M - 1) / 128 >= 65535 || (N - 1) / 128 >= 65535) return fail(EMU_ERR_UNSUPPORTED, "M and N up to 65535 * 128");
+  const emu::Fp8GemmArgs g{a, lda, b, ldb, scale_a, ld_scale_a, scale_b, ld_scale_b, a_type, b_type,
+                           b_block == EMU_BLOCK_ROW, M, N, K, out_dtype, out, ldo};
+  return cuda_status(emu::launch_gemm_fp8(g, static_cast<cudaStream_t>(stream)), "emu_gemm_fp8 launch");
+}
+
+static emu_status check_kv(int32_t format, int64_t H, int64_t D) {
+  if (format != EMU_KV_FP8 && format != EMU_KV_MXFP4) return fail(EMU_ERR_INVALID_ARGUMENT, "unknown cache format %d", format);
+  if (H < 1 || H > 65536 || D < 1 || D > 65536) return fail(EMU_ERR_UNSUPPORTED, "heads and head size must be in [1, 65536]");
+  const int64_t unit = format == EMU_KV_FP8 ? 16 : 32;
+  if (D % unit != 0) return fail(EMU_ERR_K_GROUP, "head size must be a multiple of %lld", (long long)unit);
+  return EMU_OK;
+}
+
+emu_status emu_kv_write(const void* k, const void* v, int32_t dtype, int64_t tokens, int64_t heads, int64_t head_size,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                        const int64_t* slots, int32_t format, int64_t num_slots, uint8_t* k_cache, uint8_t* v_cache,
+                        void* k_scale, void* v_scale, void* stream) {
+  if (tokens < 0 || num_slots < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (dtype != EMU_DTYPE_F16 && dtype != EMU_DTYPE_BF16) return fail(EMU_ERR_INVALID_ARGUMENT, "dtype must be EMU_DTYPE_F16 or EMU_DTYPE_BF16");
+  const emu_status st = check_kv(format, heads, head_size);
+  if (st != EMU_OK) return st;
+  if (tokens == 0 || num_slots == 0) return ok();
+  if (!k || !slots || !k_cache || !k_scale || (v && (!v_cache || !v_scale)))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return fail(EMU_ERR_INVALID_ARGUMENT, "k, v and slots must be aligned to their elements");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || (format == EMU_KV_FP8 && (!aligned(k_scale, 4) || !aligned(v_scale, 4))))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "caches must be 16-byte aligned, f32 scales 4-byte");
+  if (tokens > 0x7FFFFFFFll) return fail(EMU_ERR_UNSUPPORTED, "more than 2^31 - 1 tokens");
+  const emu::KvWriteArgs a{{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, tokens, heads, head_size,
+                           slots, num_slots, {k_cache, v_cache}, {k_scale, v_scale}, dtype, format};
+  return cuda_status(emu::launch_kv_write(a, static_cast<cudaStream_t>(stream)), "emu_kv_write launch");
+}
+
+emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const void* k_scale, const void* v_scale,
+                       int32_t format, int64_t num_pages, int64_t page_size, int64_t heads, int64_t head_size,
+                       const int32_t* block_table, int64_t sequences, int64_t table_cols, int64_t table_stride,
+                       const int32_t* cu_lens, int64_t total, int32_t out_dtype, void* k_out, void* v_out,
+                       int64_t k_token_stride, int64_t v_token_stride, void* stream) {
+  if (num_pages < 0 || sequences < 0 || table_cols < 0 || total < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (page_size < 1) return fail(EMU_ERR_INVALID_ARGUMENT, "page_size must be positive");
+  if (!float_dtype(out_dtype)) return fail(EMU_ERR_INVALID_ARGUMENT, "out_dtype must be EMU_DTYPE_F16, EMU_DTYPE_BF16 or EMU_DTYPE_F32");
+  const emu_status st = check_kv(format, heads, head_size);
+  if (st != EMU_OK) return st;
+  if (total == 0 || sequences == 0) return ok();
+  if (!cu_lens || !k_out || (v_cache && !v_out) || (table_cols > 0 && !block_table) ||
+      (num_pages > 0 && (!k_cache || !k_scale || (v_cache && !v_scale))))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (table_stride < table_cols && sequences > 1) return fail(EMU_ERR_INVALID_ARGUMENT, "table_stride (%lld) must be at least table_cols (%lld)", (long long)table_stride, (long long)table_cols);
+  if (k_token_stride < heads * head_size || (v_cache && v_token_stride < heads * head_size))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "output rows must hold heads * head_size elements");
+  const int esz = out_dtype == EMU_DTYPE_F32 ? 4 : 2;
+  if (!aligned(block_table, 4) || !aligned(cu_lens, 4) || !aligned(k_out, esz) || !aligned(v_out, esz))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "block_table, cu_lens and the outputs must be aligned to their elements");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || (format == EMU_KV_FP8 && (!aligned(k_scale, 4) || !aligned(v_scale, 4))))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "caches must be 16-byte aligned, f32 scales 4-byte");
+  if (total > 0x7FFFFFFFll) return fail(EMU_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
+  const emu::KvReadArgs a{{k_cache, v_cache}, {k_scale, v_scale}, num_pages, page_size, heads, head_size, block_table, sequences,
+                          table_cols, table_stride, cu_lens, total, {k_out, v_cache ? v_out : nullptr},
+                          {k_token_stride, v_token_stride}, out_dtype, format};
+  return cuda_status(emu::launch_kv_read(a, static_cast<cudaStream_t>(stream)), "emu_kv_read launch");
 }
 
 }  // extern "C"

@@ -1373,6 +1373,9 @@ long long set_wait_limit(long long cycles) {
   return tc::g_wait_limit.exchange(cycles > 0 ? cycles : tc::DRAIN_LIMIT);
 }
 
+long long current_wait_limit() { return tc::g_wait_limit.load(); }
+int current_hold_first_ready() { return tc::g_hold_first_ready.load(); }
+
 void set_hold_first_ready(int enable) { tc::g_hold_first_ready.store(enable ? 1 : 0); }
 
 cudaError_t take_wait_error(int* code) {

@@ -68,6 +68,9 @@ size_t gemm_tc_path_offset(int fmt, int64_t M, int64_t N, int64_t K);
 long long set_wait_limit(long long cycles);
 // test hook: later tensor-core launches withhold the first accumulator-ready signal (gemm_tc.cu)
 void set_hold_first_ready(int enable);
+// the values that the two setters left, for the other tensor-core launches
+long long current_wait_limit();
+int current_hold_first_ready();
 // this device's first timed-out wait code since the last call (0 = none), then cleared
 cudaError_t take_wait_error(int* code);
 bool gemm_tc_supported(int fmt, int w_reduce, int64_t M, int64_t N, int64_t K);
@@ -78,6 +81,57 @@ cudaError_t launch_gemm_tc(const uint8_t* A, const uint8_t* B, const uint8_t* SA
 
 cudaError_t launch_quant(int sf_vec, const void* x, int dtype, int64_t M, int64_t K,
                          const float* global_scale, uint8_t* q, uint8_t* sf, cudaStream_t stream);
+
+// Block-scaled 8-bit quantiser (quant_fp8.cu); q or qt may be null.
+cudaError_t launch_quant_fp8(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fp8_type, int block,
+                             uint8_t* q, int64_t ldq, float* scale, int64_t lds, uint8_t* qt, int64_t ldqt,
+                             float* scale_t, int64_t ldst, cudaStream_t stream);
+
+// Block-scaled 8-bit matrix product (gemm_fp8.cu).
+struct Fp8GemmArgs {
+  const uint8_t* a;
+  int64_t lda;
+  const uint8_t* b;
+  int64_t ldb;
+  const float* sa;
+  int64_t ldsa;
+  const float* sb;
+  int64_t ldsb;
+  int a_type, b_type, b_rows;   // EMU_FP8_*; b_rows: a scale per row of B and block, else per 128 x 128 tile
+  int64_t M, N, K;
+  int out_dtype;                // EMU_DTYPE_*
+  void* out;
+  int64_t ldo;
+};
+cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream);
+// as take_wait_error, for the 8-bit product's waits
+cudaError_t take_fp8_wait_error(int* code);
+
+// Quantised key/value cache (kv_cache.cu).
+struct KvWriteArgs {
+  const void* x[2];             // keys, values (the second may be null)
+  int64_t token_stride[2], head_stride[2];
+  int64_t T, H, D;
+  const int64_t* slots;
+  int64_t num_slots;
+  uint8_t* q[2];
+  void* scale[2];
+  int dtype, format;
+};
+cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t stream);
+struct KvReadArgs {
+  const uint8_t* q[2];
+  const void* scale[2];
+  int64_t num_pages, page_size, H, D;
+  const int32_t* table;
+  int64_t B, table_cols, table_stride;
+  const int32_t* cu_lens;
+  int64_t total;
+  void* out[2];
+  int64_t token_stride[2];
+  int out_dtype, format;
+};
+cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream);
 
 // sets emu_last_error() of the calling thread to `message` and returns s (capi.cu)
 int32_t record_failure(int32_t s, const char* message);

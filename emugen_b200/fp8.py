@@ -1,0 +1,235 @@
+"""Block-scaled 8-bit floating point: the quantiser, the matrix product and a linear layer with its
+backward pass.
+
+Codes are ``torch.float8_e4m3fn`` or ``torch.float8_e5m2``; every block of 128 carries one f32 scale:
+blocks of 1 x 128 along the rows ("row", activations and gradients) or 128 x 128 tiles ("tile",
+weights).  An element stands for code * scale.
+
+  quant_fp8   x -> codes and scales, and on request those of the transposed matrix in the same pass
+  gemm_fp8    a @ b.T of two quantised matrices on the tensor cores, f32 sums
+  linear_fp8  x @ weight.T with all three products of a training step in 8 bits
+
+The kernels run on the inputs' device and its current stream, allocate only their outputs (through
+torch's allocator) and do not synchronise, so that CUDA graphs can capture them.  The reference has no 8-bit path.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+_FP8 = {torch.float8_e4m3fn: _lib.EMU_FP8_E4M3, torch.float8_e5m2: _lib.EMU_FP8_E5M2}
+_DTYPE = {torch.float16: _lib.EMU_DTYPE_F16, torch.bfloat16: _lib.EMU_DTYPE_BF16, torch.float32: _lib.EMU_DTYPE_F32}
+_BLOCKS = {"row": _lib.EMU_BLOCK_ROW, "tile": _lib.EMU_BLOCK_TILE}
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _on(dev: torch.device):
+    """Make `dev` current for the call (nothing to do where it already is)."""
+    return torch.cuda.device(dev.index)
+
+
+def _codes(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """[rows, cols] codes whose rows start on 16 bytes, as the product wants them."""
+    pitch = (cols + 15) // 16 * 16
+    q = torch.empty((rows, pitch), dtype=dtype, device=dev)
+    return q if pitch == cols else q[:, :cols]
+
+
+def _row_scales(rows: int, blocks: int, dev: torch.device) -> torch.Tensor:
+    """[rows, blocks] scales stored block after block, each block's row a multiple of 4 floats."""
+    pitch = (rows + 3) // 4 * 4
+    s = torch.empty((blocks, pitch), dtype=torch.float32, device=dev).t()
+    return s if pitch == rows else s[:rows]
+
+
+def quant_fp8(x: torch.Tensor, *, block: str = "row", dtype: torch.dtype = torch.float8_e4m3fn,
+              transposed: bool = False):
+    """x [..., K] (fp16 / bf16 / f32, leading dimensions flattened to M rows) -> (q, scale), or with
+    `transposed` (q, scale, qt, scale_t), the second pair being x.T quantised in the same pass.
+
+    q [M, K], qt [K, M]: codes of `dtype`; their rows start on 16-byte boundaries (so they need not be
+    contiguous).  block "row": scale [M, ceil(K / 128)] and scale_t [K, ceil(M / 128)], stored block after
+    block (strides 1, rows rounded up to 4); block "tile": scale [ceil(M / 128), ceil(K / 128)] and its
+    transpose.  scale = max(max |x| / F, 2^-126) in f32 over the block's finite elements (F: the type's
+    largest value), code = the nearest value to x / scale, ties to even; NaN and infinities become NaN."""
+    if dtype not in _FP8:
+        raise RuntimeError(f"quant_fp8 dtype must be torch.float8_e4m3fn or torch.float8_e5m2, got {dtype}")
+    if block not in _BLOCKS:
+        raise ValueError(f"block must be 'row' or 'tile', got {block!r}")
+    if x.dtype not in _DTYPE:
+        raise RuntimeError(f"quantiser input must be float16, bfloat16 or float32, got {x.dtype}")
+    if x.dim() == 0:
+        raise RuntimeError("quantiser input must have at least one dimension")
+    L = _lib.load()
+    dev = _lib._device_for(x)
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.shape[:-1].numel(), 0)
+    if x.device != dev:
+        x = x.to(dev)
+    M, K = x.shape
+    if x.stride(1) != 1 and K > 1 or x.stride(0) < K and M > 1:   # overlapping or column-strided rows
+        x = x.contiguous()
+    ldx = max(x.stride(0), K) if M > 1 else K
+    q = _codes(M, K, dtype, dev)
+    qt = _codes(K, M, dtype, dev) if transposed else None
+    if block == "row":
+        s = _row_scales(M, _blocks(K), dev)
+        st = _row_scales(K, _blocks(M), dev) if transposed else None
+        lds, ldst = (M + 3) // 4 * 4, (K + 3) // 4 * 4
+    else:
+        s = torch.empty((_blocks(M), _blocks(K)), dtype=torch.float32, device=dev)
+        st = torch.empty((_blocks(K), _blocks(M)), dtype=torch.float32, device=dev) if transposed else None
+        lds, ldst = _blocks(K), _blocks(M)
+    if M and K:
+        with _on(dev):
+            status = L.emu_quant_fp8(x.data_ptr(), _DTYPE[x.dtype], M, K, ldx, _FP8[dtype], _BLOCKS[block],
+                                     q.data_ptr(), (K + 15) // 16 * 16, s.data_ptr(), lds,
+                                     qt.data_ptr() if transposed else None, (M + 15) // 16 * 16,
+                                     st.data_ptr() if transposed else None, ldst, _lib._stream(dev))
+        _lib._check(status)
+    return (q, s, qt, st) if transposed else (q, s)
+
+
+def _operand(t: torch.Tensor, dev: torch.device, name: str):
+    """(tensor kept alive, pitch in bytes): rows that start on 16 bytes, copied there if they do not."""
+    if t.device != dev:
+        t = t.to(dev)
+    rows, cols = t.shape
+    if cols and rows and (t.stride(1) != 1 and cols > 1 or rows > 1 and (t.stride(0) % 16 or t.stride(0) < cols)
+                          or t.data_ptr() % 16):
+        c = _codes(rows, cols, t.dtype, dev)
+        c.view(torch.uint8).copy_(t.view(torch.uint8))
+        t = c
+    return t, t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
+
+
+def _scale_rows(s: torch.Tensor, dev: torch.device):
+    """(tensor kept alive, floats between blocks): scales stored block after block on 16-byte rows that can
+    be read up to a multiple of 4, copied there if they are not."""
+    if s.device != dev:
+        s = s.to(dev)
+    rows, blocks = s.shape
+    r4 = (rows + 3) // 4 * 4
+    ld = s.stride(1) if blocks > 1 else r4
+    good = (rows == 1 or s.stride(0) == 1) and ld % 4 == 0 and ld >= r4 and s.data_ptr() % 16 == 0
+    if good and r4 != rows:
+        end = s.storage_offset() + (blocks - 1) * ld + r4
+        good = end * 4 <= s.untyped_storage().nbytes()
+    if not good:
+        c = _row_scales(rows, blocks, dev)
+        c.copy_(s)
+        s, ld = c, r4
+    return s, ld
+
+
+def gemm_fp8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, *,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [M, K] @ b [N, K].T with quant_fp8's codes and scales -> [M, N] fp16 / bf16 / f32.
+
+    scale_a [M, ceil(K / 128)]: a scale for each row of a and block of K.  scale_b: the same for b
+    ([N, ceil(K / 128)]) or one for each 128 x 128 tile ([ceil(N / 128), ceil(K / 128)]).  a and b may be of
+    different 8-bit types.  Sums in f32, one rounding at the end, the same result every run.  Operands
+    and scales laid out otherwise than quant_fp8 leaves them are copied first."""
+    if a.dim() != 2 or b.dim() != 2 or scale_a.dim() != 2 or scale_b.dim() != 2:
+        raise RuntimeError("a, b, scale_a and scale_b must be 2D")
+    if a.dtype not in _FP8 or b.dtype not in _FP8:
+        raise RuntimeError(f"a and b must be float8_e4m3fn or float8_e5m2, got {a.dtype} and {b.dtype}")
+    if scale_a.dtype != torch.float32 or scale_b.dtype != torch.float32:
+        raise RuntimeError("scale_a and scale_b must be float32")
+    if out_dtype not in _DTYPE:
+        raise RuntimeError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K:
+        raise RuntimeError("K mismatch between a and b")
+    kb = _blocks(K)
+    if tuple(scale_a.shape) != (M, kb):
+        raise RuntimeError(f"scale_a must be [{M}, {kb}], got {list(scale_a.shape)}")
+    rows = tuple(scale_b.shape) == (N, kb)
+    if not rows and tuple(scale_b.shape) != (_blocks(N), kb):
+        raise RuntimeError(f"scale_b must be [{N}, {kb}] or [{_blocks(N)}, {kb}], got {list(scale_b.shape)}")
+    L = _lib.load()
+    on_cpu = not (a.is_cuda or b.is_cuda or scale_a.is_cuda or scale_b.is_cuda)
+    dev = _lib._device_for(a, b, scale_a, scale_b)
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if M and N:
+        with _on(dev):
+            if K:
+                a_, lda = _operand(a, dev, "a")
+                b_, ldb = _operand(b, dev, "b")
+                sa, ldsa = _scale_rows(scale_a, dev)
+                if rows:
+                    sb, ldsb = _scale_rows(scale_b, dev)
+                else:
+                    sb = scale_b.to(dev).contiguous()
+                    ldsb = kb
+                status = L.emu_gemm_fp8(a_.data_ptr(), lda, _FP8[a.dtype], b_.data_ptr(), ldb, _FP8[b.dtype],
+                                        sa.data_ptr(), ldsa, sb.data_ptr(), ldsb,
+                                        _lib.EMU_BLOCK_ROW if rows else _lib.EMU_BLOCK_TILE, M, N, K,
+                                        _DTYPE[out_dtype], out.data_ptr(), N, _lib._stream(dev))
+                _lib._check(status)
+            else:
+                out.zero_()
+    if on_cpu:
+        _lib.device_status(dev)
+        return out.cpu()
+    return out
+
+
+class _LinearFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        need_x, need_w = ctx.needs_input_grad
+        x2 = x.reshape(-1, x.shape[-1])
+        # the transposed codes serve the backward pass: x.T for the weight's gradient, weight.T for x's
+        q = quant_fp8(x2, transposed=need_w)
+        w = quant_fp8(weight, block="tile", transposed=need_x)
+        y = gemm_fp8(q[0], w[0], q[1], w[1], out_dtype=x.dtype)
+        ctx.save_for_backward(*(q[2:] if need_w else (None, None)), *(w[2:] if need_x else (None, None)))
+        ctx.x_shape, ctx.x_dtype, ctx.w_dtype = x.shape, x.dtype, weight.dtype
+        return y.reshape(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xt, xts, wt, wts = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad
+        dy2 = dy.reshape(-1, dy.shape[-1])
+        g = quant_fp8(dy2, transposed=need_w)
+        dx = dw = None
+        if need_x:
+            dx = gemm_fp8(g[0], wt, g[1], wts, out_dtype=ctx.x_dtype).reshape(ctx.x_shape)
+        if need_w:
+            dw = gemm_fp8(g[2], xt, g[3], xts, out_dtype=ctx.w_dtype)
+        return dx, dw
+
+
+def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """x [..., K] @ weight [N, K].T -> [..., N] in x's dtype, differentiable in both.
+
+    With Q the quantiser (E4M3; rows in blocks of 128, the weight in 128 x 128 tiles):
+      y  = Q(x) Q(weight)^T,   dx = Q(dy) Q(weight),   dw = Q(dy^T) Q(x^T)^T
+    (the gradients treat Q as the identity).  The forward pass keeps the 8-bit transposes of x and the weight
+    for the backward pass, not x itself.  fp16, bf16 or f32 CUDA tensors of one device and dtype.
+
+    A backward pass that a CUDA graph is to capture must be the leaves' only live graph: run the warm-up on
+    the capturing stream's side and drop its outputs first (torch.cuda.make_graphed_callables does), as for
+    every torch operator."""
+    if x.dim() < 1 or weight.dim() != 2:
+        raise RuntimeError("x must have at least one dimension and weight two")
+    if x.shape[-1] != weight.shape[1]:
+        raise RuntimeError("K mismatch between x and weight")
+    if x.dtype != weight.dtype or x.dtype not in _DTYPE:
+        raise RuntimeError(f"x and weight must share one of float16, bfloat16, float32, got {x.dtype} and {weight.dtype}")
+    if not x.is_cuda or x.device != weight.device:
+        raise RuntimeError("x and weight must be on the same CUDA device")
+    return _LinearFp8.apply(x, weight)
+
+
+__all__ = ["quant_fp8", "gemm_fp8", "linear_fp8"]

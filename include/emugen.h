@@ -373,6 +373,78 @@ EMU_API emu_status emu_dequant_fp4(const uint8_t* q, const uint8_t* sf, int64_t 
                                    int64_t sf_cols, int32_t format, const float* global_scale,
                                    float* out, void* stream);
 
+/* 8-bit element types and block shapes of the operators below. */
+enum { EMU_FP8_E4M3 = 0,   /* largest 448, no infinities   */
+       EMU_FP8_E5M2 = 1    /* largest 57344                */ };
+enum { EMU_BLOCK_ROW = 0,  /* 1 x 128: 128 consecutive elements of a row */
+       EMU_BLOCK_TILE = 1  /* 128 x 128                                  */ };
+
+/*
+ * Block-scaled 8-bit quantiser: x [M][K] (fp16 / bf16 / f32, rows ldx elements apart) -> codes q [M][K]
+ * (rows ldq bytes apart) and one f32 scale per block, and / or the same of the transposed matrix: qt [K][M],
+ * scale_t.  The last block of a row or column may be short.
+ *   scale = max(max |x| / F rounded to f32, 2^-126) over the block's finite elements, F = 448 (E4M3) / 57344 (E5M2)
+ *   code  = the 8-bit value nearest to x / scale (the exact quotient), ties to even; NaN for NaN and infinities
+ * EMU_BLOCK_ROW: blocks of 128 along a row (transposed: down a column);
+ *   scale of (row m, block kb) at scale[kb * ld_scale + m], of (column k, block mb) at scale_t[mb * ld_scale_t + k].
+ * EMU_BLOCK_TILE: scale of tile (mb, kb) at scale[mb * ld_scale + kb] and at scale_t[kb * ld_scale_t + mb].
+ * q or qt may be NULL (not wanted, with its scale).  q and qt 16-byte aligned, ldq and ldqt multiples of 16; the
+ * bytes between K (M) and ldq (ldqt) are left as they were.  No reference counterpart (EmuGen has FP4 only).
+ */
+EMU_API emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, int32_t fp8_type,
+                                 int32_t block, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, uint8_t* qt,
+                                 int64_t ldqt, float* scale_t, int64_t ld_scale_t, void* stream);
+
+/*
+ * Block-scaled 8-bit matrix product on the tensor cores:
+ *   out[m][n] = sum_kb scale_a(m, kb) * scale_b(n, kb) * sum_{k in block kb} a[m][k] * b[n][k]
+ * a [M][K], b [N][K] codes (a_type / b_type EMU_FP8_*, rows lda / ldb bytes apart), both as emu_quant_fp8 leaves them:
+ *   scale_a: EMU_BLOCK_ROW layout; scale_b: b_block's layout (a scale per row of b, or per 128 x 128 tile).
+ * Sums in f32, one rounding to out_dtype (EMU_DTYPE_*) at the end; the same result every run.  A NaN code or
+ * scale makes NaN exactly those outputs that it enters.  out [M][N], rows ldo elements apart.  K = 0 gives zeros.
+ * a, b 16-byte aligned, lda and ldb multiples of 16 (bytes past K are not used).  Scale rows of the row layout start
+ * on 16 bytes, ld_scale is a multiple of 4, and they can be read up to M (N) rounded up to a multiple of 4.
+ * A device pipeline wait that runs out is reported by emu_device_status.  No reference counterpart.
+ */
+EMU_API emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, const uint8_t* b, int64_t ldb,
+                                int32_t b_type, const float* scale_a, int64_t ld_scale_a, const float* scale_b,
+                                int64_t ld_scale_b, int32_t b_block, int64_t M, int64_t N, int64_t K,
+                                int32_t out_dtype, void* out, int64_t ldo, void* stream);
+
+/* Formats of the quantised key/value cache. */
+enum { EMU_KV_FP8 = 0,     /* E4M3 codes, an f32 scale per 128 elements of a (token, head) row (emu_quant_fp8's) */
+       EMU_KV_MXFP4 = 1    /* packed e2m1 codes, a scale byte u (2^(u - 127)) per 32 elements (emu_quant_mxfp4's) */ };
+
+/*
+ * Write keys and values into a quantised cache: token t's row of head h (k[t * k_token_stride + h * k_head_stride + d],
+ * d < head_size; fp16 / bf16) is quantised into slot slots[t].  The cache is contiguous:
+ *   codes  [num_slots][heads][head_size]  (MXFP4: head_size / 2 bytes, element 2j in the low nibble of byte j)
+ *   scales [num_slots][heads][ceil(head_size / 128)] f32   (MXFP4: [..][head_size / 32] bytes)
+ * (pages of P slots: slot = page * P + place).  A slot that is negative or not below num_slots writes nothing; where
+ * several tokens have the same slot, the last one's row is kept.  v may be NULL (a cache of one tensor).  head_size is a
+ * multiple of 16 (MXFP4: 32).  FP8: NaN and infinities become NaN.  MXFP4 (which has neither): for finite rows
+ * emu_quant_mxfp4's bytes; NaN is passed over by the scale.  Caches 16-byte aligned.  No reference counterpart.
+ */
+EMU_API emu_status emu_kv_write(const void* k, const void* v, int32_t dtype, int64_t tokens, int64_t heads,
+                                int64_t head_size, int64_t k_token_stride, int64_t k_head_stride,
+                                int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, int32_t format,
+                                int64_t num_slots, uint8_t* k_cache, uint8_t* v_cache, void* k_scale, void* v_scale,
+                                void* stream);
+
+/*
+ * Read the rows of a batch of sequences back from a quantised cache (emu_kv_write's layout, num_pages * page_size slots):
+ * row r of the outputs, cu_lens[b] <= r < cu_lens[b + 1], is position i = r - cu_lens[b] of sequence b, from page
+ * block_table[b * table_stride + i / page_size].  cu_lens: sequences + 1 non-decreasing values, cu_lens[0] = 0.
+ * Outputs [total][heads][head_size], rows k_token_stride / v_token_stride elements apart: code * scale, rounded once to
+ * out_dtype.  Rows of a page that does not exist (negative, not below num_pages, past table_cols) are zeros; rows
+ * that no sequence has are left as they were.  v_cache may be NULL.  No reference counterpart.
+ */
+EMU_API emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const void* k_scale,
+                               const void* v_scale, int32_t format, int64_t num_pages, int64_t page_size, int64_t heads,
+                               int64_t head_size, const int32_t* block_table, int64_t sequences, int64_t table_cols,
+                               int64_t table_stride, const int32_t* cu_lens, int64_t total, int32_t out_dtype,
+                               void* k_out, void* v_out, int64_t k_token_stride, int64_t v_token_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
