@@ -188,16 +188,16 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
       const float sb = p.b_rows ? slot[BN + quarter * 32 + lane] : sb_t;
 #pragma unroll
       for (int j = 0; j < BN; j += 16) {
-        float v[16];
-        ptx::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + ac * BN + j, v);
-        ptx::tmem_wait_ld();
+        uint32_t v[16];
+        ptx::tmem_ld_regs(tmem + ((uint32_t)(quarter * 32) << 16) + ac * BN + j, v);
+        ptx::tmem_wait_regs(v);
 #pragma unroll
         for (int u = 0; u < 16; u += 4) {
           const float4 s4 = *reinterpret_cast<const float4*>(slot + j + u);
-          acc[j + u] = __fmaf_rn(v[u], __fmul_rn(sb, s4.x), acc[j + u]);
-          acc[j + u + 1] = __fmaf_rn(v[u + 1], __fmul_rn(sb, s4.y), acc[j + u + 1]);
-          acc[j + u + 2] = __fmaf_rn(v[u + 2], __fmul_rn(sb, s4.z), acc[j + u + 2]);
-          acc[j + u + 3] = __fmaf_rn(v[u + 3], __fmul_rn(sb, s4.w), acc[j + u + 3]);
+          acc[j + u] = __fmaf_rn(__uint_as_float(v[u]), __fmul_rn(sb, s4.x), acc[j + u]);
+          acc[j + u + 1] = __fmaf_rn(__uint_as_float(v[u + 1]), __fmul_rn(sb, s4.y), acc[j + u + 1]);
+          acc[j + u + 2] = __fmaf_rn(__uint_as_float(v[u + 2]), __fmul_rn(sb, s4.z), acc[j + u + 2]);
+          acc[j + u + 3] = __fmaf_rn(__uint_as_float(v[u + 3]), __fmul_rn(sb, s4.w), acc[j + u + 3]);
         }
       }
       ptx::tc_fence_before();
@@ -243,6 +243,275 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
     }
   }
   ptx::cluster_sync();                                             // no CTA leaves while its sums are read
+}
+
+
+// ------------------------------------------------------------------------------ large products
+// A pair of CTAs computes a 256 x 256 output tile with cta_group::2 MMAs: each CTA stages 128 rows of A
+// and 128 of B (32 KB per block of K instead of 48 KB for the same MMA time alone, so that L2 keeps up)
+// and holds the 128 x 256 accumulators of its rows of A, twice.  Persistent: one pair per two SMs.
+//   warp 0      producer: TMA into the ring (signalling the leader's barriers), bulk copies of the scales
+//   warp 1      TMEM owner; in the leader, the MMA issuer
+//   warps 4-11  epilogue: a thread owns one row and 128 columns in registers; per block of K it reads
+//               them from TMEM and adds scale * block sum, two columns per instruction.
+//               B_ROWS = false: 128 columns share one scale of B, so the factor is one number per thread;
+//               B_ROWS = true: the block sum is multiplied by the column's scale first.
+constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
+constexpr int P_NSTAGE = 5;
+constexpr int P_NSCALE = 8;
+constexpr int P_SCALE = (128 + 256) * 4;
+constexpr int P_STORE = 8 * 32 * 128;            // per epilogue warp: 32 rows x 128 bytes of output
+constexpr int P_BARS = 2 * P_NSTAGE + 2 * P_NSCALE + 2 + 1;
+constexpr int P_SMEM = 1024 + P_NSTAGE * P_STAGE + P_STORE + P_NSCALE * P_SCALE + P_BARS * 8 + 16;
+constexpr int P_THREADS = 384;
+// 128 threads x 40 + 256 x 232 = 64512 = 384 x 168, what the CTA is launched with
+constexpr int P_REG_LOW = 40, P_REG_HIGH = 232;
+constexpr int P_BAND = 8;                        // tile raster: bands of 8 row tiles (2048 rows of A stay in L2)
+static_assert(P_SMEM <= 232448, "shared memory per CTA");
+
+__device__ __forceinline__ void pair_tile(int64_t t, int64_t tiles_m, int64_t tiles_n, int64_t& tm, int64_t& tn) {
+  const int64_t per_band = P_BAND * tiles_n, band = t / per_band, first = band * P_BAND;
+  const int64_t gm = min(tiles_m - first, (int64_t)P_BAND), idx = t % per_band;
+  tm = first + idx % gm;
+  tn = idx / gm;
+}
+
+template <bool B_ROWS>
+__global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                                     const __grid_constant__ CUtensorMap map_b,
+                                                                     const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* store = smem + P_NSTAGE * P_STAGE;
+  float* scales = reinterpret_cast<float*>(store + P_STORE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + P_NSCALE * (P_SCALE / 4));
+  // a block's MMAs have completed: its stage may be filled again (producers), its accumulator read (epilogue)
+  uint64_t* done = full + P_NSTAGE;
+  uint64_t* s_full = done + P_NSTAGE;
+  uint64_t* s_empty = s_full + P_NSCALE;
+  uint64_t* acc_empty = s_empty + P_NSCALE;
+  uint64_t* drained = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const int64_t tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, tiles = tiles_m * tiles_n;
+  const int64_t first = blockIdx.x / 2, stride = gridDim.x / 2;
+
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&map_a);
+    ptx::prefetch_tmap(&map_b);
+    for (int i = 0; i < P_NSTAGE; ++i) ptx::mbar_init(&full[i], 1), ptx::mbar_init(&done[i], 1);
+    for (int i = 0; i < P_NSCALE; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&s_empty[i], 8);
+    for (int i = 0; i < 2; ++i) ptx::mbar_init(&acc_empty[i], 16);   // both CTAs' warps
+    ptx::mbar_init(drained, 1);
+    ptx::fence_mbar_init();
+  }
+  __syncwarp();
+  ptx::cluster_sync();                                               // barriers of both CTAs exist
+  if (warp == 1) {
+    ptx::tmem_alloc2(tmem_slot, 512);
+    ptx::tmem_relinquish2();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+
+  // no load may be in flight across the register split: the TMEM address is read after it
+  if (warp < 4) {
+    ptx::setmaxnreg_dec<P_REG_LOW>();
+    if (warp == 0 && lane == 0) {
+      const int64_t m_pad = (p.M + 3) & ~(int64_t)3, n_pad = (p.N + 3) & ~(int64_t)3;
+      bool ok = true;
+      int64_t i = 0;
+      for (int64_t t = first; t < tiles && ok; t += stride) {
+        int64_t tm, tn;
+        pair_tile(t, tiles_m, tiles_n, tm, tn);
+        const int64_t m0 = tm * 256 + rank * 128, n0 = tn * 256;
+        const uint32_t a_bytes = (uint32_t)max((int64_t)0, min((int64_t)128, m_pad - m0)) * 4;
+        const uint32_t b_bytes = B_ROWS ? (uint32_t)min((int64_t)256, n_pad - n0) * 4 : 0;
+        for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
+          const int st = (int)(i % P_NSTAGE), sc = (int)(i % P_NSCALE);
+          if (i >= P_NSCALE && !wait_or_record(&s_empty[sc], (uint32_t)(i / P_NSCALE - 1) & 1, p.wait_limit, 10)) { ok = false; break; }
+          if (i >= P_NSTAGE && !wait_or_record(&done[st], (uint32_t)(i / P_NSTAGE - 1) & 1, p.wait_limit, 11)) { ok = false; break; }
+          const uint32_t bar = ptx::map_shared(ptx::smem_u32(&full[st]), 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&full[st], 2 * P_STAGE);   // both CTAs' bytes
+          ptx::tma_load_2d_pair(smem + st * P_STAGE, &map_a, bar, kb * BK, (int)m0);
+          ptx::tma_load_2d_pair(smem + st * P_STAGE + 128 * BK, &map_b, bar, kb * BK, (int)(n0 + rank * 128));
+          float* slot = scales + sc * (P_SCALE / 4);
+          ptx::mbar_arrive_expect_tx(&s_full[sc], a_bytes + b_bytes);
+          if (a_bytes) ptx::bulk_load(slot, p.sa + kb * p.ldsa + m0, a_bytes, &s_full[sc]);
+          if (b_bytes) ptx::bulk_load(slot + 128, p.sb + kb * p.ldsb + n0, b_bytes, &s_full[sc]);
+        }
+      }
+      // every copy has landed before the CTA may exit: the leader's barriers count both CTAs' tiles, the
+      // final cluster barrier holds the other CTA until then.  After a failed wait the CTAs may have
+      // stopped at different blocks: then time for copies in flight.
+      for (int64_t j = max((int64_t)0, i - P_NSCALE); j < i; ++j)
+        wait_or_record(&s_full[j % P_NSCALE], (uint32_t)(j / P_NSCALE) & 1, DRAIN_LIMIT, 12);
+      if (ok && rank == 0) {
+        for (int64_t j = max((int64_t)0, i - P_NSTAGE); j < i; ++j)
+          ok = ok && wait_or_record(&full[j % P_NSTAGE], (uint32_t)(j / P_NSTAGE) & 1, p.wait_limit, 12);
+      }
+      if (!ok) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) {}
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      const uint32_t tmem = *tmem_slot;
+      bool ok = true;
+      int64_t i = 0;
+      for (int64_t t = first; t < tiles && ok; t += stride) {
+        for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
+          const int st = (int)(i % P_NSTAGE), ac = (int)(i & 1);
+          if (i >= 2 && !wait_or_record(&acc_empty[ac], (uint32_t)(i / 2 - 1) & 1, p.wait_limit, 13)) { ok = false; break; }
+          if (!wait_or_record(&full[st], (uint32_t)(i / P_NSTAGE) & 1, p.wait_limit, 14)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st * P_STAGE));
+          const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(smem + st * P_STAGE + 128 * BK));
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem + ac * 256, da + 2 * k, db + 2 * k, p.idesc, k > 0);
+          if (!(i == 0 && p.hold_first_ready)) ptx::mma2_commit_both(&done[st]);
+        }
+      }
+      ptx::mma2_commit_both(drained);
+      wait_or_record(drained, 0, DRAIN_LIMIT, 15);
+    }
+  } else {
+    ptx::setmaxnreg_inc<P_REG_HIGH>();
+    const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;     // TMEM lanes, columns
+    const uint32_t lane_base = *tmem_slot + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    uint8_t* buf = store + ew * (32 * 128);
+    const int64_t blocks_n = (p.N + 127) / 128;
+    const uint32_t empty_bar = ptx::map_shared(ptx::smem_u32(acc_empty), 0);
+    bool ok = true;
+    int64_t i = 0;
+    for (int64_t t = first; t < tiles && ok; t += stride) {
+      int64_t tm, tn;
+      pair_tile(t, tiles_m, tiles_n, tm, tn);
+      const int64_t nb = min(tn * 2 + half, blocks_n - 1);
+      const float* sb_tile = p.sb + nb * p.ldsb;
+      uint64_t acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      float sb_next = B_ROWS ? 0.0f : __ldg(sb_tile);
+      uint32_t v[2][32];
+      if (!warp_wait_or_record(&done[i % P_NSTAGE], (uint32_t)(i / P_NSTAGE) & 1, p.wait_limit, 17)) { ok = false; break; }
+      ptx::tc_fence_after();
+      ptx::tmem_ld_regs(lane_base + (uint32_t)(i & 1) * 256, v[0]);
+      for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
+        const int sc = (int)(i % P_NSCALE), ac = (int)(i & 1);
+        const float sb = sb_next;
+        if (!B_ROWS && kb + 1 < p.kb_count) sb_next = __ldg(sb_tile + kb + 1);
+        if (!warp_wait_or_record(&s_full[sc], (uint32_t)(i / P_NSCALE) & 1, p.wait_limit, 16)) { ok = false; break; }
+        const float* slot = scales + sc * (P_SCALE / 4);
+        const float sa = slot[quarter * 32 + lane];
+        const float f = B_ROWS ? sa : __fmul_rn(sa, sb);
+        const uint64_t f2 = ptx::pack2(f, f);
+        bool next = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ptx::tmem_wait_regs(v[c & 1]);
+          // the next 32 columns travel while these are added up
+          if (c < 3) {
+            ptx::tmem_ld_regs(lane_base + ac * 256 + (c + 1) * 32, v[(c + 1) & 1]);
+          } else {
+            ptx::tc_fence_before();                                  // all of this block is in registers
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac * 8);
+            if (kb + 1 < p.kb_count) {
+              next = __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(&done[(i + 1) % P_NSTAGE], (uint32_t)((i + 1) / P_NSTAGE) & 1));
+              if (next) {
+                ptx::tc_fence_after();
+                ptx::tmem_ld_regs(lane_base + (ac ^ 1) * 256, v[0]);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            uint64_t x = ptx::join2(v[c & 1][2 * j], v[c & 1][2 * j + 1]);
+            if (B_ROWS) x = ptx::mul2(x, *reinterpret_cast<const uint64_t*>(slot + 128 + half * 128 + c * 32 + 2 * j));
+            acc[c * 16 + j] = ptx::fma2(x, f2, acc[c * 16 + j]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s_empty[sc]);
+        if (!next && kb + 1 < p.kb_count) {
+          if (!warp_wait_or_record(&done[(i + 1) % P_NSTAGE], (uint32_t)((i + 1) / P_NSTAGE) & 1, p.wait_limit, 17)) { ok = false; break; }
+          ptx::tc_fence_after();
+          ptx::tmem_ld_regs(lane_base + (ac ^ 1) * 256, v[0]);
+        }
+      }
+      if (!ok) break;
+      // output: 128 bytes of each of the warp's 32 rows at a time, turned in shared memory so that a
+      // row's bytes leave together; 16-byte pieces are spread over the banks by the row's low bits
+      const int64_t row0 = tm * 256 + rank * 128 + quarter * 32, col0 = tn * 256 + half * 128;
+      const int esz = p.out_mode == EMU_DTYPE_F32 ? 4 : 2;
+      const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * esz)) & 15) == 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (esz == 2 && (c & 1)) continue;                           // 64 16-bit columns at a time, or 32 of f32
+        __syncwarp();
+        if (esz == 4) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const uint64_t x = acc[c * 16 + 2 * u], y = acc[c * 16 + 2 * u + 1];
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) =
+                make_uint4((uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32));
+          }
+        } else if (c < 3) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t x = acc[(c * 16 + 4 * u + e) & 63];
+              if (p.out_mode == EMU_DTYPE_BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(ptx::lo2(x), ptx::hi2(x));
+                w[e] = reinterpret_cast<const uint32_t&>(h);
+              } else {
+                const __half2 h = __floats2half2_rn(ptx::lo2(x), ptx::hi2(x));
+                w[e] = reinterpret_cast<const uint32_t&>(h);
+              }
+            }
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        const int u = lane & 7, per = 16 / esz;                      // elements of a 16-byte piece
+        const int64_t col = col0 + c * 32 + u * per;
+#pragma unroll
+        for (int r4 = 0; r4 < 8; ++r4) {
+          const int r = r4 * 4 + (lane >> 3);
+          const int64_t row = row0 + r;
+          if (row >= p.M || col >= p.N) continue;
+          const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
+          uint8_t* dst = static_cast<uint8_t*>(p.out) + (row * p.ldo + col) * esz;
+          if (vec && col + per <= p.N) {
+            *reinterpret_cast<uint4*>(dst) = w;
+          } else {
+            const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (e >= per || col + e >= p.N) break;
+              if (esz == 4) reinterpret_cast<uint32_t*>(dst)[e] = q[e & 3];
+              else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(q[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();                                               // both CTAs are done with both memories
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc2(*tmem_slot, 512);
+    // the leader's last signal to this CTA's shared memory has arrived before it goes
+    if (rank == 1 && lane == 0) wait_or_record(drained, 0, DRAIN_LIMIT, 15);
+  }
 }
 
 // ------------------------------------------------------------------------------ host side
@@ -302,6 +571,29 @@ cudaError_t launch_skinny(const Fp8GemmArgs& g, Params p, int sms, cudaStream_t 
   return cudaLaunchKernelEx(&cfg, kernel, mb, ma, p);
 }
 
+template <bool B_ROWS>
+cudaError_t launch_pair(const Fp8GemmArgs& g, Params p, int sms, cudaStream_t stream) {
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, g.a, g.M, g.K, g.lda, 128) || !make_map(&mb, g.b, g.N, g.K, g.ldb, 128)) return cudaErrorUnknown;
+  auto kernel = gemm_fp8_pair_kernel<B_ROWS>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+  if (e != cudaSuccess) return e;
+  p.idesc = ptx::idesc_f8_f32(256, 256, g.a_type, g.b_type);
+  const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
+  cfg.blockDim = dim3(P_THREADS);
+  cfg.dynamicSmemBytes = P_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
+}
+
 }  // namespace
 
 cudaError_t take_fp8_wait_error(int* code) {
@@ -323,6 +615,7 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
   p.out = g.out, p.ldo = g.ldo, p.out_mode = g.out_dtype;
   p.wait_limit = current_wait_limit();
   p.hold_first_ready = current_hold_first_ready();
+  if (g.M > 128) return g.b_rows ? launch_pair<true>(g, p, sms, stream) : launch_pair<false>(g, p, sms, stream);
   if (g.M <= 16) return launch_skinny<16>(g, p, sms, stream);
   if (g.M <= 32) return launch_skinny<32>(g, p, sms, stream);
   if (g.M <= 64) return launch_skinny<64>(g, p, sms, stream);
