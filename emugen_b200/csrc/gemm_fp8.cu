@@ -276,6 +276,16 @@ __device__ __forceinline__ void pair_tile(int64_t t, int64_t tiles_m, int64_t ti
   tn = idx / gm;
 }
 
+// A place in a ring of N barriers and the parity of its current round; a division by N for each block would
+// put a chain of multiplications in every role's loop.
+template <int N> struct Ring {
+  int at = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) at = 0, parity ^= 1;
+  }
+};
+
 template <bool B_ROWS>
 __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b,
@@ -323,35 +333,44 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
     if (warp == 0 && lane == 0) {
       const int64_t m_pad = (p.M + 3) & ~(int64_t)3, n_pad = (p.N + 3) & ~(int64_t)3;
       bool ok = true;
-      int64_t i = 0;
+      Ring<P_NSTAGE> st;
+      Ring<P_NSCALE> sc;
+      int filled = 0, s_filled = 0;                                  // slots in their first round need no wait
       for (int64_t t = first; t < tiles && ok; t += stride) {
         int64_t tm, tn;
         pair_tile(t, tiles_m, tiles_n, tm, tn);
         const int64_t m0 = tm * 256 + rank * 128, n0 = tn * 256;
         const uint32_t a_bytes = (uint32_t)max((int64_t)0, min((int64_t)128, m_pad - m0)) * 4;
         const uint32_t b_bytes = B_ROWS ? (uint32_t)min((int64_t)256, n_pad - n0) * 4 : 0;
-        for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
-          const int st = (int)(i % P_NSTAGE), sc = (int)(i % P_NSCALE);
-          if (i >= P_NSCALE && !wait_or_record(&s_empty[sc], (uint32_t)(i / P_NSCALE - 1) & 1, p.wait_limit, 10)) { ok = false; break; }
-          if (i >= P_NSTAGE && !wait_or_record(&done[st], (uint32_t)(i / P_NSTAGE - 1) & 1, p.wait_limit, 11)) { ok = false; break; }
-          const uint32_t bar = ptx::map_shared(ptx::smem_u32(&full[st]), 0);
-          if (rank == 0) ptx::mbar_arrive_expect_tx(&full[st], 2 * P_STAGE);   // both CTAs' bytes
-          ptx::tma_load_2d_pair(smem + st * P_STAGE, &map_a, bar, kb * BK, (int)m0);
-          ptx::tma_load_2d_pair(smem + st * P_STAGE + 128 * BK, &map_b, bar, kb * BK, (int)(n0 + rank * 128));
-          float* slot = scales + sc * (P_SCALE / 4);
-          ptx::mbar_arrive_expect_tx(&s_full[sc], a_bytes + b_bytes);
-          if (a_bytes) ptx::bulk_load(slot, p.sa + kb * p.ldsa + m0, a_bytes, &s_full[sc]);
-          if (b_bytes) ptx::bulk_load(slot + 128, p.sb + kb * p.ldsb + n0, b_bytes, &s_full[sc]);
+        for (int kb = 0; kb < p.kb_count; ++kb) {
+          if (s_filled == P_NSCALE && !wait_or_record(&s_empty[sc.at], sc.parity ^ 1, p.wait_limit, 10)) { ok = false; break; }
+          if (filled == P_NSTAGE && !wait_or_record(&done[st.at], st.parity ^ 1, p.wait_limit, 11)) { ok = false; break; }
+          const uint32_t bar = ptx::map_shared(ptx::smem_u32(&full[st.at]), 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&full[st.at], 2 * P_STAGE);   // both CTAs' bytes
+          ptx::tma_load_2d_pair(smem + st.at * P_STAGE, &map_a, bar, kb * BK, (int)m0);
+          ptx::tma_load_2d_pair(smem + st.at * P_STAGE + 128 * BK, &map_b, bar, kb * BK, (int)(n0 + rank * 128));
+          float* slot = scales + sc.at * (P_SCALE / 4);
+          ptx::mbar_arrive_expect_tx(&s_full[sc.at], a_bytes + b_bytes);
+          if (a_bytes) ptx::bulk_load(slot, p.sa + kb * p.ldsa + m0, a_bytes, &s_full[sc.at]);
+          if (b_bytes) ptx::bulk_load(slot + 128, p.sb + kb * p.ldsb + n0, b_bytes, &s_full[sc.at]);
+          st.next();
+          sc.next();
+          if (filled < P_NSTAGE) ++filled;
+          if (s_filled < P_NSCALE) ++s_filled;
         }
       }
       // every copy has landed before the CTA may exit: the leader's barriers count both CTAs' tiles, the
       // final cluster barrier holds the other CTA until then.  After a failed wait the CTAs may have
       // stopped at different blocks: then time for copies in flight.
-      for (int64_t j = max((int64_t)0, i - P_NSCALE); j < i; ++j)
-        wait_or_record(&s_full[j % P_NSCALE], (uint32_t)(j / P_NSCALE) & 1, DRAIN_LIMIT, 12);
+      const Ring<P_NSCALE> sc_end = sc;
+      for (int j = 0; j < P_NSCALE; ++j, sc.next())                  // oldest first: slots of the round before, then of this one
+        if (j >= P_NSCALE - s_filled)
+          wait_or_record(&s_full[sc.at], sc.at < sc_end.at ? sc_end.parity : sc_end.parity ^ 1, DRAIN_LIMIT, 12);
       if (ok && rank == 0) {
-        for (int64_t j = max((int64_t)0, i - P_NSTAGE); j < i; ++j)
-          ok = ok && wait_or_record(&full[j % P_NSTAGE], (uint32_t)(j / P_NSTAGE) & 1, p.wait_limit, 12);
+        const Ring<P_NSTAGE> st_end = st;
+        for (int j = 0; j < P_NSTAGE; ++j, st.next())
+          if (j >= P_NSTAGE - filled)
+            ok = ok && wait_or_record(&full[st.at], st.at < st_end.at ? st_end.parity : st_end.parity ^ 1, p.wait_limit, 12);
       }
       if (!ok) {
         const long long t0 = clock64();
@@ -359,19 +378,24 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       const uint32_t tmem = *tmem_slot;
-      bool ok = true;
-      int64_t i = 0;
+      bool ok = true, first_block = true;
+      Ring<P_NSTAGE> st;
+      Ring<2> ac;
+      int filled = 0;
       for (int64_t t = first; t < tiles && ok; t += stride) {
-        for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
-          const int st = (int)(i % P_NSTAGE), ac = (int)(i & 1);
-          if (i >= 2 && !wait_or_record(&acc_empty[ac], (uint32_t)(i / 2 - 1) & 1, p.wait_limit, 13)) { ok = false; break; }
-          if (!wait_or_record(&full[st], (uint32_t)(i / P_NSTAGE) & 1, p.wait_limit, 14)) { ok = false; break; }
+        for (int kb = 0; kb < p.kb_count; ++kb) {
+          if (filled == 2 && !wait_or_record(&acc_empty[ac.at], ac.parity ^ 1, p.wait_limit, 13)) { ok = false; break; }
+          if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
           ptx::tc_fence_after();
-          const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st * P_STAGE));
-          const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(smem + st * P_STAGE + 128 * BK));
+          const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE));
+          const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE + 128 * BK));
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem + ac * 256, da + 2 * k, db + 2 * k, p.idesc, k > 0);
-          if (!(i == 0 && p.hold_first_ready)) ptx::mma2_commit_both(&done[st]);
+          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem + ac.at * 256, da + 2 * k, db + 2 * k, p.idesc, k > 0);
+          if (!(first_block && p.hold_first_ready)) ptx::mma2_commit_both(&done[st.at]);
+          first_block = false;
+          st.next();
+          ac.next();
+          if (filled < 2) ++filled;
         }
       }
       ptx::mma2_commit_both(drained);
@@ -385,7 +409,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
     const int64_t blocks_n = (p.N + 127) / 128;
     const uint32_t empty_bar = ptx::map_shared(ptx::smem_u32(acc_empty), 0);
     bool ok = true;
-    int64_t i = 0;
+    Ring<P_NSTAGE> st;
+    Ring<P_NSCALE> sc;
+    uint32_t ac = 0;                                                 // TMEM column of the block's accumulator
     for (int64_t t = first; t < tiles && ok; t += stride) {
       int64_t tm, tn;
       pair_tile(t, tiles_m, tiles_n, tm, tn);
@@ -396,50 +422,60 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       for (int j = 0; j < 64; ++j) acc[j] = 0;
       float sb_next = B_ROWS ? 0.0f : __ldg(sb_tile);
       uint32_t v[2][32];
-      if (!warp_wait_or_record(&done[i % P_NSTAGE], (uint32_t)(i / P_NSTAGE) & 1, p.wait_limit, 17)) { ok = false; break; }
+      if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
       ptx::tc_fence_after();
-      ptx::tmem_ld_regs(lane_base + (uint32_t)(i & 1) * 256, v[0]);
-      for (int kb = 0; kb < p.kb_count; ++kb, ++i) {
-        const int sc = (int)(i % P_NSCALE), ac = (int)(i & 1);
+      ptx::tmem_ld_regs(lane_base + ac, v[0]);
+      for (int kb = 0; kb < p.kb_count; ++kb) {
+        const bool more = kb + 1 < p.kb_count;
         const float sb = sb_next;
-        if (!B_ROWS && kb + 1 < p.kb_count) sb_next = __ldg(sb_tile + kb + 1);
-        if (!warp_wait_or_record(&s_full[sc], (uint32_t)(i / P_NSCALE) & 1, p.wait_limit, 16)) { ok = false; break; }
-        const float* slot = scales + sc * (P_SCALE / 4);
+        if (!B_ROWS && more) sb_next = __ldg(sb_tile + kb + 1);
+        if (!warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
+        const float* slot = scales + sc.at * (P_SCALE / 4);
         const float sa = slot[quarter * 32 + lane];
         const float f = B_ROWS ? sa : __fmul_rn(sa, sb);
         const uint64_t f2 = ptx::pack2(f, f);
+        st.next();
         bool next = false;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           ptx::tmem_wait_regs(v[c & 1]);
           // the next 32 columns travel while these are added up
           if (c < 3) {
-            ptx::tmem_ld_regs(lane_base + ac * 256 + (c + 1) * 32, v[(c + 1) & 1]);
+            ptx::tmem_ld_regs(lane_base + ac + (c + 1) * 32, v[(c + 1) & 1]);
           } else {
             ptx::tc_fence_before();                                  // all of this block is in registers
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac * 8);
-            if (kb + 1 < p.kb_count) {
-              next = __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(&done[(i + 1) % P_NSTAGE], (uint32_t)((i + 1) / P_NSTAGE) & 1));
+            if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac / 32);   // 8 bytes per 256 columns
+            ac ^= 256;
+            if (more) {
+              next = __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(&done[st.at], st.parity));
               if (next) {
                 ptx::tc_fence_after();
-                ptx::tmem_ld_regs(lane_base + (ac ^ 1) * 256, v[0]);
+                ptx::tmem_ld_regs(lane_base + ac, v[0]);
               }
             }
           }
+          const float4* sb4 = reinterpret_cast<const float4*>(slot + 128 + half * 128 + c * 32);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < 16; j += 2) {
             uint64_t x = ptx::join2(v[c & 1][2 * j], v[c & 1][2 * j + 1]);
-            if (B_ROWS) x = ptx::mul2(x, *reinterpret_cast<const uint64_t*>(slot + 128 + half * 128 + c * 32 + 2 * j));
+            uint64_t y = ptx::join2(v[c & 1][2 * j + 2], v[c & 1][2 * j + 3]);
+            if (B_ROWS) {
+              const float4 s4 = sb4[j / 2];
+              x = ptx::mul2(x, ptx::pack2(s4.x, s4.y));
+              y = ptx::mul2(y, ptx::pack2(s4.z, s4.w));
+            }
             acc[c * 16 + j] = ptx::fma2(x, f2, acc[c * 16 + j]);
+            acc[c * 16 + j + 1] = ptx::fma2(y, f2, acc[c * 16 + j + 1]);
           }
         }
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&s_empty[sc]);
-        if (!next && kb + 1 < p.kb_count) {
-          if (!warp_wait_or_record(&done[(i + 1) % P_NSTAGE], (uint32_t)((i + 1) / P_NSTAGE) & 1, p.wait_limit, 17)) { ok = false; break; }
+        if (lane == 0) ptx::mbar_arrive(&s_empty[sc.at]);
+        sc.next();
+        if (more && !next) {
+          if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
           ptx::tc_fence_after();
-          ptx::tmem_ld_regs(lane_base + (ac ^ 1) * 256, v[0]);
+          ptx::tmem_ld_regs(lane_base + ac, v[0]);
         }
       }
       if (!ok) break;
