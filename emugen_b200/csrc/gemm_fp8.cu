@@ -250,16 +250,19 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
 // A pair of CTAs computes a 256 x 256 output tile with cta_group::2 MMAs: each CTA stages 128 rows of A
 // and 128 of B (32 KB per block of K instead of 48 KB for the same MMA time alone, so that L2 keeps up)
 // and holds the 128 x 256 accumulators of its rows of A, twice.  Persistent: one pair per two SMs.
-//   warp 0      producer: TMA into the ring (signalling the leader's barriers), bulk copies of the scales
-//   warp 1      TMEM owner; in the leader, the MMA issuer
+//   warp 0      producer: TMA into the ring (signalling the leader's barriers); B_ROWS: bulk copies of the column scales
+//   warps 1, 2  in the leader, the MMA issuers, one for each accumulator: a block's waits, four MMAs and
+//               commit take one thread ~970 clocks, the MMAs themselves 512, so two threads take turns
+//               (warp 1 owns the TMEM)
 //   warps 4-11  epilogue: a thread owns one row and 128 columns in registers; per block of K it reads
-//               them from TMEM and adds scale * block sum, two columns per instruction.
+//               them from TMEM and adds scale * block sum.  (The f32x2 form of the multiply-add was slower:
+//               its register pairs cost a move each, 484 against 268 us for the epilogue alone at 8192^3.)
 //               B_ROWS = false: 128 columns share one scale of B, so the factor is one number per thread;
 //               B_ROWS = true: the block sum is multiplied by the column's scale first.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
 constexpr int P_NSTAGE = 5;
 constexpr int P_NSCALE = 8;
-constexpr int P_SCALE = (128 + 256) * 4;
+constexpr int P_SCALE = 256 * 4;                 // column scales (B_ROWS)
 constexpr int P_STORE = 8 * 32 * 128;            // per epilogue warp: 32 rows x 128 bytes of output
 constexpr int P_BARS = 2 * P_NSTAGE + 2 * P_NSCALE + 2 + 1;
 constexpr int P_SMEM = 1024 + P_NSTAGE * P_STAGE + P_STORE + P_NSCALE * P_SCALE + P_BARS * 8 + 16;
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
     for (int i = 0; i < P_NSTAGE; ++i) ptx::mbar_init(&full[i], 1), ptx::mbar_init(&done[i], 1);
     for (int i = 0; i < P_NSCALE; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&s_empty[i], 8);
     for (int i = 0; i < 2; ++i) ptx::mbar_init(&acc_empty[i], 16);   // both CTAs' warps
-    ptx::mbar_init(drained, 1);
+    ptx::mbar_init(drained, 2);
     ptx::fence_mbar_init();
   }
   __syncwarp();
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
   if (warp < 4) {
     ptx::setmaxnreg_dec<P_REG_LOW>();
     if (warp == 0 && lane == 0) {
-      const int64_t m_pad = (p.M + 3) & ~(int64_t)3, n_pad = (p.N + 3) & ~(int64_t)3;
+      const int64_t n_pad = (p.N + 3) & ~(int64_t)3;
       bool ok = true;
       Ring<P_NSTAGE> st;
       Ring<P_NSCALE> sc;
@@ -340,19 +343,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         int64_t tm, tn;
         pair_tile(t, tiles_m, tiles_n, tm, tn);
         const int64_t m0 = tm * 256 + rank * 128, n0 = tn * 256;
-        const uint32_t a_bytes = (uint32_t)max((int64_t)0, min((int64_t)128, m_pad - m0)) * 4;
-        const uint32_t b_bytes = B_ROWS ? (uint32_t)min((int64_t)256, n_pad - n0) * 4 : 0;
+        const uint32_t b_bytes = (uint32_t)min((int64_t)256, n_pad - n0) * 4;
         for (int kb = 0; kb < p.kb_count; ++kb) {
-          if (s_filled == P_NSCALE && !wait_or_record(&s_empty[sc.at], sc.parity ^ 1, p.wait_limit, 10)) { ok = false; break; }
+          if (B_ROWS && s_filled == P_NSCALE && !wait_or_record(&s_empty[sc.at], sc.parity ^ 1, p.wait_limit, 10)) { ok = false; break; }
           if (filled == P_NSTAGE && !wait_or_record(&done[st.at], st.parity ^ 1, p.wait_limit, 11)) { ok = false; break; }
           const uint32_t bar = ptx::map_shared(ptx::smem_u32(&full[st.at]), 0);
           if (rank == 0) ptx::mbar_arrive_expect_tx(&full[st.at], 2 * P_STAGE);   // both CTAs' bytes
           ptx::tma_load_2d_pair(smem + st.at * P_STAGE, &map_a, bar, kb * BK, (int)m0);
           ptx::tma_load_2d_pair(smem + st.at * P_STAGE + 128 * BK, &map_b, bar, kb * BK, (int)(n0 + rank * 128));
-          float* slot = scales + sc.at * (P_SCALE / 4);
-          ptx::mbar_arrive_expect_tx(&s_full[sc.at], a_bytes + b_bytes);
-          if (a_bytes) ptx::bulk_load(slot, p.sa + kb * p.ldsa + m0, a_bytes, &s_full[sc.at]);
-          if (b_bytes) ptx::bulk_load(slot + 128, p.sb + kb * p.ldsb + n0, b_bytes, &s_full[sc.at]);
+          if (B_ROWS) {
+            ptx::mbar_arrive_expect_tx(&s_full[sc.at], b_bytes);
+            ptx::bulk_load(scales + sc.at * (P_SCALE / 4), p.sb + kb * p.ldsb + n0, b_bytes, &s_full[sc.at]);
+          }
           st.next();
           sc.next();
           if (filled < P_NSTAGE) ++filled;
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       // stopped at different blocks: then time for copies in flight.
       const Ring<P_NSCALE> sc_end = sc;
       for (int j = 0; j < P_NSCALE; ++j, sc.next())                  // oldest first: slots of the round before, then of this one
-        if (j >= P_NSCALE - s_filled)
+        if (B_ROWS && j >= P_NSCALE - s_filled)
           wait_or_record(&s_full[sc.at], sc.at < sc_end.at ? sc_end.parity : sc_end.parity ^ 1, DRAIN_LIMIT, 12);
       if (ok && rank == 0) {
         const Ring<P_NSTAGE> st_end = st;
@@ -376,26 +378,26 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         const long long t0 = clock64();
         while (clock64() - t0 < 200000) {}
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-      const uint32_t tmem = *tmem_slot;
+    } else if ((warp == 1 || warp == 2) && lane == 0 && rank == 0) {
+      const uint32_t tmem = *tmem_slot + (warp - 1) * 256;
+      uint64_t* acc_free = &acc_empty[warp - 1];
       bool ok = true, first_block = true;
       Ring<P_NSTAGE> st;
-      Ring<2> ac;
-      int filled = 0;
+      uint32_t parity = 1;                                           // of the accumulator's round before: free at first
+      int turn = 1;
       for (int64_t t = first; t < tiles && ok; t += stride) {
-        for (int kb = 0; kb < p.kb_count; ++kb) {
-          if (filled == 2 && !wait_or_record(&acc_empty[ac.at], ac.parity ^ 1, p.wait_limit, 13)) { ok = false; break; }
+        for (int kb = 0; kb < p.kb_count; ++kb, st.next(), turn ^= 3) {
+          if (turn != warp) continue;                                // the other warp's block
+          if (!wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
           if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
+          parity ^= 1;
           ptx::tc_fence_after();
           const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE));
           const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE + 128 * BK));
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem + ac.at * 256, da + 2 * k, db + 2 * k, p.idesc, k > 0);
-          if (!(first_block && p.hold_first_ready)) ptx::mma2_commit_both(&done[st.at]);
+          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem, da + 2 * k, db + 2 * k, p.idesc, k > 0);
+          if (!(first_block && warp == 1 && p.hold_first_ready)) ptx::mma2_commit_both(&done[st.at]);
           first_block = false;
-          st.next();
-          ac.next();
-          if (filled < 2) ++filled;
         }
       }
       ptx::mma2_commit_both(drained);
@@ -417,23 +419,28 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       pair_tile(t, tiles_m, tiles_n, tm, tn);
       const int64_t nb = min(tn * 2 + half, blocks_n - 1);
       const float* sb_tile = p.sb + nb * p.ldsb;
-      uint64_t acc[64];
+      float acc[128];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0;
-      float sb_next = B_ROWS ? 0.0f : __ldg(sb_tile);
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      // this row's scale and the column block's, read three blocks ahead
+      const float* sa_row = p.sa + min(tm * 256 + rank * 128 + quarter * 32 + lane, p.M - 1);
+      float sa1 = __ldg(sa_row), sa2 = p.kb_count > 1 ? __ldg(sa_row + p.ldsa) : 0.0f;
+      float sa3 = p.kb_count > 2 ? __ldg(sa_row + 2 * p.ldsa) : 0.0f, sb3 = B_ROWS || p.kb_count < 3 ? 1.0f : __ldg(sb_tile + 2);
+      float sb1 = B_ROWS ? 1.0f : __ldg(sb_tile), sb2 = B_ROWS || p.kb_count < 2 ? 1.0f : __ldg(sb_tile + 1);
       uint32_t v[2][32];
       if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
       ptx::tc_fence_after();
       ptx::tmem_ld_regs(lane_base + ac, v[0]);
       for (int kb = 0; kb < p.kb_count; ++kb) {
         const bool more = kb + 1 < p.kb_count;
-        const float sb = sb_next;
-        if (!B_ROWS && more) sb_next = __ldg(sb_tile + kb + 1);
-        if (!warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
+        const float f = B_ROWS ? sa1 : __fmul_rn(sa1, sb1);
+        sa1 = sa2, sb1 = sb2, sa2 = sa3, sb2 = sb3;
+        if (kb + 3 < p.kb_count) {
+          sa3 = __ldg(sa_row + (kb + 3) * p.ldsa);
+          if (!B_ROWS) sb3 = __ldg(sb_tile + kb + 3);
+        }
+        if (B_ROWS && !warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
         const float* slot = scales + sc.at * (P_SCALE / 4);
-        const float sa = slot[quarter * 32 + lane];
-        const float f = B_ROWS ? sa : __fmul_rn(sa, sb);
-        const uint64_t f2 = ptx::pack2(f, f);
         st.next();
         bool next = false;
 #pragma unroll
@@ -448,30 +455,33 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
             if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac / 32);   // 8 bytes per 256 columns
             ac ^= 256;
             if (more) {
-              next = __all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(&done[st.at], st.parity));
+              next = __all_sync(0xFFFFFFFFu, ptx::mbar_test_wait(&done[st.at], st.parity));
               if (next) {
                 ptx::tc_fence_after();
                 ptx::tmem_ld_regs(lane_base + ac, v[0]);
               }
             }
           }
-          const float4* sb4 = reinterpret_cast<const float4*>(slot + 128 + half * 128 + c * 32);
+          const float4* sb4 = reinterpret_cast<const float4*>(slot + half * 128 + c * 32);
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            uint64_t x = ptx::join2(v[c & 1][2 * j], v[c & 1][2 * j + 1]);
-            uint64_t y = ptx::join2(v[c & 1][2 * j + 2], v[c & 1][2 * j + 3]);
+          for (int j = 0; j < 32; j += 4) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[c & 1][j + e]);
             if (B_ROWS) {
-              const float4 s4 = sb4[j / 2];
-              x = ptx::mul2(x, ptx::pack2(s4.x, s4.y));
-              y = ptx::mul2(y, ptx::pack2(s4.z, s4.w));
+              const float4 s4 = sb4[j / 4];
+              x[0] = __fmul_rn(x[0], s4.x), x[1] = __fmul_rn(x[1], s4.y);
+              x[2] = __fmul_rn(x[2], s4.z), x[3] = __fmul_rn(x[3], s4.w);
             }
-            acc[c * 16 + j] = ptx::fma2(x, f2, acc[c * 16 + j]);
-            acc[c * 16 + j + 1] = ptx::fma2(y, f2, acc[c * 16 + j + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c * 32 + j + e] = __fmaf_rn(x[e], f, acc[c * 32 + j + e]);
           }
         }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&s_empty[sc.at]);
-        sc.next();
+        if (B_ROWS) {
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&s_empty[sc.at]);
+          sc.next();
+        }
         if (more && !next) {
           if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
           ptx::tc_fence_after();
@@ -491,9 +501,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         if (esz == 4) {
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const uint64_t x = acc[c * 16 + 2 * u], y = acc[c * 16 + 2 * u + 1];
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) =
-                make_uint4((uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32));
+            const float* x = acc + c * 32 + 4 * u;
+            *reinterpret_cast<float4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
           }
         } else if (c < 3) {
 #pragma unroll
@@ -501,12 +510,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t x = acc[(c * 16 + 4 * u + e) & 63];
+              const float lo = acc[(c * 32 + 8 * u + 2 * e) & 127], hi = acc[(c * 32 + 8 * u + 2 * e + 1) & 127];
               if (p.out_mode == EMU_DTYPE_BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(ptx::lo2(x), ptx::hi2(x));
+                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
                 w[e] = reinterpret_cast<const uint32_t&>(h);
               } else {
-                const __half2 h = __floats2half2_rn(ptx::lo2(x), ptx::hi2(x));
+                const __half2 h = __floats2half2_rn(lo, hi);
                 w[e] = reinterpret_cast<const uint32_t&>(h);
               }
             }
