@@ -1,11 +1,13 @@
 // Rounding to the 8-bit formats exactly as defined: code = nearest value of the format to the quotient
 // x / scale (scale an f32), ties to even.
 //
-// A product x * (1 / scale) is within 2 units of f32's last place of the quotient, so it rounds to the
-// same code unless the quotient lies that near to a border between two codes.  Those few elements
-// (about one in 2^16, or all exact ties of 16-bit inputs) are decided by comparing |x| with
-// border * scale, a product of at most 4 + 24 bits that f64 holds exactly.  A division for each
-// element would cost twice the quantiser's instructions and still collapse near-ties into ties.
+// x is multiplied by two f32 numbers that enclose 1 / scale (a relative 2^-21 below and above it, wider
+// than the errors of the reciprocal and the product) and both products are converted: where the two
+// codes agree, the quotient between them has that code too.  They differ for quotients that lie that
+// near to a border between two codes -- about one element in 2^15, and all exact ties, which 16-bit
+// inputs meet often under power-of-two scales -- and then |x| is compared with border * scale, a product
+// of at most 5 + 24 bits that f64 holds exactly.  Two products and two conversions cost less than one
+// division, which would still turn near-ties into ties.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -18,107 +20,164 @@ namespace f8 {
 
 template <int TYPE> struct Fmt;
 template <> struct Fmt<EMU_FP8_E4M3> {
-  static constexpr int BITS = 3;                       // stored significand bits
   static constexpr float MAX = 448.0f;
-  static constexpr float MIN_NORMAL = 0x1p-6f;
   static constexpr __nv_fp8_interpretation_t KIND = __NV_E4M3;
 };
 template <> struct Fmt<EMU_FP8_E5M2> {
-  static constexpr int BITS = 2;
   static constexpr float MAX = 57344.0f;
-  static constexpr float MIN_NORMAL = 0x1p-14f;
   static constexpr __nv_fp8_interpretation_t KIND = __NV_E5M2;
 };
+constexpr uint32_t NAN_CODE = 0x7Fu;   // a NaN of both types
 
-// |x| for the group maximum: 0 for NaN and infinities, which are stored as NaN and scale nothing.
-__device__ __forceinline__ float finite_magnitude(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? __uint_as_float(b) : 0.0f;
+// 8 consecutive elements as they were read, two 16-bit elements to a word.
+template <typename T> struct Raw {
+  static constexpr int WORDS = 2 * sizeof(T);
+  uint32_t w[WORDS];
+};
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
-// The group's scale: the smallest normal f32 for groups that hold (almost) nothing, so that 1 / scale
-// stays finite.
-template <int TYPE>
-__device__ __forceinline__ float scale_of(float amax) {
-  return fmaxf(__fdiv_rn(amax, Fmt<TYPE>::MAX), 0x1p-126f);
+template <typename T> __device__ __forceinline__ float element(const Raw<T>& r, int i);
+template <> __device__ __forceinline__ float element(const Raw<float>& r, int i) { return __uint_as_float(r.w[i]); }
+template <> __device__ __forceinline__ float element(const Raw<__nv_bfloat16>& r, int i) {
+  return __uint_as_float(i & 1 ? r.w[i / 2] & 0xFFFF0000u : r.w[i / 2] << 16);
+}
+template <> __device__ __forceinline__ float element(const Raw<__half>& r, int i) {
+  return __half2float(__ushort_as_half((unsigned short)(i & 1 ? r.w[i / 2] >> 16 : r.w[i / 2])));
 }
 
-// y ~ x / scale, near a border of the format?
-template <int TYPE>
-__device__ __forceinline__ bool near_border(float y) {
-  constexpr int D = 23 - Fmt<TYPE>::BITS;              // bits of an f32 significand that the format drops
-  constexpr uint32_t HALF = 1u << (D - 1);
-  const float a = fabsf(y);
-  // below the smallest normal the step is that of the first binade: adding its start aligns the bits
-  const float t = a < Fmt<TYPE>::MIN_NORMAL ? a + Fmt<TYPE>::MIN_NORMAL : a;
-  return (__float_as_uint(t) & ((1u << D) - 1u)) - (HALF - 8u) <= 16u;
+// Magnitudes are compared as bit patterns, which order like the values, infinities and NaN above all of
+// them.  Such a top tells that the block needs finite_top.
+template <typename T> __device__ __forceinline__ uint32_t top_bits(const Raw<T>& r) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, r.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max_u16x2(m, r.w[i] & 0x7FFF7FFFu);
+    return max(m & 0xFFFFu, m >> 16);
+  }
+}
+template <typename T> __device__ __forceinline__ bool special(uint32_t bits);
+template <> __device__ __forceinline__ bool special<float>(uint32_t b) { return b >= 0x7F800000u; }
+template <> __device__ __forceinline__ bool special<__half>(uint32_t b) { return b >= 0x7C00u; }
+template <> __device__ __forceinline__ bool special<__nv_bfloat16>(uint32_t b) { return b >= 0x7F80u; }
+template <typename T> __device__ __forceinline__ float bits_to_float(uint32_t b);
+template <> __device__ __forceinline__ float bits_to_float<float>(uint32_t b) { return __uint_as_float(b); }
+template <> __device__ __forceinline__ float bits_to_float<__half>(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+template <> __device__ __forceinline__ float bits_to_float<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
+// one element's magnitude bits, 0 for NaN and infinities (which are stored as NaN and scale nothing)
+template <typename T> __device__ __forceinline__ uint32_t finite_bits(const Raw<T>& r, int i) {
+  uint32_t b;
+  if constexpr (sizeof(T) == 4) b = r.w[i] & 0x7FFFFFFFu;
+  else b = (i & 1 ? r.w[i / 2] >> 16 : r.w[i / 2]) & 0x7FFFu;
+  return special<T>(b) ? 0u : b;
+}
+template <typename T> __device__ __forceinline__ uint32_t finite_top_bits(const Raw<T>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(r, i));
+  return m;
 }
 
-// y near a border: the border itself if |x| / scale is exactly there, else a value clearly on its side.
-template <int TYPE>
-__device__ __noinline__ float settle(float x, float y, float scale) {
-  constexpr int D = 23 - Fmt<TYPE>::BITS;
-  const float a = fabsf(y);
-  const bool sub = a < Fmt<TYPE>::MIN_NORMAL;
-  const float t = sub ? a + Fmt<TYPE>::MIN_NORMAL : a;
-  float mid = __uint_as_float((__float_as_uint(t) & ~((1u << D) - 1u)) | (1u << (D - 1)));
-  if (sub) mid -= Fmt<TYPE>::MIN_NORMAL;
-  const double q = fabs((double)x), m = __dmul_rn((double)mid, (double)scale);
-  if (y != y) return y;
-  const float r = q > m ? mid * (1.0f + 0x1p-10f) : q < m ? mid * (1.0f - 0x1p-10f) : mid;
-  return copysignf(r, y);
+// A block's scale and the two numbers around its reciprocal.  The smallest normal f32 for blocks that hold
+// (almost) nothing, so that 1 / scale stays finite.
+struct Scale {
+  float s, lo, hi;
+};
+template <int TYPE> __device__ __forceinline__ Scale scale_of(float amax) {
+  Scale r;
+  r.s = fmaxf(__fdiv_rn(amax, Fmt<TYPE>::MAX), 0x1p-126f);
+  const float inv = __frcp_rn(r.s);
+  r.lo = __fmul_rn(inv, 1.0f - 0x1p-21f);
+  r.hi = __fmul_rn(inv, 1.0f + 0x1p-21f);
+  return r;
 }
 
-// 8 elements -> 8 codes (byte i = element i).  inv = 1 / scale in f32.
-template <int TYPE>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8], float scale, float inv) {
+template <int TYPE> __device__ __forceinline__ uint32_t cvt2(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, Fmt<TYPE>::KIND);
+}
+
+// The code of x where the two products' codes differ; `lo` is the one nearer to zero.
+template <int TYPE> __device__ __noinline__ uint32_t settle(float x, float scale, uint32_t lo) {
+  const uint32_t m = lo & 0x7Fu;
+  const __half_raw a = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)m, Fmt<TYPE>::KIND);
+  const __half_raw b = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(m + 1), Fmt<TYPE>::KIND);
+  const double mid = 0.5 * ((double)__half2float(__half(a)) + (double)__half2float(__half(b)));
+  const double q = fabs((double)x), t = __dmul_rn(mid, (double)scale);
+  return (lo & 0x80u) | (q > t ? m + 1 : q < t ? m : m + (m & 1u));
+}
+
+// 8 elements -> 8 codes (byte i = element i).
+template <int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s) {
+  uint32_t lo[4], hi[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = cvt2<TYPE>(__fmul_rn(x[2 * i], s.lo), __fmul_rn(x[2 * i + 1], s.lo));
+    hi[i] = cvt2<TYPE>(__fmul_rn(x[2 * i], s.hi), __fmul_rn(x[2 * i + 1], s.hi));
+  }
+  uint2 w = make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
+  const uint2 h = make_uint2(__byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
+  if ((w.x ^ h.x) | (w.y ^ h.y)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t& word = i < 4 ? w.x : w.y;
+      const uint32_t other = i < 4 ? h.x : h.y;
+      const int sh = 8 * (i & 3);
+      if (((word ^ other) >> sh) & 0xFFu) {
+        const uint32_t c = settle<TYPE>(x[i], s.s, (word >> sh) & 0xFFu);
+        word = (word & ~(0xFFu << sh)) | (c << sh);
+      }
+    }
+  }
+  return w;
+}
+
+// The same for a block that holds NaN or infinities: they become NaN.
+template <int TYPE> __device__ __noinline__ uint2 encode8_special(float x0, float x1, float x2, float x3, float x4, float x5,
+                                                                  float x6, float x7, float s, float lo, float hi) {
+  const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
   float y[8];
-  bool near_any = false;
+  uint2 bad = make_uint2(0, 0);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    y[i] = __fmaf_rn(x[i], 0.0f, __fmul_rn(x[i], inv));   // x * 0 turns an infinity into NaN and adds nothing else
-    near_any |= near_border<TYPE>(y[i]);
+    const bool b = (__float_as_uint(x[i]) & 0x7FFFFFFFu) >= 0x7F800000u;
+    y[i] = b ? 0.0f : x[i];
+    if (b) (i < 4 ? bad.x : bad.y) |= NAN_CODE << (8 * (i & 3));
   }
-  if (near_any) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (near_border<TYPE>(y[i])) y[i] = settle<TYPE>(x[i], y[i], scale);
-  }
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, Fmt<TYPE>::KIND);
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  const uint2 w = encode8<TYPE>(y, Scale{s, lo, hi});
+  return make_uint2(w.x | bad.x, w.y | bad.y);
 }
-
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s, bool specials) {
+  if (specials) return encode8_special<TYPE>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s.s, s.lo, s.hi);
+  return encode8<TYPE>(x, s);
+}
 
 // 8 consecutive elements, `valid` of them in range (the others 0).  VEC: p is 16-byte aligned.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int valid, float (&x)[8]) {
+__device__ __forceinline__ void load8(const T* p, int valid, Raw<T>& r) {
   if (VEC && valid >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        T lo, hi;
-        reinterpret_cast<uint16_t&>(lo) = (uint16_t)u[i];
-        reinterpret_cast<uint16_t&>(hi) = (uint16_t)(u[i] >> 16);
-        x[2 * i] = to_float<T>(lo);
-        x[2 * i + 1] = to_float<T>(hi);
-      }
-    } else {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    for (int i = 0; i < Raw<T>::WORDS / 4; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < valid ? to_float<T>(p[i]) : 0.0f;
+  for (int i = 0; i < Raw<T>::WORDS; ++i) r.w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= valid) continue;
+    if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(p[i]);
+    else r.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+  }
 }
 
 // 8 codes to q (8-byte aligned), `valid` of them in range.

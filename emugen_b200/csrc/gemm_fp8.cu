@@ -388,8 +388,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       for (int64_t t = first; t < tiles && ok; t += stride) {
         for (int kb = 0; kb < p.kb_count; ++kb, st.next(), turn ^= 3) {
           if (turn != warp) continue;                                // the other warp's block
-          if (!wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
+          // the stage filled long ago as a rule, the accumulator comes free last
           if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
+          if (!wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
           parity ^= 1;
           ptx::tc_fence_after();
           const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE));

@@ -72,20 +72,27 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteArgs a, int 
     const int64_t slot = have ? own[i] : -1;
     const bool live = have && !dead[i] && slot >= 0 && slot < a.num_slots;
     const int valid = live && d < a.D ? 8 : 0;               // D is a multiple of 16
-    float v[8];
+    f8::Raw<T> r;
     f8::load8<T, VEC>(static_cast<const T*>(a.x[which]) + (i0 + i) * a.token_stride[which] + h * a.head_stride[which] + d,
-                      valid, v);
+                      valid, r);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f8::element(r, e);
     const int64_t row = slot * a.H + h;
     if (FORMAT == EMU_KV_FP8) {
-      float top = 0.0f;
+      uint32_t top = f8::top_bits(r);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, f8::finite_magnitude(v[e]));
+      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const bool sp = f8::special<T>(top);
+      if (__any_sync(0xFFFFFFFFu, sp)) {
+        top = f8::finite_top_bits(r);
 #pragma unroll
-      for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      const float s = f8::scale_of<EMU_FP8_E4M3>(top);
-      const uint2 w = f8::encode8<EMU_FP8_E4M3>(v, s, __frcp_rn(s));
+        for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      }
+      const f8::Scale s = f8::scale_of<EMU_FP8_E4M3>(f8::bits_to_float<T>(top));
+      const uint2 w = f8::encode8<EMU_FP8_E4M3>(v, s, sp);
       if (valid) *reinterpret_cast<uint2*>(a.q[which] + row * a.D + d) = w;
-      if (live && lane16 == 0) static_cast<float*>(a.scale[which])[row * G + g] = s;
+      if (live && lane16 == 0) static_cast<float*>(a.scale[which])[row * G + g] = s.s;
     } else {
       // as quant_fp4_kernel<T, 32>: the same roundings and flushes, so the same bytes
       float top = 0.0f;

@@ -33,18 +33,25 @@ __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict
     const int64_t k = kb * 128 + lane16 * 8;
     const bool live = row < M && kb < kb_count;
     const int valid = live ? (int)min((int64_t)8, max((int64_t)0, K - k)) : 0;
+    f8::Raw<T> r;
+    f8::load8<T, VEC>(x + row * ldx + k, valid, r);
+    uint32_t top = f8::top_bits(r);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const bool sp = f8::special<T>(top);
+    if (__any_sync(0xFFFFFFFFu, sp)) {                       // (rare) leave out what is not finite
+      top = f8::finite_top_bits(r);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    }
+    const f8::Scale sc = f8::scale_of<TYPE>(f8::bits_to_float<T>(top));
     float v[8];
-    f8::load8<T, VEC>(x + row * ldx + k, valid, v);
-    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, f8::finite_magnitude(v[i]));
-#pragma unroll
-    for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float s = f8::scale_of<TYPE>(top);
-    const uint2 w = f8::encode8<TYPE>(v, s, __frcp_rn(s));
+    for (int i = 0; i < 8; ++i) v[i] = f8::element(r, i);
+    const uint2 w = f8::encode8<TYPE>(v, sc, sp);
     if (!live) continue;
     f8::store8(q + row * ldq + k, w, valid);
-    if (lane16 == 0) scale[kb * lds + row] = s;
+    if (lane16 == 0) scale[kb * lds + row] = sc.s;
   }
 }
 
@@ -60,98 +67,144 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
                                                              float* __restrict__ scale_t, int64_t ldst) {
   constexpr int PITCH = 136;                               // bytes per transposed row: 8-byte aligned, rows 34 banks apart
   __shared__ __align__(16) uint8_t tr[128 * PITCH];
-  __shared__ float col_top[8][128];
+  __shared__ uint32_t col_top[8][128];
   const int tid = threadIdx.x, cx = tid & 15, ry = tid >> 4, warp = tid >> 5;
   const int64_t tiles_k = (K + 127) / 128;
   const int64_t mb = blockIdx.x / tiles_k, kb = blockIdx.x % tiles_k;
   const int64_t r0 = mb * 128 + ry * 8, c0 = kb * 128 + cx * 8;
   const int valid_c = (int)min((int64_t)8, max((int64_t)0, K - c0));
   const int valid_r = (int)min((int64_t)8, max((int64_t)0, M - r0));
-  float v[8][8];
+  f8::Raw<T> r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f8::load8<T, VEC>(x + (r0 + i) * ldx + c0, i < valid_r ? valid_c : 0, v[i]);
+  for (int i = 0; i < 8; ++i) f8::load8<T, VEC>(x + (r0 + i) * ldx + c0, i < valid_r ? valid_c : 0, r[i]);
 
-  float row_top[8], ct[8];
+  uint32_t row_top[8], ct[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ct[j] = 0.0f;
+  for (int i = 0; i < 8; ++i) row_top[i] = f8::top_bits(r[i]);
+  // specials anywhere in the tile (rare): every maximum is taken again over the finite elements
+  uint32_t any = row_top[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    row_top[i] = 0.0f;
+  for (int i = 1; i < 8; ++i) any = max(any, row_top[i]);
+  const bool sp = __syncthreads_or(f8::special<T>(any));
+  if (sp) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = f8::finite_magnitude(v[i][j]);
-      row_top[i] = fmaxf(row_top[i], a);
-      ct[j] = fmaxf(ct[j], a);
-    }
+    for (int i = 0; i < 8; ++i) row_top[i] = f8::finite_top_bits(r[i]);
   }
   if (!TILE) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t pair[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4; ++i) {                          // two rows' tops to a word
+        pair[i] = row_top[2 * i] | (row_top[2 * i + 1] << 16);
 #pragma unroll
-      for (int o = 8; o; o >>= 1) row_top[i] = fmaxf(row_top[i], __shfl_xor_sync(0xFFFFFFFFu, row_top[i], o));
+        for (int o = 8; o; o >>= 1) pair[i] = f8::max_u16x2(pair[i], __shfl_xor_sync(0xFFFFFFFFu, pair[i], o));
+        row_top[2 * i] = pair[i] & 0xFFFFu, row_top[2 * i + 1] = pair[i] >> 16;
+      }
+      if (qt) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ct[j] = fmaxf(ct[j], __shfl_xor_sync(0xFFFFFFFFu, ct[j], 16));   // the warp's two row groups
-      if ((tid & 16) == 0) col_top[warp][cx * 8 + j] = ct[j];
+        for (int j = 0; j < 4; ++j) {                        // two columns' tops to a word
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t e = sp ? f8::finite_bits(r[i], 2 * j) | (f8::finite_bits(r[i], 2 * j + 1) << 16) : r[i].w[j] & 0x7FFF7FFFu;
+            m = f8::max_u16x2(m, e);
+          }
+          m = f8::max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));   // the warp's two row groups
+          ct[2 * j] = m & 0xFFFFu, ct[2 * j + 1] = m >> 16;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int o = 8; o; o >>= 1) row_top[i] = max(row_top[i], __shfl_xor_sync(0xFFFFFFFFu, row_top[i], o));
+      if (qt) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          ct[j] = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ct[j] = max(ct[j], sp ? f8::finite_bits(r[i], j) : r[i].w[j] & 0x7FFFFFFFu);
+          ct[j] = max(ct[j], __shfl_xor_sync(0xFFFFFFFFu, ct[j], 16));
+        }
+      }
+    }
+    if (qt && (tid & 16) == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        *reinterpret_cast<uint4*>(&col_top[warp][cx * 8 + j]) = make_uint4(ct[j], ct[j + 1], ct[j + 2], ct[j + 3]);
     }
   } else {
-    float top = row_top[0];
+    uint32_t top = row_top[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, row_top[i]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int i = 1; i < 8; ++i) top = max(top, row_top[i]);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
     if ((tid & 31) == 0) col_top[warp][0] = top;
   }
   __syncthreads();
-  float tile_s = 0.0f, tile_inv = 0.0f;
+  f8::Scale ts{};
   if (TILE) {
-    float top = col_top[0][0];
+    uint32_t top = col_top[0][0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, col_top[w][0]);
-    tile_s = f8::scale_of<TYPE>(top);
-    tile_inv = __frcp_rn(tile_s);
+    for (int w = 1; w < 8; ++w) top = max(top, col_top[w][0]);
+    ts = f8::scale_of<TYPE>(f8::bits_to_float<T>(top));
     if (tid == 0) {
-      if (q) scale[mb * lds + kb] = tile_s;
-      if (qt) scale_t[kb * ldst + mb] = tile_s;
+      if (q) scale[mb * lds + kb] = ts.s;
+      if (qt) scale_t[kb * ldst + mb] = ts.s;
     }
   }
   uint2 rows8[8];                                          // TILE: the rows' codes, shared by both outputs
   if (q || TILE) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float s = TILE ? tile_s : f8::scale_of<TYPE>(row_top[i]);
-      const float inv = TILE ? tile_inv : __frcp_rn(s);
-      rows8[i] = f8::encode8<TYPE>(v[i], s, inv);
+      const f8::Scale s = TILE ? ts : f8::scale_of<TYPE>(f8::bits_to_float<T>(row_top[i]));
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = f8::element(r[i], j);
+      rows8[i] = f8::encode8<TYPE>(v, s, sp);
       if (q && i < valid_r) {
         f8::store8(q + (r0 + i) * ldq + c0, rows8[i], valid_c);
-        if (!TILE && cx == 0) scale[kb * lds + r0 + i] = s;
+        if (!TILE && cx == 0) scale[kb * lds + r0 + i] = s.s;
       }
     }
   }
   if (!qt) return;
+  if (TILE) {
+    // 8 x 8 bytes turned: column j's bytes of rows 0-3 and 4-7
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint2 w;
-    if (TILE) {
-      uint32_t lo = 0, hi = 0;
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo |= (((j < 4 ? rows8[i].x : rows8[i].y) >> (8 * (j & 3))) & 0xFFu) << (8 * i);
-        hi |= (((j < 4 ? rows8[i + 4].x : rows8[i + 4].y) >> (8 * (j & 3))) & 0xFFu) << (8 * i);
+      for (int u = 0; u < 4; ++u) {
+        const int j = g * 4 + u;
+        uint32_t c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = g ? rows8[i].y : rows8[i].x;
+        const uint32_t sel = (uint32_t)u | (uint32_t)(u + 4) << 4;   // byte u of each of two words
+        const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], sel), __byte_perm(c[2], c[3], sel), 0x5410);
+        const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], sel), __byte_perm(c[6], c[7], sel), 0x5410);
+        *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = make_uint2(lo, hi);
       }
-      w = make_uint2(lo, hi);
-    } else {
-      float top = col_top[0][cx * 8 + j];
+  } else {
+    uint32_t top[8];
 #pragma unroll
-      for (int u = 1; u < 8; ++u) top = fmaxf(top, col_top[u][cx * 8 + j]);
-      const float s = f8::scale_of<TYPE>(top);
+    for (int j = 0; j < 8; ++j) top[j] = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const uint4 t4 = *reinterpret_cast<const uint4*>(&col_top[u][cx * 8 + j]);
+        top[j] = max(top[j], t4.x), top[j + 1] = max(top[j + 1], t4.y);
+        top[j + 2] = max(top[j + 2], t4.z), top[j + 3] = max(top[j + 3], t4.w);
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const f8::Scale s = f8::scale_of<TYPE>(f8::bits_to_float<T>(top[j]));
       float c[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = v[i][j];
-      w = f8::encode8<TYPE>(c, s, __frcp_rn(s));
-      if (ry == 0 && j < valid_c) scale_t[mb * ldst + c0 + j] = s;
+      for (int i = 0; i < 8; ++i) c[i] = f8::element(r[i], j);
+      const uint2 w = f8::encode8<TYPE>(c, s, sp);
+      if (ry == 0 && j < valid_c) scale_t[mb * ldst + c0 + j] = s.s;
+      *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = w;
     }
-    *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = w;
   }
   __syncthreads();
   // 16 threads write one transposed row of 128 codes
