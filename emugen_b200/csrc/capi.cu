@@ -493,7 +493,7 @@ emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_t K, int
     return fail(EMU_ERR_INVALID_ARGUMENT, "code rows must start on 16-byte boundaries");
   if ((q && ld_scale < (block == EMU_BLOCK_ROW ? M : kb)) || (qt && ld_scale_t < (block == EMU_BLOCK_ROW ? K : mb)))
     return fail(EMU_ERR_INVALID_ARGUMENT, "scale rows too short");
-  if (mb > 0x7FFFFFFF / kb || (M - 1) / 4 + 1 > 0x7FFFFFFF / ((kb - 1) / 4 + 1))
+  if (mb > 0x7FFFFFFF / kb)
     return fail(EMU_ERR_UNSUPPORTED, "more than 2^31 - 1 blocks");
   return cuda_status(emu::launch_quant_fp8(x, dtype, M, K, ldx, fp8_type, block, q, ldq, scale, ld_scale, qt, ldqt, scale_t,
                                            ld_scale_t, static_cast<cudaStream_t>(stream)),

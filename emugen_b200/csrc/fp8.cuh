@@ -1,13 +1,19 @@
 // Rounding to the 8-bit formats exactly as defined: code = nearest value of the format to the quotient
-// x / scale (scale an f32), ties to even.
+// x / scale, ties to even, where scale = fl32(amax / F), F = 7 * 2^n the type's largest value.
 //
-// x is multiplied by two f32 numbers that enclose 1 / scale (a relative 2^-21 below and above it, wider
-// than the errors of the reciprocal and the product) and both products are converted: where the two
-// codes agree, the quotient between them has that code too.  They differ for quotients that lie that
-// near to a border between two codes -- about one element in 2^15, and all exact ties, which 16-bit
-// inputs meet often under power-of-two scales -- and then |x| is compared with border * scale, a product
-// of at most 5 + 24 bits that f64 holds exactly.  Two products and two conversions cost less than one
-// division, which would still turn near-ties into ties.
+// 16-bit inputs.  F * x / amax is a quotient of short integers: against a border between two codes (an
+// odd multiple of half a step, at most 5 bits) it is either equal or at least a relative 2^-16 away, since
+// 7 x and border * amax have at most 14 and 16 bits.  Where it is equal, x / scale lies on the side that the
+// rounding of scale decides, for the whole block alike: below the border if F * scale > amax, above it if
+// F * scale < amax, on it if scale is exact.  So one product with 1 / scale, made a relative 2^-21
+// smaller or larger, rounds every element right; where scale is exact, the product is rounded to 20 bits
+// first, which takes its error away and leaves ties ties.
+//
+// f32 inputs.  x is multiplied by two numbers that enclose 1 / scale (a relative 2^-21 around it) and both
+// products are converted: where the codes agree, the quotient between them has that code too.  Where they
+// differ, border * scale - |x| is taken in one fused multiply-add, whose sign is exact.
+//
+// A division for each element would cost more than either and still turn near-ties into ties.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,10 +27,14 @@ namespace f8 {
 template <int TYPE> struct Fmt;
 template <> struct Fmt<EMU_FP8_E4M3> {
   static constexpr float MAX = 448.0f;
+  static constexpr int BITS = 3;                 // stored significand bits
+  static constexpr float REBIAS = 0x1p120f;      // f32's exponent bias over the type's
   static constexpr __nv_fp8_interpretation_t KIND = __NV_E4M3;
 };
 template <> struct Fmt<EMU_FP8_E5M2> {
   static constexpr float MAX = 57344.0f;
+  static constexpr int BITS = 2;
+  static constexpr float REBIAS = 0x1p112f;
   static constexpr __nv_fp8_interpretation_t KIND = __NV_E5M2;
 };
 constexpr uint32_t NAN_CODE = 0x7Fu;   // a NaN of both types
@@ -86,17 +96,28 @@ template <typename T> __device__ __forceinline__ uint32_t finite_top_bits(const 
   return m;
 }
 
-// A block's scale and the two numbers around its reciprocal.  The smallest normal f32 for blocks that hold
-// (almost) nothing, so that 1 / scale stays finite.
+// A block's scale with what its elements are multiplied by: `lo` and `hi` around the reciprocal (f32), or `lo`
+// alone (16-bit inputs; `exact`: rounded products).  The smallest normal f32 for blocks that hold (almost)
+// nothing, so that 1 / scale stays finite.
 struct Scale {
   float s, lo, hi;
+  bool exact;
 };
-template <int TYPE> __device__ __forceinline__ Scale scale_of(float amax) {
+template <typename T, int TYPE> __device__ __forceinline__ Scale scale_of(float amax) {
   Scale r;
-  r.s = fmaxf(__fdiv_rn(amax, Fmt<TYPE>::MAX), 0x1p-126f);
+  const float d = __fdiv_rn(amax, Fmt<TYPE>::MAX);
+  r.s = fmaxf(d, 0x1p-126f);
   const float inv = __frcp_rn(r.s);
-  r.lo = __fmul_rn(inv, 1.0f - 0x1p-21f);
-  r.hi = __fmul_rn(inv, 1.0f + 0x1p-21f);
+  if constexpr (sizeof(T) == 4) {
+    r.lo = __fmul_rn(inv, 1.0f - 0x1p-21f);
+    r.hi = __fmul_rn(inv, 1.0f + 0x1p-21f);
+    r.exact = false;
+  } else {
+    const float e = __fmaf_rn(Fmt<TYPE>::MAX, r.s, -amax);
+    r.exact = e == 0.0f || d < 0x1p-126f;                      // (a scale of 2^-126 has an exact reciprocal)
+    r.lo = r.exact ? inv : __fmul_rn(inv, e > 0.0f ? 1.0f - 0x1p-21f : 1.0f + 0x1p-21f);
+    r.hi = r.lo;
+  }
   return r;
 }
 
@@ -104,44 +125,59 @@ template <int TYPE> __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, Fmt<TYPE>::KIND);
 }
 
-// The code of x where the two products' codes differ; `lo` is the one nearer to zero.
-template <int TYPE> __device__ __noinline__ uint32_t settle(float x, float scale, uint32_t lo) {
+// The code of x where the two products' codes differ; `lo` is the one nearer to zero.  The border above it
+// is its code with half a step more, read as an f32 (subnormals included) and rebiased.
+template <int TYPE> __device__ __forceinline__ uint32_t settle(float x, float scale, uint32_t lo) {
   const uint32_t m = lo & 0x7Fu;
-  const __half_raw a = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)m, Fmt<TYPE>::KIND);
-  const __half_raw b = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(m + 1), Fmt<TYPE>::KIND);
-  const double mid = 0.5 * ((double)__half2float(__half(a)) + (double)__half2float(__half(b)));
-  const double q = fabs((double)x), t = __dmul_rn(mid, (double)scale);
-  return (lo & 0x80u) | (q > t ? m + 1 : q < t ? m : m + (m & 1u));
+  const float mid = __fmul_rn(__uint_as_float((2u * m + 1u) << (22 - Fmt<TYPE>::BITS)), Fmt<TYPE>::REBIAS);
+  if (scale < 0x1p-60f) x *= 0x1p60f, scale *= 0x1p60f;      // the difference must not underflow
+  const float d = __fmaf_rn(mid, scale, -fabsf(x));
+  return (lo & 0x80u) | (m + (d < 0.0f ? 1u : d > 0.0f ? 0u : m & 1u));
 }
-
-// 8 elements -> 8 codes (byte i = element i).
-template <int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s) {
-  uint32_t lo[4], hi[4];
+// Out of line: few elements of f32 inputs come here, and its code eight times over would not stay in the
+// instruction cache.
+template <int TYPE> __device__ __noinline__ uint2 settle8(float x0, float x1, float x2, float x3, float x4, float x5,
+                                                          float x6, float x7, float scale, uint2 w, uint2 h) {
+  const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = cvt2<TYPE>(__fmul_rn(x[2 * i], s.lo), __fmul_rn(x[2 * i + 1], s.lo));
-    hi[i] = cvt2<TYPE>(__fmul_rn(x[2 * i], s.hi), __fmul_rn(x[2 * i + 1], s.hi));
-  }
-  uint2 w = make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
-  const uint2 h = make_uint2(__byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
-  if ((w.x ^ h.x) | (w.y ^ h.y)) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t& word = i < 4 ? w.x : w.y;
-      const uint32_t other = i < 4 ? h.x : h.y;
-      const int sh = 8 * (i & 3);
-      if (((word ^ other) >> sh) & 0xFFu) {
-        const uint32_t c = settle<TYPE>(x[i], s.s, (word >> sh) & 0xFFu);
-        word = (word & ~(0xFFu << sh)) | (c << sh);
-      }
+  for (int i = 0; i < 8; ++i) {
+    uint32_t& word = i < 4 ? w.x : w.y;
+    const int sh = 8 * (i & 3);
+    if (((word ^ (i < 4 ? h.x : h.y)) >> sh) & 0xFFu) {
+      const uint32_t c = settle<TYPE>(x[i], scale, (word >> sh) & 0xFFu);
+      word = (word & ~(0xFFu << sh)) | (c << sh);
     }
   }
   return w;
 }
 
+// 8 elements -> 8 codes (byte i = element i).
+template <typename T, int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s) {
+  uint32_t lo[4];
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[i], s.lo);
+  if (sizeof(T) == 2 && s.exact) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __uint_as_float((__float_as_uint(y[i]) + 8u) & ~15u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lo[i] = cvt2<TYPE>(y[2 * i], y[2 * i + 1]);
+  const uint2 w = make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
+  if constexpr (sizeof(T) == 4) {
+    uint32_t hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = cvt2<TYPE>(__fmul_rn(x[2 * i], s.hi), __fmul_rn(x[2 * i + 1], s.hi));
+    const uint2 h = make_uint2(__byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
+    if ((w.x ^ h.x) | (w.y ^ h.y)) return settle8<TYPE>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s.s, w, h);
+  }
+  return w;
+}
+
 // The same for a block that holds NaN or infinities: they become NaN.
-template <int TYPE> __device__ __noinline__ uint2 encode8_special(float x0, float x1, float x2, float x3, float x4, float x5,
-                                                                  float x6, float x7, float s, float lo, float hi) {
+template <typename T, int TYPE>
+__device__ __noinline__ uint2 encode8_special(float x0, float x1, float x2, float x3, float x4, float x5, float x6,
+                                              float x7, Scale s) {
   const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
   float y[8];
   uint2 bad = make_uint2(0, 0);
@@ -151,12 +187,12 @@ template <int TYPE> __device__ __noinline__ uint2 encode8_special(float x0, floa
     y[i] = b ? 0.0f : x[i];
     if (b) (i < 4 ? bad.x : bad.y) |= NAN_CODE << (8 * (i & 3));
   }
-  const uint2 w = encode8<TYPE>(y, Scale{s, lo, hi});
+  const uint2 w = encode8<T, TYPE>(y, s);
   return make_uint2(w.x | bad.x, w.y | bad.y);
 }
-template <int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s, bool specials) {
-  if (specials) return encode8_special<TYPE>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s.s, s.lo, s.hi);
-  return encode8<TYPE>(x, s);
+template <typename T, int TYPE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], const Scale& s, bool specials) {
+  if (specials) return encode8_special<T, TYPE>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s);
+  return encode8<T, TYPE>(x, s);
 }
 
 // 8 consecutive elements, `valid` of them in range (the others 0).  VEC: p is 16-byte aligned.

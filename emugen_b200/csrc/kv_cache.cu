@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteArgs a, int 
 #pragma unroll
         for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       }
-      const f8::Scale s = f8::scale_of<EMU_FP8_E4M3>(f8::bits_to_float<T>(top));
-      const uint2 w = f8::encode8<EMU_FP8_E4M3>(v, s, sp);
+      const f8::Scale s = f8::scale_of<T, EMU_FP8_E4M3>(f8::bits_to_float<T>(top));
+      const uint2 w = f8::encode8<T, EMU_FP8_E4M3>(v, s, sp);
       if (valid) *reinterpret_cast<uint2*>(a.q[which] + row * a.D + d) = w;
       if (live && lane16 == 0) static_cast<float*>(a.scale[which])[row * G + g] = s.s;
     } else {

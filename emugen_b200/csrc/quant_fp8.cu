@@ -18,40 +18,45 @@
 namespace emu {
 namespace {
 
-// Rows in 1 x 128 blocks.  16 lanes hold one block, 8 elements each; a CTA of 256 threads takes 4 rows
-// x 4 blocks at a time (1 KB of consecutive 16-bit input per row).
-template <typename T, int TYPE, bool VEC>
+// Rows in 1 x 128 blocks.  16 lanes hold one block, 8 elements each; a CTA of 256 threads takes 4 U rows
+// x 4 blocks (1 KB of consecutive 16-bit input per row), U loads in flight per thread.
+template <typename T, int TYPE, bool VEC, int U>
 __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
                                                              uint8_t* __restrict__ q, int64_t ldq,
                                                              float* __restrict__ scale, int64_t lds) {
   const int lane16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int64_t kb_count = (K + 127) / 128;
-  const int64_t tiles_k = (kb_count + 3) / 4, tiles_m = (M + 3) / 4;
-  for (int64_t t = blockIdx.x; t < tiles_k * tiles_m; t += gridDim.x) {
-    const int64_t row = t / tiles_k * 4 + (grp >> 2);
-    const int64_t kb = t % tiles_k * 4 + (grp & 3);
-    const int64_t k = kb * 128 + lane16 * 8;
-    const bool live = row < M && kb < kb_count;
-    const int valid = live ? (int)min((int64_t)8, max((int64_t)0, K - k)) : 0;
-    f8::Raw<T> r;
-    f8::load8<T, VEC>(x + row * ldx + k, valid, r);
-    uint32_t top = f8::top_bits(r);
+  const int64_t kb = (int64_t)blockIdx.x * 4 + (grp & 3), k = kb * 128 + lane16 * 8;
+  const int valid_k = (int)min((int64_t)8, max((int64_t)0, K - k));
+  for (int64_t m0 = (int64_t)blockIdx.y * (4 * U); m0 < M; m0 += (int64_t)gridDim.y * (4 * U)) {
+    const int64_t row0 = m0 + (grp >> 2);
+    f8::Raw<T> r[U];
 #pragma unroll
-    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const bool sp = f8::special<T>(top);
-    if (__any_sync(0xFFFFFFFFu, sp)) {                       // (rare) leave out what is not finite
-      top = f8::finite_top_bits(r);
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + 4 * u;
+      f8::load8<T, VEC>(x + row * ldx + k, row < M ? valid_k : 0, r[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + 4 * u;
+      uint32_t top = f8::top_bits(r[u]);
 #pragma unroll
       for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    }
-    const f8::Scale sc = f8::scale_of<TYPE>(f8::bits_to_float<T>(top));
-    float v[8];
+      const bool sp = f8::special<T>(top);
+      if (__any_sync(0xFFFFFFFFu, sp)) {                     // (rare) leave out what is not finite
+        top = f8::finite_top_bits(r[u]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = f8::element(r, i);
-    const uint2 w = f8::encode8<TYPE>(v, sc, sp);
-    if (!live) continue;
-    f8::store8(q + row * ldq + k, w, valid);
-    if (lane16 == 0) scale[kb * lds + row] = sc.s;
+        for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      }
+      const f8::Scale sc = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top));
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = f8::element(r[u], i);
+      const uint2 w = f8::encode8<T, TYPE>(v, sc, sp);
+      if (row >= M || kb >= kb_count) continue;
+      f8::store8(q + row * ldq + k, w, valid_k);
+      if (lane16 == 0) scale[kb * lds + row] = sc.s;
+    }
   }
 }
 
@@ -69,8 +74,8 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
   __shared__ __align__(16) uint8_t tr[128 * PITCH];
   __shared__ uint32_t col_top[8][128];
   const int tid = threadIdx.x, cx = tid & 15, ry = tid >> 4, warp = tid >> 5;
-  const int64_t tiles_k = (K + 127) / 128;
-  const int64_t mb = blockIdx.x / tiles_k, kb = blockIdx.x % tiles_k;
+  const int tiles_k = (int)((K + 127) / 128);              // the grid holds below 2^31 tiles
+  const int64_t mb = blockIdx.x / (unsigned)tiles_k, kb = blockIdx.x % (unsigned)tiles_k;
   const int64_t r0 = mb * 128 + ry * 8, c0 = kb * 128 + cx * 8;
   const int valid_c = (int)min((int64_t)8, max((int64_t)0, K - c0));
   const int valid_r = (int)min((int64_t)8, max((int64_t)0, M - r0));
@@ -146,7 +151,7 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
     uint32_t top = col_top[0][0];
 #pragma unroll
     for (int w = 1; w < 8; ++w) top = max(top, col_top[w][0]);
-    ts = f8::scale_of<TYPE>(f8::bits_to_float<T>(top));
+    ts = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top));
     if (tid == 0) {
       if (q) scale[mb * lds + kb] = ts.s;
       if (qt) scale_t[kb * ldst + mb] = ts.s;
@@ -156,11 +161,11 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
   if (q || TILE) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const f8::Scale s = TILE ? ts : f8::scale_of<TYPE>(f8::bits_to_float<T>(row_top[i]));
+      const f8::Scale s = TILE ? ts : f8::scale_of<T, TYPE>(f8::bits_to_float<T>(row_top[i]));
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = f8::element(r[i], j);
-      rows8[i] = f8::encode8<TYPE>(v, s, sp);
+      rows8[i] = f8::encode8<T, TYPE>(v, s, sp);
       if (q && i < valid_r) {
         f8::store8(q + (r0 + i) * ldq + c0, rows8[i], valid_c);
         if (!TILE && cx == 0) scale[kb * lds + r0 + i] = s.s;
@@ -197,11 +202,11 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
       }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const f8::Scale s = f8::scale_of<TYPE>(f8::bits_to_float<T>(top[j]));
+      const f8::Scale s = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top[j]));
       float c[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) c[i] = f8::element(r[i], j);
-      const uint2 w = f8::encode8<TYPE>(c, s, sp);
+      const uint2 w = f8::encode8<T, TYPE>(c, s, sp);
       if (ry == 0 && j < valid_c) scale_t[mb * ldst + c0 + j] = s.s;
       *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = w;
     }
@@ -221,13 +226,26 @@ template <typename T, int TYPE>
 cudaError_t launch_t(const T* x, int64_t M, int64_t K, int64_t ldx, int block, uint8_t* q, int64_t ldq, float* scale,
                      int64_t lds, uint8_t* qt, int64_t ldqt, float* scale_t, int64_t ldst, cudaStream_t stream) {
   // rows that start on 16 bytes are read 16 bytes at a time
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
   const int64_t kb = (K + 127) / 128, mb = (M + 127) / 128;
   if (block == EMU_BLOCK_ROW && !qt) {
-    const int64_t tiles = ((kb + 3) / 4) * ((M + 3) / 4);
-    const unsigned grid = (unsigned)std::min<int64_t>(tiles, 0x7FFFFFFF);
-    if (vec) quant_fp8_rows_kernel<T, TYPE, true><<<grid, 256, 0, stream>>>(x, M, K, ldx, q, ldq, scale, lds);
-    else quant_fp8_rows_kernel<T, TYPE, false><<<grid, 256, 0, stream>>>(x, M, K, ldx, q, ldq, scale, lds);
+    // many rows: 16 per CTA with four loads in flight per thread; few: 4 per CTA, so that more SMs work
+    const int64_t tiles_k = (kb + 3) / 4;
+    const bool deep = tiles_k * ((M + 15) / 16) >= 2 * sms;
+#define EMU_ROWS(V, U)                                                                                             \
+  quant_fp8_rows_kernel<T, TYPE, V, U>                                                                             \
+      <<<dim3((unsigned)tiles_k, (unsigned)std::min<int64_t>((M + 4 * U - 1) / (4 * U), 65535)), 256, 0, stream>>>( \
+          x, M, K, ldx, q, ldq, scale, lds)
+    if (vec) {
+      if (deep) EMU_ROWS(true, 4);
+      else EMU_ROWS(true, 1);
+    } else {
+      EMU_ROWS(false, 1);
+    }
+#undef EMU_ROWS
     return cudaGetLastError();
   }
   const unsigned grid = (unsigned)(kb * mb);
