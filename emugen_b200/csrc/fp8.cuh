@@ -99,22 +99,28 @@ template <typename T> __device__ __forceinline__ uint32_t finite_top_bits(const 
 // A block's scale with what its elements are multiplied by: `lo` and `hi` around the reciprocal (f32), or `lo`
 // alone (16-bit inputs; `exact`: rounded products).  The smallest normal f32 for blocks that hold (almost)
 // nothing, so that 1 / scale stays finite.
+// (lo and hi: the reciprocal's error, 2^-23, the product's, 2^-24, and scale's own stay within the 2^-21.)
 struct Scale {
   float s, lo, hi;
   bool exact;
 };
 template <typename T, int TYPE> __device__ __forceinline__ Scale scale_of(float amax) {
   Scale r;
-  const float d = __fdiv_rn(amax, Fmt<TYPE>::MAX);
+  // amax / F rounded to nearest: the product with the rounded 1 / F, corrected once by its exact remainder
+  // (Markstein 1990); below 2^-126, where remainders would underflow, the result is not used
+  constexpr float RCP = 1.0f / Fmt<TYPE>::MAX;
+  const float d0 = __fmul_rn(amax, RCP);
+  const float d = __fmaf_rn(__fmaf_rn(-d0, Fmt<TYPE>::MAX, amax), RCP, d0);
   r.s = fmaxf(d, 0x1p-126f);
-  const float inv = __frcp_rn(r.s);
+  float inv;                                                   // to 1 unit of the last place
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(r.s));
   if constexpr (sizeof(T) == 4) {
     r.lo = __fmul_rn(inv, 1.0f - 0x1p-21f);
     r.hi = __fmul_rn(inv, 1.0f + 0x1p-21f);
     r.exact = false;
   } else {
     const float e = __fmaf_rn(Fmt<TYPE>::MAX, r.s, -amax);
-    r.exact = e == 0.0f || d < 0x1p-126f;                      // (a scale of 2^-126 has an exact reciprocal)
+    r.exact = e == 0.0f || d < 0x1p-126f;
     r.lo = r.exact ? inv : __fmul_rn(inv, e > 0.0f ? 1.0f - 0x1p-21f : 1.0f + 0x1p-21f);
     r.hi = r.lo;
   }

@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp8.cuh"
@@ -36,19 +37,35 @@ __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict
       const int64_t row = row0 + 4 * u;
       f8::load8<T, VEC>(x + row * ldx + k, row < M ? valid_k : 0, r[u]);
     }
+    uint32_t top[U];
+    bool sp = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      top[u] = f8::top_bits(r[u]);
+      sp |= f8::special<T>(top[u]);
+    }
+    sp = __any_sync(0xFFFFFFFFu, sp);
+    if (sp) {                                                // (rare) leave out what is not finite
+#pragma unroll
+      for (int u = 0; u < U; ++u) top[u] = f8::finite_top_bits(r[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (sizeof(T) == 2 && U > 1) {                         // two rows' tops to a word
+        if (u & 1) continue;
+        uint32_t two = top[u] | top[(u + 1) % U] << 16;
+#pragma unroll
+        for (int o = 8; o; o >>= 1) two = f8::max_u16x2(two, __shfl_xor_sync(0xFFFFFFFFu, two, o));
+        top[u] = two & 0xFFFFu, top[(u + 1) % U] = two >> 16;
+      } else {
+#pragma unroll
+        for (int o = 8; o; o >>= 1) top[u] = max(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], o));
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = row0 + 4 * u;
-      uint32_t top = f8::top_bits(r[u]);
-#pragma unroll
-      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      const bool sp = f8::special<T>(top);
-      if (__any_sync(0xFFFFFFFFu, sp)) {                     // (rare) leave out what is not finite
-        top = f8::finite_top_bits(r[u]);
-#pragma unroll
-        for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      }
-      const f8::Scale sc = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top));
+      const f8::Scale sc = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top[u]));
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = f8::element(r[u], i);
@@ -65,7 +82,7 @@ __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict
 // transposed codes go through shared memory so that both outputs are written in 128-byte runs.
 // TILE: one scale for the tile; otherwise one per row (q) and one per column (qt).
 template <typename T, int TYPE, bool VEC, bool TILE>
-__global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
+__global__ void __launch_bounds__(256, TILE ? 1 : sizeof(T) == 2 ? 3 : 2) quant_fp8_tile_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
                                                              uint8_t* __restrict__ q, int64_t ldq,
                                                              float* __restrict__ scale, int64_t lds,
                                                              uint8_t* __restrict__ qt, int64_t ldqt,
@@ -157,60 +174,67 @@ __global__ void __launch_bounds__(256) quant_fp8_tile_kernel(const T* __restrict
       if (qt) scale_t[kb * ldst + mb] = ts.s;
     }
   }
-  uint2 rows8[8];                                          // TILE: the rows' codes, shared by both outputs
-  if (q || TILE) {
+  // encoded twice over in the code, with and without the test for what is not finite
+  auto encode = [&](auto specials) {
+    constexpr bool SP = decltype(specials)::value;
+    uint2 rows8[8];                                          // TILE: the rows' codes, shared by both outputs
+    if (q || TILE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const f8::Scale s = TILE ? ts : f8::scale_of<T, TYPE>(f8::bits_to_float<T>(row_top[i]));
-      float v[8];
+      for (int i = 0; i < 8; ++i) {
+        const f8::Scale s = TILE ? ts : f8::scale_of<T, TYPE>(f8::bits_to_float<T>(row_top[i]));
+        float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = f8::element(r[i], j);
-      rows8[i] = f8::encode8<T, TYPE>(v, s, sp);
-      if (q && i < valid_r) {
-        f8::store8(q + (r0 + i) * ldq + c0, rows8[i], valid_c);
-        if (!TILE && cx == 0) scale[kb * lds + r0 + i] = s.s;
+        for (int j = 0; j < 8; ++j) v[j] = f8::element(r[i], j);
+        rows8[i] = f8::encode8<T, TYPE>(v, s, SP);
+        if (q && i < valid_r) {
+          f8::store8(q + (r0 + i) * ldq + c0, rows8[i], valid_c);
+          if (!TILE && cx == 0) scale[kb * lds + r0 + i] = s.s;
+        }
       }
     }
-  }
+    if (!qt) return;
+    if (TILE) {
+      // 8 x 8 bytes turned: column j's bytes of rows 0-3 and 4-7
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = g * 4 + u;
+          uint32_t c[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[i] = g ? rows8[i].y : rows8[i].x;
+          const uint32_t sel = (uint32_t)u | (uint32_t)(u + 4) << 4;   // byte u of each of two words
+          const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], sel), __byte_perm(c[2], c[3], sel), 0x5410);
+          const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], sel), __byte_perm(c[6], c[7], sel), 0x5410);
+          *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = make_uint2(lo, hi);
+        }
+    } else {
+      uint32_t top[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const uint4 t4 = *reinterpret_cast<const uint4*>(&col_top[u][cx * 8 + j]);
+          top[j] = max(top[j], t4.x), top[j + 1] = max(top[j + 1], t4.y);
+          top[j + 2] = max(top[j + 2], t4.z), top[j + 3] = max(top[j + 3], t4.w);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const f8::Scale s = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top[j]));
+        float c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = f8::element(r[i], j);
+        const uint2 w = f8::encode8<T, TYPE>(c, s, SP);
+        if (ry == 0 && j < valid_c) scale_t[mb * ldst + c0 + j] = s.s;
+        *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = w;
+      }
+    }
+  };
+  if (sp) encode(std::true_type{});
+  else encode(std::false_type{});
   if (!qt) return;
-  if (TILE) {
-    // 8 x 8 bytes turned: column j's bytes of rows 0-3 and 4-7
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = g * 4 + u;
-        uint32_t c[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = g ? rows8[i].y : rows8[i].x;
-        const uint32_t sel = (uint32_t)u | (uint32_t)(u + 4) << 4;   // byte u of each of two words
-        const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], sel), __byte_perm(c[2], c[3], sel), 0x5410);
-        const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], sel), __byte_perm(c[6], c[7], sel), 0x5410);
-        *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = make_uint2(lo, hi);
-      }
-  } else {
-    uint32_t top[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top[j] = 0;
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const uint4 t4 = *reinterpret_cast<const uint4*>(&col_top[u][cx * 8 + j]);
-        top[j] = max(top[j], t4.x), top[j + 1] = max(top[j + 1], t4.y);
-        top[j + 2] = max(top[j + 2], t4.z), top[j + 3] = max(top[j + 3], t4.w);
-      }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const f8::Scale s = f8::scale_of<T, TYPE>(f8::bits_to_float<T>(top[j]));
-      float c[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = f8::element(r[i], j);
-      const uint2 w = f8::encode8<T, TYPE>(c, s, sp);
-      if (ry == 0 && j < valid_c) scale_t[mb * ldst + c0 + j] = s.s;
-      *reinterpret_cast<uint2*>(tr + (cx * 8 + j) * PITCH + ry * 8) = w;
-    }
-  }
   __syncthreads();
   // 16 threads write one transposed row of 128 codes
 #pragma unroll
