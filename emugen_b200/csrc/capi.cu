@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/emugen.h"
@@ -41,6 +42,19 @@ bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p
 emu_status emu::record_failure(emu_status s, const char* message) {
   g_last_error = message;
   return s;
+}
+
+int emu::sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& k = known[dev & 63];
+  int n = dev < 64 ? k.load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    if (dev < 64) k.store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 extern "C" {

@@ -591,12 +591,25 @@ bool make_map(CUtensorMap* m, const uint8_t* base, int64_t rows, int64_t K, int6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Raises a kernel's shared-memory limit, once for each device.
+template <typename Kernel> cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int BN>
 cudaError_t launch_skinny(const Fp8GemmArgs& g, Params p, int sms, cudaStream_t stream) {
   CUtensorMap ma, mb;
   if (!make_map(&mb, g.b, g.N, g.K, g.ldb, LANES) || !make_map(&ma, g.a, g.M, g.K, g.lda, BN)) return cudaErrorUnknown;
   auto kernel = gemm_fp8_skinny_kernel<BN>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(kernel, Cfg<BN>::SMEM, done);
   if (e != cudaSuccess) return e;
   p.idesc = ptx::idesc_f8_f32(LANES, BN, g.b_type, g.a_type);
   const int64_t tiles_n = (g.N + LANES - 1) / LANES, tiles_m = (g.M + BN - 1) / BN;
@@ -622,7 +635,8 @@ cudaError_t launch_pair(const Fp8GemmArgs& g, Params p, int sms, cudaStream_t st
   CUtensorMap ma, mb;
   if (!make_map(&ma, g.a, g.M, g.K, g.lda, 128) || !make_map(&mb, g.b, g.N, g.K, g.ldb, 128)) return cudaErrorUnknown;
   auto kernel = gemm_fp8_pair_kernel<B_ROWS>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(kernel, P_SMEM, done);
   if (e != cudaSuccess) return e;
   p.idesc = ptx::idesc_f8_f32(256, 256, g.a_type, g.b_type);
   const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
@@ -650,9 +664,7 @@ cudaError_t take_fp8_wait_error(int* code) {
 }
 
 cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   Params p{};
   p.sa = g.sa, p.sb = g.sb, p.ldsa = g.ldsa, p.ldsb = g.ldsb;
   p.M = g.M, p.N = g.N;

@@ -82,6 +82,9 @@ cudaError_t launch_gemm_tc(const uint8_t* A, const uint8_t* B, const uint8_t* SA
 cudaError_t launch_quant(int sf_vec, const void* x, int dtype, int64_t M, int64_t K,
                          const float* global_scale, uint8_t* q, uint8_t* sf, cudaStream_t stream);
 
+// The current device's number of SMs, asked of the runtime once for each device (capi.cu).
+int sm_count();
+
 // Block-scaled 8-bit quantiser (quant_fp8.cu); q or qt may be null.
 cudaError_t launch_quant_fp8(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fp8_type, int block,
                              uint8_t* q, int64_t ldq, float* scale, int64_t lds, uint8_t* qt, int64_t ldqt,

@@ -245,9 +245,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
 }  // namespace
 
 cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t stream) {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   // up to 16 tokens to each of 4 CTAs of 256 threads per SM; longer calls 2 CTAs of 1024 threads per SM, so that
   // fewer CTAs read all later slots (find_overwritten)
   const bool wide = a.T > 64 * (int64_t)sms;
@@ -276,9 +274,7 @@ cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t stream) {
 }
 
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream) {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   // up to 32 rows per CTA, fewer while the SMs (8 CTAs of 256 threads each) are not filled twice
   const int per_cta = (int)std::min<int64_t>(READ_ROWS, (a.total + 16 * sms - 1) / (16 * sms));
   const unsigned grid = (unsigned)((a.total + per_cta - 1) / per_cta);

@@ -250,9 +250,7 @@ template <typename T, int TYPE>
 cudaError_t launch_t(const T* x, int64_t M, int64_t K, int64_t ldx, int block, uint8_t* q, int64_t ldq, float* scale,
                      int64_t lds, uint8_t* qt, int64_t ldqt, float* scale_t, int64_t ldst, cudaStream_t stream) {
   // rows that start on 16 bytes are read 16 bytes at a time
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
   const int64_t kb = (K + 127) / 128, mb = (M + 127) / 128;
   if (block == EMU_BLOCK_ROW && !qt) {

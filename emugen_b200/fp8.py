@@ -14,6 +14,8 @@ torch's allocator) and do not synchronise, so that CUDA graphs can capture them.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -28,9 +30,14 @@ def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
-def _on(dev: torch.device):
-    """Make `dev` current for the call (nothing to do where it already is)."""
-    return torch.cuda.device(dev.index)
+_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(dev).cuda_stream without its objects
+
+
+def _on(index: int):
+    """Make device `index` current for the call.  Where it already is, as in most calls, entering and
+    leaving torch.cuda.device would cost a small launch's time."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _codes(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
@@ -43,7 +50,7 @@ def _codes(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch
 def _row_scales(rows: int, blocks: int, dev: torch.device) -> torch.Tensor:
     """[rows, blocks] scales stored block after block, each block's row a multiple of 4 floats."""
     pitch = (rows + 3) // 4 * 4
-    s = torch.empty((blocks, pitch), dtype=torch.float32, device=dev).t()
+    s = torch.empty_strided((pitch, blocks), (1, pitch), dtype=torch.float32, device=dev)
     return s if pitch == rows else s[:rows]
 
 
@@ -65,48 +72,61 @@ def quant_fp8(x: torch.Tensor, *, block: str = "row", dtype: torch.dtype = torch
         raise RuntimeError(f"quantiser input must be float16, bfloat16 or float32, got {x.dtype}")
     if x.dim() == 0:
         raise RuntimeError("quantiser input must have at least one dimension")
-    L = _lib.load()
-    dev = _lib._device_for(x)
-    x = x.detach()
+    if not x.is_cuda:
+        x = x.to(_lib._device_for(x))
+    if x.requires_grad:
+        x = x.detach()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.shape[:-1].numel(), 0)
-    if x.device != dev:
-        x = x.to(dev)
+    return _quant(x, _BLOCKS[block], dtype, transposed)
+
+
+def _quant(x: torch.Tensor, block: int, dtype: torch.dtype, transposed: bool):
+    """quant_fp8 of a checked CUDA matrix."""
+    dev = x.device
     M, K = x.shape
-    if x.stride(1) != 1 and K > 1 or x.stride(0) < K and M > 1:   # overlapping or column-strided rows
+    ldx, inner = x.stride()
+    if inner != 1 and K > 1 or ldx < K and M > 1:   # overlapping or column-strided rows
         x = x.contiguous()
-    ldx = max(x.stride(0), K) if M > 1 else K
+        ldx = K
+    mb, kb = _blocks(M), _blocks(K)
     q = _codes(M, K, dtype, dev)
-    qt = _codes(K, M, dtype, dev) if transposed else None
-    if block == "row":
-        s = _row_scales(M, _blocks(K), dev)
-        st = _row_scales(K, _blocks(M), dev) if transposed else None
-        lds, ldst = (M + 3) // 4 * 4, (K + 3) // 4 * 4
+    if block == _lib.EMU_BLOCK_ROW:
+        s, lds = _row_scales(M, kb, dev), (M + 3) // 4 * 4
     else:
-        s = torch.empty((_blocks(M), _blocks(K)), dtype=torch.float32, device=dev)
-        st = torch.empty((_blocks(K), _blocks(M)), dtype=torch.float32, device=dev) if transposed else None
-        lds, ldst = _blocks(K), _blocks(M)
+        s, lds = torch.empty((mb, kb), dtype=torch.float32, device=dev), kb
+    qt = st = None
+    ldst = 0
+    if transposed:
+        qt = _codes(K, M, dtype, dev)
+        if block == _lib.EMU_BLOCK_ROW:
+            st, ldst = _row_scales(K, mb, dev), (K + 3) // 4 * 4
+        else:
+            st, ldst = torch.empty((kb, mb), dtype=torch.float32, device=dev), mb
     if M and K:
-        with _on(dev):
-            status = L.emu_quant_fp8(x.data_ptr(), _DTYPE[x.dtype], M, K, ldx, _FP8[dtype], _BLOCKS[block],
+        L = _lib.load()
+        with _on(dev.index):
+            status = L.emu_quant_fp8(x.data_ptr(), _DTYPE[x.dtype], M, K, ldx if M > 1 else K, _FP8[dtype], block,
                                      q.data_ptr(), (K + 15) // 16 * 16, s.data_ptr(), lds,
                                      qt.data_ptr() if transposed else None, (M + 15) // 16 * 16,
-                                     st.data_ptr() if transposed else None, ldst, _lib._stream(dev))
-        _lib._check(status)
+                                     st.data_ptr() if transposed else None, ldst, _raw_stream(dev.index))
+        if status:
+            _lib._check(status)
     return (q, s, qt, st) if transposed else (q, s)
 
 
-def _operand(t: torch.Tensor, dev: torch.device, name: str):
+def _operand(t: torch.Tensor, dev: torch.device):
     """(tensor kept alive, pitch in bytes): rows that start on 16 bytes, copied there if they do not."""
     if t.device != dev:
         t = t.to(dev)
     rows, cols = t.shape
-    if cols and rows and (t.stride(1) != 1 and cols > 1 or rows > 1 and (t.stride(0) % 16 or t.stride(0) < cols)
-                          or t.data_ptr() % 16):
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1 or rows > 1 and (ld % 16 or ld < cols) or t.data_ptr() % 16:
         c = _codes(rows, cols, t.dtype, dev)
         c.view(torch.uint8).copy_(t.view(torch.uint8))
         t = c
-    return t, t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
+        ld = t.stride(0)
+    return t, ld if rows > 1 else (cols + 15) // 16 * 16
 
 
 def _scale_rows(s: torch.Tensor, dev: torch.device):
@@ -116,11 +136,12 @@ def _scale_rows(s: torch.Tensor, dev: torch.device):
         s = s.to(dev)
     rows, blocks = s.shape
     r4 = (rows + 3) // 4 * 4
-    ld = s.stride(1) if blocks > 1 else r4
-    good = (rows == 1 or s.stride(0) == 1) and ld % 4 == 0 and ld >= r4 and s.data_ptr() % 16 == 0
+    inner, ld = s.stride()
+    if blocks == 1:
+        ld = r4
+    good = (rows == 1 or inner == 1) and ld % 4 == 0 and ld >= r4 and s.data_ptr() % 16 == 0
     if good and r4 != rows:
-        end = s.storage_offset() + (blocks - 1) * ld + r4
-        good = end * 4 <= s.untyped_storage().nbytes()
+        good = (s.storage_offset() + (blocks - 1) * ld + r4) * 4 <= s.untyped_storage().nbytes()
     if not good:
         c = _row_scales(rows, blocks, dev)
         c.copy_(s)
@@ -154,31 +175,40 @@ def gemm_fp8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: t
     rows = tuple(scale_b.shape) == (N, kb)
     if not rows and tuple(scale_b.shape) != (_blocks(N), kb):
         raise RuntimeError(f"scale_b must be [{N}, {kb}] or [{_blocks(N)}, {kb}], got {list(scale_b.shape)}")
-    L = _lib.load()
-    on_cpu = not (a.is_cuda or b.is_cuda or scale_a.is_cuda or scale_b.is_cuda)
+    if a.is_cuda:
+        return _gemm(a, b, scale_a, scale_b, rows, out_dtype, a.device)
+    on_cpu = not (b.is_cuda or scale_a.is_cuda or scale_b.is_cuda)
     dev = _lib._device_for(a, b, scale_a, scale_b)
-    out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    if M and N:
-        with _on(dev):
-            if K:
-                a_, lda = _operand(a, dev, "a")
-                b_, ldb = _operand(b, dev, "b")
-                sa, ldsa = _scale_rows(scale_a, dev)
-                if rows:
-                    sb, ldsb = _scale_rows(scale_b, dev)
-                else:
-                    sb = scale_b.to(dev).contiguous()
-                    ldsb = kb
-                status = L.emu_gemm_fp8(a_.data_ptr(), lda, _FP8[a.dtype], b_.data_ptr(), ldb, _FP8[b.dtype],
-                                        sa.data_ptr(), ldsa, sb.data_ptr(), ldsb,
-                                        _lib.EMU_BLOCK_ROW if rows else _lib.EMU_BLOCK_TILE, M, N, K,
-                                        _DTYPE[out_dtype], out.data_ptr(), N, _lib._stream(dev))
-                _lib._check(status)
-            else:
-                out.zero_()
+    out = _gemm(a, b, scale_a, scale_b, rows, out_dtype, dev)
     if on_cpu:
         _lib.device_status(dev)
         return out.cpu()
+    return out
+
+
+def _gemm(a, b, scale_a, scale_b, rows: bool, out_dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """gemm_fp8 of checked operands on `dev`; rows: scale_b has a row for each of b's."""
+    M, K = a.shape
+    N = b.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if not (M and N):
+        return out
+    with _on(dev.index):
+        if not K:
+            return out.zero_()
+        a_, lda = _operand(a, dev)
+        b_, ldb = _operand(b, dev)
+        sa, ldsa = _scale_rows(scale_a, dev)
+        if rows:
+            sb, ldsb = _scale_rows(scale_b, dev)
+        else:
+            sb, ldsb = scale_b.to(dev).contiguous(), scale_b.shape[1]
+        status = _lib.load().emu_gemm_fp8(a_.data_ptr(), lda, _FP8[a.dtype], b_.data_ptr(), ldb, _FP8[b.dtype],
+                                          sa.data_ptr(), ldsa, sb.data_ptr(), ldsb,
+                                          _lib.EMU_BLOCK_ROW if rows else _lib.EMU_BLOCK_TILE, M, N, K,
+                                          _DTYPE[out_dtype], out.data_ptr(), N, _raw_stream(dev.index))
+    if status:
+        _lib._check(status)
     return out
 
 
@@ -186,27 +216,31 @@ class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
         need_x, need_w = ctx.needs_input_grad
-        x2 = x.reshape(-1, x.shape[-1])
+        dev, dtype = x.device, x.dtype
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         # the transposed codes serve the backward pass: x.T for the weight's gradient, weight.T for x's
-        q = quant_fp8(x2, transposed=need_w)
-        w = quant_fp8(weight, block="tile", transposed=need_x)
-        y = gemm_fp8(q[0], w[0], q[1], w[1], out_dtype=x.dtype)
+        q = _quant(x2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
+        w = _quant(weight, _lib.EMU_BLOCK_TILE, torch.float8_e4m3fn, need_x)
+        y = _gemm(q[0], w[0], q[1], w[1], False, dtype, dev)
         ctx.save_for_backward(*(q[2:] if need_w else (None, None)), *(w[2:] if need_x else (None, None)))
-        ctx.x_shape, ctx.x_dtype, ctx.w_dtype = x.shape, x.dtype, weight.dtype
-        return y.reshape(*x.shape[:-1], weight.shape[0])
+        ctx.x_shape = x.shape
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         xt, xts, wt, wts = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad
-        dy2 = dy.reshape(-1, dy.shape[-1])
-        g = quant_fp8(dy2, transposed=need_w)
+        dev, dtype = dy.device, dy.dtype
+        dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
+        g = _quant(dy2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
         dx = dw = None
         if need_x:
-            dx = gemm_fp8(g[0], wt, g[1], wts, out_dtype=ctx.x_dtype).reshape(ctx.x_shape)
+            dx = _gemm(g[0], wt, g[1], wts, False, dtype, dev)
+            if len(ctx.x_shape) != 2:
+                dx = dx.reshape(ctx.x_shape)
         if need_w:
-            dw = gemm_fp8(g[2], xt, g[3], xts, out_dtype=ctx.w_dtype)
+            dw = _gemm(g[2], xt, g[3], xts, True, dtype, dev)
         return dx, dw
 
 

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .fp8 import _DTYPE, _on
+from .fp8 import _DTYPE, _on, _raw_stream
 
 
 def make_kv_cache(num_pages: int, page_size: int, heads: int, head_size: int, fmt: str = "fp8", *,
@@ -107,12 +107,13 @@ def write_kv_cache(k: torch.Tensor, v: Optional[torch.Tensor], slots: torch.Tens
         v = v.contiguous()
     slots = slots.contiguous()
     L = _lib.load()
-    with _on(dev):
+    with _on(dev.index):
         status = L.emu_kv_write(k.data_ptr(), _ptr(v), _DTYPE[k.dtype], k.shape[0], heads, D, k.stride(0), k.stride(1),
                                 0 if v is None else v.stride(0), 0 if v is None else v.stride(1), slots.data_ptr(),
                                 fmt, pages * page_size, k_cache.data_ptr(), _ptr(v_cache), k_scale.data_ptr(),
-                                _ptr(v_scale), _lib._stream(dev))
-    _lib._check(status)
+                                _ptr(v_scale), _raw_stream(dev.index))
+    if status:
+        _lib._check(status)
 
 
 def read_kv_cache(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], k_scale: torch.Tensor,
@@ -164,13 +165,14 @@ def read_kv_cache(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], k_scal
     cu_lens = cu_lens.contiguous()
     row = heads * D
     L = _lib.load()
-    with _on(dev):
+    with _on(dev.index):
         status = L.emu_kv_read(k_cache.data_ptr(), _ptr(v_cache), k_scale.data_ptr(), _ptr(v_scale), fmt, pages, page_size,
                                heads, D, block_table.data_ptr(), B, cols, max(block_table.stride(0), cols),
                                cu_lens.data_ptr(), total, _DTYPE[k_out.dtype], k_out.data_ptr(), _ptr(v_out),
                                k_out.stride(0) if total > 1 else row,
-                               0 if v_out is None else v_out.stride(0) if total > 1 else row, _lib._stream(dev))
-    _lib._check(status)
+                               0 if v_out is None else v_out.stride(0) if total > 1 else row, _raw_stream(dev.index))
+    if status:
+        _lib._check(status)
     return k_out, v_out
 
 
