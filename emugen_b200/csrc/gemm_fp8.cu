@@ -14,7 +14,7 @@
 //
 //   warp 0      TMA: a 128 x 128 tile of B and a BN x 128 tile of A per block of K into a ring; bulk copies
 //               of the block's scales into a second ring
-//   warp 1      TMEM owner and MMA issuer
+//   warps 1, 6  MMA issuers in turn (warp 1 owns the TMEM)
 //   warps 2-5   epilogue: a thread owns one row of B (a TMEM lane) and BN accumulators
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -32,7 +32,7 @@ namespace {
 
 constexpr int BK = 128;                         // bytes of K per stage: one scale block, one 128-byte swizzle row
 constexpr int LANES = 128;
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;
 constexpr long long DRAIN_LIMIT = 1ll << 31;    // waits for copies / MMAs already in flight
 
 struct Params {
@@ -81,7 +81,7 @@ template <int BN> struct Cfg {
 };
 
 template <int BN>
-__global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(THREADS, BN == 128 ? 0 : 2) gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_b,
                                                                   const __grid_constant__ CUtensorMap map_a,
                                                                   const Params p) {
   using C = Cfg<BN>;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
     for (int i = 0; i < C::NSTAGE; ++i) ptx::mbar_init(&full[i], 1), ptx::mbar_init(&empty[i], 1);
     for (int i = 0; i < C::NSCALE; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&s_empty[i], 4);
     for (int i = 0; i < C::NACC; ++i) ptx::mbar_init(&acc_full[i], 1), ptx::mbar_init(&acc_empty[i], 4);
-    ptx::mbar_init(drained, 1);
+    ptx::mbar_init(drained, 2);
     *failed = 0;
     ptx::fence_mbar_init();
   }
@@ -153,9 +153,13 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
       for (int j = max(0, i - C::NSCALE); j < i; ++j)
         wait_or_record(&s_full[j % C::NSCALE], (j / C::NSCALE) & 1, DRAIN_LIMIT, 12);
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 6) {
     if (lane == 0) {
-      for (int i = 0; i < steps; ++i) {
+      // Two issuers, blocks in turn: NACC is even, so each has its own accumulators.  The accumulator is
+      // waited for first: it is free once block i - NACC has been read, so the stage's last block, i - NSTAGE,
+      // has landed, and the parity of the stage's barrier cannot be that of two rounds before.
+      static_assert(C::NACC % 2 == 0 && C::NSTAGE >= C::NACC, "see above");
+      for (int i = warp == 1 ? 0 : 1; i < steps; i += 2) {
         const int st = i % C::NSTAGE, ac = i % C::NACC;
         if (i >= C::NACC && !wait_or_record(&acc_empty[ac], (i / C::NACC - 1) & 1, p.wait_limit, 13)) break;
         if (!wait_or_record(&full[st], (i / C::NSTAGE) & 1, p.wait_limit, 14)) break;
@@ -165,8 +169,8 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)                          // 32 bytes of K per MMA: +2 in the descriptor
           ptx::mma_f8(tmem + ac * BN, da + 2 * k, db + 2 * k, p.idesc, k > 0);
-        ptx::mma_commit(&empty[st]);
         if (!(i == 0 && p.hold_first_ready)) ptx::mma_commit(&acc_full[ac]);
+        ptx::mma_commit(&empty[st]);
       }
       ptx::mma_commit(drained);
       wait_or_record(drained, 0, DRAIN_LIMIT, 15);
@@ -225,20 +229,26 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
 
   // partial sums: [column][lane] in the ring's place, then each CTA adds up its share of the columns
   float* part = reinterpret_cast<float*>(smem);
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const int l = (warp & 3) * 32 + lane;
 #pragma unroll
     for (int j = 0; j < BN; ++j) part[j * LANES + l] = *failed ? __int_as_float(0x7FC00000) : acc[j];
   }
   ptx::cluster_sync();
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const int l = (warp & 3) * 32 + lane;
     const int64_t n = n0 + l;
     const int j0 = BN * rank / split, j1 = BN * (rank + 1) / split;
+    uint32_t base[8];
+#pragma unroll
+    for (uint32_t r = 0; r < 8; ++r) base[r] = ptx::map_shared(ptx::smem_u32(part + l), r < split ? r : rank);
+#pragma unroll 2
     for (int j = j0; j < j1; ++j) {
-      const uint32_t at = ptx::smem_u32(part + j * LANES + l);
-      float s = 0.0f;
-      for (uint32_t r = 0; r < split; ++r) s = __fadd_rn(s, ptx::ld_shared_cluster(ptx::map_shared(at, r)));
+      float v[8], s = 0.0f;
+#pragma unroll
+      for (uint32_t r = 0; r < 8; ++r) v[r] = r < split ? ptx::ld_shared_cluster(base[r] + j * (LANES * 4)) : 0.0f;
+#pragma unroll
+      for (uint32_t r = 0; r < 8; ++r) s = r < split ? __fadd_rn(s, v[r]) : s;
       if (n < p.N && m0 + j < p.M) store_out(p.out, (m0 + j) * p.ldo + n, s, p.out_mode);
     }
   }
@@ -260,7 +270,7 @@ __global__ void __launch_bounds__(THREADS) gemm_fp8_skinny_kernel(const __grid_c
 //               B_ROWS = false: 128 columns share one scale of B, so the factor is one number per thread;
 //               B_ROWS = true: the block sum is multiplied by the column's scale first.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
-constexpr int P_NSTAGE = 5;
+constexpr int P_NSTAGE = 5;                      // at least 2: see the issuers' waits
 constexpr int P_NSCALE = 8;
 constexpr int P_SCALE = 256 * 4;                 // column scales (B_ROWS)
 constexpr int P_STORE = 8 * 32 * 128;            // per epilogue warp: 32 rows x 128 bytes of output
@@ -388,9 +398,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       for (int64_t t = first; t < tiles && ok; t += stride) {
         for (int kb = 0; kb < p.kb_count; ++kb, st.next(), turn ^= 3) {
           if (turn != warp) continue;                                // the other warp's block
-          // the stage filled long ago as a rule, the accumulator comes free last
-          if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
+          // The accumulator first: it is free once the epilogue has read block i - 2, so every block up to
+          // there has landed, among them the stage's last one, i - 5.  Only then can the parity of the
+          // stage's barrier not be taken for that of two rounds before (its rounds alternate between
+          // the issuers, so this thread has not waited for the one between).
           if (!wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
+          if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
           parity ^= 1;
           ptx::tc_fence_after();
           const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE));

@@ -400,3 +400,17 @@ def test_wait_limit_is_reported(M):
     _lib.device_status()
     out = fp8.gemm_fp8(*dev, out_dtype=torch.float32)
     assert (out.cpu().double().numpy() == O.gemm(a, b, sa, sb)[0]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 65536, 4096), (30, 40000, 2000), (100, 20000, 4096), (140, 20000, 4000)])
+@pytest.mark.parametrize("rows", [False, True])
+def test_gemm_many_blocks_and_ctas_exact(M, N, K, rows):
+    """More tiles than the SMs hold at once and many blocks of K each, the same call repeated: integers, so that a
+    stage read before it has landed would show.  The reference product is torch's in f64, on the GPU."""
+    a, b, sa, sb = [t.cuda() for t in _operands(M, N, K, E4, E4, rows, 17, True)]
+    kb = sa.shape[1]
+    full = lambda q, s: q.double() * s.double().repeat_interleave(128, 1)[:, :K]
+    ref = full(a, sa) @ full(b, sb if rows else sb.repeat_interleave(128, 0)[:N]).t()
+    for _ in range(4):
+        out = fp8.gemm_fp8(a, b, sa, sb, out_dtype=torch.float32)
+        assert torch.equal(out.double(), ref)
