@@ -542,7 +542,7 @@ emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, const uin
   if (b_block == EMU_BLOCK_TILE && (!aligned(scale_b, 4) || ld_scale_b < kb))
     return fail(EMU_ERR_SCALE_SHAPE, "scale_b: rows of at least ceil(K / 128) floats");
   if (K > 0x7FFFFF00ll) return fail(EMU_ERR_UNSUPPORTED, "K too large");
-  if ((M - 1) / 128 >= 65535 || (N - 1) / 128 >= 65535) return fail(EMU_ERR_UNSUPPORTED, "M and N up to 65535 * 128");
+  if ((M - 1) / 64 >= 65535 || (N - 1) / 128 >= 65535) return fail(EMU_ERR_UNSUPPORTED, "M up to 65535 * 64, N up to 65535 * 128");
   const emu::Fp8GemmArgs g{a, lda, b, ldb, scale_a, ld_scale_a, scale_b, ld_scale_b, a_type, b_type,
                            b_block == EMU_BLOCK_ROW, M, N, K, out_dtype, out, ldo};
   return cuda_status(emu::launch_gemm_fp8(g, static_cast<cudaStream_t>(stream)), "emu_gemm_fp8 launch");

@@ -7,7 +7,7 @@
 // it by the two scales and add it to f32 accumulators in registers, so the scales' f32 product and the
 // sum over blocks never pass through fewer than 32 bits.
 //
-// One kernel (this file's first form): the rows of B are the MMA's 128 lanes and BN rows of A its columns
+// Few rows of A (gemm_fp8_skinny_kernel): the rows of B are the MMA's 128 lanes and BN rows of A its columns
 // ("weights by tokens"), so that few rows of A cost few columns; the blocks of K are split over the CTAs
 // of a cluster where the tiles alone would leave SMs idle, their partial sums meeting in distributed
 // shared memory in rank order (the same result every run).
@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -70,18 +71,18 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, float v, int mod
 
 template <int BN> struct Cfg {
   static constexpr int STAGE = (LANES + BN) * BK;
-  static constexpr int NSTAGE = BN <= 32 ? 5 : BN == 64 ? 4 : 3;     // ~100 KB: two CTAs share an SM
+  static constexpr int NSTAGE = BN <= 32 ? 5 : 4;                    // ~100 KB: two CTAs share an SM
   static constexpr int NSCALE = 8;                                    // scale slots: BN + 128 floats each
   static constexpr int SCALE = (BN + LANES) * 4;
-  static constexpr int NACC = BN <= 64 ? 4 : 2;                       // TMEM accumulators
-  static constexpr int TMEM_COLS = NACC * BN < 32 ? 32 : NACC * BN;   // <= 256: two CTAs share an SM's 512
+  static constexpr int NACC = 4;                                      // TMEM accumulators
+  static constexpr int TMEM_COLS = NACC * BN;                         // <= 256: two CTAs share an SM's 512
   static constexpr int BARS = 2 * NSTAGE + 2 * NSCALE + 2 * NACC + 1;
   static constexpr int SMEM = 1024 + NSTAGE * STAGE + NSCALE * SCALE + BARS * 8 + 16;
   static_assert(NSTAGE * STAGE >= BN * LANES * 4, "the ring holds the partial sums afterwards");
 };
 
 template <int BN>
-__global__ void __launch_bounds__(THREADS, BN == 128 ? 0 : 2) gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_b,
                                                                   const __grid_constant__ CUtensorMap map_a,
                                                                   const Params p) {
   using C = Cfg<BN>;
@@ -238,19 +239,31 @@ __global__ void __launch_bounds__(THREADS, BN == 128 ? 0 : 2) gemm_fp8_skinny_ke
   if (warp >= 2 && warp < 6) {
     const int l = (warp & 3) * 32 + lane;
     const int64_t n = n0 + l;
-    const int j0 = BN * rank / split, j1 = BN * (rank + 1) / split;
-    uint32_t base[8];
+    auto add_up = [&](auto parts) {
+      constexpr int S = decltype(parts)::value;
+      constexpr int COLS = BN / S, CH = COLS < 8 ? COLS : 8;       // this CTA's columns, loads of CH of them at once
+      uint32_t base[S];
 #pragma unroll
-    for (uint32_t r = 0; r < 8; ++r) base[r] = ptx::map_shared(ptx::smem_u32(part + l), r < split ? r : rank);
-#pragma unroll 2
-    for (int j = j0; j < j1; ++j) {
-      float v[8], s = 0.0f;
+      for (int r = 0; r < S; ++r) base[r] = ptx::map_shared(ptx::smem_u32(part + (int)rank * COLS * LANES + l), r);
+      for (int j = 0; j < COLS; j += CH) {
+        float v[S][CH];
 #pragma unroll
-      for (uint32_t r = 0; r < 8; ++r) v[r] = r < split ? ptx::ld_shared_cluster(base[r] + j * (LANES * 4)) : 0.0f;
+        for (int r = 0; r < S; ++r)
 #pragma unroll
-      for (uint32_t r = 0; r < 8; ++r) s = r < split ? __fadd_rn(s, v[r]) : s;
-      if (n < p.N && m0 + j < p.M) store_out(p.out, (m0 + j) * p.ldo + n, s, p.out_mode);
-    }
+          for (int c = 0; c < CH; ++c) v[r][c] = ptx::ld_shared_cluster(base[r] + (j + c) * (LANES * 4));
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          float sum = v[0][c];
+#pragma unroll
+          for (int r = 1; r < S; ++r) sum = __fadd_rn(sum, v[r][c]);
+          const int64_t m = m0 + (int)rank * COLS + j + c;
+          if (n < p.N && m < p.M) store_out(p.out, m * p.ldo + n, sum, p.out_mode);
+        }
+      }
+    };
+    if (split == 8) add_up(std::integral_constant<int, 8>{});
+    else if (split == 4) add_up(std::integral_constant<int, 4>{});
+    else add_up(std::integral_constant<int, 2>{});
   }
   ptx::cluster_sync();                                             // no CTA leaves while its sums are read
 }
@@ -537,24 +550,42 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
           }
         }
         __syncwarp();
-        const int u = lane & 7, per = 16 / esz;                      // elements of a 16-byte piece
-        const int64_t col = col0 + c * 32 + u * per;
+        const int64_t colc = col0 + c * 32;
+        if (vec) {
+          // 8 lanes write 128 bytes of a row
+          const int u = lane & 7, per = 16 / esz;                    // elements of a 16-byte piece
+          const int64_t col = colc + u * per;
 #pragma unroll
-        for (int r4 = 0; r4 < 8; ++r4) {
-          const int r = r4 * 4 + (lane >> 3);
-          const int64_t row = row0 + r;
-          if (row >= p.M || col >= p.N) continue;
-          const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
-          uint8_t* dst = static_cast<uint8_t*>(p.out) + (row * p.ldo + col) * esz;
-          if (vec && col + per <= p.N) {
-            *reinterpret_cast<uint4*>(dst) = w;
-          } else {
-            const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+          for (int r4 = 0; r4 < 8; ++r4) {
+            const int r = r4 * 4 + (lane >> 3);
+            if (row0 + r >= p.M || col >= p.N) continue;
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + ((row0 + r) * p.ldo + col) * esz;
+            if (col + per <= p.N) {
+              *reinterpret_cast<uint4*>(dst) = w;
+            } else {
+              const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (e >= per || col + e >= p.N) break;
-              if (esz == 4) reinterpret_cast<uint32_t*>(dst)[e] = q[e & 3];
-              else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(q[e >> 1] >> (16 * (e & 1)));
+              for (int e = 0; e < 8; ++e) {
+                if (e >= per || col + e >= p.N) break;
+                if (esz == 4) reinterpret_cast<uint32_t*>(dst)[e] = q[e & 3];
+                else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(q[e >> 1] >> (16 * (e & 1)));
+              }
+            }
+          }
+        } else {
+          // rows that do not start on 16 bytes: the warp writes a row's 128 bytes, 4 to a lane (or two
+          // 16-bit elements by themselves where rows start on 2 bytes)
+          const int64_t col = colc + lane * (4 / esz);
+          const bool words = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * esz)) & 3) == 0;
+          for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + ((row0 + r) * p.ldo + col) * esz;
+            if (words && col + 4 / esz <= p.N) {
+              *reinterpret_cast<uint32_t*>(dst) = w;
+            } else {
+              if (col < p.N) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
+              if (col + 1 < p.N) reinterpret_cast<uint16_t*>(dst)[1] = (uint16_t)(w >> 16);
             }
           }
         }
@@ -626,7 +657,8 @@ cudaError_t launch_skinny(const Fp8GemmArgs& g, Params p, int sms, cudaStream_t 
   if (e != cudaSuccess) return e;
   p.idesc = ptx::idesc_f8_f32(LANES, BN, g.b_type, g.a_type);
   const int64_t tiles_n = (g.N + LANES - 1) / LANES, tiles_m = (g.M + BN - 1) / BN;
-  // split K while CTAs fit twice into the SMs and each keeps at least two blocks
+  // split K (in powers of two: the kernel adds up 2, 4 or 8 parts) while the CTAs fit twice into the SMs and
+  // each keeps at least two blocks
   int split = 1;
   while (split < 8 && tiles_n * tiles_m * split * 2 <= 2 * sms && p.kb_count >= split * 4) split *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -686,11 +718,20 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
   p.out = g.out, p.ldo = g.ldo, p.out_mode = g.out_dtype;
   p.wait_limit = current_wait_limit();
   p.hold_first_ready = current_hold_first_ready();
-  if (g.M > 128) return g.b_rows ? launch_pair<true>(g, p, sms, stream) : launch_pair<false>(g, p, sms, stream);
+  // Up to 64 rows of A are one column tile of the skinny kernel: each byte of B is read once.  Beyond, the two
+  // kernels' times by what they do, in us (measured over 65 .. 4096 rows, 512 .. 14336 columns and K, within
+  // 15%): the skinny one 6.5 + its tiles' blocks of K / 300 (B200 whole), the pairs 3.5 + for each wave of tiles
+  // 0.53 (0.85 with a scale per row of B) a block + 2.3 to store.  E.g. 128 x 4096 x 4096: 14.1 against 22.3;
+  // 128 x 14336 x 4096: 28.1 against 23.5; 1024 x 4096 x 4096: 53 against 24.
+  const int64_t kb = p.kb_count;
+  const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256), pairs = std::max(1, sms / 2);
+  const double t_pair = 3.5 + (double)((tiles + pairs - 1) / pairs) * ((g.b_rows ? 0.85 : 0.53) * kb + 2.3);
+  const double t_skinny = 6.5 + (double)((g.M + 63) / 64) * (double)((g.N + 127) / 128) * (double)kb / 300.0;
+  if (g.M > 64 && t_pair < t_skinny)
+    return g.b_rows ? launch_pair<true>(g, p, sms, stream) : launch_pair<false>(g, p, sms, stream);
   if (g.M <= 16) return launch_skinny<16>(g, p, sms, stream);
   if (g.M <= 32) return launch_skinny<32>(g, p, sms, stream);
-  if (g.M <= 64) return launch_skinny<64>(g, p, sms, stream);
-  return launch_skinny<128>(g, p, sms, stream);
+  return launch_skinny<64>(g, p, sms, stream);
 }
 
 }  // namespace emu
