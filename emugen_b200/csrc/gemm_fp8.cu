@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
   uint64_t* drained = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   const int64_t tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, tiles = tiles_m * tiles_n;
   const int64_t first = blockIdx.x / 2, stride = gridDim.x / 2;
@@ -401,7 +401,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         const long long t0 = clock64();
         while (clock64() - t0 < 200000) {}
       }
-    } else if ((warp == 1 || warp == 2) && lane == 0 && rank == 0) {
+    } else if ((warp == 1 || warp == 2) && rank == 0) {
+      // The whole warp walks the blocks and one elected lane issues: descriptors then stay in uniform
+      // registers, from which the MMAs take them.
       const uint32_t tmem = *tmem_slot + (warp - 1) * 256;
       uint64_t* acc_free = &acc_empty[warp - 1];
       bool ok = true, first_block = true;
@@ -411,24 +413,29 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       for (int64_t t = first; t < tiles && ok; t += stride) {
         for (int kb = 0; kb < p.kb_count; ++kb, st.next(), turn ^= 3) {
           if (turn != warp) continue;                                // the other warp's block
-          // The accumulator first: it is free once the epilogue has read block i - 2, so every block up to
-          // there has landed, among them the stage's last one, i - 5.  Only then can the parity of the
-          // stage's barrier not be taken for that of two rounds before (its rounds alternate between
-          // the issuers, so this thread has not waited for the one between).
-          if (!wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
-          if (!wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
+          // The stage first: it filled long ago as a rule, the accumulator comes free last.  The parity of
+          // the stage's barrier cannot be that of two rounds before, although the round between was the
+          // other issuer's: this one has waited for the accumulator of block i - 2, that is for block i - 4
+          // to be read, so the stage's last block, i - 5, has landed.
+          static_assert(P_NSTAGE >= 4, "see above");
+          if (!warp_wait_or_record(&full[st.at], st.parity, p.wait_limit, 14)) { ok = false; break; }
+          if (!warp_wait_or_record(acc_free, parity, p.wait_limit, 13)) { ok = false; break; }
           parity ^= 1;
           ptx::tc_fence_after();
           const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE));
           const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(smem + st.at * P_STAGE + 128 * BK));
+          if (ptx::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem, da + 2 * k, db + 2 * k, p.idesc, k > 0);
-          if (!(first_block && warp == 1 && p.hold_first_ready)) ptx::mma2_commit_both(&done[st.at]);
+            for (int k = 0; k < BK / 32; ++k) ptx::mma2_f8(tmem, da + 2 * k, db + 2 * k, p.idesc, k > 0);
+            if (!(first_block && warp == 1 && p.hold_first_ready)) ptx::mma2_commit_both(&done[st.at]);
+          }
+          __syncwarp();
           first_block = false;
         }
       }
-      ptx::mma2_commit_both(drained);
-      wait_or_record(drained, 0, DRAIN_LIMIT, 15);
+      if (ptx::elect_one()) ptx::mma2_commit_both(drained);
+      __syncwarp();
+      warp_wait_or_record(drained, 0, DRAIN_LIMIT, 15);
     }
   } else {
     ptx::setmaxnreg_inc<P_REG_HIGH>();
