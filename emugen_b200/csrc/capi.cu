@@ -551,6 +551,7 @@ emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, const uin
 static emu_status check_kv(int32_t format, int64_t H, int64_t D) {
   if (format != EMU_KV_FP8 && format != EMU_KV_MXFP4) return fail(EMU_ERR_INVALID_ARGUMENT, "unknown cache format %d", format);
   if (H < 1 || H > 65536 || D < 1 || D > 65536) return fail(EMU_ERR_UNSUPPORTED, "heads and head size must be in [1, 65536]");
+  if (H * D > (1ll << 28)) return fail(EMU_ERR_UNSUPPORTED, "heads * head_size up to 2^28");
   const int64_t unit = format == EMU_KV_FP8 ? 16 : 32;
   if (D % unit != 0) return fail(EMU_ERR_K_GROUP, "head size must be a multiple of %lld", (long long)unit);
   return EMU_OK;

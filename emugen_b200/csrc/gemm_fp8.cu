@@ -444,6 +444,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
     uint8_t* buf = store + ew * (32 * 128);
     const int64_t blocks_n = (p.N + 127) / 128;
     const uint32_t empty_bar = ptx::map_shared(ptx::smem_u32(acc_empty), 0);
+    // columns of one TMEM load (with column scales 16 were faster than 32: 122 against 128 us at 4096^3)
+    constexpr int LD = B_ROWS ? 16 : 32, CHUNKS = 128 / LD;
     bool ok = true;
     Ring<P_NSTAGE> st;
     Ring<P_NSCALE> sc;
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       float sa1 = __ldg(sa_row), sa2 = p.kb_count > 1 ? __ldg(sa_row + p.ldsa) : 0.0f;
       float sa3 = p.kb_count > 2 ? __ldg(sa_row + 2 * p.ldsa) : 0.0f, sb3 = B_ROWS || p.kb_count < 3 ? 1.0f : __ldg(sb_tile + 2);
       float sb1 = B_ROWS ? 1.0f : __ldg(sb_tile), sb2 = B_ROWS || p.kb_count < 2 ? 1.0f : __ldg(sb_tile + 1);
-      uint32_t v[2][32];
+      uint32_t v[2][LD];
       if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
       ptx::tc_fence_after();
       ptx::tmem_ld_regs(lane_base + ac, v[0]);
@@ -478,11 +480,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         st.next();
         bool next = false;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < CHUNKS; ++c) {
+          const ulonglong2* sb4 = reinterpret_cast<const ulonglong2*>(slot + half * 128 + c * LD);
           ptx::tmem_wait_regs(v[c & 1]);
-          // the next 32 columns travel while these are added up
-          if (c < 3) {
-            ptx::tmem_ld_regs(lane_base + ac + (c + 1) * 32, v[(c + 1) & 1]);
+          // the next columns travel while these are added up
+          if (c + 1 < CHUNKS) {
+            ptx::tmem_ld_regs(lane_base + ac + (c + 1) * LD, v[(c + 1) & 1]);
           } else {
             ptx::tc_fence_before();                                  // all of this block is in registers
             __syncwarp();
@@ -496,19 +499,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
               }
             }
           }
-          const float4* sb4 = reinterpret_cast<const float4*>(slot + half * 128 + c * 32);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
+          for (int j = 0; j < LD; j += 4) {
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[c & 1][j + e]);
             if (B_ROWS) {
-              const float4 s4 = sb4[j / 4];
-              x[0] = __fmul_rn(x[0], s4.x), x[1] = __fmul_rn(x[1], s4.y);
-              x[2] = __fmul_rn(x[2], s4.z), x[3] = __fmul_rn(x[3], s4.w);
+              // two products per instruction: here the pairs lie as they were loaded
+              const ulonglong2 s = sb4[j / 4];
+              const uint64_t lo = ptx::mul2(ptx::join2(v[c & 1][j], v[c & 1][j + 1]), s.x);
+              const uint64_t hi = ptx::mul2(ptx::join2(v[c & 1][j + 2], v[c & 1][j + 3]), s.y);
+              x[0] = ptx::lo2(lo), x[1] = ptx::hi2(lo), x[2] = ptx::lo2(hi), x[3] = ptx::hi2(hi);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c * 32 + j + e] = __fmaf_rn(x[e], f, acc[c * 32 + j + e]);
+            for (int e = 0; e < 4; ++e) acc[c * LD + j + e] = __fmaf_rn(x[e], f, acc[c * LD + j + e]);
           }
         }
         if (B_ROWS) {
@@ -728,11 +732,11 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
   // Up to 64 rows of A are one column tile of the skinny kernel: each byte of B is read once.  Beyond, the two
   // kernels' times by what they do, in us (measured over 65 .. 4096 rows, 512 .. 14336 columns and K, within
   // 15%): the skinny one 6.5 + its tiles' blocks of K / 300 (B200 whole), the pairs 3.5 + for each wave of tiles
-  // 0.53 (0.85 with a scale per row of B) a block + 2.3 to store.  E.g. 128 x 4096 x 4096: 14.1 against 22.3;
+  // 0.53 (0.8 with a scale per row of B) a block + 2.3 to store.  E.g. 128 x 4096 x 4096: 14.1 against 22.3;
   // 128 x 14336 x 4096: 28.1 against 23.5; 1024 x 4096 x 4096: 53 against 24.
   const int64_t kb = p.kb_count;
   const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256), pairs = std::max(1, sms / 2);
-  const double t_pair = 3.5 + (double)((tiles + pairs - 1) / pairs) * ((g.b_rows ? 0.85 : 0.53) * kb + 2.3);
+  const double t_pair = 3.5 + (double)((tiles + pairs - 1) / pairs) * ((g.b_rows ? 0.8 : 0.53) * kb + 2.3);
   const double t_skinny = 6.5 + (double)((g.M + 63) / 64) * (double)((g.N + 127) / 128) * (double)kb / 300.0;
   if (g.M > 64 && t_pair < t_skinny)
     return g.b_rows ? launch_pair<true>(g, p, sms, stream) : launch_pair<false>(g, p, sms, stream);

@@ -66,7 +66,7 @@ def _write(**kw):
 
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(T=-1), 1, "negative size"), (dict(n=-1), 1, "negative size"), (dict(dtype=2), 1, "dtype must be"),
-    (dict(fmt=2), 1, "cache format"), (dict(H=0), 8, "heads"), (dict(D=72), 3, "multiple of 16"),
+    (dict(fmt=2), 1, "cache format"), (dict(H=0), 8, "heads"), (dict(H=65536, D=65536), 8, "2^28"), (dict(D=72), 3, "multiple of 16"),
     (dict(fmt=1, D=48), 3, "multiple of 32"), (dict(k=None), 1, "NULL"), (dict(vc=None), 1, "NULL"), (dict(ks=None), 1, "NULL"),
     (dict(slots=P + 4), 1, "aligned"), (dict(k=P + 1), 1, "aligned"), (dict(kc=P + 8), 1, "16-byte"),
     (dict(ks=P + 2), 1, "4-byte"),
