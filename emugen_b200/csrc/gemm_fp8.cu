@@ -530,77 +530,73 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       // output: 128 bytes of each of the warp's 32 rows at a time, turned in shared memory so that a
       // row's bytes leave together; 16-byte pieces are spread over the banks by the row's low bits
       const int64_t row0 = tm * 256 + rank * 128 + quarter * 32, col0 = tn * 256 + half * 128;
-      const int esz = p.out_mode == EMU_DTYPE_F32 ? 4 : 2;
-      const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * esz)) & 15) == 0;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
+      auto write = [&](auto* out) {
+        using O = std::remove_pointer_t<decltype(out)>;
+        constexpr int PER = 16 / sizeof(O), COLS = 8 * PER;          // elements of a piece, of 128 bytes
+        out += row0 * p.ldo + col0;
+        const int cols = (int)min((int64_t)128, p.N - col0);
+        const uintptr_t mis = reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * sizeof(O));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (esz == 2 && (c & 1)) continue;                           // 64 16-bit columns at a time, or 32 of f32
-        __syncwarp();
-        if (esz == 4) {
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const float* x = acc + c * 32 + 4 * u;
-            *reinterpret_cast<float4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
-          }
-        } else if (c < 3) {
+        for (int c = 0; c < 128; c += COLS) {
+          __syncwarp();
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float lo = acc[(c * 32 + 8 * u + 2 * e) & 127], hi = acc[(c * 32 + 8 * u + 2 * e + 1) & 127];
-              if (p.out_mode == EMU_DTYPE_BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+              if constexpr (sizeof(O) == 4) {
+                w[e] = __float_as_uint(acc[c + 4 * u + e]);
+              } else if constexpr (std::is_same<O, __half>::value) {
+                const __half2 h = __floats2half2_rn(acc[c + 8 * u + 2 * e], acc[c + 8 * u + 2 * e + 1]);
                 w[e] = reinterpret_cast<const uint32_t&>(h);
               } else {
-                const __half2 h = __floats2half2_rn(lo, hi);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[c + 8 * u + 2 * e], acc[c + 8 * u + 2 * e + 1]);
                 w[e] = reinterpret_cast<const uint32_t&>(h);
               }
             }
             *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        }
-        __syncwarp();
-        const int64_t colc = col0 + c * 32;
-        if (vec) {
-          // 8 lanes write 128 bytes of a row
-          const int u = lane & 7, per = 16 / esz;                    // elements of a 16-byte piece
-          const int64_t col = colc + u * per;
+          __syncwarp();
+          if ((mis & 15) == 0) {
+            // 8 lanes write 128 bytes of a row
+            const int u = lane & 7, col = c + u * PER;
+            O* dst = out + (lane >> 3) * p.ldo + col;
 #pragma unroll
-          for (int r4 = 0; r4 < 8; ++r4) {
-            const int r = r4 * 4 + (lane >> 3);
-            if (row0 + r >= p.M || col >= p.N) continue;
-            const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
-            uint8_t* dst = static_cast<uint8_t*>(p.out) + ((row0 + r) * p.ldo + col) * esz;
-            if (col + per <= p.N) {
-              *reinterpret_cast<uint4*>(dst) = w;
-            } else {
-              const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+            for (int r4 = 0; r4 < 8; ++r4, dst += 4 * p.ldo) {
+              const int r = r4 * 4 + (lane >> 3);
+              if (r >= rows || col >= cols) continue;
+              const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
+              if (col + PER <= cols) {
+                *reinterpret_cast<uint4*>(dst) = w;
+              } else {
+                const O* x = reinterpret_cast<const O*>(buf + r * 128 + ((u ^ (r & 7)) * 16));
+                for (int e = 0; col + e < cols; ++e) dst[e] = x[e];
+              }
+            }
+          } else {
+            // rows that do not start on 16 bytes: the warp writes a row's 128 bytes, 4 to a lane (or two
+            // 16-bit elements by themselves where rows start on 2 bytes)
+            constexpr int EL = 4 / sizeof(O);
+            const int col = c + lane * EL;
+            O* dst = out + col;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r, dst += p.ldo) {
+              const uint8_t* x = buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4;
+              if ((mis & 3) == 0 && col + EL <= cols) {
+                *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(x);
+              } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                if (e >= per || col + e >= p.N) break;
-                if (esz == 4) reinterpret_cast<uint32_t*>(dst)[e] = q[e & 3];
-                else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(q[e >> 1] >> (16 * (e & 1)));
+                for (int e = 0; e < EL; ++e)
+                  if (col + e < cols) dst[e] = reinterpret_cast<const O*>(x)[e];
               }
             }
           }
-        } else {
-          // rows that do not start on 16 bytes: the warp writes a row's 128 bytes, 4 to a lane (or two
-          // 16-bit elements by themselves where rows start on 2 bytes)
-          const int64_t col = colc + lane * (4 / esz);
-          const bool words = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ldo * esz)) & 3) == 0;
-          for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
-            uint8_t* dst = static_cast<uint8_t*>(p.out) + ((row0 + r) * p.ldo + col) * esz;
-            if (words && col + 4 / esz <= p.N) {
-              *reinterpret_cast<uint32_t*>(dst) = w;
-            } else {
-              if (col < p.N) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
-              if (col + 1 < p.N) reinterpret_cast<uint16_t*>(dst)[1] = (uint16_t)(w >> 16);
-            }
-          }
         }
-      }
+      };
+      if (p.out_mode == EMU_DTYPE_BF16) write(static_cast<__nv_bfloat16*>(p.out));
+      else if (p.out_mode == EMU_DTYPE_F16) write(static_cast<__half*>(p.out));
+      else write(static_cast<float*>(p.out));
     }
   }
 
