@@ -505,6 +505,9 @@ emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_t K, int
   if ((q && ldq < K) || (qt && ldqt < M)) return fail(EMU_ERR_INVALID_ARGUMENT, "code rows must hold K (transposed: M) bytes");
   if ((q && (ldq % 16 != 0 || !aligned(q, 16))) || (qt && (ldqt % 16 != 0 || !aligned(qt, 16))))
     return fail(EMU_ERR_INVALID_ARGUMENT, "code rows must start on 16-byte boundaries");
+  const uintptr_t esz = dtype == EMU_DTYPE_F32 ? 4 : 2;
+  if (!aligned(x, esz) || !aligned(scale, 4) || !aligned(scale_t, 4))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "x and the scales must be aligned to their elements");
   if ((q && ld_scale < (block == EMU_BLOCK_ROW ? M : kb)) || (qt && ld_scale_t < (block == EMU_BLOCK_ROW ? K : mb)))
     return fail(EMU_ERR_INVALID_ARGUMENT, "scale rows too short");
   if (mb > 0x7FFFFFFF / kb)

@@ -212,19 +212,24 @@ def _gemm(a, b, scale_a, scale_b, rows: bool, out_dtype: torch.dtype, dev: torch
     return out
 
 
+def _linear(x: torch.Tensor, weight: torch.Tensor, need_x: bool, need_w: bool):
+    """(y, x's codes and scales as `quant_fp8` gives them, weight's): with the transposes that the wanted
+    gradients need -- x.T for the weight's, weight.T for x's."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    q = _quant(x2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
+    w = _quant(weight, _lib.EMU_BLOCK_TILE, torch.float8_e4m3fn, need_x)
+    y = _gemm(q[0], w[0], q[1], w[1], False, x.dtype, x.device)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0]), q, w
+
+
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
         need_x, need_w = ctx.needs_input_grad
-        dev, dtype = x.device, x.dtype
-        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        # the transposed codes serve the backward pass: x.T for the weight's gradient, weight.T for x's
-        q = _quant(x2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
-        w = _quant(weight, _lib.EMU_BLOCK_TILE, torch.float8_e4m3fn, need_x)
-        y = _gemm(q[0], w[0], q[1], w[1], False, dtype, dev)
+        y, q, w = _linear(x, weight, need_x, need_w)
         ctx.save_for_backward(*(q[2:] if need_w else (None, None)), *(w[2:] if need_x else (None, None)))
         ctx.x_shape = x.shape
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -252,9 +257,9 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     (the gradients treat Q as the identity).  The forward pass keeps the 8-bit transposes of x and the weight
     for the backward pass, not x itself.  fp16, bf16 or f32 CUDA tensors of one device and dtype.
 
-    A backward pass that a CUDA graph is to capture must be the leaves' only live graph: run the warm-up on
-    the capturing stream's side and drop its outputs first (torch.cuda.make_graphed_callables does), as for
-    every torch operator."""
+    A backward pass that a CUDA graph is to capture follows torch's rule for every operator: no eager graph of
+    the same leaves may be alive (their gradient accumulators belong to its stream, and torch ends the process over
+    it) -- warm up on a side stream and drop the outputs first, as torch.cuda.make_graphed_callables does."""
     if x.dim() < 1 or weight.dim() != 2:
         raise RuntimeError("x must have at least one dimension and weight two")
     if x.shape[-1] != weight.shape[1]:
@@ -263,6 +268,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         raise RuntimeError(f"x and weight must share one of float16, bfloat16, float32, got {x.dtype} and {weight.dtype}")
     if not x.is_cuda or x.device != weight.device:
         raise RuntimeError("x and weight must be on the same CUDA device")
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        return _linear(x.detach(), weight.detach(), False, False)[0]
     return _LinearFp8.apply(x, weight)
 
 

@@ -18,7 +18,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, fp8, kvcache
 
 _OUT_DTYPE = {_lib.EMU_OUT_F16: torch.float16, _lib.EMU_OUT_BF16_VIA_F16: torch.bfloat16,
               _lib.EMU_OUT_F32: torch.float32}
@@ -86,4 +86,60 @@ def _mxfp_fake(a_fp4, b_fp4, scale_a, scale_b, group_size=32, m_chunk_size=128, 
     return a_fp4.new_empty((a_fp4.shape[0], b_fp4.shape[0]), dtype=torch.float16)
 
 
-__all__ = ["gemm", "emulated_scaled_fp4_mm", "emulated_mxfp4_mm"]
+@torch.library.custom_op("emugen::quant_fp8", mutates_args=())
+def quant_fp8(x: torch.Tensor, block: str = "row", dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
+    """Block-scaled 8-bit quantiser: (codes [M, K], scales), laid out as fp8.quant_fp8 does."""
+    return fp8.quant_fp8(x, block=block, dtype=dtype)
+
+
+@quant_fp8.register_fake
+def _quant_fp8_fake(x, block="row", dtype=torch.float8_e4m3fn):
+    M, K = x.numel() // x.shape[-1] if x.shape[-1] else x.shape[:-1].numel(), x.shape[-1]
+    kb = fp8._blocks(K)
+    s = (fp8._row_scales(M, kb, x.device) if block == "row"
+         else torch.empty((fp8._blocks(M), kb), dtype=torch.float32, device=x.device))
+    return fp8._codes(M, K, dtype, x.device), s
+
+
+@torch.library.custom_op("emugen::gemm_fp8", mutates_args=())
+def gemm_fp8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Block-scaled 8-bit product a [M, K] @ b [N, K].T -> [M, N]."""
+    return fp8.gemm_fp8(a, b, scale_a, scale_b, out_dtype=out_dtype)
+
+
+@gemm_fp8.register_fake
+def _gemm_fp8_fake(a, b, scale_a, scale_b, out_dtype=torch.bfloat16):
+    torch._check(a.dim() == 2 and b.dim() == 2, lambda: "a, b, scale_a and scale_b must be 2D")
+    torch._check(a.shape[1] == b.shape[1], lambda: "K mismatch between a and b")
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("emugen::write_kv_cache", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def write_kv_cache(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Quantise k and v [tokens, heads, head_size] into their slots of the cache."""
+    kvcache.write_kv_cache(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+
+
+@write_kv_cache.register_fake
+def _write_kv_cache_fake(k, v, slots, k_cache, v_cache, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op("emugen::read_kv_cache", mutates_args=())
+def read_kv_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_table: torch.Tensor, cu_lens: torch.Tensor, total: int,
+                  dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows of a batch of sequences, packed: (k, v) [total, heads, head_size]."""
+    return kvcache.read_kv_cache(k_cache, v_cache, k_scale, v_scale, block_table, cu_lens, total=total, dtype=dtype)
+
+
+@read_kv_cache.register_fake
+def _read_kv_cache_fake(k_cache, v_cache, k_scale, v_scale, block_table, cu_lens, total, dtype=torch.bfloat16):
+    D = k_cache.shape[3] if k_cache.dtype == torch.float8_e4m3fn else 2 * k_cache.shape[3]
+    shape = (total, k_cache.shape[2], D)
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+__all__ = ["gemm", "emulated_scaled_fp4_mm", "emulated_mxfp4_mm", "quant_fp8", "gemm_fp8", "write_kv_cache", "read_kv_cache"]

@@ -1,6 +1,7 @@
 /*
  * emugen.h — C ABI of libemugen.so, the B200 (sm_100a) implementation of EmuGen's emulated
- * NVFP4 / MXFP4 scaled GEMM and of the FP4 quantisation that feeds it.
+ * NVFP4 / MXFP4 scaled GEMM and of the FP4 quantisation that feeds it, with block-scaled 8-bit
+ * operators beside them (quantiser, matrix product, quantised key/value cache).
  *
  * Conventions (every entry point):
  *   - All tensor arguments are DEVICE pointers owned by the caller; nothing is allocated or freed
@@ -404,6 +405,7 @@ EMU_API emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_
  * scale makes NaN exactly those outputs that it enters.  out [M][N], rows ldo elements apart.  K = 0 gives zeros.
  * a, b 16-byte aligned, lda and ldb multiples of 16 (bytes past K are not used).  Scale rows of the row layout start
  * on 16 bytes, ld_scale is a multiple of 4, and they can be read up to M (N) rounded up to a multiple of 4.
+ * M up to 65535 * 64, N up to 65535 * 128.
  * A device pipeline wait that runs out is reported by emu_device_status.  No reference counterpart.
  */
 EMU_API emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, const uint8_t* b, int64_t ldb,
@@ -422,7 +424,7 @@ enum { EMU_KV_FP8 = 0,     /* E4M3 codes, an f32 scale per 128 elements of a (to
  *   scales [num_slots][heads][ceil(head_size / 128)] f32   (MXFP4: [..][head_size / 32] bytes)
  * (pages of P slots: slot = page * P + place).  A slot that is negative or not below num_slots writes nothing; where
  * several tokens have the same slot, the last one's row is kept.  v may be NULL (a cache of one tensor).  head_size is a
- * multiple of 16 (MXFP4: 32).  FP8: NaN and infinities become NaN.  MXFP4 (which has neither): for finite rows
+ * multiple of 16 (MXFP4: 32), heads * head_size at most 2^28.  FP8: NaN and infinities become NaN.  MXFP4 (which has neither): for finite rows
  * emu_quant_mxfp4's bytes; NaN is passed over by the scale.  Caches 16-byte aligned.  No reference counterpart.
  */
 EMU_API emu_status emu_kv_write(const void* k, const void* v, int32_t dtype, int64_t tokens, int64_t heads,

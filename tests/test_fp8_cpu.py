@@ -25,7 +25,7 @@ def _quant(**kw):
     (dict(block=2), 1, "unknown block"), (dict(x=None), 1, "NULL"), (dict(q=None, qt=None), 1, "NULL"),
     (dict(s=None), 1, "NULL"), (dict(st=None), 1, "NULL"), (dict(ldx=199), 1, "ldx"), (dict(ldq=192), 1, "code rows"),
     (dict(ldq=201), 1, "16-byte"), (dict(q=P + 8), 1, "16-byte"), (dict(qt=P + 1), 1, "16-byte"), (dict(ldqt=2), 1, "code rows"),
-    (dict(lds=3), 1, "scale rows"), (dict(ldst=199), 1, "scale rows"), (dict(block=1, lds=1), 1, "scale rows"),
+    (dict(x=P + 1), 1, "aligned"), (dict(s=P + 2), 1, "aligned"), (dict(lds=3), 1, "scale rows"), (dict(ldst=199), 1, "scale rows"), (dict(block=1, lds=1), 1, "scale rows"),
     (dict(M=1 << 40, ldqt=1 << 40, lds=1 << 40), 8, "2^31"),
 ])
 def test_quant_refusals(kw, status, msg):
@@ -167,3 +167,22 @@ def test_signatures_match_the_header():
     for name, n in (("emu_quant_fp8", 16), ("emu_gemm_fp8", 18), ("emu_kv_write", 18), ("emu_kv_read", 21)):
         assert len(getattr(L, name).argtypes) == n
         assert getattr(L, name).restype is ctypes.c_int32
+
+
+def test_ops_fakes_give_the_layouts():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import emugen_b200.ops  # noqa: F401
+
+    with FakeTensorMode():
+        x = torch.empty(7, 200, dtype=torch.bfloat16)
+        q, s = torch.ops.emugen.quant_fp8(x)
+        assert q.shape == (7, 200) and q.stride() == (208, 1) and s.shape == (7, 2) and s.stride() == (1, 8)
+        w, ws = torch.ops.emugen.quant_fp8(torch.empty(300, 200, dtype=torch.bfloat16), "tile")
+        assert ws.shape == (3, 2)
+        out = torch.ops.emugen.gemm_fp8(q, w, s, ws, torch.float32)
+        assert out.shape == (7, 300) and out.dtype == torch.float32
+        c = torch.empty(4, 16, 2, 32, dtype=torch.uint8)
+        k, v = torch.ops.emugen.read_kv_cache(c, c, c[..., :2], c[..., :2], torch.empty(1, 2, dtype=torch.int32),
+                                              torch.empty(2, dtype=torch.int32), 9)
+        assert k.shape == v.shape == (9, 2, 64)

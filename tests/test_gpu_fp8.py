@@ -132,7 +132,9 @@ def _operands(M, N, K, at, bt, rows, seed, exact):
 # one row to many, short and ragged K, one block to many, N below, at and past the tiles
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 300, 4096), (2, 17, 33), (7, 1000, 130), (16, 128, 1024), (17, 129, 257), (33, 256, 2000),
           (64, 64, 64), (65, 130, 384), (100, 1500, 1111), (128, 128, 128), (129, 257, 129), (200, 96, 5000), (255, 511, 640),
-          (300, 1000, 520), (513, 640, 256), (1024, 1024, 1024), (1300, 2304, 392)]
+          (300, 1000, 520), (513, 640, 256), (1024, 1024, 1024), (1300, 2304, 392),
+          # large enough for the CTA pairs: ragged in every direction, one block of K, several tiles a pair
+          (1111, 1501, 2000), (2049, 2300, 130), (4100, 4000, 260), (257, 20000, 512), (3000, 2900, 100)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -166,7 +168,7 @@ def test_gemm_same_result_every_run():
         assert torch.equal(first, fp8.gemm_fp8(a, b, sa, sb, out_dtype=torch.float32))
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 200, 300), (150, 300, 600), (700, 800, 640)])
+@pytest.mark.parametrize("M,N,K", [(5, 200, 300), (150, 300, 600), (700, 800, 640), (2000, 2100, 300)])
 @pytest.mark.parametrize("rows", [False, True])
 def test_gemm_nan_stays_in_its_row_and_column(M, N, K, rows):
     a, b, sa, sb = _operands(M, N, K, E4, E4, rows, 11, True)
@@ -222,7 +224,7 @@ def test_gemm_other_layouts_are_copied():
 
 def test_gemm_output_rows_apart():
     """The C entry with ldo > N: what lies between the rows and behind the last stays."""
-    for M, N, K in ((3, 130, 256), (200, 300, 256)):
+    for M, N, K in ((3, 130, 256), (200, 300, 256), (2000, 2101, 256), (2000, 2104, 256)):
         a, b, sa, sb = [t.cuda() for t in _operands(M, N, K, E4, E4, False, 2, True)]
         sa4 = torch.zeros(2, (M + 3) // 4 * 4, device="cuda")
         sa4[:, :M] = sa.t()
@@ -248,7 +250,7 @@ def test_gemm_empty():
 
 def test_streams_and_graph():
     """On a side stream, two streams at once, and captured and replayed on new inputs."""
-    sets = [[t.cuda() for t in _operands(m, 900, 3000, E4, E4, False, m, True)] for m in (3, 40, 300)]
+    sets = [[t.cuda() for t in _operands(m, n, 3000, E4, E4, False, m, True)] for m, n in ((3, 900), (40, 900), (300, 900), (2000, 2500))]
     want = [fp8.gemm_fp8(*s, out_dtype=torch.float32) for s in sets]
     streams = [torch.cuda.Stream() for _ in sets]
     torch.cuda.synchronize()
@@ -349,6 +351,11 @@ def test_linear_partial_gradients_and_expanded_gradient():
     assert not fp8.linear_fp8(x, w).requires_grad
     with torch.no_grad():
         assert torch.equal(fp8.linear_fp8(x, w), full)
+    one = fp8.linear_fp8(x[3], w)                       # a vector
+    assert one.shape == (48,) and torch.equal(one, fp8.linear_fp8(x[3:4], w)[0])
+    p, q = x.clone().requires_grad_(), w.clone().requires_grad_()
+    with torch.no_grad():                               # nothing is kept where nothing is to be differentiated
+        assert fp8.linear_fp8(p, q).grad_fn is None
     e = torch.zeros(0, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     v = w.clone().requires_grad_()
     fp8.linear_fp8(e, v).sum().backward()
@@ -378,11 +385,11 @@ def test_linear_training_step_captured():
     assert torch.equal(y, y2) and torch.equal(dx, dx2) and torch.equal(dw, dw2)
 
 
-@pytest.mark.parametrize("M", [8, 300])
-def test_wait_limit_is_reported(M):
+@pytest.mark.parametrize("M,N", [(8, 256), (300, 256), (2048, 2048)])   # skinny (split over K), skinny, CTA pairs
+def test_wait_limit_is_reported(M, N):
     """A withheld ready signal: the bounded wait runs out, the kernel returns, the status tells, and the
     next product is right."""
-    a, b, sa, sb = _operands(M, 256, 512, E4, E4, False, 6, True)
+    a, b, sa, sb = _operands(M, N, 512, E4, E4, False, 6, True)
     dev = [t.cuda() for t in (a, b, sa, sb)]
     _lib.device_status()
     old = _lib.set_wait_limit(1_000_000)
@@ -414,3 +421,19 @@ def test_gemm_many_blocks_and_ctas_exact(M, N, K, rows):
     for _ in range(4):
         out = fp8.gemm_fp8(a, b, sa, sb, out_dtype=torch.float32)
         assert torch.equal(out.double(), ref)
+
+
+def test_registered_operators():
+    import emugen_b200.ops  # noqa: F401
+
+    x = _x(33, 200, torch.bfloat16, special=False).cuda()
+    w = _x(70, 200, torch.bfloat16, seed=1, special=False).cuda()
+
+    def f(x, w):
+        q, s = torch.ops.emugen.quant_fp8(x)
+        v, t = torch.ops.emugen.quant_fp8(w, "tile")
+        return torch.ops.emugen.gemm_fp8(q, v, s, t) * 2
+
+    want = fp8.linear_fp8(x, w) * 2
+    assert torch.equal(f(x, w), want)
+    assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x, w), want)

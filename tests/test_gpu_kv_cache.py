@@ -245,3 +245,19 @@ def test_refusals():
                          ((table, cu), dict(out=(k, k), total=2), "total must"), ((table, cu), dict(out=(k.transpose(1, 2).contiguous().transpose(1, 2),) * 2), "contiguous")]:
         with pytest.raises(RuntimeError, match=msg):
             kvcache.read_kv_cache(*cache, *bad, **kw)
+
+
+def test_registered_operators():
+    import emugen_b200.ops  # noqa: F401
+
+    k, v = _kv(20, 2, 64, torch.bfloat16, 1).cuda(), _kv(20, 2, 64, torch.bfloat16, 2).cuda()
+    a, b = kvcache.make_kv_cache(3, 8, 2, 64, "mxfp4"), kvcache.make_kv_cache(3, 8, 2, 64, "mxfp4")
+    slots = torch.arange(20, device="cuda")
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    torch.ops.emugen.write_kv_cache(k, v, slots, *a)
+    kvcache.write_kv_cache(k, v, slots, *b)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    for x, y in zip(torch.ops.emugen.read_kv_cache(*a, table, cu, 20), kvcache.read_kv_cache(*b, table, cu, total=20)):
+        assert torch.equal(x, y)
