@@ -16,6 +16,8 @@
 //               of the block's scales into a second ring
 //   warps 1, 6  MMA issuers in turn (warp 1 owns the TMEM)
 //   warps 2-5   epilogue: a thread owns one row of B (a TMEM lane) and BN accumulators
+// Bound: reading B.  B200: 1 x 128256 x 4096 83 us (96% of the measured copy rate), 32 x 14336 x 4096 16.6 us (floor 9.2;
+// about 5 us are the launch, the pipeline's fill and the parts' exchange: 1 x 512 x 4096 takes 5.4).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -282,6 +284,11 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __gri
 //               its register pairs cost a move each, 484 against 268 us for the epilogue alone at 8192^3.)
 //               B_ROWS = false: 128 columns share one scale of B, so the factor is one number per thread;
 //               B_ROWS = true: the block sum is multiplied by the column's scale first.
+// Bound: the epilogue's turn-around.  A block's MMAs take 512 clocks; its sums reach the epilogue about 450 clocks
+// after that, take 270 to load (TMEM's rate) and 400 to add up, so with two accumulators a block comes every
+// 850 clocks or so.  B200: 4096^3 72 us (1.91 PFLOP/s; 118 with column scales), 8192^3 490 us (2.24 PFLOP/s, the clock
+// already lowered by the power limit: MMAs and loads alone take 366).  Other splits were no faster: 128-column
+// MMAs with four accumulators 72, sixteen epilogue warps of 64 columns 95, one issuer 89 us at 4096^3.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
 constexpr int P_NSTAGE = 5;                      // at least 2: see the issuers' waits
 constexpr int P_NSCALE = 8;

