@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __gri
 // already lowered by the power limit: MMAs and loads alone take 366).  Other splits were no faster: 128-column
 // MMAs with four accumulators 72, sixteen epilogue warps of 64 columns 95, one issuer 89 us at 4096^3.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
-constexpr int P_NSTAGE = 5;                      // at least 2: see the issuers' waits
+constexpr int P_NSTAGE = 5;                      // at least 4: see the issuers' waits
 constexpr int P_NSCALE = 8;
 constexpr int P_SCALE = 256 * 4;                 // column scales (B_ROWS)
 constexpr int P_STORE = 8 * 32 * 128;            // per epilogue warp: 32 rows x 128 bytes of output

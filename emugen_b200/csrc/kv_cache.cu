@@ -25,7 +25,11 @@ namespace {
 constexpr int MAX_TOKENS = 1024;      // tokens per CTA of the write kernel
 constexpr int BUCKETS = 4096;
 
-// A CTA's slots, hashed: chains of its tokens by the slot's low bits.
+// A slot's bucket: the top bits of its product with 2^64 / golden ratio (Knuth), which spreads consecutive
+// slots and those a power of two apart alike.
+__device__ __forceinline__ int bucket_of(int64_t slot) { return (int)(((uint64_t)slot * 0x9E3779B97F4A7C15ull) >> 52); }
+
+// A CTA's slots, hashed: chains of its tokens by bucket.
 struct Slots {
   int64_t own[MAX_TOKENS];
   int16_t next[MAX_TOKENS];
@@ -43,11 +47,11 @@ __device__ __forceinline__ void find_overwritten(const int64_t* __restrict__ slo
   for (int i = threadIdx.x; i < n; i += blockDim.x) s.own[i] = slots[i0 + i], s.dead[i] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (s.own[i] >= 0) s.next[i] = (int16_t)(atomicExch(&s.head[s.own[i] & (BUCKETS - 1)], i + 1) - 1);
+    if (s.own[i] >= 0) s.next[i] = (int16_t)(atomicExch(&s.head[bucket_of(s.own[i])], i + 1) - 1);
   __syncthreads();
   auto look_up = [&](int64_t slot, int64_t j) {
     if (slot < 0) return;                                    // padding: writes nothing
-    for (int i = s.head[slot & (BUCKETS - 1)] - 1; i >= 0; i = s.next[i])
+    for (int i = s.head[bucket_of(slot)] - 1; i >= 0; i = s.next[i])
       if (s.own[i] == slot && i0 + i < j) s.dead[i] = 1;
   };
   int64_t j = i0 + 1 + threadIdx.x;
@@ -90,18 +94,20 @@ __global__ void __launch_bounds__(NT) kv_write_kernel(const __grid_constant__ Kv
     const int64_t stride = which ? a.token_stride[1] : a.token_stride[0];
     const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + h * (which ? a.head_stride[1] : a.head_stride[0]) + d +
                  (i0 + first) * stride;
+    // (the count of rounds is the same for every lane group of a warp, whatever its `first`)
     const bool mine = have && d < D;                         // D is a multiple of 16
     // code and scale places of this lane in slot 0, and from slot to slot
     const int q_row = FORMAT == EMU_KV_FP8 ? H * D : H * (D / 2), s_row = FORMAT == EMU_KV_FP8 ? H * G : H * (D / 32);
     uint8_t* q = (which ? a.q[1] : a.q[0]) + (FORMAT == EMU_KV_FP8 ? h * D + d : (h * D + d) / 2);
     void* sc = which ? a.scale[1] : a.scale[0];
     const int s_at = FORMAT == EMU_KV_FP8 ? hg : (h * D + d) / 32;
-    for (int t0 = first; t0 < n; t0 += side * U, x += (int64_t)side * U * stride) {
+    for (int t0 = 0; t0 < n; t0 += side * U, x += (int64_t)side * U * stride) {
       f8::Raw<T> r[U];
       int64_t slot[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        slot[u] = have && t0 + u * side < n ? sl.own[t0 + u * side] : -1;
+        const int i = t0 + first + u * side;
+        slot[u] = have && i < n ? sl.own[i] : -1;
         f8::load8<T, VEC>(x + u * side * stride, mine && slot[u] >= 0 ? 8 : 0, r[u]);
       }
 #pragma unroll

@@ -261,3 +261,30 @@ def test_registered_operators():
         assert torch.equal(x, y)
     for x, y in zip(torch.ops.emugen.read_kv_cache(*a, table, cu, 20), kvcache.read_kv_cache(*b, table, cu, total=20)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("H,D", [(3, 128), (1, 32), (5, 48), (7, 64), (1, 144)])
+@pytest.mark.parametrize("T", [1, 2, 601, 1500])
+@pytest.mark.parametrize("values", [False, True])
+def test_odd_numbers_of_groups(H, D, T, values):
+    """Lane groups of one warp that belong to different tokens, with and without a value cache."""
+    k, v = _kv(T, H, D, torch.bfloat16, 1), _kv(T, H, D, torch.bfloat16, 2)
+    c = kvcache.make_kv_cache(T // 16 + 1, 16, H, D, values=values)
+    slots = torch.randperm((T // 16 + 1) * 16, generator=torch.Generator().manual_seed(T))[:T]
+    kvcache.write_kv_cache(k.cuda(), v.cuda() if values else None, slots.cuda(), *c)
+    for x, codes, scales in ((k, c[0], c[2]),) + (((v, c[1], c[3]),) if values else ()):
+        want_c, want_s = _rows(x.reshape(-1, D), "fp8")
+        assert torch.equal(_bytes(codes).reshape(-1, H, D)[slots].reshape(want_c.shape), want_c)
+        assert torch.equal(scales.cpu().reshape(-1, H, scales.shape[-1])[slots].reshape(want_s.shape), want_s)
+
+
+def test_slots_far_apart_and_many_times():
+    """Slots a power of two apart (one bucket of a low-bits hash) and one slot for all tokens."""
+    T, H, D = 900, 1, 32
+    k = _kv(T, H, D, torch.bfloat16, 3).cuda()
+    c = kvcache.make_kv_cache(T, 4096, H, D, values=False)
+    kvcache.write_kv_cache(k, None, torch.arange(T, device="cuda") * 4096, c[0], None, c[2], None)
+    want_c, want_s = _rows(k.cpu().reshape(T, D), "fp8")
+    assert torch.equal(_bytes(c[0])[:, 0].reshape(T, D), want_c) and torch.equal(c[2].cpu()[:, 0].reshape(T, 1), want_s)
+    kvcache.write_kv_cache(k, None, torch.full((T,), 7, device="cuda"), c[0], None, c[2], None)
+    assert torch.equal(_bytes(c[0])[0, 7].reshape(1, D), want_c[-1:]) and c[2].cpu()[0, 7, 0, 0] == want_s[-1, 0]
