@@ -5,8 +5,8 @@
 //   code  = nearest 8-bit value to x / scale, ties to even (fp8.cuh); NaN for NaN and infinities.
 //
 // Each input element is read once and kept in registers between the maximum and the rounding.  What bounds
-// the kernels is their arithmetic (ALU pipe 58% busy) before the memory: 8192 x 8192 bf16 on B200, rows 49 us
-// (201 MB: floor 31), rows and columns 88 us (272 MB: floor 42), tiles 39 us, tiles with the transpose 55 us.
+// the kernels is their arithmetic (ALU pipe 58% busy) before the memory: 8192 x 8192 bf16 on B200, rows 48 us
+// (201 MB: floor 31), rows and columns 88 us (272 MB: floor 42), tiles 37 us, tiles with the transpose 54 us.
 // A division or a border test for each element took rows and columns to 255 us (fp8.cuh).
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -24,9 +24,9 @@ namespace {
 // Rows in 1 x 128 blocks.  16 lanes hold one block, 8 elements each; a CTA of 256 threads takes 4 U rows
 // x 4 blocks (1 KB of consecutive 16-bit input per row), U loads in flight per thread.
 template <typename T, int TYPE, bool VEC, int U>
-__global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                                                             uint8_t* __restrict__ q, int64_t ldq,
-                                                             float* __restrict__ scale, int64_t lds) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 0)
+    quant_fp8_rows_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
+                          float* __restrict__ scale, int64_t lds) {
   const int lane16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int64_t kb_count = (K + 127) / 128;
   const int64_t kb = (int64_t)blockIdx.x * 4 + (grp & 3), k = kb * 128 + lane16 * 8;
@@ -85,11 +85,10 @@ __global__ void __launch_bounds__(256) quant_fp8_rows_kernel(const T* __restrict
 // TILE: one scale for the tile, its codes turned as bytes; otherwise one per row (q) and one per column (qt),
 // each element rounded twice (88 us at 8192 x 8192 bf16; two passes over the input would read 134 MB more).
 template <typename T, int TYPE, bool VEC, bool TILE>
-__global__ void __launch_bounds__(256, TILE ? 1 : sizeof(T) == 2 ? 3 : 2) quant_fp8_tile_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                                                             uint8_t* __restrict__ q, int64_t ldq,
-                                                             float* __restrict__ scale, int64_t lds,
-                                                             uint8_t* __restrict__ qt, int64_t ldqt,
-                                                             float* __restrict__ scale_t, int64_t ldst) {
+__global__ void __launch_bounds__(256, TILE ? 0 : sizeof(T) == 2 ? 3 : 2)
+    quant_fp8_tile_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
+                          uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale, int64_t lds,
+                          uint8_t* __restrict__ qt, int64_t ldqt, float* __restrict__ scale_t, int64_t ldst) {
   constexpr int PITCH = 136;                               // bytes per transposed row: 8-byte aligned, rows 34 banks apart
   __shared__ __align__(16) uint8_t tr[128 * PITCH];
   __shared__ uint32_t col_top[8][128];
