@@ -76,9 +76,12 @@ def quant_fp8(x: torch.Tensor, *, block: str = "row", dtype: torch.dtype = torch
         x = x.to(_lib._device_for(x))
     if x.requires_grad:
         x = x.detach()
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.shape[:-1].numel(), 0)
-    return _quant(x, _BLOCKS[block], dtype, transposed)
+    return _quant(_matrix(x), _BLOCKS[block], dtype, transposed)
+
+
+def _matrix(x: torch.Tensor) -> torch.Tensor:
+    """x with its leading dimensions flattened."""
+    return x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), x.shape[-1])
 
 
 def _quant(x: torch.Tensor, block: int, dtype: torch.dtype, transposed: bool):
@@ -212,41 +215,98 @@ def _gemm(a, b, scale_a, scale_b, rows: bool, out_dtype: torch.dtype, dev: torch
     return out
 
 
+def _up(n: int, m: int) -> int:
+    return (n + m - 1) // m * m
+
+
+class _Quantised:
+    """Codes and scales of a [rows, cols] matrix inside a byte buffer, at 256-byte places, as the product
+    takes them; `tile`: 128 x 128 blocks.  One buffer for a layer's operands in place of a tensor for each."""
+
+    def __init__(self, rows: int, cols: int, tile: bool, at: int = 0):
+        self.rows, self.cols, self.tile, self.codes = rows, cols, tile, at
+        self.ld = _up(cols, 16)
+        self.ld_scale = _blocks(cols) if tile else _up(rows, 4)
+        self.scale = at + _up(rows * self.ld, 256)
+        self.end = self.scale + _up(4 * self.ld_scale * (_blocks(rows) if tile else _blocks(cols)), 256)
+
+
+def _quant_into(x: torch.Tensor, block: int, q: _Quantised, base: int, t, base_t: int, stream: int) -> None:
+    """quant_fp8 of a matrix into q at address `base` and, unless t is None, of its transpose into t at base_t."""
+    ldx, inner = x.stride()
+    if inner != 1 and q.cols > 1 or ldx < q.cols and q.rows > 1:
+        x = x.contiguous()
+        ldx = q.cols
+    status = _lib.load().emu_quant_fp8(
+        x.data_ptr(), _DTYPE[x.dtype], q.rows, q.cols, ldx if q.rows > 1 else q.cols, _lib.EMU_FP8_E4M3, block,
+        base + q.codes, q.ld, base + q.scale, q.ld_scale, *((base_t + t.codes, t.ld, base_t + t.scale, t.ld_scale) if t else
+                                                            (None, 0, None, 0)), stream)
+    if status:
+        _lib._check(status)
+
+
+def _product(a: _Quantised, base_a: int, b: _Quantised, base_b: int, dtype: torch.dtype, dev: torch.device, stream: int):
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
+    status = _lib.load().emu_gemm_fp8(
+        base_a + a.codes, a.ld, _lib.EMU_FP8_E4M3, base_b + b.codes, b.ld, _lib.EMU_FP8_E4M3, base_a + a.scale, a.ld_scale,
+        base_b + b.scale, b.ld_scale, _lib.EMU_BLOCK_TILE if b.tile else _lib.EMU_BLOCK_ROW, a.rows, b.rows, a.cols,
+        _DTYPE[dtype], out.data_ptr(), b.rows, stream)
+    if status:
+        _lib._check(status)
+    return out
+
+
 def _linear(x: torch.Tensor, weight: torch.Tensor, need_x: bool, need_w: bool):
-    """(y, x's codes and scales as `quant_fp8` gives them, weight's): with the transposes that the wanted
-    gradients need -- x.T for the weight's, weight.T for x's."""
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    q = _quant(x2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
-    w = _quant(weight, _lib.EMU_BLOCK_TILE, torch.float8_e4m3fn, need_x)
-    y = _gemm(q[0], w[0], q[1], w[1], False, x.dtype, x.device)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0]), q, w
+    """(y [M, N], what the wanted gradients need): x.T's codes for the weight's, weight.T's for x's, each a
+    byte buffer or None."""
+    (M, K), N, dev = x.shape, weight.shape[0], x.device
+    if not (M and N and K):
+        return torch.zeros((M, N), dtype=x.dtype, device=dev), None, None
+    q = _Quantised(M, K, False)
+    w = _Quantised(N, K, True, q.end)
+    qt, wt = _Quantised(K, M, False) if need_w else None, _Quantised(K, N, True) if need_x else None
+    with _on(dev.index):
+        now = torch.empty(w.end, dtype=torch.uint8, device=dev)
+        xt = torch.empty(qt.end, dtype=torch.uint8, device=dev) if need_w else None
+        wtt = torch.empty(wt.end, dtype=torch.uint8, device=dev) if need_x else None
+        base, stream = now.data_ptr(), _raw_stream(dev.index)
+        _quant_into(x, _lib.EMU_BLOCK_ROW, q, base, qt, xt.data_ptr() if need_w else 0, stream)
+        _quant_into(weight, _lib.EMU_BLOCK_TILE, w, base, wt, wtt.data_ptr() if need_x else 0, stream)
+        return _product(q, base, w, base, x.dtype, dev, stream), xt, wtt
+
+
+def _linear_backward(dy: torch.Tensor, xt, wt, K: int, need_x: bool, need_w: bool):
+    """(dx [M, K], dw [N, K]), each None where it is not wanted."""
+    (M, N), dtype, dev = dy.shape, dy.dtype, dy.device
+    if not (M and N and K):
+        return (torch.zeros((M, K), dtype=dtype, device=dev) if need_x else None,
+                torch.zeros((N, K), dtype=dtype, device=dev) if need_w else None)
+    g = _Quantised(M, N, False)
+    gt = _Quantised(N, M, False, g.end) if need_w else None
+    with _on(dev.index):
+        now = torch.empty((gt or g).end, dtype=torch.uint8, device=dev)
+        base, stream = now.data_ptr(), _raw_stream(dev.index)
+        _quant_into(dy, _lib.EMU_BLOCK_ROW, g, base, gt, base, stream)
+        return (_product(g, base, _Quantised(K, N, True), wt.data_ptr(), dtype, dev, stream) if need_x else None,
+                _product(gt, base, _Quantised(K, M, False), xt.data_ptr(), dtype, dev, stream) if need_w else None)
 
 
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
         need_x, need_w = ctx.needs_input_grad
-        y, q, w = _linear(x, weight, need_x, need_w)
-        ctx.save_for_backward(*(q[2:] if need_w else (None, None)), *(w[2:] if need_x else (None, None)))
+        y, xt, wt = _linear(_matrix(x), weight, need_x, need_w)
+        ctx.save_for_backward(xt, wt)
         ctx.x_shape = x.shape
-        return y
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xt, xts, wt, wts = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad
-        dev, dtype = dy.device, dy.dtype
-        dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
-        g = _quant(dy2, _lib.EMU_BLOCK_ROW, torch.float8_e4m3fn, need_w)
-        dx = dw = None
-        if need_x:
-            dx = _gemm(g[0], wt, g[1], wts, False, dtype, dev)
-            if len(ctx.x_shape) != 2:
-                dx = dx.reshape(ctx.x_shape)
-        if need_w:
-            dw = _gemm(g[2], xt, g[3], xts, True, dtype, dev)
-        return dx, dw
+        shape = ctx.x_shape
+        dx, dw = _linear_backward(_matrix(dy), *ctx.saved_tensors, shape[-1], need_x, need_w)
+        return dx if dx is None or len(shape) == 2 else dx.reshape(shape), dw
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -269,7 +329,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     if not x.is_cuda or x.device != weight.device:
         raise RuntimeError("x and weight must be on the same CUDA device")
     if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
-        return _linear(x.detach(), weight.detach(), False, False)[0]
+        y = _linear(_matrix(x.detach()), weight.detach(), False, False)[0]
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
     return _LinearFp8.apply(x, weight)
 
 

@@ -356,6 +356,17 @@ def test_linear_partial_gradients_and_expanded_gradient():
     p, q = x.clone().requires_grad_(), w.clone().requires_grad_()
     with torch.no_grad():                               # nothing is kept where nothing is to be differentiated
         assert fp8.linear_fp8(p, q).grad_fn is None
+    for shape, n in (((2, 3, 0), 5), ((2, 0, 8), 5), ((2, 3, 8), 0)):   # nothing to add up, no rows, no columns
+        a = torch.ones(shape, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        b = torch.ones(n, shape[-1], device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        out = fp8.linear_fp8(a, b)
+        assert out.shape == (*shape[:-1], n) and (out == 0).all()
+        da, db = torch.autograd.grad(out, (a, b), torch.ones_like(out))
+        assert da.shape == a.shape and db.shape == b.shape and (da == 0).all() and (db == 0).all()
+    y = fp8.linear_fp8(p, q)                            # a second backward pass through the same graph
+    g1 = torch.autograd.grad(y, (p, q), torch.ones_like(y), retain_graph=True)
+    g2 = torch.autograd.grad(y, (p, q), torch.ones_like(y))
+    assert all(torch.equal(s, t) for s, t in zip(g1, g2))
     e = torch.zeros(0, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     v = w.clone().requires_grad_()
     fp8.linear_fp8(e, v).sum().backward()
