@@ -31,13 +31,14 @@ def _blocks(n: int) -> int:
 
 
 _HERE = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(dev).cuda_stream without its objects
+# current_stream(dev).cuda_stream and current_device() without their objects and start-up checks
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _on(index: int):
-    """Make device `index` current for the call.  Where it already is, as in most calls, entering and
-    leaving torch.cuda.device would cost a small launch's time."""
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+    """Make device `index`, which holds a tensor, current for the call.  Where it already is, as in most calls,
+    entering and leaving torch.cuda.device would cost a small launch's time."""
+    return _HERE if _current_device() == index else torch.cuda.device(index)
 
 
 def _codes(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:

@@ -69,10 +69,13 @@ def _geometry(k_cache, v_cache, k_scale, v_scale):
             raise RuntimeError("v_cache must have k_cache's shape and dtype")
         if v_scale.shape != k_scale.shape or v_scale.dtype != k_scale.dtype:
             raise RuntimeError("v_scale must have k_scale's shape and dtype")
+    device = k_cache.get_device()
     for t in (k_cache, v_cache, k_scale, v_scale):
-        if t is not None and not t.is_contiguous():
+        if t is None:
+            continue
+        if not t.is_contiguous():
             raise RuntimeError("cache tensors must be contiguous")
-        if t is not None and (not t.is_cuda or t.device != k_cache.device):
+        if device < 0 or t.get_device() != device:
             raise RuntimeError("cache tensors must be on one CUDA device")
     return fmt, pages, page_size, heads, D
 
@@ -99,7 +102,8 @@ def write_kv_cache(k: torch.Tensor, v: Optional[torch.Tensor], slots: torch.Tens
         raise RuntimeError("v must have k's shape and dtype")
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != k.shape[0]:
         raise RuntimeError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {list(slots.shape)}")
-    if k.device != dev or slots.device != dev or (v is not None and v.device != dev):
+    at = dev.index
+    if k.get_device() != at or slots.get_device() != at or (v is not None and v.get_device() != at):
         raise RuntimeError("k, v and slots must be on the cache's device")
     if k.stride(2) != 1:
         k = k.contiguous()
