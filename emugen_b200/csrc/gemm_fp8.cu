@@ -733,8 +733,8 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
   p.wait_limit = current_wait_limit();
   p.hold_first_ready = current_hold_first_ready();
   // Up to 64 rows of A are one column tile of the skinny kernel: each byte of B is read once.  Beyond, the two
-  // kernels' times by what they do, in us (measured over 65 .. 4096 rows, 512 .. 14336 columns and K, within
-  // 15%): the skinny one 6.5 + its tiles' blocks of K / 300 (B200 whole), the pairs 3.5 + for each wave of tiles
+  // kernels' times by what they do, in us (fitted over 65 .. 4096 rows, 512 .. 14336 columns and K; mostly within
+  // 15%, at worst 25%): the skinny one 6.5 + its tiles' blocks of K / 300, the pairs 3.5 + for each wave of tiles
   // 0.53 (0.8 with a scale per row of B) a block + 2.3 to store.  E.g. 128 x 4096 x 4096: 14.1 against 22.3;
   // 128 x 14336 x 4096: 28.1 against 23.5; 1024 x 4096 x 4096: 53 against 24.
   const int64_t kb = p.kb_count;
