@@ -448,3 +448,30 @@ def test_registered_operators():
     want = fp8.linear_fp8(x, w) * 2
     assert torch.equal(f(x, w), want)
     assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x, w), want)
+
+
+def test_beside_the_emulated_product_on_other_streams():
+    """The kernels that own tensor memory, at once: the emulated product, the CTA pairs and the skinny kernel."""
+    from emugen_b200 import nvfp4_global_scales, quant_nvfp4
+
+    g = torch.Generator().manual_seed(2)
+    p, r = torch.randn(1024, 1024, generator=g).half().cuda(), torch.randn(1024, 1024, generator=g).half().cuda()
+    gp, gr, alpha = nvfp4_global_scales(p, r)
+    (qp, sp), (qr, sr) = quant_nvfp4(p, gp), quant_nvfp4(r, gr)
+    emulated = lambda: _lib.gemm(qp, qr, sp, sr, fmt=0, group_size=16, w_reduce=4, stage3_rounding=0, stage4_rounding=0,
+                                 alpha=alpha, out_mode=2, path="tc")
+    big = [t.cuda() for t in _operands(2048, 2048, 2048, E4, E4, False, 3, True)]
+    few = [t.cuda() for t in _operands(40, 4000, 4096, E4, E4, True, 4, True)]
+    calls = [emulated, lambda: fp8.gemm_fp8(*big, out_dtype=torch.float32), lambda: fp8.gemm_fp8(*few, out_dtype=torch.float32)]
+    want = [f() for f in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    outs = [[] for _ in calls]
+    for _ in range(8):
+        for st, f, o in zip(streams, calls, outs):
+            with torch.cuda.stream(st):
+                o.append(f())
+    torch.cuda.synchronize()
+    _lib.device_status()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x, w) for x in o)
