@@ -176,10 +176,7 @@ __device__ __forceinline__ void tmem_wait_regs(uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_wait_regs(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-// Two f32 operations in one instruction (round to nearest, subnormals kept).
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  return (uint64_t)__float_as_uint(lo) | ((uint64_t)__float_as_uint(hi) << 32);
-}
+// Two f32 in one register pair, and their products in one instruction (round to nearest, subnormals kept).
 __device__ __forceinline__ uint64_t join2(uint32_t lo, uint32_t hi) {
   uint64_t d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
@@ -187,11 +184,6 @@ __device__ __forceinline__ uint64_t join2(uint32_t lo, uint32_t hi) {
 }
 __device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
