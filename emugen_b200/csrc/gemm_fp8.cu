@@ -4,8 +4,8 @@
 //   out[m][n] = sum_kb sa[m][kb] * sb[n or n / 128][kb] * sum_{k in block kb} A[m][k] * B[n][k]
 //
 // The inner sum of one 128-wide block is four MMAs into a fresh TMEM accumulator; CUDA cores multiply
-// it by the two scales and add it to f32 accumulators in registers, so the scales' f32 product and the
-// sum over blocks never pass through fewer than 32 bits.
+// it by the two scales and add it to f32 accumulators in registers, so neither the scaled block sums nor the
+// sum over blocks pass through fewer than 32 bits.  The scales may be any f32: see "Order of the factors".
 //
 // Few rows of A (gemm_fp8_skinny_kernel): the rows of B are the MMA's 128 lanes and BN rows of A its columns
 // ("weights by tokens"), so that few rows of A cost few columns; the blocks of K are split over the CTAs
@@ -70,6 +70,71 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, float v, int mod
   else if (mode == EMU_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(out)[i] = __float2half_rn(v);
 }
+
+// ------------------------------------------------------------------------------ Order of the factors
+// sum * sa * sb must not leave f32's range on the way where the result does not.  A block sum is 0 or between 2^-32 (two
+// smallest E5M2 codes) and 2^39 (128 products of the largest), so
+//   * times a scale in [2^-94, 2^89] it stays a normal number, and the other scale may be anything;
+//   * times a smaller scale it is off by at most 2^-150, which a second scale of at most 1 leaves below f32's last place
+//     (blocks of zeros have the quantiser's smallest scale, 2^-126, and are in this form as a rule);
+//   * where sa * sb is a normal number, the sum may be multiplied by that product;
+//   * where it is smaller, by the larger scale first: that is below 2^23 (the other is at least 2^-149) and, unless
+//     the result is below 2^-150 anyhow, at least 2^-94 (a scale of 0 goes first instead: the other may be anything);
+//   * where it is larger, by the smaller scale first: either that is below 1, or an overflow is the result's own.
+// Which of these an element takes depends on its own two scales and not on what else a warp adds up (but for the last
+// place of results below f32's normal range).
+constexpr float SCALE_LOW = 0x1p-94f, SCALE_HIGH = 0x1p89f;
+
+__device__ __forceinline__ bool in_range(float s) { return fabsf(s) >= SCALE_LOW && fabsf(s) <= SCALE_HIGH; }
+__device__ __forceinline__ bool normal_product(float f) {
+  return fabsf(f) >= 0x1p-126f && fabsf(f) <= 3.402823466e38f;       // NaN: no
+}
+struct Factors {
+  float first, second;
+};
+// The last three of these cases.
+__device__ __forceinline__ Factors factors(float sa, float sb) {
+  const float f = __fmul_rn(sa, sb);
+  if (normal_product(f)) return {1.0f, f};
+  const bool larger_first = fabsf(f) < 0x1p-126f && sa != 0.0f && sb != 0.0f;
+  return (fabsf(sa) > fabsf(sb)) == larger_first ? Factors{sa, sb} : Factors{sb, sa};
+}
+// All of them: `first` before `second` where the first two say so.
+__device__ __forceinline__ Factors factors_in_order(float first, float second) {
+  const float m = fabsf(first);
+  return (m >= SCALE_LOW || fabsf(second) <= 1.0f) && m <= SCALE_HIGH ? Factors{first, second} : factors(first, second);
+}
+// Four sums added up, each in its own order (out of line: rare, and its code many times over would cost the usual path
+// registers: 118 -> 137 us at 4096^3 with row scales of both operands).
+__device__ __noinline__ float4 add_any4(float4 x, float first, float4 second, float4 acc) {
+  const Factors a = factors_in_order(first, second.x), b = factors_in_order(first, second.y);
+  const Factors c = factors_in_order(first, second.z), d = factors_in_order(first, second.w);
+  return make_float4(__fmaf_rn(__fmul_rn(x.x, a.first), a.second, acc.x), __fmaf_rn(__fmul_rn(x.y, b.first), b.second, acc.y),
+                     __fmaf_rn(__fmul_rn(x.z, c.first), c.second, acc.z), __fmaf_rn(__fmul_rn(x.w, d.first), d.second, acc.w));
+}
+template <int N> __device__ __forceinline__ void add_any(const uint32_t (&x)[N], float first, const float* second, float* acc) {
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const float4 r = add_any4(make_float4(__uint_as_float(x[j]), __uint_as_float(x[j + 1]), __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
+                              first, *reinterpret_cast<const float4*>(second + j), make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+    acc[j] = r.x, acc[j + 1] = r.y, acc[j + 2] = r.z, acc[j + 3] = r.w;
+  }
+}
+// For the second case: whether this lane's share of the first n of `second` (shared memory; n <= 128) is at most 1.
+__device__ __forceinline__ bool at_most_one(const float* second, int n, int lane) {
+  bool ok = true;
+  if (lane * 4 < n) {
+    const float4 s = *reinterpret_cast<const float4*>(second + lane * 4);
+    const int j = n - lane * 4;
+    ok = fabsf(s.x) <= 1.0f && (j < 2 || fabsf(s.y) <= 1.0f) && (j < 3 || fabsf(s.z) <= 1.0f) && (j < 4 || fabsf(s.w) <= 1.0f);
+  }
+  return ok;
+}
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 template <int BN> struct Cfg {
   static constexpr int STAGE = (LANES + BN) * BK;
@@ -182,42 +247,68 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __gri
     const int quarter = warp & 3;                                  // the TMEM lanes this warp may read
     const int64_t n = n0 + quarter * 32 + lane;
     const float* sb_tile = p.sb + (n0 / 128) * p.ldsb;
-    for (int i = 0; i < steps; ++i) {
-      const int sc = i % C::NSCALE, ac = i % C::NACC;
-      const float sb_t = p.b_rows ? 0.0f : __ldg(sb_tile + kb0 + i);
-      if (!warp_wait_or_record(&s_full[sc], (i / C::NSCALE) & 1, p.wait_limit, 16) ||
-          !warp_wait_or_record(&acc_full[ac], (i / C::NACC) & 1, p.wait_limit, 17)) {
-        *failed = 1;
-        break;
-      }
-      ptx::tc_fence_after();
-      const float* slot = scales + sc * (C::SCALE / 4);
-      const float sb = p.b_rows ? slot[BN + quarter * 32 + lane] : sb_t;
+    const int columns = (int)min((int64_t)BN, p.M - m0);
+    // The blocks whose sums may be multiplied by the scale of B's row first, up to one whose scales need more care; from
+    // there on each element in its own order.
+    int i = 0;
+    auto add_up = [&](auto any_scales) {
+      constexpr bool ANY = decltype(any_scales)::value;
+      for (; i < steps; ++i) {
+        const int sc = i % C::NSCALE, ac = i % C::NACC;
+        const float sb_t = p.b_rows ? 0.0f : __ldg(sb_tile + kb0 + i);
+        if (!warp_wait_or_record(&s_full[sc], (i / C::NSCALE) & 1, p.wait_limit, 16)) {
+          *failed = 1;
+          return;
+        }
+        const float* slot = scales + sc * (C::SCALE / 4);
+        const float sb = !p.b_rows ? sb_t : n < p.N ? slot[BN + quarter * 32 + lane] : 1.0f;   // lanes past N have no scale
+        // one vote for the wait and the scales
+        const bool full_now = wait_or_record(&acc_full[ac], (i / C::NACC) & 1, p.wait_limit, 17);
+        if (!__all_sync(0xFFFFFFFFu, full_now && (ANY || in_range(sb)))) {
+          if (!__all_sync(0xFFFFFFFFu, full_now)) {
+            *failed = 1;
+            return;
+          }
+          if (!__all_sync(0xFFFFFFFFu, fabsf(sb) <= SCALE_HIGH && at_most_one(slot, columns, lane))) return;
+        }
+        ptx::tc_fence_after();
 #pragma unroll
-      for (int j = 0; j < BN; j += 16) {
-        uint32_t v[16];
-        ptx::tmem_ld_regs(tmem + ((uint32_t)(quarter * 32) << 16) + ac * BN + j, v);
-        ptx::tmem_wait_regs(v);
+        for (int j = 0; j < BN; j += 16) {
+          uint32_t v[16];
+          ptx::tmem_ld_regs(tmem + ((uint32_t)(quarter * 32) << 16) + ac * BN + j, v);
+          ptx::tmem_wait_regs(v);
+          if constexpr (ANY) {
+            add_any(v, sb, slot + j, acc + j);
+          } else {
 #pragma unroll
-        for (int u = 0; u < 16; u += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(slot + j + u);
-          acc[j + u] = __fmaf_rn(__uint_as_float(v[u]), __fmul_rn(sb, s4.x), acc[j + u]);
-          acc[j + u + 1] = __fmaf_rn(__uint_as_float(v[u + 1]), __fmul_rn(sb, s4.y), acc[j + u + 1]);
-          acc[j + u + 2] = __fmaf_rn(__uint_as_float(v[u + 2]), __fmul_rn(sb, s4.z), acc[j + u + 2]);
-          acc[j + u + 3] = __fmaf_rn(__uint_as_float(v[u + 3]), __fmul_rn(sb, s4.w), acc[j + u + 3]);
+            for (int u = 0; u < 16; u += 4) {
+              const float4 s4 = *reinterpret_cast<const float4*>(slot + j + u);
+              const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[j + u + e] = __fmaf_rn(__fmul_rn(__uint_as_float(v[u + e]), sb), s[e], acc[j + u + e]);
+            }
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(&acc_empty[ac]);
+          ptx::mbar_arrive(&s_empty[sc]);
         }
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        ptx::mbar_arrive(&acc_empty[ac]);
-        ptx::mbar_arrive(&s_empty[sc]);
-      }
-    }
+    };
+    add_up(std::false_type{});
+    if (i < steps && !*failed) add_up(std::true_type{});
     if (split == 1 && n < p.N && !*failed) {
+      auto write = [&](auto* out) {
+        out += m0 * p.ldo + n;
 #pragma unroll
-      for (int j = 0; j < BN; ++j)
-        if (m0 + j < p.M) store_out(p.out, (m0 + j) * p.ldo + n, acc[j], p.out_mode);
+        for (int j = 0; j < BN; ++j, out += p.ldo)
+          if (j < columns) *out = from_float<std::remove_pointer_t<decltype(out)>>(acc[j]);
+      };
+      if (p.out_mode == EMU_DTYPE_BF16) write(static_cast<__nv_bfloat16*>(p.out));
+      else if (p.out_mode == EMU_DTYPE_F16) write(static_cast<__half*>(p.out));
+      else write(static_cast<float*>(p.out));
     }
   }
 
@@ -283,11 +374,12 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __gri
 //               them from TMEM and adds scale * block sum.  (The f32x2 form of the multiply-add was slower:
 //               its register pairs cost a move each, 484 against 268 us for the epilogue alone at 8192^3.)
 //               B_ROWS = false: 128 columns share one scale of B, so the factor is one number per thread;
-//               B_ROWS = true: the block sum is multiplied by the column's scale first.
+//               B_ROWS = true: the block sum is multiplied by the row's scale, then by the column's.
 // Bound: the epilogue's turn-around.  A block's MMAs take 512 clocks; its sums reach the epilogue about 450 clocks
 // after that, take 270 to load (TMEM's rate) and 400 to add up, so with two accumulators a block comes every
-// 850 clocks or so.  B200: 4096^3 72 us (1.91 PFLOP/s; 118 with column scales), 8192^3 490 us (2.24 PFLOP/s, the clock
-// already lowered by the power limit: MMAs and loads alone take 366).  Other splits were no faster: 128-column
+// 850 clocks or so.  B200: 4096^3 74 us (1.86 PFLOP/s; 121 with column scales), 8192^3 503 us (2.19 PFLOP/s, the clock
+// already lowered by the power limit: MMAs and loads alone take 366); without the test of the scales' range 73, 119 and
+// 495.  Other splits were no faster: 128-column
 // MMAs with four accumulators 72, sixteen epilogue warps of 64 columns 95, one issuer 89 us at 4096^3.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
 constexpr int P_NSTAGE = 5;                      // at least 4: see the issuers' waits
@@ -451,8 +543,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
     uint8_t* buf = store + ew * (32 * 128);
     const int64_t blocks_n = (p.N + 127) / 128;
     const uint32_t empty_bar = ptx::map_shared(ptx::smem_u32(acc_empty), 0);
-    // columns of one TMEM load (with column scales 16 were faster than 32: 122 against 128 us at 4096^3)
-    constexpr int LD = B_ROWS ? 16 : 32, CHUNKS = 128 / LD;
+    constexpr int LD = 32, CHUNKS = 128 / LD;                        // columns of one TMEM load
     bool ok = true;
     Ring<P_NSTAGE> st;
     Ring<P_NSCALE> sc;
@@ -462,6 +553,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       pair_tile(t, tiles_m, tiles_n, tm, tn);
       const int64_t nb = min(tn * 2 + half, blocks_n - 1);
       const float* sb_tile = p.sb + nb * p.ldsb;
+      const int columns = (int)max((int64_t)0, min((int64_t)128, p.N - (tn * 2 + half) * 128));
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
@@ -470,25 +562,45 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
       float sa1 = __ldg(sa_row), sa2 = p.kb_count > 1 ? __ldg(sa_row + p.ldsa) : 0.0f;
       float sa3 = p.kb_count > 2 ? __ldg(sa_row + 2 * p.ldsa) : 0.0f, sb3 = B_ROWS || p.kb_count < 3 ? 1.0f : __ldg(sb_tile + 2);
       float sb1 = B_ROWS ? 1.0f : __ldg(sb_tile), sb2 = B_ROWS || p.kb_count < 2 ? 1.0f : __ldg(sb_tile + 1);
-      uint32_t v[2][LD];
-      if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
-      ptx::tc_fence_after();
-      ptx::tmem_ld_regs(lane_base + ac, v[0]);
-      for (int kb = 0; kb < p.kb_count; ++kb) {
-        const bool more = kb + 1 < p.kb_count;
-        const float f = B_ROWS ? sa1 : __fmul_rn(sa1, sb1);
-        sa1 = sa2, sb1 = sb2, sa2 = sa3, sb2 = sb3;
+      // B_ROWS = false: a row whose first block has the quantiser's smallest scale (zeros, as a rule all along the row) would
+      // make the product of the scales too small.  Such a row is added up 2^100 times as large, while its factors stay
+      // below 2^60; so rows of zeros among others cost nothing (4096^3: 74 us; in the last loop below 90).
+      float up = !B_ROWS && fabsf(__fmul_rn(sa1, sb1)) < 0x1p-126f ? 0x1p100f : 1.0f;
+      const float low = up == 1.0f ? 0x1p-126f : 0.0f;
+      if (!B_ROWS) sa1 = __fmul_rn(sa1, up);
+      auto next_scales = [&](int kb) {
+        sa1 = B_ROWS ? sa2 : __fmul_rn(sa2, up), sb1 = sb2, sa2 = sa3, sb2 = sb3;
         if (kb + 3 < p.kb_count) {
           sa3 = __ldg(sa_row + (kb + 3) * p.ldsa);
           if (!B_ROWS) sb3 = __ldg(sb_tile + kb + 3);
         }
+      };
+      auto factor = [&] { return B_ROWS ? sa1 : __fmul_rn(sa1, sb1); };
+      auto fine = [&](float f) { return B_ROWS ? in_range(f) : fabsf(f) >= low && fabsf(f) <= 0x1p60f; };
+      // B_ROWS: rows of scales below the range, beside columns of scales up to 1 (4096^3 with such a row in every warp 152 us)
+      auto fine_beside = [&](float f) { return fabsf(f) <= SCALE_HIGH && at_most_one(scales + sc.at * (P_SCALE / 4) + half * 128, columns, lane); };
+      uint32_t v[2][LD];
+      if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
+      ptx::tc_fence_after();
+      ptx::tmem_ld_regs(lane_base + ac, v[0]);
+      int kb = 0;
+      float f = factor();
+      bool usual = __all_sync(0xFFFFFFFFu, fine(f));
+      if (B_ROWS && !usual) {
+        if (!warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
+        usual = __all_sync(0xFFFFFFFFu, fine_beside(f));
+      }
+      // The blocks of K, up to one whose scales need more care (see "Order of the factors")
+      for (; usual && kb < p.kb_count; ++kb) {
+        const bool more = kb + 1 < p.kb_count;
+        next_scales(kb);
+        const float f1 = factor();                                   // the next block's
         if (B_ROWS && !warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
-        const float* slot = scales + sc.at * (P_SCALE / 4);
+        const float* slot = scales + sc.at * (P_SCALE / 4) + half * 128;
         st.next();
         bool next = false;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-          const ulonglong2* sb4 = reinterpret_cast<const ulonglong2*>(slot + half * 128 + c * LD);
           ptx::tmem_wait_regs(v[c & 1]);
           // the next columns travel while these are added up
           if (c + 1 < CHUNKS) {
@@ -499,7 +611,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
             if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac / 32);   // 8 bytes per 256 columns
             ac ^= 256;
             if (more) {
-              next = __all_sync(0xFFFFFFFFu, ptx::mbar_test_wait(&done[st.at], st.parity));
+              // (one vote for both: a second one for the scales cost 72 -> 75 us at 4096^3)
+              next = __all_sync(0xFFFFFFFFu, ptx::mbar_test_wait(&done[st.at], st.parity) && fine(f1));
               if (next) {
                 ptx::tc_fence_after();
                 ptx::tmem_ld_regs(lane_base + ac, v[0]);
@@ -508,18 +621,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
           }
 #pragma unroll
           for (int j = 0; j < LD; j += 4) {
-            float x[4];
+            float x[4], s[4] = {f, f, f, f};
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[c & 1][j + e]);
             if (B_ROWS) {
               // two products per instruction: here the pairs lie as they were loaded
-              const ulonglong2 s = sb4[j / 4];
-              const uint64_t lo = ptx::mul2(ptx::join2(v[c & 1][j], v[c & 1][j + 1]), s.x);
-              const uint64_t hi = ptx::mul2(ptx::join2(v[c & 1][j + 2], v[c & 1][j + 3]), s.y);
+              const float4 s4 = *reinterpret_cast<const float4*>(slot + c * LD + j);
+              s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
+              const uint64_t ff = ptx::join2(__float_as_uint(f), __float_as_uint(f));
+              const uint64_t lo = ptx::mul2(ptx::join2(v[c & 1][j], v[c & 1][j + 1]), ff);
+              const uint64_t hi = ptx::mul2(ptx::join2(v[c & 1][j + 2], v[c & 1][j + 3]), ff);
               x[0] = ptx::lo2(lo), x[1] = ptx::hi2(lo), x[2] = ptx::lo2(hi), x[3] = ptx::hi2(hi);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c * LD + j + e] = __fmaf_rn(x[e], f, acc[c * LD + j + e]);
+            for (int e = 0; e < 4; ++e) acc[c * LD + j + e] = __fmaf_rn(x[e], s[e], acc[c * LD + j + e]);
           }
         }
         if (B_ROWS) {
@@ -527,7 +642,53 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
           if (lane == 0) ptx::mbar_arrive(&s_empty[sc.at]);
           sc.next();
         }
+        f = f1;
         if (more && !next) {
+          if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
+          ptx::tc_fence_after();
+          ptx::tmem_ld_regs(lane_base + ac, v[0]);
+          usual = __all_sync(0xFFFFFFFFu, fine(f));
+          if (B_ROWS && !usual) {
+            if (!warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
+            usual = __all_sync(0xFFFFFFFFu, fine_beside(f));
+          }
+        }
+      }
+      if (!B_ROWS && !__all_sync(0xFFFFFFFFu, up == 1.0f)) {
+        const float down = up == 1.0f ? 1.0f : 0x1p-100f;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] = __fmul_rn(acc[j], down);
+        if (kb < p.kb_count) sa1 = __ldg(sa_row + kb * p.ldsa);
+        up = 1.0f;
+      }
+      // The rest: each element in its own order (no load is in flight over add_any's calls)
+      for (; ok && kb < p.kb_count; ++kb) {
+        const float sa = sa1;
+        const Factors fs = factors(sa1, sb1);
+        next_scales(kb);
+        if (B_ROWS && !warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
+        const float* slot = scales + sc.at * (P_SCALE / 4) + half * 128;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          ptx::tmem_wait_regs(v[0]);
+          if (B_ROWS) {
+            add_any(v[0], sa, slot + c * LD, acc + c * LD);
+          } else {
+#pragma unroll
+            for (int j = 0; j < LD; ++j) acc[c * LD + j] = __fmaf_rn(__fmul_rn(__uint_as_float(v[0][j]), fs.first), fs.second, acc[c * LD + j]);
+          }
+          if (c + 1 < CHUNKS) ptx::tmem_ld_regs(lane_base + ac + (c + 1) * LD, v[0]);
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive_cluster(empty_bar + ac / 32);
+          if (B_ROWS) ptx::mbar_arrive(&s_empty[sc.at]);
+        }
+        ac ^= 256;
+        st.next();
+        if (B_ROWS) sc.next();
+        if (kb + 1 < p.kb_count) {
           if (!warp_wait_or_record(&done[st.at], st.parity, p.wait_limit, 17)) { ok = false; break; }
           ptx::tc_fence_after();
           ptx::tmem_ld_regs(lane_base + ac, v[0]);

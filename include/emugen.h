@@ -401,8 +401,9 @@ EMU_API emu_status emu_quant_fp8(const void* x, int32_t dtype, int64_t M, int64_
  *   out[m][n] = sum_kb scale_a(m, kb) * scale_b(n, kb) * sum_{k in block kb} a[m][k] * b[n][k]
  * a [M][K], b [N][K] codes (a_type / b_type EMU_FP8_*, rows lda / ldb bytes apart), both as emu_quant_fp8 leaves them:
  *   scale_a: EMU_BLOCK_ROW layout; scale_b: b_block's layout (a scale per row of b, or per 128 x 128 tile).
- * Sums in f32, one rounding to out_dtype (EMU_DTYPE_*) at the end; the same result every run.  A NaN code or
- * scale makes NaN exactly those outputs that it enters.  out [M][N], rows ldo elements apart.  K = 0 gives zeros.
+ * Sums in f32, one rounding to out_dtype (EMU_DTYPE_*) at the end; the same result every run.  Scales may be any f32: a
+ * scaled sum that is an f32 is not lost because the two scales' product, or the sum times one of them, is none.  A NaN code
+ * or scale makes NaN exactly those outputs that it enters (an infinite scale: infinities, and NaN where its block sums to 0).  out [M][N], rows ldo elements apart.  K = 0 gives zeros.
  * a, b 16-byte aligned, lda and ldb multiples of 16 (bytes past K are not used).  Scale rows of the row layout start
  * on 16 bytes, ld_scale is a multiple of 4, and they can be read up to M (N) rounded up to a multiple of 4.
  * M up to 65535 * 64, N up to 65535 * 128.
