@@ -17,6 +17,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -316,7 +317,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     With Q the quantiser (E4M3; rows in blocks of 128, the weight in 128 x 128 tiles):
       y  = Q(x) Q(weight)^T,   dx = Q(dy) Q(weight),   dw = Q(dy^T) Q(x^T)^T
     (the gradients treat Q as the identity).  The forward pass keeps the 8-bit transposes of x and the weight
-    for the backward pass, not x itself.  fp16, bf16 or f32 CUDA tensors of one device and dtype.
+    for the backward pass, not x itself.  fp16, bf16 or f32 CUDA tensors of one device and dtype.  Reverse mode only: inputs
+    with a forward-mode tangent are refused.
 
     A backward pass that a CUDA graph is to capture follows torch's rule for every operator: no eager graph of
     the same leaves may be alive (their gradient accumulators belong to its stream, and torch ends the process over
@@ -327,6 +329,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         raise RuntimeError("K mismatch between x and weight")
     if x.dtype != weight.dtype or x.dtype not in _DTYPE:
         raise RuntimeError(f"x and weight must share one of float16, bfloat16, float32, got {x.dtype} and {weight.dtype}")
+    if forward_ad.unpack_dual(x).tangent is not None or forward_ad.unpack_dual(weight).tangent is not None:
+        raise RuntimeError("linear_fp8 has no forward-mode derivative")
     if not x.is_cuda or x.device != weight.device:
         raise RuntimeError("x and weight must be on the same CUDA device")
     if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
