@@ -450,10 +450,12 @@ emu_status emu_test_hold_first_ready(int32_t enable) {
 emu_status emu_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: stream");
-  int code = 0;
+  // both kernels' words are taken, so that the next call speaks for later launches alone; the first one set is told
+  int code = 0, code_fp8 = 0;
   e = emu::take_wait_error(&code);
-  if (e == cudaSuccess && code == 0) e = emu::take_fp8_wait_error(&code);
+  if (e == cudaSuccess) e = emu::take_fp8_wait_error(&code_fp8);
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: error word");
+  if (code == 0) code = code_fp8;
   if (code == 0) return ok();
   static const char* const kSite[] = {"", "producer stage slot", "producer record slot", "MMA accumulator set",
                                       "MMA stage data", "epilogue accumulator", "epilogue records",
