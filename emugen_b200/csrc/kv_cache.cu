@@ -38,35 +38,55 @@ struct Slots {
 };
 
 // dead[i] for each of this CTA's tokens i0 + i: a later token of the call has the same slot, so that token's
-// row is the one that is kept (two rows written at once would leave a mixture).  Every later slot is
-// looked up among the CTA's.  That is T / 2 reads of L2 per CTA, so a long call takes many tokens per CTA
-// (launch_kv_write): 65536 tokens over 1024 CTAs spent 0.8 ms here.
+// row is the one that is kept (two rows written at once would leave a mixture).  The CTA's own tokens are settled first,
+// which leaves each slot in its chain once, and then every token behind them is looked up.  That is T / 2 reads of L2 per
+// CTA, so a long call takes many tokens per CTA (launch_kv_write): 65536 tokens over 1024 CTAs spent 0.8 ms here.
+// Padding on either side of the cache stays out of the chains (all of it in one made 131072 such tokens 9.9 ms).
 __device__ __forceinline__ void find_overwritten(const int64_t* __restrict__ slots, int64_t T, int64_t num_slots, int64_t i0,
                                                  int n, Slots& s) {
-  for (int i = threadIdx.x; i < BUCKETS; i += blockDim.x) s.head[i] = 0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) s.own[i] = slots[i0 + i], s.dead[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (s.own[i] >= 0) s.next[i] = (int16_t)(atomicExch(&s.head[bucket_of(s.own[i])], i + 1) - 1);
-  __syncthreads();
-  auto look_up = [&](int64_t slot, int64_t j) {
-    if (slot < 0) return;                                    // padding: writes nothing
-    for (int i = s.head[bucket_of(slot)] - 1; i >= 0; i = s.next[i])
-      if (s.own[i] == slot && i0 + i < j) s.dead[i] = 1;
+  auto link = [&] {                                          // chains of the tokens that still write
+    for (int i = threadIdx.x; i < BUCKETS; i += blockDim.x) s.head[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+      if (s.own[i] >= 0 && !s.dead[i]) s.next[i] = (int16_t)(atomicExch(&s.head[bucket_of(s.own[i])], i + 1) - 1);
+    __syncthreads();
   };
-  int64_t j = i0 + 1 + threadIdx.x;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t slot = slots[i0 + i];
+    s.own[i] = slot < num_slots ? slot : -1;                 // from here on a slot below 0 is one that nothing is written to
+    s.dead[i] = 0;
+  }
+  link();                                                    // (a thread reads what it wrote itself up to the second barrier)
+  if (n > 1) {
+    bool any = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int64_t slot = s.own[i];
+      if (slot < 0) continue;
+      for (int c = s.head[bucket_of(slot)] - 1; c >= 0; c = s.next[c])
+        if (c > i && s.own[c] == slot) {
+          s.dead[i] = 1, any = true;
+          break;
+        }
+    }
+    if (__syncthreads_or(any)) link();
+  }
+  auto look_up = [&](int64_t slot) {
+    if (slot < 0 || slot >= num_slots) return;
+    for (int i = s.head[bucket_of(slot)] - 1; i >= 0; i = s.next[i])
+      if (s.own[i] == slot) s.dead[i] = 1;
+  };
+  int64_t j = i0 + n + threadIdx.x;
   for (; j + 7 * (int64_t)blockDim.x < T; j += 8 * (int64_t)blockDim.x) {
     int64_t v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = __ldg(slots + j + u * (int64_t)blockDim.x);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) look_up(v[u], j + u * (int64_t)blockDim.x);
+    for (int u = 0; u < 8; ++u) look_up(v[u]);
   }
-  for (; j < T; j += blockDim.x) look_up(slots[j], j);
+  for (; j < T; j += blockDim.x) look_up(slots[j]);
   __syncthreads();
-  // from here on a slot below 0 is one that nothing is written to
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (s.dead[i] || s.own[i] >= num_slots) s.own[i] = -1;
+    if (s.dead[i]) s.own[i] = -1;
   __syncthreads();
 }
 

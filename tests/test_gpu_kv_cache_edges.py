@@ -1,0 +1,61 @@
+"""The quantised cache at its edges: padding past the cache and repeated slots in long calls."""
+import pytest
+import torch
+
+from emugen_b200 import kvcache
+from tests.test_gpu_kv_cache import _kv
+
+pytestmark = pytest.mark.gpu
+
+
+def _written(k, slots, pages, page):
+    """The cache after one call with each slot's last row (k: every token's)."""
+    n = pages * page
+    last = torch.full((n,), -1, dtype=torch.int64)
+    live = (slots >= 0) & (slots < n)
+    at = torch.arange(len(slots))[live]
+    last.scatter_reduce_(0, slots[live], at, "amax")
+    where = torch.arange(n)[last >= 0]
+    cache = kvcache.make_kv_cache(pages, page, *k.shape[1:], values=False)
+    for w in where.split(100):                       # short calls of distinct slots
+        kvcache.write_kv_cache(k[last[w].cuda()], None, w.cuda(), cache[0], None, cache[2], None)
+    return cache
+
+
+@pytest.mark.parametrize("T,pages,padding", [(160000, 80, -1), (160000, 80, 80 * 16), (160000, 1, 1 << 40), (5000, 20, 20 * 16), (700, 3, 3 * 16)])
+def test_long_calls_with_repeated_slots_and_padding(T, pages, padding):
+    """More tokens than 1024 for each SM, every slot many times over, a third of the tokens padding before or past the cache."""
+    g = torch.Generator().manual_seed(T)
+    k = _kv(T, 1, 32, torch.bfloat16, 7).cuda()
+    slots = torch.randint(0, pages * 16, (T,), generator=g)
+    slots[torch.rand(T, generator=g) < 0.33] = padding
+    cache = kvcache.make_kv_cache(pages, 16, 1, 32, values=False)
+    kvcache.write_kv_cache(k, None, slots.cuda(), cache[0], None, cache[2], None)
+    want = _written(k, slots, pages, 16)
+    assert torch.equal(cache[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(cache[2], want[2])
+
+
+def _us(f, n=5):
+    f()
+    best = float("inf")
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("slot", [1 << 40, 5])
+def test_padding_and_repeated_slots_cost_no_more_than_rows(slot):
+    """A call whose tokens are all padding past the cache, or all of one slot, is not slower than one that writes them
+    all (a factor of two for the clock): they write next to nothing."""
+    T = 131072
+    k = _kv(T, 8, 128, torch.bfloat16, 9).cuda()
+    cache = kvcache.make_kv_cache(T // 64, 64, 8, 128, values=False)
+    many = torch.randperm(T, generator=torch.Generator().manual_seed(2)).cuda()
+    one = torch.full((T,), slot, dtype=torch.int64, device="cuda")
+    write = lambda s: kvcache.write_kv_cache(k, None, s, cache[0], None, cache[2], None)
+    assert _us(lambda: write(one)) <= 2 * _us(lambda: write(many))
