@@ -236,8 +236,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
           s[u] = __ldg(static_cast<const float*>(sc) + (slot[u] * s_row + s_at));
         } else {
           w[u].x = __ldg(reinterpret_cast<const uint32_t*>(q + slot[u] * q_row));
-          // byte 0 -> 0, 255 -> inf, as emu_dequant_fp4
-          s[u] = __uint_as_float((uint32_t)__ldg(static_cast<const uint8_t*>(sc) + (slot[u] * s_row + s_at)) << 23);
+          // 2^(byte - 127): the exponent field, but for byte 0, which is f32's subnormal 2^-127; byte 255 gives infinity
+          const uint32_t e = __ldg(static_cast<const uint8_t*>(sc) + (slot[u] * s_row + s_at));
+          s[u] = __uint_as_float(e ? e << 23 : 0x00400000u);
         }
       }
 #pragma unroll

@@ -416,7 +416,8 @@ EMU_API emu_status emu_gemm_fp8(const uint8_t* a, int64_t lda, int32_t a_type, c
 
 /* Formats of the quantised key/value cache. */
 enum { EMU_KV_FP8 = 0,     /* E4M3 codes, an f32 scale per 128 elements of a (token, head) row (emu_quant_fp8's) */
-       EMU_KV_MXFP4 = 1    /* packed e2m1 codes, a scale byte u (2^(u - 127)) per 32 elements (emu_quant_mxfp4's) */ };
+       EMU_KV_MXFP4 = 1    /* packed e2m1 codes, a scale byte u (2^(u - 127), 255: infinity) per 32 elements
+                              (emu_quant_mxfp4's) */ };
 
 /*
  * Write keys and values into a quantised cache: token t's row of head h (k[t * k_token_stride + h * k_head_stride + d],

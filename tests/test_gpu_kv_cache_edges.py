@@ -1,11 +1,38 @@
-"""The quantised cache at its edges: padding past the cache and repeated slots in long calls."""
+"""The quantised cache at its edges: scale bytes at the ends of their range, padding past the cache
+and repeated slots in long calls."""
 import pytest
 import torch
 
 from emugen_b200 import kvcache
-from tests.test_gpu_kv_cache import _kv
+from tests.test_gpu_kv_cache import E2M1, _kv
 
 pytestmark = pytest.mark.gpu
+
+
+def _read_all(cache, rows, dtype):
+    pages = cache[0].shape[0]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    return kvcache.read_kv_cache(*cache, table, cu, total=rows, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_mxfp4_scale_bytes_of_the_whole_range(dtype):
+    """Every scale byte with every code: code * 2^(byte - 127) in f32 (byte 255, 2^128: infinity), rounded to the type."""
+    cache = kvcache.make_kv_cache(4, 64, 1, 32, "mxfp4")
+    code = torch.arange(32, dtype=torch.int32) % 16
+    packed = (code[0::2] | (code[1::2] << 4)).to(torch.uint8)
+    for c, s in ((cache[0], cache[2]), (cache[1], cache[3])):
+        c.copy_(packed.expand(4, 64, 1, 16))
+        s.copy_(torch.arange(256).to(torch.uint8).reshape(4, 64, 1, 1))
+    scale = torch.pow(2.0, torch.arange(256, dtype=torch.float64) - 127)
+    scale[255] = float("inf")
+    want = (E2M1[code.long()][None] * scale[:, None]).float().to(dtype)       # exact in f32 up to its range's end
+    assert want[0].double().abs().max() == (6 * 2.0 ** -127 if dtype != torch.float16 else 0)
+    for got in _read_all(cache, 256, dtype):
+        got = got.cpu()[:, 0]
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
 
 
 def _written(k, slots, pages, page):
