@@ -257,6 +257,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
           v[e] = __fmul_rn(f.x, s[u]);
           v[e + 1] = __fmul_rn(f.y, s[u]);
         }
+        // fp8: the product (4 + 24 bits) is rounded to f32 and then to T, so a value just beside a tie of T may go the
+        // other way than in one rounding; half a step of T and of f32 bound the error.  MXFP4 products are exact.
         T* dst = out + u * side * stride;
         __align__(16) T y[8];
 #pragma unroll

@@ -439,8 +439,8 @@ EMU_API emu_status emu_kv_write(const void* k, const void* v, int32_t dtype, int
  * Read the rows of a batch of sequences back from a quantised cache (emu_kv_write's layout, num_pages * page_size slots):
  * row r of the outputs, cu_lens[b] <= r < cu_lens[b + 1], is position i = r - cu_lens[b] of sequence b, from page
  * block_table[b * table_stride + i / page_size].  cu_lens: sequences + 1 non-decreasing values, cu_lens[0] = 0.
- * Outputs [total][heads][head_size], rows k_token_stride / v_token_stride elements apart: code * scale, rounded once to
- * out_dtype.  Rows of a page that does not exist (negative, not below num_pages, past table_cols) are zeros; rows
+ * Outputs [total][heads][head_size], rows k_token_stride / v_token_stride elements apart: code * scale, rounded to f32
+ * and then to out_dtype.  Rows of a page that does not exist (negative, not below num_pages, past table_cols) are zeros; rows
  * that no sequence has are left as they were.  v_cache may be NULL.  No reference counterpart.
  */
 EMU_API emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const void* k_scale,

@@ -1,5 +1,5 @@
-"""The quantised cache at its edges: scale bytes at the ends of their range, padding past the cache
-and repeated slots in long calls."""
+"""The quantised cache at its edges: scale bytes at the ends of their range, products beside ties, padding past the
+cache and repeated slots in long calls."""
 import pytest
 import torch
 
@@ -33,6 +33,26 @@ def test_mxfp4_scale_bytes_of_the_whole_range(dtype):
         got = got.cpu()[:, 0]
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_fp8_products_are_rounded_to_f32_and_then_to_the_type(dtype):
+    """Scales whose products with a code lie beside a tie of the type: the two roundings that are documented."""
+    g = torch.Generator().manual_seed(1)
+    D = 128
+    cache = kvcache.make_kv_cache(16, 64, 1, D, values=False)
+    bits = 8 if dtype == torch.bfloat16 else 11
+    tie = torch.randint(2 ** bits, 2 ** (bits + 1), (1024,), generator=g) | 1           # bits + 1 bits, the last one set
+    code = torch.randint(1, 16, (1024, D), generator=g).float() / 8
+    scale = (tie.double() * 2.0 ** -bits / code[:, 0].double()).float()                 # code * scale next to the tie
+    scale = torch.where(torch.arange(1024) % 3 == 0, torch.nextafter(scale, torch.tensor(2.0)), scale)
+    cache[0].view(torch.uint8).copy_(code.to(torch.float8_e4m3fn).view(torch.uint8).reshape(16, 64, 1, D))
+    cache[2].copy_(scale.reshape(16, 64, 1, 1))
+    got, _ = _read_all((cache[0], None, cache[2], None), 1024, dtype)
+    f32 = code * scale[:, None]
+    assert torch.equal(got.cpu()[:, 0], f32.to(dtype))
+    once = code.double() * scale.double()[:, None]                                      # at most half a step of the type and of f32
+    assert ((got.cpu()[:, 0].double() - once).abs() <= once * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -24) + 2.0 ** -24)).all()
 
 
 def _written(k, slots, pages, page):
