@@ -593,11 +593,13 @@ emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const voi
   const emu_status st = check_kv(format, heads, head_size);
   if (st != EMU_OK) return st;
   if (total == 0 || sequences == 0) return ok();
+  // a cache without pages has no memory: there the output tells whether it holds values
+  const bool values = v_cache || (num_pages == 0 && v_out);
   if (!cu_lens || !k_out || (v_cache && !v_out) || (table_cols > 0 && !block_table) ||
       (num_pages > 0 && (!k_cache || !k_scale || (v_cache && !v_scale))))
     return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
   if (table_stride < table_cols && sequences > 1) return fail(EMU_ERR_INVALID_ARGUMENT, "table_stride (%lld) must be at least table_cols (%lld)", (long long)table_stride, (long long)table_cols);
-  if (k_token_stride < heads * head_size || (v_cache && v_token_stride < heads * head_size))
+  if (k_token_stride < heads * head_size || (values && v_token_stride < heads * head_size))
     return fail(EMU_ERR_INVALID_ARGUMENT, "output rows must hold heads * head_size elements");
   const int esz = out_dtype == EMU_DTYPE_F32 ? 4 : 2;
   if (!aligned(block_table, 4) || !aligned(cu_lens, 4) || !aligned(k_out, esz) || !aligned(v_out, esz))
@@ -606,7 +608,7 @@ emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const voi
     return fail(EMU_ERR_INVALID_ARGUMENT, "caches must be 16-byte aligned, f32 scales 4-byte");
   if (total > 0x7FFFFFFFll) return fail(EMU_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   const emu::KvReadArgs a{{k_cache, v_cache}, {k_scale, v_scale}, num_pages, page_size, heads, head_size, block_table, sequences,
-                          table_cols, table_stride, cu_lens, total, {k_out, v_cache ? v_out : nullptr},
+                          table_cols, table_stride, cu_lens, total, {k_out, values ? v_out : nullptr},
                           {k_token_stride, v_token_stride}, out_dtype, format};
   return cuda_status(emu::launch_kv_read(a, static_cast<cudaStream_t>(stream)), "emu_kv_read launch");
 }

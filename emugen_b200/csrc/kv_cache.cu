@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
   }
   __syncthreads();
   const int D = (int)a.D, H = (int)a.H, G = (D + 127) / 128;
-  const int64_t per_tensor = (int64_t)H * (D / 8), per_row = per_tensor * (a.q[1] ? 2 : 1);
+  const int64_t per_tensor = (int64_t)H * (D / 8), per_row = per_tensor * (a.out[1] ? 2 : 1);
   // short rows: the CTA's threads share out the rows too
   const int side = per_row >= 256 ? 1 : 256 / (int)per_row;
   const int first = side == 1 ? 0 : threadIdx.x / (int)per_row;

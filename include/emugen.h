@@ -441,7 +441,8 @@ EMU_API emu_status emu_kv_write(const void* k, const void* v, int32_t dtype, int
  * block_table[b * table_stride + i / page_size].  cu_lens: sequences + 1 non-decreasing values, cu_lens[0] = 0.
  * Outputs [total][heads][head_size], rows k_token_stride / v_token_stride elements apart: code * scale, rounded to f32
  * and then to out_dtype.  Rows of a page that does not exist (negative, not below num_pages, past table_cols) are zeros; rows
- * that no sequence has are left as they were.  v_cache may be NULL.  No reference counterpart.
+ * that no sequence has are left as they were.  v_cache may be NULL (v_out is left alone then, unless num_pages is 0, where
+ * both outputs that are given get zeros).  No reference counterpart.
  */
 EMU_API emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const void* k_scale,
                                const void* v_scale, int32_t format, int64_t num_pages, int64_t page_size, int64_t heads,

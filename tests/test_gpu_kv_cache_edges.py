@@ -1,5 +1,5 @@
 """The quantised cache at its edges: scale bytes at the ends of their range, products beside ties, padding past the
-cache and repeated slots in long calls."""
+cache and repeated slots in long calls, a cache without pages."""
 import pytest
 import torch
 
@@ -106,3 +106,15 @@ def test_padding_and_repeated_slots_cost_no_more_than_rows(slot):
     one = torch.full((T,), slot, dtype=torch.int64, device="cuda")
     write = lambda s: kvcache.write_kv_cache(k, None, s, cache[0], None, cache[2], None)
     assert _us(lambda: write(one)) <= 2 * _us(lambda: write(many))
+
+
+def test_a_cache_without_pages_reads_as_zeros():
+    for fmt in ("fp8", "mxfp4"):
+        cache = [t[:0] for t in kvcache.make_kv_cache(1, 16, 2, 64, fmt)]
+        table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, 3, 8], dtype=torch.int32, device="cuda")
+        out = [torch.full((9, 2, 64), 5.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        kvcache.read_kv_cache(*cache, table, cu, out=out)
+        for o in out:
+            assert (o[:8] == 0).all() and (o[8] == 5).all()
+        kvcache.write_kv_cache(*[torch.ones(3, 2, 64, dtype=torch.bfloat16, device="cuda")] * 2, torch.arange(3, device="cuda"), *cache)
