@@ -233,16 +233,17 @@ class _Quantised:
         self.end = self.scale + _up(4 * self.ld_scale * (_blocks(rows) if tile else _blocks(cols)), 256)
 
 
-def _quant_into(x: torch.Tensor, block: int, q: _Quantised, base: int, t, base_t: int, stream: int) -> None:
-    """quant_fp8 of a matrix into q at address `base` and, unless t is None, of its transpose into t at base_t."""
+def _quant_into(x: torch.Tensor, block: int, q, base: int, t, base_t: int, stream: int) -> None:
+    """quant_fp8 of a matrix into q at address `base` and of its transpose into t at base_t; either may be None."""
+    rows, cols = x.shape
     ldx, inner = x.stride()
-    if inner != 1 and q.cols > 1 or ldx < q.cols and q.rows > 1:
+    if inner != 1 and cols > 1 or ldx < cols and rows > 1:
         x = x.contiguous()
-        ldx = q.cols
+        ldx = cols
     status = _lib.load().emu_quant_fp8(
-        x.data_ptr(), _DTYPE[x.dtype], q.rows, q.cols, ldx if q.rows > 1 else q.cols, _lib.EMU_FP8_E4M3, block,
-        base + q.codes, q.ld, base + q.scale, q.ld_scale, *((base_t + t.codes, t.ld, base_t + t.scale, t.ld_scale) if t else
-                                                            (None, 0, None, 0)), stream)
+        x.data_ptr(), _DTYPE[x.dtype], rows, cols, ldx if rows > 1 else cols, _lib.EMU_FP8_E4M3, block,
+        *((base + q.codes, q.ld, base + q.scale, q.ld_scale) if q else (None, 0, None, 0)),
+        *((base_t + t.codes, t.ld, base_t + t.scale, t.ld_scale) if t else (None, 0, None, 0)), stream)
     if status:
         _lib._check(status)
 
@@ -283,8 +284,9 @@ def _linear_backward(dy: torch.Tensor, xt, wt, K: int, need_x: bool, need_w: boo
     if not (M and N and K):
         return (torch.zeros((M, K), dtype=dtype, device=dev) if need_x else None,
                 torch.zeros((N, K), dtype=dtype, device=dev) if need_w else None)
-    g = _Quantised(M, N, False)
-    gt = _Quantised(N, M, False, g.end) if need_w else None
+    # dx takes dy's codes along its rows, dw those along its columns
+    g = _Quantised(M, N, False) if need_x else None
+    gt = _Quantised(N, M, False, g.end if g else 0) if need_w else None
     with _on(dev.index):
         now = torch.empty((gt or g).end, dtype=torch.uint8, device=dev)
         base, stream = now.data_ptr(), _raw_stream(dev.index)
