@@ -65,7 +65,8 @@ def quant_fp8(x: torch.Tensor, *, block: str = "row", dtype: torch.dtype = torch
     contiguous).  block "row": scale [M, ceil(K / 128)] and scale_t [K, ceil(M / 128)], stored block after
     block (strides 1, rows rounded up to 4); block "tile": scale [ceil(M / 128), ceil(K / 128)] and its
     transpose.  scale = max(max |x| / F, 2^-126) in f32 over the block's finite elements (F: the type's
-    largest value), code = the nearest value to x / scale, ties to even; NaN and infinities become NaN."""
+    largest value), code = the nearest value to x / scale, ties to even; NaN and infinities become NaN.
+    A CPU tensor is quantised on the current GPU, where its codes and scales stay.  Not differentiable."""
     if dtype not in _FP8:
         raise RuntimeError(f"quant_fp8 dtype must be torch.float8_e4m3fn or torch.float8_e5m2, got {dtype}")
     if block not in _BLOCKS:

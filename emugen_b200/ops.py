@@ -92,13 +92,22 @@ def quant_fp8(x: torch.Tensor, block: str = "row", dtype: torch.dtype = torch.fl
     return fp8.quant_fp8(x, block=block, dtype=dtype)
 
 
+def _device(*tensors) -> torch.device:
+    """The device that _lib._device_for picks, without a GPU: the first CUDA tensor's, else the current one."""
+    for t in tensors:
+        if t.device.type == "cuda":
+            return t.device
+    return torch.device("cuda")
+
+
 @quant_fp8.register_fake
 def _quant_fp8_fake(x, block="row", dtype=torch.float8_e4m3fn):
+    dev = _device(x)
     M, K = x.numel() // x.shape[-1] if x.shape[-1] else x.shape[:-1].numel(), x.shape[-1]
     kb = fp8._blocks(K)
-    s = (fp8._row_scales(M, kb, x.device) if block == "row"
-         else torch.empty((fp8._blocks(M), kb), dtype=torch.float32, device=x.device))
-    return fp8._codes(M, K, dtype, x.device), s
+    s = (fp8._row_scales(M, kb, dev) if block == "row"
+         else torch.empty((fp8._blocks(M), kb), dtype=torch.float32, device=dev))
+    return fp8._codes(M, K, dtype, dev), s
 
 
 @torch.library.custom_op("emugen::gemm_fp8", mutates_args=())
@@ -112,7 +121,9 @@ def gemm_fp8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: t
 def _gemm_fp8_fake(a, b, scale_a, scale_b, out_dtype=torch.bfloat16):
     torch._check(a.dim() == 2 and b.dim() == 2, lambda: "a, b, scale_a and scale_b must be 2D")
     torch._check(a.shape[1] == b.shape[1], lambda: "K mismatch between a and b")
-    return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+    on_cpu = not any(t.device.type == "cuda" for t in (a, b, scale_a, scale_b))
+    dev = a.device if on_cpu else _device(a, b, scale_a, scale_b)
+    return torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype, device=dev)
 
 
 @torch.library.custom_op("emugen::write_kv_cache", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
