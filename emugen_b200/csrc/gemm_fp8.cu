@@ -16,7 +16,7 @@
 //               of the block's scales into a second ring
 //   warps 1, 6  MMA issuers in turn (warp 1 owns the TMEM)
 //   warps 2-5   epilogue: a thread owns one row of B (a TMEM lane) and BN accumulators
-// Bound: reading B.  B200: 1 x 128256 x 4096 83 us (96% of the measured copy rate), 32 x 14336 x 4096 16.6 us (floor 9.2;
+// Bound: reading B.  B200: 1 x 128256 x 4096 83 us (96% of the measured copy rate), 32 x 14336 x 4096 16.9 us (floor 9.2;
 // about 5 us are the launch, the pipeline's fill and the parts' exchange: 1 x 512 x 4096 takes 5.4).
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -112,11 +112,34 @@ __device__ __noinline__ float4 add_any4(float4 x, float first, float4 second, fl
   return make_float4(__fmaf_rn(__fmul_rn(x.x, a.first), a.second, acc.x), __fmaf_rn(__fmul_rn(x.y, b.first), b.second, acc.y),
                      __fmaf_rn(__fmul_rn(x.z, c.first), c.second, acc.z), __fmaf_rn(__fmul_rn(x.w, d.first), d.second, acc.w));
 }
+// The whole warp.  Sums of 0 are 0 (or NaN) in any order, so rows of zeros beside columns of any scale stay quick: 4096^3
+// with such rows and columns of scales above 1 in every warp 194 us; 1400 where every sum has to be looked at.
 template <int N> __device__ __forceinline__ void add_any(const uint32_t (&x)[N], float first, const float* second, float* acc) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) bits |= x[j];
+  const bool easy = __all_sync(0xFFFFFFFFu, in_range(first) || (bits & 0x7FFFFFFFu) == 0);
+  // the test once for the pairs (194 against 431 us), for every four in the skinny kernel, whose usual path then is as
+  // quick as without (64 x 4096 x 4096: 12.8 against 13.1 us)
+  constexpr bool ONCE = N > 16;
+  if (ONCE && easy) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = __fmaf_rn(__fmul_rn(__uint_as_float(x[j]), first), second[j], acc[j]);
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < N; j += 4) {
-    const float4 r = add_any4(make_float4(__uint_as_float(x[j]), __uint_as_float(x[j + 1]), __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
-                              first, *reinterpret_cast<const float4*>(second + j), make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+    const float4 s = *reinterpret_cast<const float4*>(second + j);
+    const float4 v = make_float4(__uint_as_float(x[j]), __uint_as_float(x[j + 1]), __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]));
+    float4 r = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    if (!ONCE && easy) {
+      r.x = __fmaf_rn(__fmul_rn(v.x, first), s.x, r.x);
+      r.y = __fmaf_rn(__fmul_rn(v.y, first), s.y, r.y);
+      r.z = __fmaf_rn(__fmul_rn(v.z, first), s.z, r.z);
+      r.w = __fmaf_rn(__fmul_rn(v.w, first), s.w, r.w);
+    } else {
+      r = add_any4(v, first, s, r);
+    }
     acc[j] = r.x, acc[j + 1] = r.y, acc[j + 2] = r.z, acc[j + 3] = r.w;
   }
 }
@@ -377,10 +400,10 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_fp8_skinny_kernel(const __gri
 //               B_ROWS = true: the block sum is multiplied by the row's scale, then by the column's.
 // Bound: the epilogue's turn-around.  A block's MMAs take 512 clocks; its sums reach the epilogue about 450 clocks
 // after that, take 270 to load (TMEM's rate) and 400 to add up, so with two accumulators a block comes every
-// 850 clocks or so.  B200: 4096^3 74 us (1.86 PFLOP/s; 121 with column scales), 8192^3 503 us (2.19 PFLOP/s, the clock
-// already lowered by the power limit: MMAs and loads alone take 366); without the test of the scales' range 73, 119 and
-// 495.  Other splits were no faster: 128-column
-// MMAs with four accumulators 72, sixteen epilogue warps of 64 columns 95, one issuer 89 us at 4096^3.
+// 850 clocks or so.  B200: 4096^3 74 us (1.86 PFLOP/s; 121 with column scales), 8192^3 500 us (2.20 PFLOP/s, the clock
+// already lowered by the power limit: MMAs and loads alone take 366); without the test of the scales' range 73, 120
+// and 493.  Other splits were no faster: 128-column MMAs with four accumulators 72, sixteen epilogue warps of 64
+// columns 95, one issuer 89 us at 4096^3.
 constexpr int P_STAGE = 2 * 128 * BK;            // one CTA's 128 rows of A and of B
 constexpr int P_NSTAGE = 5;                      // at least 4: see the issuers' waits
 constexpr int P_NSCALE = 8;
@@ -595,6 +618,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
         const bool more = kb + 1 < p.kb_count;
         next_scales(kb);
         const float f1 = factor();                                   // the next block's
+        const bool fine1 = fine(f1);
         if (B_ROWS && !warp_wait_or_record(&s_full[sc.at], sc.parity, p.wait_limit, 16)) { ok = false; break; }
         const float* slot = scales + sc.at * (P_SCALE / 4) + half * 128;
         st.next();
@@ -611,8 +635,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_fp8_pair_kernel(const __gri
             if (lane == 0) ptx::mbar_arrive_cluster(empty_bar + ac / 32);   // 8 bytes per 256 columns
             ac ^= 256;
             if (more) {
-              // (one vote for both: a second one for the scales cost 72 -> 75 us at 4096^3)
-              next = __all_sync(0xFFFFFFFFu, ptx::mbar_test_wait(&done[st.at], st.parity) && fine(f1));
+              // (one vote for both, without a branch: a second vote for the scales cost 72 -> 75 us at 4096^3)
+              next = __all_sync(0xFFFFFFFFu, (int)ptx::mbar_test_wait(&done[st.at], st.parity) & (int)fine1);
               if (next) {
                 ptx::tc_fence_after();
                 ptx::tmem_ld_regs(lane_base + ac, v[0]);
@@ -894,10 +918,11 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& g, cudaStream_t stream) {
   p.wait_limit = current_wait_limit();
   p.hold_first_ready = current_hold_first_ready();
   // Up to 64 rows of A are one column tile of the skinny kernel: each byte of B is read once.  Beyond, the two
-  // kernels' times by what they do, in us (fitted over 65 .. 4096 rows, 512 .. 14336 columns and K; mostly within
-  // 15%, at worst 25%): the skinny one 6.5 + its tiles' blocks of K / 300, the pairs 3.5 + for each wave of tiles
-  // 0.53 (0.8 with a scale per row of B) a block + 2.3 to store.  E.g. 128 x 4096 x 4096: 14.1 against 22.3;
-  // 128 x 14336 x 4096: 28.1 against 23.5; 1024 x 4096 x 4096: 53 against 24.
+  // kernels' times by what they do, in us: the skinny one 6.5 + its tiles' blocks of K / 300, the pairs 3.5 + for each
+  // wave of tiles 0.53 (0.8 with a scale per row of B) a block + 2.3 to store.  A rough rule: over 124 sizes of 65 .. 4096
+  // rows the median error is 14% (skinny; at worst 46%, it knows neither the split nor its own waves) and 9% (pairs;
+  // 27%), and 14 times the kernel taken is over 5% slower than the other, at worst 1.45 times.  E.g. 128 x 4096 x 4096:
+  // 14.3 against 21.1; 128 x 14336 x 4096: 26.6 against 23.2; 1024 x 4096 x 4096: 48 against 23.4.
   const int64_t kb = p.kb_count;
   const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256), pairs = std::max(1, sms / 2);
   const double t_pair = 3.5 + (double)((tiles + pairs - 1) / pairs) * ((g.b_rows ? 0.8 : 0.53) * kb + 2.3);

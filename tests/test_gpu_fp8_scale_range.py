@@ -118,3 +118,34 @@ def test_cta_pairs_over_many_blocks_exact(M, N, K, rows):
     ref = full(a, sa) @ full(b, sb if rows else sb.repeat_interleave(128, 0)[:N]).t()
     for _ in range(3):
         assert torch.equal(fp8.gemm_fp8(a, b, sa, sb, out_dtype=torch.float32).double(), ref)
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES + [(700, 2300, 4000)])
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("kind", ["zeros", "zeros and largest", "small"])
+def test_scales_that_change_along_k(M, N, K, rows, kind):
+    """Blocks of zeros (the quantiser's smallest scale, or the largest one) among others in every order, the first block
+    of a row among them, and rows whose blocks are all below the range: exact."""
+    g = torch.Generator().manual_seed(M + N)
+    kb, nb = -(-K // 128), N if rows else -(-N // 128)
+    a, b = _codes(M, K, E4, 1.0 if kind != "small" else 128.0, 1), _codes(N, K, E4, 1.0 if kind != "small" else 128.0, 2)
+    ea, eb = torch.randint(-1, 2, (M, kb), generator=g), torch.randint(-1, 2, (nb, kb), generator=g)
+    if kind == "small":
+        ea = ea * 0 - 126 + 2 * torch.randint(0, 2, (M, kb), generator=g)
+        eb = eb * 0 - 18
+    else:
+        dead = torch.rand(M, kb, generator=g) < torch.rand(M, 1, generator=g)       # some rows all dead, some none
+        dead[::7, 0] = True
+        ea[dead] = -126
+        if kind != "zeros":
+            ea[dead & (torch.rand(M, kb, generator=g) < 0.1)] = 127
+        a = (a.float() * (~dead).repeat_interleave(128, 1)[:, :K].cuda()).to(E4)
+        dead = torch.rand(nb, kb, generator=g) < 0.05
+        eb[dead] = -126
+        d = dead if rows else dead.repeat_interleave(128, 0)[:N]
+        b = (b.float() * (~d).repeat_interleave(128, 1)[:, :K].cuda()).to(E4)
+    sa, sb = (torch.ldexp(torch.ones(e.shape), e).cuda() for e in (ea, eb))
+    out = fp8.gemm_fp8(a, b, sa, sb, out_dtype=torch.float32)
+    full = lambda q, s: q.double() * s.double().repeat_interleave(128, 1)[:, :K]
+    ref = full(a, sa) @ full(b, sb if rows else sb.repeat_interleave(128, 0)[:N]).t()
+    assert torch.equal(out, ref.float())
