@@ -4,9 +4,9 @@
 //   EMU_KV_FP8    E4M3 codes, one f32 scale per 128 elements of a row (the quantiser of quant_fp8.cu)
 //   EMU_KV_MXFP4  e2m1 codes, one power-of-two scale byte per 32 elements (the quantiser of quant.cu)
 //
-// Measured on B200 with 8 heads of 128 (bf16): reading 131072 rows back 137 us from fp8 (814 MB: 91% of the
-// measured copy rate) and 119 us from MXFP4 (679 MB: 87%); writing 65536 tokens 94 us (407 MB: floor 62), where
-// the quantiser's arithmetic bounds it; 32 tokens 3.5 us, the launch.
+// Measured on B200 with 8 heads of 128 (bf16): reading 131072 rows back 135 us from fp8 (814 MB: 92% of the
+// measured copy rate) and 118 us from MXFP4 (679 MB: 88%); writing 65536 tokens 95 us (407 MB: floor 62), where
+// the quantiser's arithmetic bounds it; 32 tokens 3.6 us, where a launch is about 1.7: the rest is find_overwritten.
 #include <cuda_fp4.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -281,7 +281,7 @@ cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t stream) {
   const int sms = sm_count();
   // A token to a CTA of 256 threads while four CTAs per SM take them all; longer calls one CTA of 1024 threads
   // per SM, so that fewer CTAs read all later slots (8 heads of 128, fp8: 256 tokens 4.2 against 4.9 us,
-  // 2048 tokens 9.0 against 6.5, 65536 tokens 136 against 94)
+  // 2048 tokens 9.0 against 6.9, 65536 tokens 136 against 95)
   const bool wide = a.T > 4 * (int64_t)sms;
   const int64_t ctas = wide ? sms : a.T;
   const int per_cta = (int)std::min<int64_t>(MAX_TOKENS, (a.T + ctas - 1) / ctas);
@@ -309,7 +309,8 @@ cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream) {
   const int sms = sm_count();
-  // up to 32 rows per CTA, fewer while the SMs (8 CTAs of 256 threads each) are not filled twice
+  // up to 32 rows per CTA, fewer while there are not 16 CTAs for each SM, which holds four at a time (56 to 61 registers
+  // for 16-bit outputs)
   const int per_cta = (int)std::min<int64_t>(READ_ROWS, (a.total + 16 * sms - 1) / (16 * sms));
   const unsigned grid = (unsigned)((a.total + per_cta - 1) / per_cta);
   const int esz = a.out_dtype == EMU_DTYPE_F32 ? 4 : 2;

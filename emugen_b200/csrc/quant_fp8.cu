@@ -5,8 +5,10 @@
 //   code  = nearest 8-bit value to x / scale, ties to even (fp8.cuh); NaN for NaN and infinities.
 //
 // Each input element is read once and kept in registers between the maximum and the rounding.  What bounds
-// the kernels is their arithmetic (ALU pipe 58% busy) before the memory: 8192 x 8192 bf16 on B200, rows 48 us
-// (201 MB: floor 31), rows and columns 88 us (272 MB: floor 42), tiles 37 us, tiles with the transpose 54 us.
+// the kernels is their arithmetic (ALU pipe 58% busy) before the memory: 8192 x 8192 bf16 on B200, rows 45 us
+// (203 MB: floor 31), rows and columns 86 us (272 MB: floor 42), tiles 35 us, tiles with the transpose 51 us; f32, two
+// products and conversions an element, rows 72 us (338 MB: floor 52), rows and columns 116 us (407 MB: floor 62), tiles
+// 58 us, tiles with the transpose 81 us.
 // A division or a border test for each element took rows and columns to 255 us (fp8.cuh).
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 0)
 // columns 8 * (tid % 16) ..).  Row maxima meet in 16 lanes, column maxima in shared memory.  The
 // transposed codes go through shared memory so that both outputs are written in 128-byte runs.
 // TILE: one scale for the tile, its codes turned as bytes; otherwise one per row (q) and one per column (qt),
-// each element rounded twice (88 us at 8192 x 8192 bf16; two passes over the input would read 134 MB more).
+// each element rounded twice (86 us at 8192 x 8192 bf16; two passes over the input would read 134 MB more).
 template <typename T, int TYPE, bool VEC, bool TILE>
 __global__ void __launch_bounds__(256, TILE ? 0 : sizeof(T) == 2 ? 3 : 2)
     quant_fp8_tile_kernel(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
