@@ -78,9 +78,10 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, float v, int mod
 //   * times a smaller scale it is off by at most 2^-150, which a second scale of at most 1 leaves below f32's last place
 //     (blocks of zeros have the quantiser's smallest scale, 2^-126, and are in this form as a rule);
 //   * where sa * sb is a normal number, the sum may be multiplied by that product;
-//   * where it is smaller, by the larger scale first: that is below 2^23 (the other is at least 2^-149) and, unless
-//     the result is below 2^-150 anyhow, at least 2^-94 (a scale of 0 goes first instead: the other may be anything);
-//   * where it is larger, by the smaller scale first: either that is below 1, or an overflow is the result's own.
+//   * where it is smaller, by the larger scale first: that is below 2^23 (the other is at least 2^-149), and where it takes
+//     the sum below the normal range, both are below 2^-94 and the result below 2^-150 (a scale of 0 goes first instead:
+//     the other may be anything);
+//   * where it is larger, by the smaller scale first: that is at least 1, so an overflow is the result's own.
 // Which of these an element takes depends on its own two scales and not on what else a warp adds up (but for the last
 // place of results below f32's normal range).
 constexpr float SCALE_LOW = 0x1p-94f, SCALE_HIGH = 0x1p89f;
