@@ -11,15 +11,17 @@ Python modules mirror the reference interfaces that call it:
 and, beyond the reference, block-scaled 8-bit operators:
 
   emugen_b200.fp8             quantiser, matrix product, linear layer with its backward pass
-  emugen_b200.kvcache         quantised key/value cache (8 or 4 bits): write, read back
+  emugen_b200.kvcache         quantised key/value cache (8 or 4 bits): write, read back, attention of one token over it
+  emugen_b200.attention       norms of queries and keys with the position rotation, attention over packed sequences
 """
 from . import _lib
 from ._lib import EmuError, gemm, nvfp4_global_scales, quant_mxfp4, quant_nvfp4
+from .attention import packed_attention, qk_norm_rope
 from .fp8 import gemm_fp8, linear_fp8, quant_fp8
-from .kvcache import make_kv_cache, read_kv_cache, write_kv_cache
+from .kvcache import attend_kv_cache, make_kv_cache, read_kv_cache, write_kv_cache
 
 __all__ = ["EmuError", "gemm", "nvfp4_global_scales", "quant_mxfp4", "quant_nvfp4", "quant_fp8", "gemm_fp8", "linear_fp8",
-           "make_kv_cache", "write_kv_cache", "read_kv_cache", "load_library"]
+           "make_kv_cache", "write_kv_cache", "read_kv_cache", "attend_kv_cache", "qk_norm_rope", "packed_attention", "load_library"]
 
 
 def load_library():

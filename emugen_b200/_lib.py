@@ -31,7 +31,9 @@ SYMBOLS = ("emu_abi_version", "emu_last_error", "emu_status_string", "emu_gemm",
            "emu_gemm_ws", "emu_gemm_tc_path_offset", "emu_gemm_static", "emu_nvfp4_global_scales", "emu_nvfp4_amax",
            "emu_nvfp4_scales_from_amax", "emu_quant_nvfp4", "emu_quant_mxfp4",
            "emu_gemm_model", "emu_gemm_sweep", "emu_gemm_compare", "emu_gemm_batch", "emu_compare", "emu_dequant_fp4", "emu_device_status",
-           "emu_set_wait_limit", "emu_test_hold_first_ready", "emu_quant_fp8", "emu_gemm_fp8", "emu_kv_write", "emu_kv_read")
+           "emu_set_wait_limit", "emu_test_hold_first_ready", "emu_quant_fp8", "emu_gemm_fp8", "emu_kv_write", "emu_kv_read",
+           "emu_qk_norm_rope", "emu_qk_norm_rope_workspace_size", "emu_qk_norm_rope_backward", "emu_attention",
+           "emu_attention_backward_workspace_size", "emu_attention_backward", "emu_kv_attend_workspace_size", "emu_kv_attend")
 STATIC_SCRATCH_BYTES = 64 << 20   # EMU_STATIC_SCRATCH_BYTES
 
 
@@ -39,6 +41,26 @@ class EmuGemmParams(ctypes.Structure):
     _fields_ = [("format", ctypes.c_int32), ("group_size", ctypes.c_int32), ("w_reduce", ctypes.c_int32),
                 ("stage3_rounding", ctypes.c_int32), ("stage4_rounding", ctypes.c_int32),
                 ("out_mode", ctypes.c_int32)]
+
+
+class EmuNormRopeArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("cos", ctypes.c_void_p),
+                ("sin", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("tokens", ctypes.c_int64),
+                ("table_rows", ctypes.c_int64), ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32),
+                ("head_size", ctypes.c_int32), ("half", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class EmuAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("cu_q", ctypes.c_void_p),
+                ("cu_k", ctypes.c_void_p), ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64),
+                ("sequences", ctypes.c_int64), ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32),
+                ("head_size", ctypes.c_int32), ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
 
 
 class EmuCompareStats(ctypes.Structure):
@@ -143,6 +165,24 @@ def load() -> ctypes.CDLL:
         L.emu_kv_read.restype = i32
         L.emu_kv_read.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp, i64, i64, i64, vp, i64, i32, vp, vp,
                                   i64, i64, vp]
+        norm_rope, attention, size = ctypes.POINTER(EmuNormRopeArgs), ctypes.POINTER(EmuAttentionArgs), ctypes.c_size_t
+        L.emu_qk_norm_rope.restype = i32
+        L.emu_qk_norm_rope.argtypes = [norm_rope, vp, vp, vp]
+        L.emu_qk_norm_rope_workspace_size.restype = size
+        L.emu_qk_norm_rope_workspace_size.argtypes = [i32]
+        L.emu_qk_norm_rope_backward.restype = i32
+        L.emu_qk_norm_rope_backward.argtypes = [norm_rope, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, size, vp]
+        L.emu_attention.restype = i32
+        L.emu_attention.argtypes = [attention, vp, vp, vp]
+        L.emu_attention_backward_workspace_size.restype = size
+        L.emu_attention_backward_workspace_size.argtypes = [attention]
+        L.emu_attention_backward.restype = i32
+        L.emu_attention_backward.argtypes = [attention, vp, vp, vp, i64, i64, vp, vp, vp, vp, size, vp]
+        L.emu_kv_attend_workspace_size.restype = size
+        L.emu_kv_attend_workspace_size.argtypes = [i64, i32, i32, i32]
+        L.emu_kv_attend.restype = i32
+        L.emu_kv_attend.argtypes = [vp, i64, i64, i32, i64, i32, i32, i32, ctypes.c_float, i32, vp, vp, vp, vp, i64, i64,
+                                    vp, i64, i64, vp, vp, vp, vp, size, vp]
         v = L.emu_abi_version()
         if v != ABI_VERSION:
             raise ImportError(f"libemugen ABI version {v}, expected {ABI_VERSION}: rebuild it")

@@ -1,0 +1,168 @@
+// What the kernels of attention over packed sequences share: which keys a query sees, and the formulas row by row.
+//
+// Query i of a sequence with nq queries and nk keys sees keys 0 .. nk - 1, or with the causal mask those up to
+// i + nk - nq (the last query stands on the last key).  With s_ij = scale q_i . k_j over the keys seen:
+//   lse_i = log sum_j exp(s_ij),  p_ij = exp(s_ij - lse_i),  o_i = sum_j p_ij v_j     (no key: o = 0, lse = -inf)
+// and for dO:  dp_ij = dO_i . v_j,  delta_i = dO_i . o_i,  ds_ij = p_ij (dp_ij - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dO_i
+// (dk and dv over the query heads that share the key head).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace emu {
+namespace attn {
+
+// Rows [begin, end) of sequence b, inside the tensor whatever the cumulative lengths say.
+struct Rows {
+  int64_t begin, end;
+  __device__ __forceinline__ int64_t count() const { return end - begin; }
+};
+__device__ __forceinline__ Rows rows_of(const int32_t* cu, int64_t b, int64_t total) {
+  Rows r;
+  r.begin = min(max((int64_t)cu[b], (int64_t)0), total);
+  r.end = min(max((int64_t)cu[b + 1], r.begin), total);
+  return r;
+}
+// The sequence that holds row t, or B for a row behind the last one.
+__device__ __forceinline__ int64_t sequence_of(const int32_t* cu, int64_t B, int64_t t) {
+  int64_t lo = 0, hi = B;
+  while (lo < hi) {
+    const int64_t m = (lo + hi) / 2;
+    if ((int64_t)cu[m + 1] > t) hi = m;
+    else lo = m + 1;
+  }
+  return lo;
+}
+
+template <typename T> __device__ __forceinline__ float widen(T v);
+template <> __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+
+// One row at a time, a warp to a row: lane l holds elements l, l + 32, l + 64 and l + 96 of it.  Nothing that the mask
+// hides is read, so that infinities and NaN there reach no result.
+struct Lanes {
+  float v[4];
+};
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+template <typename T> __device__ __forceinline__ Lanes load_row(const T* p, int D) {
+  Lanes r;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = lane + 32 * i < D ? widen<T>(p[lane + 32 * i]) : 0.0f;
+  return r;
+}
+__device__ __forceinline__ float dot(const Lanes& a, const Lanes& b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = __fmaf_rn(a.v[i], b.v[i], s);
+  return warp_sum(s);
+}
+template <typename T> __device__ __forceinline__ void store_row(T* p, int D, const Lanes& r, float f) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < D) p[lane + 32 * i] = narrow<T>(__fmul_rn(r.v[i], f));
+}
+
+// The keys that query t of sequence b sees: the first `n` of the sequence's.
+struct Seen {
+  Rows k;
+  int64_t n;
+};
+__device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t) {
+  const Rows q = rows_of(a.cu_q, b, a.Tq);
+  Seen s;
+  s.k = rows_of(a.cu_k, b, a.Tk);
+  s.n = s.k.count();
+  if (a.causal) s.n = max((int64_t)0, min(s.n, t - q.begin + 1 + s.k.count() - q.count()));
+  return s;
+}
+
+// o_t and lse_t of one head.
+template <typename T> __device__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h) {
+  const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
+  const int kh = h / (a.Hq / a.Hk);
+  const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];
+  const T* v = static_cast<const T*>(a.v) + kh * a.v_stride[1];
+  Seen s{{0, 0}, 0};
+  if (b < a.B) s = seen_by(a, b, t);
+  const Lanes x = load_row(q, a.D);
+  Lanes o{};
+  float m = -INFINITY, l = 0.0f;
+  for (int64_t j = s.k.begin; j < s.k.begin + s.n; ++j) {
+    const float z = __fmul_rn(dot(x, load_row(k + j * a.k_stride[0], a.D)), a.scale);
+    const float top = fmaxf(m, z);
+    const float shift = top == -INFINITY ? 0.0f : top;
+    const float old = expf(m - shift), p = expf(z - shift);
+    const Lanes y = load_row(v + j * a.v_stride[0], a.D);
+    l = __fmaf_rn(l, old, p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(p, y.v[i], __fmul_rn(o.v[i], old));
+    m = top;
+  }
+  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, a.D, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
+  if ((threadIdx.x & 31) == 0 && a.lse) a.lse[(int64_t)h * a.Tq + t] = l > 0.0f ? m + logf(l) : l == 0.0f ? -INFINITY : l;
+}
+
+// dq_t of one head.
+template <typename T> __device__ void row_dq(const AttnArgs& a, const float* delta, int64_t b, int64_t t, int h) {
+  const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
+  const T* g = static_cast<const T*>(a.dout) + t * a.dout_stride[0] + h * a.dout_stride[1];
+  const int kh = h / (a.Hq / a.Hk);
+  const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];
+  const T* v = static_cast<const T*>(a.v) + kh * a.v_stride[1];
+  Seen s{{0, 0}, 0};
+  if (b < a.B) s = seen_by(a, b, t);
+  const Lanes x = load_row(q, a.D), y = load_row(g, a.D);
+  const float lse = a.lse[(int64_t)h * a.Tq + t], dl = delta[(int64_t)h * a.Tq + t];
+  Lanes o{};
+  for (int64_t j = s.k.begin; j < s.k.begin + s.n; ++j) {
+    const Lanes kj = load_row(k + j * a.k_stride[0], a.D);
+    const float p = expf(__fmaf_rn(dot(x, kj), a.scale, -lse));
+    const float ds = __fmul_rn(p, dot(y, load_row(v + j * a.v_stride[0], a.D)) - dl);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(ds, kj.v[i], o.v[i]);
+  }
+  store_row(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D, a.D, o, a.scale);
+}
+
+// dk_t and dv_t of one key head (t: a row of the keys; either may be left out).
+template <typename T> __device__ void row_dkdv(const AttnArgs& a, const float* delta, int64_t b, int64_t t, int kh) {
+  Lanes ok{}, ov{};
+  if (b < a.B) {
+    const Rows q = rows_of(a.cu_q, b, a.Tq), kr = rows_of(a.cu_k, b, a.Tk);
+    const Lanes kj = load_row(static_cast<const T*>(a.k) + t * a.k_stride[0] + kh * a.k_stride[1], a.D);
+    const Lanes vj = load_row(static_cast<const T*>(a.v) + t * a.v_stride[0] + kh * a.v_stride[1], a.D);
+    const int64_t first = a.causal ? max((int64_t)0, (t - kr.begin) - (kr.count() - q.count())) : 0;
+    const int group = a.Hq / a.Hk;
+    for (int h = kh * group; h < (kh + 1) * group; ++h)
+      for (int64_t i = q.begin + first; i < q.end; ++i) {
+        const Lanes x = load_row(static_cast<const T*>(a.q) + i * a.q_stride[0] + h * a.q_stride[1], a.D);
+        const Lanes g = load_row(static_cast<const T*>(a.dout) + i * a.dout_stride[0] + h * a.dout_stride[1], a.D);
+        const float p = expf(__fmaf_rn(dot(x, kj), a.scale, -a.lse[(int64_t)h * a.Tq + i]));
+        const float ds = __fmul_rn(p, dot(g, vj) - delta[(int64_t)h * a.Tq + i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ok.v[e] = __fmaf_rn(ds, x.v[e], ok.v[e]);
+          ov.v[e] = __fmaf_rn(p, g.v[e], ov.v[e]);
+        }
+      }
+  }
+  if (a.dk) store_row(static_cast<T*>(a.dk) + (t * a.Hk + kh) * a.D, a.D, ok, a.scale);
+  if (a.dv) store_row(static_cast<T*>(a.dv) + (t * a.Hk + kh) * a.D, a.D, ov, 1.0f);
+}
+
+}  // namespace attn
+}  // namespace emu

@@ -613,4 +613,194 @@ emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, const voi
   return cuda_status(emu::launch_kv_read(a, static_cast<cudaStream_t>(stream)), "emu_kv_read launch");
 }
 
+static emu_status check_norm_rope(const emu_norm_rope_args* p) {
+  if (!p) return fail(EMU_ERR_INVALID_ARGUMENT, "args must not be NULL");
+  if (p->tokens < 0 || p->table_rows < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (!float_dtype(p->dtype)) return fail(EMU_ERR_INVALID_ARGUMENT, "dtype must be EMU_DTYPE_F16, EMU_DTYPE_BF16 or EMU_DTYPE_F32");
+  if (p->heads_q < 1 || p->heads_q > 65536 || p->heads_k < 1 || p->heads_k > 65536) return fail(EMU_ERR_UNSUPPORTED, "heads must be in [1, 65536]");
+  if (p->head_size < 8 || p->head_size > 256 || p->head_size % 8 != 0) return fail(EMU_ERR_UNSUPPORTED, "head size must be a multiple of 8 up to 256");
+  if (p->half < 0 || 2 * p->half > p->head_size || (!p->interleaved && p->half % 8 != 0))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "half (%d) must be at most head_size / 2, a multiple of 8 unless interleaved", p->half);
+  if (!(p->eps >= 0.0f)) return fail(EMU_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  if (p->tokens > (1ll << 40)) return fail(EMU_ERR_UNSUPPORTED, "too many tokens");
+  if (p->tokens == 0) return EMU_OK;
+  if (!p->q || !p->k || !p->positions || (p->half > 0 && p->table_rows > 0 && (!p->cos || !p->sin)))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  const uintptr_t esz = p->dtype == EMU_DTYPE_F32 ? 4 : 2;
+  if (!aligned(p->q, esz) || !aligned(p->k, esz) || !aligned(p->q_weight, esz) || !aligned(p->k_weight, esz) || !aligned(p->cos, 4) ||
+      !aligned(p->sin, 4) || !aligned(p->positions, 8))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+  return EMU_OK;
+}
+
+static emu::NormRopeArgs norm_rope_args(const emu_norm_rope_args* p, void* q_out, void* k_out) {
+  emu::NormRopeArgs a{};
+  a.x[0] = p->q, a.x[1] = p->k;
+  a.token_stride[0] = p->q_token_stride, a.token_stride[1] = p->k_token_stride;
+  a.head_stride[0] = p->q_head_stride, a.head_stride[1] = p->k_head_stride;
+  a.heads[0] = p->heads_q, a.heads[1] = p->heads_k;
+  a.weight[0] = p->q_weight, a.weight[1] = p->k_weight;
+  a.cos = p->cos, a.sin = p->sin, a.table_rows = p->table_rows, a.half = p->half;
+  a.positions = p->positions, a.T = p->tokens, a.D = p->head_size, a.eps = p->eps;
+  a.interleaved = p->interleaved, a.dtype = p->dtype;
+  a.y[0] = q_out, a.y[1] = k_out;
+  return a;
+}
+
+emu_status emu_qk_norm_rope(const emu_norm_rope_args* p, void* q_out, void* k_out, void* stream) {
+  const emu_status st = check_norm_rope(p);
+  if (st != EMU_OK) return st;
+  if (p->tokens == 0) return ok();
+  if (!q_out || !k_out) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(q_out, 16) || !aligned(k_out, 16)) return fail(EMU_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned");
+  return cuda_status(emu::launch_norm_rope(norm_rope_args(p, q_out, k_out), false, static_cast<cudaStream_t>(stream)), "emu_qk_norm_rope launch");
+}
+
+size_t emu_qk_norm_rope_workspace_size(int32_t head_size) { return head_size > 0 ? emu::norm_rope_workspace(head_size) : 0; }
+
+emu_status emu_qk_norm_rope_backward(const emu_norm_rope_args* p, const void* q_grad, const void* k_grad,
+                                     int64_t q_grad_token_stride, int64_t q_grad_head_stride, int64_t k_grad_token_stride,
+                                     int64_t k_grad_head_stride, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  const emu_status st = check_norm_rope(p);
+  if (st != EMU_OK) return st;
+  const size_t esz = p->dtype == EMU_DTYPE_F32 ? 4 : 2;
+  if (!aligned(dq_weight, esz) || !aligned(dk_weight, esz)) return fail(EMU_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+  if (p->tokens == 0) {   // empty sums
+    cudaError_t e = cudaSuccess;
+    if (dq_weight) e = cudaMemsetAsync(dq_weight, 0, esz * p->head_size, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess && dk_weight) e = cudaMemsetAsync(dk_weight, 0, esz * p->head_size, static_cast<cudaStream_t>(stream));
+    return cuda_status(e, "emu_qk_norm_rope_backward memset");
+  }
+  if (!q_grad || !k_grad || !dq || !dk || !workspace) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(q_grad, esz) || !aligned(k_grad, esz)) return fail(EMU_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+  if (!aligned(dq, 16) || !aligned(dk, 16) || !aligned(workspace, 16)) return fail(EMU_ERR_INVALID_ARGUMENT, "outputs and workspace must be 16-byte aligned");
+  const size_t need = emu::norm_rope_workspace(p->head_size);
+  if (workspace_bytes < need) return fail(EMU_ERR_INVALID_ARGUMENT, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  emu::NormRopeArgs a = norm_rope_args(p, dq, dk);
+  a.dy[0] = q_grad, a.dy[1] = k_grad;
+  a.dy_token_stride[0] = q_grad_token_stride, a.dy_token_stride[1] = k_grad_token_stride;
+  a.dy_head_stride[0] = q_grad_head_stride, a.dy_head_stride[1] = k_grad_head_stride;
+  a.dw[0] = dq_weight, a.dw[1] = dk_weight;
+  a.partial = static_cast<float*>(workspace);
+  return cuda_status(emu::launch_norm_rope(a, true, static_cast<cudaStream_t>(stream)), "emu_qk_norm_rope_backward launch");
+}
+
+static emu_status check_attention(const emu_attention_args* p) {
+  if (!p) return fail(EMU_ERR_INVALID_ARGUMENT, "args must not be NULL");
+  if (p->total_q < 0 || p->total_k < 0 || p->sequences < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (p->dtype != EMU_DTYPE_F16 && p->dtype != EMU_DTYPE_BF16) return fail(EMU_ERR_INVALID_ARGUMENT, "dtype must be EMU_DTYPE_F16 or EMU_DTYPE_BF16");
+  if (p->heads_q < 1 || p->heads_k < 1 || p->heads_q > 65535) return fail(EMU_ERR_UNSUPPORTED, "heads must be in [1, 65535]");
+  if (p->heads_q % p->heads_k != 0) return fail(EMU_ERR_INVALID_ARGUMENT, "heads_q (%d) must be a multiple of heads_k (%d)", p->heads_q, p->heads_k);
+  if (p->head_size < 8 || p->head_size > 128 || p->head_size % 8 != 0) return fail(EMU_ERR_UNSUPPORTED, "head size must be a multiple of 8 up to 128");
+  if (!(p->scale > 0.0f) || p->scale > 3.402823466e38f) return fail(EMU_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (p->total_q > 0x7FFFFFFFll - 4096 || p->total_k > 0x7FFFFFFFll - 4096) return fail(EMU_ERR_UNSUPPORTED, "too many rows");
+  if (p->sequences > 0x7FFFFFFll) return fail(EMU_ERR_UNSUPPORTED, "too many sequences");
+  if (!p->cu_q || !p->cu_k || !aligned(p->cu_q, 4) || !aligned(p->cu_k, 4))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "cu_q and cu_k must be 4-byte aligned pointers");
+  if ((p->total_q > 0 && !p->q) || (p->total_k > 0 && (!p->k || !p->v))) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, 16)) return fail(EMU_ERR_INVALID_ARGUMENT, "q, k and v must be 16-byte aligned");
+  const int64_t strides[] = {p->q_token_stride, p->q_head_stride, p->k_token_stride, p->k_head_stride, p->v_token_stride, p->v_head_stride};
+  for (int64_t s : strides)
+    if (s < 8 || s % 8 != 0 || s >= (1ll << 38)) return fail(EMU_ERR_INVALID_ARGUMENT, "strides must be positive multiples of 8 elements");
+  return EMU_OK;
+}
+
+static emu::AttnArgs attention_args(const emu_attention_args* p) {
+  emu::AttnArgs a{};
+  a.q = p->q, a.k = p->k, a.v = p->v;
+  a.q_stride[0] = p->q_token_stride, a.q_stride[1] = p->q_head_stride;
+  a.k_stride[0] = p->k_token_stride, a.k_stride[1] = p->k_head_stride;
+  a.v_stride[0] = p->v_token_stride, a.v_stride[1] = p->v_head_stride;
+  a.Tq = p->total_q, a.Tk = p->total_k, a.B = p->sequences;
+  a.Hq = p->heads_q, a.Hk = p->heads_k, a.D = p->head_size, a.dtype = p->dtype, a.causal = p->causal != 0;
+  a.cu_q = p->cu_q, a.cu_k = p->cu_k, a.scale = p->scale;
+  return a;
+}
+
+emu_status emu_attention(const emu_attention_args* p, void* out, float* lse, void* stream) {
+  const emu_status st = check_attention(p);
+  if (st != EMU_OK) return st;
+  if (p->total_q == 0) return ok();
+  if (!out) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(out, 16) || !aligned(lse, 4)) return fail(EMU_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned, lse 4-byte");
+  emu::AttnArgs a = attention_args(p);
+  a.out = out, a.lse = lse;
+  return cuda_status(emu::launch_attention(a, static_cast<cudaStream_t>(stream)), "emu_attention launch");
+}
+
+size_t emu_attention_backward_workspace_size(const emu_attention_args* p) {
+  if (!p || p->total_q < 0 || p->total_k < 0 || p->heads_q < 1 || p->heads_k < 1) return 0;
+  return emu::attention_backward_workspace(p->total_q, p->total_k, p->heads_q, p->heads_k);
+}
+
+emu_status emu_attention_backward(const emu_attention_args* p, const void* out, const float* lse, const void* dout,
+                                  int64_t dout_token_stride, int64_t dout_head_stride, void* dq, void* dk, void* dv,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const emu_status st = check_attention(p);
+  if (st != EMU_OK) return st;
+  if (!aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return fail(EMU_ERR_INVALID_ARGUMENT, "gradients must be 16-byte aligned");
+  if (p->total_q == 0) {   // empty sums
+    const size_t bytes = (size_t)p->total_k * p->heads_k * p->head_size * 2;
+    cudaError_t e = cudaSuccess;
+    if (dk && bytes) e = cudaMemsetAsync(dk, 0, bytes, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess && dv && bytes) e = cudaMemsetAsync(dv, 0, bytes, static_cast<cudaStream_t>(stream));
+    return cuda_status(e, "emu_attention_backward memset");
+  }
+  if (!out || !lse || !dout || !workspace) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (!aligned(out, 16) || !aligned(dout, 16) || !aligned(lse, 4) || !aligned(workspace, 256))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "out and dout must be 16-byte aligned, lse 4-byte, workspace 256-byte");
+  if (dout_token_stride < 8 || dout_token_stride % 8 != 0 || dout_head_stride < 8 || dout_head_stride % 8 != 0 ||
+      dout_token_stride >= (1ll << 38) || dout_head_stride >= (1ll << 38))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "strides must be positive multiples of 8 elements");
+  const size_t need = emu_attention_backward_workspace_size(p);
+  if (workspace_bytes < need) return fail(EMU_ERR_INVALID_ARGUMENT, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  emu::AttnArgs a = attention_args(p);
+  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
+  a.dout = dout, a.dout_stride[0] = dout_token_stride, a.dout_stride[1] = dout_head_stride;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.workspace = workspace;
+  return cuda_status(emu::launch_attention_backward(a, static_cast<cudaStream_t>(stream)), "emu_attention_backward launch");
+}
+
+size_t emu_kv_attend_workspace_size(int64_t sequences, int32_t heads_q, int32_t heads, int32_t head_size) {
+  if (sequences < 1 || heads_q < 1 || heads < 1 || head_size < 1) return 0;
+  return emu::kv_attend_workspace(sequences, heads_q, heads, head_size);
+}
+
+emu_status emu_kv_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype, int64_t sequences,
+                         int32_t heads_q, int32_t heads, int32_t head_size, float scale, int32_t format, const uint8_t* k_cache,
+                         const uint8_t* v_cache, const void* k_scale, const void* v_scale, int64_t num_pages,
+                         int64_t page_size, const int32_t* block_table, int64_t table_cols, int64_t table_stride,
+                         const int32_t* lens, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  if (num_pages < 0 || sequences < 0 || table_cols < 0) return fail(EMU_ERR_INVALID_ARGUMENT, "negative size");
+  if (page_size < 1) return fail(EMU_ERR_INVALID_ARGUMENT, "page_size must be positive");
+  if (dtype != EMU_DTYPE_F16 && dtype != EMU_DTYPE_BF16) return fail(EMU_ERR_INVALID_ARGUMENT, "dtype must be EMU_DTYPE_F16 or EMU_DTYPE_BF16");
+  const emu_status st = check_kv(format, heads, head_size);
+  if (st != EMU_OK) return st;
+  if (head_size > 256) return fail(EMU_ERR_UNSUPPORTED, "head size must be at most 256");
+  if (heads_q < 1 || heads_q > 65536 || heads_q % heads != 0) return fail(EMU_ERR_INVALID_ARGUMENT, "heads_q (%d) must be a positive multiple of the cache's heads (%d)", heads_q, heads);
+  if (!(scale > 0.0f) || scale > 3.402823466e38f) return fail(EMU_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (sequences > 0x7FFFFFFFll / heads_q) return fail(EMU_ERR_UNSUPPORTED, "sequences * heads_q up to 2^31 - 1");
+  if (num_pages > (1ll << 40) / page_size || table_cols > (1ll << 40) / page_size) return fail(EMU_ERR_UNSUPPORTED, "too many slots");
+  if (sequences == 0) return ok();
+  if (!q || !lens || !out || (table_cols > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
+  if (table_stride < table_cols && sequences > 1) return fail(EMU_ERR_INVALID_ARGUMENT, "table_stride (%lld) must be at least table_cols (%lld)", (long long)table_stride, (long long)table_cols);
+  if (!aligned(q, 2) || !aligned(lens, 4) || !aligned(block_table, 4) || !aligned(lse, 4) || !aligned(out, 16))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements, out 16-byte");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || (format == EMU_KV_FP8 && (!aligned(k_scale, 4) || !aligned(v_scale, 4))))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "caches must be 16-byte aligned, f32 scales 4-byte");
+  const size_t need = emu::kv_attend_workspace(sequences, heads_q, heads, head_size);
+  if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "workspace needs %zu bytes, 256-byte aligned, got %zu", need, workspace_bytes);
+  emu::KvAttendArgs a{};
+  a.q = q, a.q_stride[0] = q_token_stride, a.q_stride[1] = q_head_stride;
+  a.cache[0] = k_cache, a.cache[1] = v_cache, a.scales[0] = k_scale, a.scales[1] = v_scale;
+  a.num_pages = num_pages, a.page_size = page_size;
+  a.Hq = heads_q, a.Hk = heads, a.D = head_size, a.dtype = dtype, a.format = format;
+  a.table = block_table, a.B = sequences, a.table_cols = table_cols, a.table_stride = table_stride;
+  a.lens = lens, a.scale = scale, a.out = out, a.lse = lse, a.workspace = workspace;
+  return cuda_status(emu::launch_kv_attend(a, static_cast<cudaStream_t>(stream)), "emu_kv_attend launch");
+}
+
 }  // extern "C"

@@ -136,6 +136,73 @@ struct KvReadArgs {
 };
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream);
 
+// Norms of queries and keys with the position rotation (norm_rope.cu).  Index 0: queries, 1: keys.
+constexpr int NORM_ROPE_CTAS = 4;   // most CTAs for each SM that write a share of the weights' gradients
+struct NormRopeArgs {
+  const void* x[2];
+  int64_t token_stride[2], head_stride[2];
+  int64_t heads[2];
+  const void* weight[2];        // may be null
+  const float* cos;
+  const float* sin;             // [table_rows][half]
+  int64_t table_rows, half;
+  const int64_t* positions;
+  int64_t T, D;
+  float eps;
+  int interleaved, dtype;
+  void* y[2];                   // contiguous outputs: y, or dx in the backward pass
+  const void* dy[2];            // backward pass from here on
+  int64_t dy_token_stride[2], dy_head_stride[2];
+  void* dw[2];
+  float* partial;               // norm_rope_workspace bytes
+  int chunks[2], heads_per_unit;   // set by the launcher
+};
+size_t norm_rope_workspace(int64_t D);
+cudaError_t launch_norm_rope(NormRopeArgs a, bool back, cudaStream_t stream);
+
+// Attention over packed sequences (attention.cu).
+struct AttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride[2], k_stride[2], v_stride[2];   // elements between tokens, between heads
+  int64_t Tq, Tk, B;
+  int Hq, Hk, D, dtype, causal;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  float scale;
+  void* out;                    // [Tq][Hq][D]
+  float* lse;                   // [Hq][Tq]
+  const void* dout;             // backward pass from here on
+  int64_t dout_stride[2];
+  void* dq;
+  void* dk;
+  void* dv;                     // contiguous; any of the three may be null
+  void* workspace;
+};
+size_t attention_backward_workspace(int64_t Tq, int64_t Tk, int Hq, int Hk);
+cudaError_t launch_attention(const AttnArgs& a, cudaStream_t stream);
+cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream);
+
+// Attention of one token for each sequence over the quantised cache (kv_attend.cu).
+struct KvAttendArgs {
+  const void* q;                // [B][Hq][D], strides in elements
+  int64_t q_stride[2];
+  const uint8_t* cache[2];
+  const void* scales[2];
+  int64_t num_pages, page_size;
+  int Hq, Hk, D, dtype, format;
+  const int32_t* table;
+  int64_t B, table_cols, table_stride;
+  const int32_t* lens;
+  float scale;
+  void* out;                    // [B][Hq][D]
+  float* lse;                   // [B][Hq], may be null
+  void* workspace;
+};
+size_t kv_attend_workspace(int64_t B, int Hq, int Hk, int D);
+cudaError_t launch_kv_attend(const KvAttendArgs& a, cudaStream_t stream);
+
 // sets emu_last_error() of the calling thread to `message` and returns s (capi.cu)
 int32_t record_failure(int32_t s, const char* message);
 

@@ -1,4 +1,4 @@
-"""Quantised key/value cache: rows (token, head) written to their slots in 8 or 4 bits and read back.
+"""Quantised key/value cache: rows (token, head) written to their slots in 8 or 4 bits, read back, and attended to.
 
 A cache is four tensors (make_kv_cache): codes and scales of the keys and of the values, page by page:
 
@@ -6,6 +6,8 @@ A cache is four tensors (make_kv_cache): codes and scales of the keys and of the
             (emugen_b200.fp8's quantiser, blocks of 128 along a row)
   "mxfp4"   packed e2m1 uint8 [pages, page_size, heads, head_size / 2], scale bytes [..., head_size / 32]
             (quant_mxfp4's codes and exponents, without its swizzle)
+
+attend_kv_cache is the attention of one new token for each sequence over its rows, read as they are stored.
 
 Slot s is place s % page_size of page s // page_size.  The kernels run on the cache's device and its
 current stream and synchronise nothing.  The reference has no cache.
@@ -180,4 +182,54 @@ def read_kv_cache(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], k_scal
     return k_out, v_out
 
 
-__all__ = ["make_kv_cache", "write_kv_cache", "read_kv_cache"]
+def attend_kv_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+                    scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of one new token for each sequence over its cached rows: [sequences, query heads, head_size].
+
+    q [sequences, query heads, head_size] (fp16 / bf16; any sequence and head strides); its heads are a multiple of the
+    cache's, query head h reading the cache's head h // (query heads // heads).  lens int32 [sequences]: sequence b sees its
+    positions 0 .. lens[b] - 1, from pages block_table[b] (int32 [sequences, pages of a sequence]); write the new token's
+    own row first.  Positions on a page that does not exist are not seen, and a sequence that sees none gets zeros.
+    scale: of the scores (default head_size ** -0.5).  With return_lse also f32 [sequences, query heads]: the logarithm of
+    the sum of exp(score), -inf where nothing is seen.  head_size up to 256.  Scores, sums and the softmax in f32, the
+    weights of the values rounded to fp16; the same result every run.  Not differentiable."""
+    if v_cache is None or v_scale is None:
+        raise RuntimeError("attend_kv_cache needs a cache of keys and values")
+    fmt, pages, page_size, heads, D = _geometry(k_cache, v_cache, k_scale, v_scale)
+    dev = k_cache.device
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] < 1 or q.shape[1] % heads:
+        raise RuntimeError(f"q must be [sequences, a multiple of {heads}, {D}], got {list(q.shape)}")
+    B, Hq = q.shape[0], q.shape[1]
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise RuntimeError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {list(block_table.shape)}")
+    if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != B:
+        raise RuntimeError(f"lens must be int32 [{B}], got {lens.dtype} {list(lens.shape)}")
+    at = dev.index
+    if q.get_device() != at or block_table.get_device() != at or lens.get_device() != at:
+        raise RuntimeError("q, block_table and lens must be on the cache's device")
+    cols = block_table.shape[1]
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if block_table.stride(1) != 1 and cols > 1 or block_table.stride(0) < cols and B > 1:
+        block_table = block_table.contiguous()
+    lens = lens.contiguous()
+    L = _lib.load()
+    with _on(at):
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+        need = L.emu_kv_attend_workspace_size(B, Hq, heads, D)
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        status = L.emu_kv_attend(q.data_ptr(), q.stride(0), q.stride(1), _DTYPE[q.dtype], B, Hq, heads, D,
+                                 D ** -0.5 if scale is None else float(scale), fmt, k_cache.data_ptr(), v_cache.data_ptr(),
+                                 k_scale.data_ptr(), v_scale.data_ptr(), pages, page_size, block_table.data_ptr(), cols,
+                                 max(block_table.stride(0), cols), lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(work),
+                                 need, _raw_stream(at))
+    if status:
+        _lib._check(status)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["make_kv_cache", "write_kv_cache", "read_kv_cache", "attend_kv_cache"]

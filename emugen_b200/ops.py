@@ -18,7 +18,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib, fp8, kvcache
+from . import _lib, attention, fp8, kvcache
 
 _OUT_DTYPE = {_lib.EMU_OUT_F16: torch.float16, _lib.EMU_OUT_BF16_VIA_F16: torch.bfloat16,
               _lib.EMU_OUT_F32: torch.float32}
@@ -153,4 +153,45 @@ def _read_kv_cache_fake(k_cache, v_cache, k_scale, v_scale, block_table, cu_lens
     return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
 
 
-__all__ = ["gemm", "emulated_scaled_fp4_mm", "emulated_mxfp4_mm", "quant_fp8", "gemm_fp8", "write_kv_cache", "read_kv_cache"]
+@torch.library.custom_op("emugen::attend_kv_cache", mutates_args=())
+def attend_kv_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of one new token for each sequence over its cached rows: [sequences, query heads, head_size]."""
+    return kvcache.attend_kv_cache(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, scale=scale)
+
+
+@attend_kv_cache.register_fake
+def _attend_kv_cache_fake(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("emugen::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                 cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, eps: float = 1e-6,
+                 interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norms of queries and keys [tokens, heads, head_size] with the position rotation (without gradients)."""
+    with torch.no_grad():
+        return attention.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=eps, interleaved=interleaved)
+
+
+@qk_norm_rope.register_fake
+def _qk_norm_rope_fake(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("emugen::packed_attention", mutates_args=())
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: Optional[torch.Tensor] = None,
+                     causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
+    """Attention over packed sequences [tokens, heads, head_size] (without gradients)."""
+    with torch.no_grad():
+        return attention.packed_attention(q, k, v, cu_q, cu_k, causal=causal, scale=scale)
+
+
+@packed_attention.register_fake
+def _packed_attention_fake(q, k, v, cu_q, cu_k=None, causal=True, scale=None):
+    return q.new_empty(q.shape)
+
+
+__all__ = ["gemm", "emulated_scaled_fp4_mm", "emulated_mxfp4_mm", "quant_fp8", "gemm_fp8", "write_kv_cache", "read_kv_cache",
+           "attend_kv_cache", "qk_norm_rope", "packed_attention"]

@@ -450,6 +450,94 @@ EMU_API emu_status emu_kv_read(const uint8_t* k_cache, const uint8_t* v_cache, c
                                int64_t table_stride, const int32_t* cu_lens, int64_t total, int32_t out_dtype,
                                void* k_out, void* v_out, int64_t k_token_stride, int64_t v_token_stride, void* stream);
 
+/*
+ * Norms of queries and keys for each head with the position rotation, in one pass.  For a row x of head_size elements
+ * (token t, one head), weight w (of its tensor, NULL: ones) and angle row p = positions[t]:
+ *   z = x / sqrt(mean(x^2) + eps) * w
+ *   out = z with pairs of its first 2 * half elements turned: (a, b) -> (a cos - b sin, b cos + a sin), cos and sin of pair i
+ *   at [p * half + i]; the pairs are (z[i], z[i + half]), or with `interleaved` (z[2 i], z[2 i + 1]).
+ * Sums in f32, one rounding at the end.  A negative position is padding: its rows are zeros and give no gradients.  A
+ * position not below table_rows gives NaN where elements are turned.  q, k and their gradients: fp16 / bf16 / f32 with any
+ * token and head strides (elements); outputs contiguous [tokens][heads][head_size], 16-byte aligned.  head_size is a multiple
+ * of 8 up to 256, 2 * half <= head_size; half is a multiple of 8 unless interleaved, and 0 for no turn.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  int64_t tokens, table_rows;
+  int32_t heads_q, heads_k, head_size, half, dtype, interleaved;
+  float eps;
+} emu_norm_rope_args;
+EMU_API emu_status emu_qk_norm_rope(const emu_norm_rope_args* args, void* q_out, void* k_out, void* stream);
+/*
+ * Its gradients: dq and dk (contiguous, 16-byte aligned) from q_grad and k_grad, and those of the weights, dq_weight and
+ * dk_weight [head_size] (NULL: not wanted), in the inputs' dtype.  The weights' sums are made in one order, the same result
+ * every run.  workspace: emu_qk_norm_rope_workspace_size(head_size) bytes on the device, 16-byte aligned.
+ */
+EMU_API size_t emu_qk_norm_rope_workspace_size(int32_t head_size);
+EMU_API emu_status emu_qk_norm_rope_backward(const emu_norm_rope_args* args, const void* q_grad, const void* k_grad,
+                                             int64_t q_grad_token_stride, int64_t q_grad_head_stride,
+                                             int64_t k_grad_token_stride, int64_t k_grad_head_stride, void* dq, void* dk,
+                                             void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                                             void* stream);
+
+/*
+ * Attention over packed sequences: sequence b has the queries cu_q[b] .. cu_q[b + 1] - 1 and the keys and values
+ * cu_k[b] .. cu_k[b + 1] - 1 (int32 [sequences + 1] on the device, non-decreasing from 0).  Query i of nq sees every key of
+ * its sequence, or with `causal` those up to i + nk - nq: the last query stands on the last of the nk keys.
+ *   out = sum_j p_j v_j,  p = softmax over the keys seen of scale * q . k_j;  query head h uses key head h / (heads_q / heads_k)
+ * A query that sees no key gets zeros, as do rows behind the last sequence.  Keys and values that the mask hides reach no
+ * result, whatever they hold.  Scores, sums and the softmax's statistics in f32; p is rounded to the inputs' dtype for its
+ * product.  lse f32 [heads_q][total_q] (may be NULL): log of the sum of exp(score), -infinity for a query without keys.
+ * dtype fp16 / bf16; head_size a multiple of 8 up to 128; tensors 16-byte aligned, strides multiples of 8 elements; out is
+ * contiguous [total_q][heads_q][head_size].  scale positive.  The same result every run.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t total_q, total_k, sequences;
+  int32_t heads_q, heads_k, head_size, dtype, causal;
+  float scale;
+} emu_attention_args;
+EMU_API emu_status emu_attention(const emu_attention_args* args, void* out, float* lse, void* stream);
+/*
+ * Its gradients from dout: dq [total_q][heads_q][head_size], dk and dv [total_k][heads_k][head_size], contiguous, each may be
+ * NULL (not wanted).  out and lse are emu_attention's.  ds = p (dout . v - dout . out) is rounded to the inputs' dtype for
+ * its products (fp16: scaled by a power of two that keeps it in range).  No atomic additions: the same result every run.
+ * workspace: emu_attention_backward_workspace_size(args) bytes on the device, 256-byte aligned.
+ */
+EMU_API size_t emu_attention_backward_workspace_size(const emu_attention_args* args);
+EMU_API emu_status emu_attention_backward(const emu_attention_args* args, const void* out, const float* lse,
+                                          const void* dout, int64_t dout_token_stride, int64_t dout_head_stride, void* dq,
+                                          void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of one new token for each sequence over a quantised cache (emu_kv_write's layout, num_pages * page_size slots):
+ * out[b][h] = sum_j p_j v_j over the positions j < lens[b] of sequence b, in page block_table[b * table_stride + j / page_size],
+ * p = softmax of scale * q[b][h] . k_j; query head h uses the cache's head h / (heads_q / heads).  Positions on a page that
+ * does not exist (negative, not below num_pages, past table_cols) are not seen; a sequence that sees none gets zeros.
+ * q fp16 / bf16 [sequences][heads_q][head_size] (any strides, elements), out contiguous, lse f32 [sequences][heads_q] (may be
+ * NULL) as in emu_attention.  head_size up to 256.  workspace: emu_kv_attend_workspace_size bytes (may be 0) on the device,
+ * 256-byte aligned.  The same result every run.
+ */
+EMU_API size_t emu_kv_attend_workspace_size(int64_t sequences, int32_t heads_q, int32_t heads, int32_t head_size);
+EMU_API emu_status emu_kv_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,
+                                 int64_t sequences, int32_t heads_q, int32_t heads, int32_t head_size, float scale,
+                                 int32_t format, const uint8_t* k_cache, const uint8_t* v_cache, const void* k_scale,
+                                 const void* v_scale, int64_t num_pages, int64_t page_size, const int32_t* block_table,
+                                 int64_t table_cols, int64_t table_stride, const int32_t* lens, void* out, float* lse,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
