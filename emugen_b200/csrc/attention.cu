@@ -1,60 +1,311 @@
-// Attention over packed sequences and its gradients (the formulas: attention.cuh), a warp to a row.
+// Attention over packed sequences, forward pass (the formulas: attention.cuh), on the 5th-generation tensor cores.
+//
+// A CTA owns two tiles of up to 128 rows and walks over the keys in tiles of 128: S = Q K^T into tensor memory, one pass
+// over S by the tile's warpgroup with the running maximum and sum of the softmax, P in 16 bits back into S's place, O += P V
+// with P from tensor memory.  A row is (token, query head of the group): the tile holds all heads that share a key head, so
+// that K and V are staged once for them and few queries still fill it.
+//
+//   warps 0-3, 4-7   softmax of the first and the second tile, a thread to a row; at the end its row's output
+//   warp 8           MMA issuer: for each tile in turn O += P V of the tile of keys before, then S of the next, so that
+//                    the tensor cores work on one tile while the other's softmax runs.  Owns the tensor memory.
+//   warp 9           TMA: Q once, then K and V tiles through a ring
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/emugen.h"
 #include "attention.cuh"
+#include "attention_tc.cuh"
+#include "tc_ptx.cuh"
 
 namespace emu {
 namespace {
 
 using namespace attn;
 
-enum { FORWARD, DELTA, DQ, DKDV };
+constexpr int THREADS = 384;                                // warps 10 and 11 fill up the third warpgroup
+// 128 threads x 40 + 256 x 232 = 64512 = 384 x 168, what the CTA is launched with
+constexpr int REG_LOW = 40, REG_HIGH = 232;
 
-template <typename T, int WHAT> __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ AttnArgs a) {
-  const int heads = WHAT == DKDV ? a.Hk : a.Hq;
-  const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), total = WHAT == DKDV ? a.Tk : a.Tq;
-  if (u >= total * heads) return;
-  const int64_t t = u / heads;
-  const int h = (int)(u - t * heads);
-  float* delta = static_cast<float*>(a.workspace);
-  if (WHAT == DELTA) {
-    const Lanes o = load_row(static_cast<const T*>(a.out) + (t * a.Hq + h) * a.D, a.D);
-    const float d = dot(o, load_row(static_cast<const T*>(a.dout) + t * a.dout_stride[0] + h * a.dout_stride[1], a.D));
-    if ((threadIdx.x & 31) == 0) delta[(int64_t)h * a.Tq + t] = d;
-    return;
+template <int DP> struct Fwd {
+  static constexpr int TILE = 128 * DP * 2;                 // 128 rows of DP elements, as DP / 64 boxes of 128 x 128 bytes
+  static constexpr int SLOTS = DP == 128 ? 5 : 8;           // ring of K and V tiles in turn
+  static constexpr int BARS = 1 + 2 * SLOTS + 2 + 2 + 2;
+  static constexpr int SMEM = 1024 + 2 * TILE + SLOTS * TILE + BARS * 8 + 16;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+// tensor memory columns: S (and P) of both tiles, O of both tiles
+constexpr uint32_t S_COL = 0, O_COL = 256;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
+                                                              const __grid_constant__ Tiling tl) {
+  using C = Fwd<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  const Unit u = unit_of(a, tl, a.cu_q, a.Tq, 2);
+  if (!u.any) return;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const Rows qr = u.rows;
+  const Rows kr = u.b < a.B ? rows_of(a.cu_k, u.b, a.Tk) : Rows{0, 0};
+  const int64_t nq = qr.count(), nk = kr.count();
+  // keys that the unit's last token sees
+  const int64_t last = min(u.t0 + 2 * tl.tokens, qr.end) - 1 - qr.begin;
+  const int64_t most = a.causal ? max((int64_t)0, min(nk, last + 1 + nk - nq)) : nk;
+  const int tiles = (int)((most + 127) / 128);
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* ring = smem + 2 * C::TILE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + C::SLOTS * C::TILE);
+  uint64_t* kv_full = q_full + 1;
+  uint64_t* kv_empty = kv_full + C::SLOTS;
+  uint64_t* s_full = kv_empty + C::SLOTS;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&map_q), ptx::prefetch_tmap(&map_k), ptx::prefetch_tmap(&map_v);
+    ptx::mbar_init(q_full, 1);
+    for (int i = 0; i < C::SLOTS; ++i) ptx::mbar_init(&kv_full[i], 1), ptx::mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < 2; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&p_full[i], 128), ptx::mbar_init(&o_full[i], 1);
+    ptx::fence_mbar_init();
   }
-  const int64_t b = sequence_of(WHAT == DKDV ? a.cu_k : a.cu_q, a.B, t);
-  if (WHAT == FORWARD) row_forward<T>(a, b, t, h);
-  else if (WHAT == DQ) row_dq<T>(a, delta, b, t, h);
-  else if (WHAT == DKDV) row_dkdv<T>(a, delta, b, t, h);
+  if (warp == 8) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  // no load may be in flight across the register split: the TMEM address is read after it
+  if (warp >= 8) {
+    ptx::setmaxnreg_dec<REG_LOW>();
+    if (warp == 9 && lane == 0 && tiles) {
+      const int head = u.kh * tl.group + u.chunk * tl.heads;
+      ptx::mbar_arrive_expect_tx(q_full, 2 * (DP / 64) * tl.heads * tl.tokens * 128);
+      for (int i = 0; i < 2; ++i)
+        for (int x = 0; x < DP / 64; ++x)
+          ptx::tma_load_3d(smem + i * C::TILE + x * 16384, &map_q, q_full, x * 64, head, (int)(u.t0 + i * tl.tokens));
+      Ring<C::SLOTS> r;
+      bool ok = true;
+      int i = 0;
+      for (; i < 2 * tiles; ++i, r.next()) {
+        if (i >= C::SLOTS && !wait_or_record(&kv_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_FWD_SLOT)) { ok = false; break; }
+        ptx::mbar_arrive_expect_tx(&kv_full[r.at], C::TILE);
+        for (int x = 0; x < DP / 64; ++x)
+          ptx::tma_load_3d(ring + r.at * C::TILE + x * 16384, i & 1 ? &map_v : &map_k, &kv_full[r.at], x * 64, u.kh, (int)(kr.begin + (i >> 1) * 128));
+      }
+      if (!ok) {                                             // every copy has landed before the CTA exits
+        wait_or_record(q_full, 0, DRAIN_LIMIT, WAIT_DRAIN);
+        for (int j = max(0, i - C::SLOTS); j < i; ++j) wait_or_record(&kv_full[j % C::SLOTS], (j / C::SLOTS) & 1, DRAIN_LIMIT, WAIT_DRAIN);
+      }
+    } else if (warp == 8 && tiles) {
+      const uint32_t tmem = *tmem_slot;
+      constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+      const uint32_t id_s = ptx::idesc_16_f32(128, 128, BF, false), id_o = ptx::idesc_16_f32(128, tl.d16, BF, true);
+      const int steps = tl.d16 / 16;
+      bool ok = warp_wait_or_record(q_full, 0, tl.wait_limit, WAIT_FWD_Q);
+      auto scores = [&](int i, int slot) {                   // S_i = Q_i K^T
+        const uint32_t q = ptx::smem_u32(smem + i * C::TILE), k = ptx::smem_u32(ring + slot * C::TILE);
+        for (int s = 0; s < steps; ++s) {
+          const uint32_t at = (s / 4) * 16384 + (s % 4) * 32;
+          ptx::mma_f16(tmem + S_COL + i * 128, ptx::smem_desc_sw128(q + at), ptx::smem_desc_sw128(k + at), id_s, s > 0);
+        }
+      };
+      auto values = [&](int i, int slot, bool more) {        // O_i += P_i V
+        const uint64_t v = ptx::smem_desc_mn_sw128(ptx::smem_u32(ring + slot * C::TILE), 16384);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          ptx::mma_f16_ta(tmem + O_COL + i * DP, tmem + S_COL + i * 128 + s * 8, v + s * 128, id_o, more || s > 0);
+      };
+      Ring<C::SLOTS> k, v;                                   // of the keys and of the values before them
+      v.next();
+      uint32_t parity = 0;                                   // of P
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (j > 0 && !warp_wait_or_record(&kv_full[v.at], v.parity, tl.wait_limit, WAIT_FWD_V)) { ok = false; break; }
+        if (!warp_wait_or_record(&kv_full[k.at], k.parity, tl.wait_limit, WAIT_FWD_K)) { ok = false; break; }
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j > 0 && !warp_wait_or_record(&p_full[i], parity ^ 1, tl.wait_limit, WAIT_FWD_P)) ok = false;
+          ptx::tc_fence_after();
+          if (ok && ptx::elect_one()) {
+            if (j > 0) values(i, v.at, j > 1);
+            scores(i, k.at);
+            if (!(j == 0 && i == 0 && tl.hold_first_ready)) ptx::mma_commit(&s_full[i]);
+          }
+          __syncwarp();
+        }
+        if (ok && ptx::elect_one()) {
+          if (j > 0) ptx::mma_commit(&kv_empty[v.at]);
+          ptx::mma_commit(&kv_empty[k.at]);
+        }
+        __syncwarp();
+        k.next(), k.next();
+        if (j > 0) v.next(), v.next();
+        parity ^= 1;
+      }
+      if (ok) ok = warp_wait_or_record(&kv_full[v.at], v.parity, tl.wait_limit, WAIT_FWD_V);
+      for (int i = 0; i < 2; ++i) {
+        if (ok) ok = warp_wait_or_record(&p_full[i], parity ^ 1, tl.wait_limit, WAIT_FWD_P);
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          if (ok) values(i, v.at, tiles > 1);
+          ptx::mma_commit(&o_full[i]);                       // after a failed wait too: the MMAs in flight are waited for
+        }
+        __syncwarp();
+      }
+      warp_wait_or_record(&o_full[1], 0, DRAIN_LIMIT, WAIT_DRAIN);
+    }
+  } else {
+    ptx::setmaxnreg_inc<REG_HIGH>();
+    const uint32_t tmem = *tmem_slot;
+    // softmax of tile i, row r
+    const int i = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_at = lanes + S_COL + i * 128, o_at = lanes + O_COL + i * DP;
+    const int64_t t = u.t0 + i * tl.tokens + r / tl.heads;
+    const int gh = u.chunk * tl.heads + r % tl.heads, h = u.kh * tl.group + gh;
+    const bool mine = r < tl.heads * tl.tokens && gh < tl.group && t < qr.end;
+    // this row sees the first n keys
+    const int64_t n = !mine ? 0 : a.causal ? max((int64_t)0, min(nk, t - qr.begin + 1 + nk - nq)) : nk;
+    // all rows of the tile see the first n0
+    const int64_t first = a.causal ? u.t0 + i * tl.tokens - qr.begin + 1 + nk - nq : nk;
+    const float c = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      if (!warp_wait_or_record(&s_full[i], j & 1, tl.wait_limit, WAIT_FWD_S)) { ok = false; break; }
+      ptx::tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_ld_regs(s_at + 32 * x, s[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_wait_regs(s[x]);
+      if ((int64_t)(j + 1) * 128 > first || (int64_t)(j + 1) * 128 > nk) {      // the same for the whole tile
+        const int lim = (int)max((int64_t)0, min((int64_t)128, n - (int64_t)j * 128));
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (x * 32 + e >= lim) s[x][e] = 0xFF800000u;
+      }
+      float top[4] = {m, m, m, m};
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
+      const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      // The weights are held to the maximum up to a factor of 2^8: P stays below 2^8, l and O in range, and most
+      // tiles need no correction of O.
+      const bool grow = (tm - m) * c > 8.0f;
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+        const float f = tm == -INFINITY ? 1.0f : exp2f((m - tm) * c);
+        l *= f;
+        m = tm;
+        if (j > 0) {
+#pragma unroll
+          for (int x = 0; x < DP; x += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_regs(o_at + x, o);
+            ptx::tmem_wait_regs(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            ptx::tmem_st_regs(o_at + x, o);
+          }
+        }
+      }
+      const float shift = m == -INFINITY ? 0.0f : -m * c;
+      const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int x = 0; x < 4; x += 2) {
+        uint32_t p[32];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t z = ptx::fma2(ptx::join2(s[x + y][e], s[x + y][e + 1]), c2, sh2);
+            const float p0 = exp2_approx(ptx::lo2(z)), p1 = exp2_approx(ptx::hi2(z));
+            sum[y] = ptx::add2(sum[y], ptx::join2(__float_as_uint(p0), __float_as_uint(p1)));
+            p[y * 16 + e / 2] = pack2<T>(p0, p1);
+          }
+        ptx::tmem_st_regs(s_at + 16 * x, p);
+      }
+      const uint64_t all = ptx::add2(sum[0], sum[1]);
+      l += ptx::lo2(all) + ptx::hi2(all);
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(&p_full[i]);
+    }
+    bool redo = false;
+    if (ok && tiles) ok = warp_wait_or_record(&o_full[i], 0, tl.wait_limit, WAIT_FWD_O);
+    ptx::tc_fence_after();
+    const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
+    float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
+#pragma unroll
+    for (int x = 0; x < DP; x += 32) {
+      uint32_t o[32];
+      if (tiles) {
+        ptx::tmem_ld_regs(o_at + x, o);
+        ptx::tmem_wait_regs(o);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // a row without keys gives zeros, whatever its place held
+          const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
+          if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
+          w[k] = pack2<T>(v0, v1);
+        }
+        if (mine && ok && x + e < a.D) *reinterpret_cast<uint4*>(out + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
+    // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
+    // from the keys that they see alone.  (Where the sum is NaN, the scores are, and the row is NaN by right.)
+    redo = mine && ok && worst != 0.0f && l > 0.0f;
+    for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
+      const int src = __ffs(rows) - 1;
+      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src));
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(*tmem_slot, 512);
+  }
 }
 
-template <typename T, int WHAT> void launch_rows(const AttnArgs& a, cudaStream_t stream) {
-  const int64_t rows = WHAT == DKDV ? a.Tk * a.Hk : a.Tq * a.Hq;
-  if (rows) attention_rows_kernel<T, WHAT><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(a);
-}
-template <typename T> void launch_back(const AttnArgs& a, cudaStream_t stream) {
-  launch_rows<T, DELTA>(a, stream);
-  if (a.dq) launch_rows<T, DQ>(a, stream);
-  if (a.dk || a.dv) launch_rows<T, DKDV>(a, stream);
+template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
+  CUtensorMap mq, mk, mv;
+  const Tiling tl = tiling_of(a);
+  if (!make_rows_map(&mq, a.q, a.Tq, a.Hq, a.D, a.q_stride, a.dtype, tl.heads, tl.tokens) ||
+      !make_rows_map(&mk, a.k, a.Tk, a.Hk, a.D, a.k_stride, a.dtype, 1, 128) || !make_rows_map(&mv, a.v, a.Tk, a.Hk, a.D, a.v_stride, a.dtype, 1, 128))
+    return cudaErrorUnknown;
+  auto kernel = attention_kernel<T, DP>;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(kernel, Fwd<DP>::SMEM, done);
+  if (e != cudaSuccess) return e;
+  const int64_t grid = units(a.Tq, a.B, 2 * tl.tokens) * tl.chunks * a.Hk;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  kernel<<<(unsigned)grid, THREADS, Fwd<DP>::SMEM, stream>>>(mq, mk, mv, a, tl);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-size_t attention_backward_workspace(int64_t Tq, int64_t, int Hq, int) { return (size_t)Tq * Hq * sizeof(float); }
+cudaError_t take_attention_wait_error(int* code) { return take_error(code); }
 
 cudaError_t launch_attention(const AttnArgs& a, cudaStream_t stream) {
-  if (a.dtype == EMU_DTYPE_F16) launch_rows<__half, FORWARD>(a, stream);
-  else launch_rows<__nv_bfloat16, FORWARD>(a, stream);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream) {
-  if (a.dtype == EMU_DTYPE_F16) launch_back<__half>(a, stream);
-  else launch_back<__nv_bfloat16>(a, stream);
-  return cudaGetLastError();
+  const bool half = a.dtype == EMU_DTYPE_F16;
+  if (a.D <= 64) return half ? launch<__half, 64>(a, stream) : launch<__nv_bfloat16, 64>(a, stream);
+  return half ? launch<__half, 128>(a, stream) : launch<__nv_bfloat16, 128>(a, stream);
 }
 
 }  // namespace emu

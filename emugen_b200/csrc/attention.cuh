@@ -91,7 +91,7 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t)
 }
 
 // o_t and lse_t of one head.
-template <typename T> __device__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h) {
+template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h) {
   const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
   const int kh = h / (a.Hq / a.Hk);
   const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];

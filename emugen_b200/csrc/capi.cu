@@ -450,12 +450,14 @@ emu_status emu_test_hold_first_ready(int32_t enable) {
 emu_status emu_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: stream");
-  // both kernels' words are taken, so that the next call speaks for later launches alone; the first one set is told
-  int code = 0, code_fp8 = 0;
+  // every kernel's word is taken, so that the next call speaks for later launches alone; the first one set is told
+  int code = 0, code_fp8 = 0, code_attention = 0;
   e = emu::take_wait_error(&code);
   if (e == cudaSuccess) e = emu::take_fp8_wait_error(&code_fp8);
+  if (e == cudaSuccess) e = emu::take_attention_wait_error(&code_attention);
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: error word");
   if (code == 0) code = code_fp8;
+  if (code == 0) code = code_attention;
   if (code == 0) return ok();
   static const char* const kSite[] = {"", "producer stage slot", "producer record slot", "MMA accumulator set",
                                       "MMA stage data", "epilogue accumulator", "epilogue records",
@@ -463,7 +465,10 @@ emu_status emu_device_status(void* stream) {
                                       "8-bit product: producer scale slot", "8-bit product: producer stage slot",
                                       "8-bit product: copy drain", "8-bit product: MMA accumulator",
                                       "8-bit product: MMA stage data", "8-bit product: MMA drain",
-                                      "8-bit product: epilogue scales", "8-bit product: epilogue accumulator"};
+                                      "8-bit product: epilogue scales", "8-bit product: epilogue accumulator",
+                                      "attention: producer slot", "attention: queries", "attention: keys",
+                                      "attention: values", "attention: weights", "attention: scores",
+                                      "attention: output", "attention: drain"};
   constexpr int kSites = (int)(sizeof(kSite) / sizeof(kSite[0]));
   return fail(EMU_ERR_TIMEOUT,
               "a tensor-core pipeline wait ran out (code %d: %s); outputs of the calls on this device since the "
