@@ -285,6 +285,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
 template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
   const Tiling tl = tiling_of(a);
+  const cudaError_t bound = bind_context();
+  if (bound != cudaSuccess) return bound;
   if (!make_rows_map(&mq, a.q, a.Tq, a.Hq, a.D, a.q_stride, a.dtype, tl.heads, tl.tokens) ||
       !make_rows_map(&mk, a.k, a.Tk, a.Hk, a.D, a.k_stride, a.dtype, 1, 128) || !make_rows_map(&mv, a.v, a.Tk, a.Hk, a.D, a.v_stride, a.dtype, 1, 128))
     return cudaErrorUnknown;

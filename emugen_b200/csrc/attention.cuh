@@ -69,11 +69,20 @@ __device__ __forceinline__ float dot(const Lanes& a, const Lanes& b) {
   for (int i = 0; i < 4; ++i) s = __fmaf_rn(a.v[i], b.v[i], s);
   return warp_sum(s);
 }
-template <typename T> __device__ __forceinline__ void store_row(T* p, int D, const Lanes& r, float f) {
+// Elements [d0, d1) of the row.
+template <typename T> __device__ __forceinline__ void store_row(T* p, int d0, int d1, const Lanes& r, float f) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < D) p[lane + 32 * i] = narrow<T>(__fmul_rn(r.v[i], f));
+    if (lane + 32 * i >= d0 && lane + 32 * i < d1) p[lane + 32 * i] = narrow<T>(__fmul_rn(r.v[i], f));
+}
+// Whether every element of the row is NaN: nothing that is added changes it any more.
+__device__ __forceinline__ bool settled(const Lanes& r, int D) {
+  const int lane = threadIdx.x & 31;
+  bool nan = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) nan = nan && (isnan(r.v[i]) || lane + 32 * i >= D);
+  return __all_sync(0xFFFFFFFFu, nan);
 }
 
 // The keys that query t of sequence b sees: the first `n` of the sequence's.
@@ -90,7 +99,7 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t)
   return s;
 }
 
-// o_t and lse_t of one head.
+// o_t of one head.
 template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h) {
   const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
   const int kh = h / (a.Hq / a.Hk);
@@ -111,13 +120,16 @@ template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs
 #pragma unroll
     for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(p, y.v[i], __fmul_rn(o.v[i], old));
     m = top;
+    if (settled(o, a.D)) break;
   }
-  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, a.D, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
-  if ((threadIdx.x & 31) == 0 && a.lse) a.lse[(int64_t)h * a.Tq + t] = l > 0.0f ? m + logf(l) : l == 0.0f ? -INFINITY : l;
+  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, 0, a.D, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
 }
 
-// dq_t of one head.
-template <typename T> __device__ void row_dq(const AttnArgs& a, const float* delta, int64_t b, int64_t t, int h) {
+// A query's shift -lse log2 e and its delta, at [t * Hq + h].
+__device__ __forceinline__ float2 stat_of(const float2* stats, const AttnArgs& a, int64_t t, int h) { return stats[t * a.Hq + h]; }
+
+// Elements [d0, d1) of dq_t of one head.
+template <typename T> __device__ __forceinline__ void row_dq(const AttnArgs& a, const float2* stats, int64_t b, int64_t t, int h, int d0, int d1) {
   const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
   const T* g = static_cast<const T*>(a.dout) + t * a.dout_stride[0] + h * a.dout_stride[1];
   const int kh = h / (a.Hq / a.Hk);
@@ -126,42 +138,44 @@ template <typename T> __device__ void row_dq(const AttnArgs& a, const float* del
   Seen s{{0, 0}, 0};
   if (b < a.B) s = seen_by(a, b, t);
   const Lanes x = load_row(q, a.D), y = load_row(g, a.D);
-  const float lse = a.lse[(int64_t)h * a.Tq + t], dl = delta[(int64_t)h * a.Tq + t];
+  const float2 st = stat_of(stats, a, t, h);
+  const float c = a.scale * 1.4426950408889634f;
   Lanes o{};
   for (int64_t j = s.k.begin; j < s.k.begin + s.n; ++j) {
     const Lanes kj = load_row(k + j * a.k_stride[0], a.D);
-    const float p = expf(__fmaf_rn(dot(x, kj), a.scale, -lse));
-    const float ds = __fmul_rn(p, dot(y, load_row(v + j * a.v_stride[0], a.D)) - dl);
+    const float p = exp2f(__fmaf_rn(dot(x, kj), c, st.x));
+    const float ds = __fmul_rn(p, dot(y, load_row(v + j * a.v_stride[0], a.D)) - st.y);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(ds, kj.v[i], o.v[i]);
+    if (settled(o, a.D)) break;
   }
-  store_row(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D, a.D, o, a.scale);
+  store_row(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D, d0, d1, o, a.scale);
 }
 
-// dk_t and dv_t of one key head (t: a row of the keys; either may be left out).
-template <typename T> __device__ void row_dkdv(const AttnArgs& a, const float* delta, int64_t b, int64_t t, int kh) {
-  Lanes ok{}, ov{};
+// dk_t (KEYS) or dv_t of one key head, t a row of the keys.
+template <typename T, bool KEYS> __device__ __forceinline__ void row_dkv(const AttnArgs& a, const float2* stats, int64_t b, int64_t t, int kh) {
+  Lanes o{};
   if (b < a.B) {
     const Rows q = rows_of(a.cu_q, b, a.Tq), kr = rows_of(a.cu_k, b, a.Tk);
     const Lanes kj = load_row(static_cast<const T*>(a.k) + t * a.k_stride[0] + kh * a.k_stride[1], a.D);
     const Lanes vj = load_row(static_cast<const T*>(a.v) + t * a.v_stride[0] + kh * a.v_stride[1], a.D);
     const int64_t first = a.causal ? max((int64_t)0, (t - kr.begin) - (kr.count() - q.count())) : 0;
     const int group = a.Hq / a.Hk;
-    for (int h = kh * group; h < (kh + 1) * group; ++h)
-      for (int64_t i = q.begin + first; i < q.end; ++i) {
+    const float c = a.scale * 1.4426950408889634f;
+    bool done = false;
+    for (int h = kh * group; h < (kh + 1) * group && !done; ++h)
+      for (int64_t i = q.begin + first; i < q.end && !done; ++i) {
         const Lanes x = load_row(static_cast<const T*>(a.q) + i * a.q_stride[0] + h * a.q_stride[1], a.D);
         const Lanes g = load_row(static_cast<const T*>(a.dout) + i * a.dout_stride[0] + h * a.dout_stride[1], a.D);
-        const float p = expf(__fmaf_rn(dot(x, kj), a.scale, -a.lse[(int64_t)h * a.Tq + i]));
-        const float ds = __fmul_rn(p, dot(g, vj) - delta[(int64_t)h * a.Tq + i]);
+        const float2 st = stat_of(stats, a, i, h);
+        const float p = exp2f(__fmaf_rn(dot(x, kj), c, st.x));
+        const float w = KEYS ? __fmul_rn(p, dot(g, vj) - st.y) : p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ok.v[e] = __fmaf_rn(ds, x.v[e], ok.v[e]);
-          ov.v[e] = __fmaf_rn(p, g.v[e], ov.v[e]);
-        }
+        for (int e = 0; e < 4; ++e) o.v[e] = __fmaf_rn(w, KEYS ? x.v[e] : g.v[e], o.v[e]);
+        done = settled(o, a.D);
       }
   }
-  if (a.dk) store_row(static_cast<T*>(a.dk) + (t * a.Hk + kh) * a.D, a.D, ok, a.scale);
-  if (a.dv) store_row(static_cast<T*>(a.dv) + (t * a.Hk + kh) * a.D, a.D, ov, 1.0f);
+  store_row(static_cast<T*>(KEYS ? a.dk : a.dv) + (t * a.Hk + kh) * a.D, 0, a.D, o, KEYS ? a.scale : 1.0f);
 }
 
 }  // namespace attn

@@ -21,6 +21,7 @@ constexpr long long DRAIN_LIMIT = 1ll << 31;    // waits for copies / MMAs alrea
 // Codes of the waits (emu_device_status).
 enum {
   WAIT_FWD_SLOT = 18, WAIT_FWD_Q, WAIT_FWD_K, WAIT_FWD_V, WAIT_FWD_P, WAIT_FWD_S, WAIT_FWD_O, WAIT_DRAIN,
+  WAIT_BACK_SLOT, WAIT_BACK_FIXED, WAIT_BACK_TILE, WAIT_BACK_STATS, WAIT_BACK_S, WAIT_BACK_P, WAIT_BACK_DP, WAIT_BACK_DS, WAIT_BACK_DONE,
 };
 
 static __device__ int g_wait_error;             // code of the first wait that ran out since the last read (0 = none)
@@ -126,6 +127,14 @@ inline EncodeTiledFn get_encode() {
     return static_cast<EncodeTiledFn>(nullptr);
   }();
   return fn;
+}
+
+// Makes the current device's context this thread's: encoding a tensor map is a driver call, which takes what is current, and
+// in a thread without earlier CUDA calls (an autograd worker) nothing is.
+inline cudaError_t bind_context() {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  return e == cudaSuccess ? cudaSetDevice(dev) : e;
 }
 
 // Rows [tokens][heads][D] of 16-bit elements with 128-byte swizzle: boxes of 64 elements x box_heads x box_tokens; what is

@@ -451,13 +451,15 @@ emu_status emu_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: stream");
   // every kernel's word is taken, so that the next call speaks for later launches alone; the first one set is told
-  int code = 0, code_fp8 = 0, code_attention = 0;
+  int code = 0, code_fp8 = 0, code_attention = 0, code_back = 0;
   e = emu::take_wait_error(&code);
   if (e == cudaSuccess) e = emu::take_fp8_wait_error(&code_fp8);
   if (e == cudaSuccess) e = emu::take_attention_wait_error(&code_attention);
+  if (e == cudaSuccess) e = emu::take_attention_backward_wait_error(&code_back);
   if (e != cudaSuccess) return cuda_status(e, "emu_device_status: error word");
   if (code == 0) code = code_fp8;
   if (code == 0) code = code_attention;
+  if (code == 0) code = code_back;
   if (code == 0) return ok();
   static const char* const kSite[] = {"", "producer stage slot", "producer record slot", "MMA accumulator set",
                                       "MMA stage data", "epilogue accumulator", "epilogue records",
@@ -468,7 +470,11 @@ emu_status emu_device_status(void* stream) {
                                       "8-bit product: epilogue scales", "8-bit product: epilogue accumulator",
                                       "attention: producer slot", "attention: queries", "attention: keys",
                                       "attention: values", "attention: weights", "attention: scores",
-                                      "attention: output", "attention: drain"};
+                                      "attention: output", "attention: drain",
+                                      "attention gradients: producer slot", "attention gradients: fixed tiles",
+                                      "attention gradients: tiles", "attention gradients: statistics",
+                                      "attention gradients: scores", "attention gradients: weights",
+                                      "attention gradients: dp", "attention gradients: ds", "attention gradients: sums"};
   constexpr int kSites = (int)(sizeof(kSite) / sizeof(kSite[0]));
   return fail(EMU_ERR_TIMEOUT,
               "a tensor-core pipeline wait ran out (code %d: %s); outputs of the calls on this device since the "

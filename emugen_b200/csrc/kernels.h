@@ -185,6 +185,7 @@ cudaError_t launch_attention(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream);
 // as take_wait_error, for the waits of attention's kernels
 cudaError_t take_attention_wait_error(int* code);
+cudaError_t take_attention_backward_wait_error(int* code);
 
 // Attention of one token for each sequence over the quantised cache (kv_attend.cu).
 struct KvAttendArgs {

@@ -10,6 +10,9 @@ import math
 import torch
 
 F = 2.0 ** -23
+# A weight exp(s) below f32's smallest normal number, 2^-126, is made 0 (and bf16 has the same smallest one): with the
+# rounding at that border, a weight may be off by 2^-125 whatever its size.
+LOWEST = 2.0 ** -125
 
 
 def half_step(dtype):
@@ -63,7 +66,7 @@ def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None):
             used = seen.any(0)
             c0 = torch.where(used[:, None], c, 0.0)
             o = p @ c0
-            p_err = p * (rel + pu) + (2.0 ** -31 if q.dtype == torch.float16 else 0.0) * seen
+            p_err = p * (rel + pu) + ((2.0 ** -31 if q.dtype == torch.float16 else 0.0) + LOWEST) * seen
             o_t = (p_err + F * n * p) @ c0.abs() + u * o.abs() + low
             out[i0:i1, h], out_t[i0:i1, h] = o, o_t
             if do is None:
@@ -74,14 +77,14 @@ def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None):
             a0, b0 = torch.where(some[:, None], a, 0.0), torch.where(used[:, None], b, 0.0)
             b_err = rel + 2 * lse_t[h, i0:i1, None] + F * 4 * lse[h, i0:i1, None].abs().nan_to_num(0, 0, 0)
             dv[j0:j1, g] += p.t() @ w
-            dv_t[j0:j1, g] += (p * (b_err + u + F * (nq + 64))).t() @ w.abs()
+            dv_t[j0:j1, g] += (p * (b_err + u + F * (nq + 64)) + LOWEST * seen).t() @ w.abs()
             dp = w @ c0.t()
             delta = (w * o).sum(1, keepdim=True)
             dp_err = F * (D + 4) * (w.abs() @ c0.abs().t()) + F * (D + 4) * (w * o).abs().sum(1, keepdim=True) + (w.abs() * o_t).sum(1, keepdim=True)
             ds = p * (dp - delta)
             # (fp16: held to 2^-24 of a bound on |dp - delta| times 2^-15)
             bound = 2 * w.norm(dim=1).amax() * c0.norm(dim=1).amax()
-            ds_err = ds.abs() * (b_err + u) + p * dp_err + (bound * 2.0 ** -36 if q.dtype == torch.float16 else 0.0) * seen
+            ds_err = ds.abs() * (b_err + u) + p * dp_err + LOWEST * (1 + (dp - delta).abs()) * seen + (bound * 2.0 ** -36 if q.dtype == torch.float16 else 0.0) * seen
             dq[i0:i1, h] = ds @ b0 * scale
             dq_t[i0:i1, h] = (ds_err + F * n * ds.abs()) @ b0.abs() * scale
             dk[j0:j1, g] += ds.t() @ a0 * scale

@@ -280,6 +280,22 @@ def test_streams_and_graph_replay():
         assert all(torch.equal(a, b) for a, b in zip(r, w))
 
 
+def test_fresh_thread():
+    """A thread whose first CUDA work is this call."""
+    import threading
+
+    q, k, v, _ = _make([90], [90], 4, 2, 64, torch.bfloat16, 16)
+    c = _tensor([0, 90])
+    want = attention.packed_attention(q, k, v, c)
+    torch.cuda.synchronize()
+    got = []
+    t = threading.Thread(target=lambda: got.append(attention.packed_attention(q, k, v, c)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want)
+
+
 def test_empty_calls():
     for tq, tk, B in ((0, 0, 0), (0, 5, 1), (6, 0, 1), (6, 5, 0)):
         q = torch.randn(tq, 4, 64, device="cuda", dtype=torch.float16, requires_grad=True)
