@@ -24,9 +24,10 @@ def tiny(dtype):
     return {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}[dtype]
 
 
-def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None):
+def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None, v_low=None):
     """{name: (value, tolerance)} for out, lse and, with do, dq, dk, dv; a head and a sequence at a time.  Hidden keys and
-    values are left out of the sums altogether.  p_step: half a step of the type that the weights are rounded to."""
+    values are left out of the sums altogether.  p_step: half a step of the type that the weights are rounded to; v_low
+    (v's shape): the error of one key's share of the output where its weight is below that type's normal numbers."""
     dev = q.device
     u, D = half_step(q.dtype), q.shape[2]
     pu = u if p_step is None else p_step
@@ -68,6 +69,8 @@ def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None):
             o = p @ c0
             p_err = p * (rel + pu) + ((2.0 ** -31 if q.dtype == torch.float16 else 0.0) + LOWEST) * seen
             o_t = (p_err + F * n * p) @ c0.abs() + u * o.abs() + low
+            if v_low is not None:
+                o_t = o_t + seen.double() @ v_low[j0:j1, g]
             out[i0:i1, h], out_t[i0:i1, h] = o, o_t
             if do is None:
                 continue

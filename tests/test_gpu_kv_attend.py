@@ -47,7 +47,8 @@ def _make(lens, Hq, Hk, D, page, fmt, dtype, seed, spread=1.0):
 def _want(q, cache, table, lens, fmt, scale, page):
     k, v = (_stored(cache[i], cache[i + 2], fmt) for i in (0, 1))
     pages = cache[0].shape[0]
-    ks, vs, cu = [], [], [0]
+    block = 128 if fmt == "fp8" else 32
+    ks, vs, low, cu = [], [], [], [0]
     for b, n in enumerate(lens.tolist()):
         n = max(0, min(n, table.shape[1] * page))
         pos = torch.arange(n)
@@ -55,8 +56,15 @@ def _want(q, cache, table, lens, fmt, scale, page):
         ok = (pg >= 0) & (pg < pages)
         at = (pg * page + pos % page)[ok]
         ks.append(k[at]), vs.append(v[at]), cu.append(cu[-1] + len(at))
+        # A weight p * scale is put to 2^6 times its share of at most twice the largest scale of the values' block (some p
+        # is 1 or more) and rounded to fp16: half a subnormal step, 2^-25, is 2^-31 of that scale, times the code.
+        s = cache[3].cpu().flatten(0, 1)[at].double() if fmt == "fp8" else torch.pow(2.0, cache[3].cpu().flatten(0, 1)[at].double() - 127)
+        s = s.nan_to_num(0, 0, 0)
+        code = v[at].abs() / s.repeat_interleave(block, -1)[..., :v.shape[-1]].clamp(min=1e-300)
+        top = s.amax(0, keepdim=True) if len(at) else s
+        low.append((code * top.repeat_interleave(block, -1)[..., :v.shape[-1]] * 2.0 ** -31).nan_to_num(0, 0, 0))
     kk, vv = torch.cat(ks).cuda(), torch.cat(vs).cuda()
-    r = O.attention(q, kk, vv, list(range(len(lens) + 1)), cu, False, scale, p_step=2.0 ** -11)
+    r = O.attention(q, kk, vv, list(range(len(lens) + 1)), cu, False, scale, p_step=2.0 ** -11, v_low=torch.cat(low).cuda())
     return r["out"], (r["lse"][0].t(), r["lse"][1].t())
 
 
