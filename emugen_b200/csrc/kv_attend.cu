@@ -69,39 +69,56 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Copies into shared memory that are waited for later.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool any) {
   const int n = any ? 16 : 0;                                // 0: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy4(uint32_t dst, const uint8_t* src, bool any) {
+  const int n = any ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <int N> __device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+}
+// two fp16 factors of a power of two each
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// 2^e as fp16 bits: subnormal below -14, 0 below -24, infinity above 15
+__device__ __forceinline__ uint32_t half_pow2(int e) { return e > 15 ? 0x7C00u : e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u; }
 
-// The shapes of a format at a padded head size.
+// Who holds which of a row's DP elements.  Keys (k = 16 to an MMA, 4 lanes to a key): lane c's are KX places of KW words.
+// Values (8 lanes to a row): lane g's are VX places of VW words.  A stage holds 16 rows of keys, 16 of values and their scales; its
+// rows are 16 bytes further apart than they are long, so that the lanes that read together meet different banks.
 template <int FORMAT, int DP> struct Shape {
   static constexpr bool FP8 = FORMAT == EMU_KV_FP8;
   static constexpr int ROW = FP8 ? DP : DP / 2;              // bytes of a row of codes
-  static constexpr int CHUNKS = ROW / 16;
-  static constexpr int BLOCKS = FP8 ? (DP + 127) / 128 : DP / 32;
-  static constexpr int CODES = KEYS * ROW;                   // keys (or values) of a stage
-  static constexpr int SCALES = BLOCKS * KEYS * 4;           // [block][key], 32 bits each
-  static constexpr int STAGE = 2 * (CODES + SCALES);
+  static constexpr int KW = ROW >= 64 ? 4 : 2, KX = ROW / (16 * KW);
+  static constexpr int VW = ROW >= 128 ? 4 : ROW / 32, VX = ROW / (32 * VW);
+  static constexpr int BLOCKS = FP8 ? (DP + 127) / 128 : 1;  // separately scaled sums of the scores, weights of the values
+  static constexpr int CODES = FP8 ? 4 : 8;                  // codes in a word
+  static constexpr int PITCH = ROW + 16, SCALE = FP8 ? 4 * BLOCKS : DP == 256 ? 8 : 4;   // bytes from row to row, of a row's scales
+  static constexpr int STAGE = 2 * KEYS * (PITCH + SCALE);
   static constexpr int STAGES = FP8 && DP >= 128 ? 3 : 4;    // what ctas_per_sm leaves room for
-  static constexpr int JOIN = 16 * (DP + 4) * 4;             // a warp's sums
-  static constexpr int WARP = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
-  static constexpr int SMEM = WARPS * WARP + WARPS * 16 * 8 + WARPS * STAGES * 4 + 64;
+  static constexpr int CHUNKS = ROW / 16, COPIES = KEYS * CHUNKS / 32;   // 16-byte copies of a row, of keys (values) to a lane
+  static_assert(CHUNKS <= 32 && COPIES >= 1, "a lane copies at least one chunk of a step");
+  // bytes of lane c's place x
+  static __host__ __device__ constexpr int key_place(int c, int x) { return (KX == 1 ? c : 8 * (x / 2) + 2 * c + x % 2) * 4 * KW; }
+  static __host__ __device__ constexpr int value_place(int g, int x) { return (g + 8 * x) * 4 * VW; }
 };
-// Where chunk `c` of row r lies: lines of 128 bytes, the chunk's place in its line turned so that the lanes that read
-// together meet all banks (K: 8 rows and 4 neighbours each; V: every other row and 8 neighbours).
-template <int FORMAT, int DP, bool VALUES> __device__ __forceinline__ uint32_t place(int r, int c) {
-  using S = Shape<FORMAT, DP>;
-  const int at = r * S::CHUNKS + c, line = at >> 3;
-  int turn;
-  if (S::FP8) {
-    if (DP == 64) turn = (line * 2) & 7;
-    else turn = VALUES ? r & 7 : (r & 1) * 4;
-  } else {
-    turn = DP == 64 ? line & 1 : DP == 128 ? line & 3 : r & 7;
-  }
-  return (uint32_t)(line * 128 + ((at & 7) ^ turn) * 16);
-}
+constexpr int JOIN = 4;                                      // floats between the rows of the join's buffer
 
 // The tiles of a sequence (of each of its heads).
 __device__ __forceinline__ int64_t tiles_of(const KvAttendArgs& a, int64_t b) {
@@ -177,21 +194,23 @@ struct Ending {
 };
 
 // As many as registers (and shared memory) allow.
-constexpr int ctas_per_sm(int DP, bool two) { return DP == 256 ? 2 : DP == 128 && two ? 3 : 4; }
+constexpr int ctas_per_sm(int format, int DP, bool two) { return DP == 256 ? 2 : DP == 128 && (two || format == EMU_KV_FP8) ? 3 : 4; }
 constexpr int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 template <typename T, int FORMAT, int DP, bool TWO>
-__global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ Plan pl) {
+__global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ Plan pl) {
   using S = Shape<FORMAT, DP>;
   // d-tiles of 16 (DT), those of a block of values (PER), groups of 8 heads (R)
-  constexpr int STAGES = S::STAGES, NB = S::BLOCKS, STEPS = DP / 16, DT = DP / 16, PER = DT / NB, R = TWO ? 2 : 1;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int NB = S::BLOCKS, STEPS = DP / 16, DT = DP / 16, PER = DT / NB, R = TWO ? 2 : 1;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t tmp[WARPS], found[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  uint8_t* mine = smem + warp * S::WARP;
-  float2* join_ml = reinterpret_cast<float2*>(smem + WARPS * S::WARP);            // [warp][16]
-  uint32_t* live = reinterpret_cast<uint32_t*>(join_ml + WARPS * 16) + warp * STAGES;
-  const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
+  constexpr int STAGES = S::STAGES, RING = STAGES * S::STAGE;
+  static_assert(RING >= 8 * (DP + JOIN) * 4, "the ring holds the warp's sums afterwards");
+  uint8_t* ring = smem + warp * RING;
+  const uint32_t ring_u = (uint32_t)__cvta_generic_to_shared(ring);
+  float* sums = reinterpret_cast<float*>(ring);              // [8 rows][DP + 4]
+  float2* join_ml = reinterpret_cast<float2*>(smem + WARPS * RING);                // [warp][8]
   const int D = a.D, HV = a.Hk * pl.groups, group = a.Hq / a.Hk;
   const Parts parts = parts_of(a.workspace, pl.ctas, pl.rows, D);
 
@@ -245,99 +264,115 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(con
     // ---- steps of 16 keys; the warps take them in turn
     const int key0 = (int)(tile0 * TILE) + warp * KEYS, end = (int)min((int64_t)len, tile1 * TILE);
     const int steps = (int)(tile1 - tile0);
-    const int my = lane & 15;
-    // the page of this lane's key of step i (of all of the step's keys); -1 past the end
+    const int RB = S::FP8 ? D : D / 2, nb = S::FP8 ? (D + 127) / 128 : D / 32;
+    constexpr int SZ = S::FP8 ? 4 : 1;                       // bytes of a scale
+    // from slot to slot, in bytes (16 slots stay below 2^32)
+    const uint32_t head_row = (uint32_t)(a.Hk * RB), head_scale = (uint32_t)(a.Hk * nb * SZ);
+    // The page of step i's keys (of its key lane % 16 where a step may lie in several); -1 past the end.
     auto page_of = [&](int i) {
-      const int key = key0 + i * TILE + (pl.whole_steps ? 0 : my);
+      const int key = key0 + i * TILE + (pl.whole_steps ? 0 : lane & 15);
       return i < steps && key < end ? __ldg(table + (uint32_t)key / pl.page_size) : -1;
     };
-    const int RB = S::FP8 ? D : D / 2, nb = S::FP8 ? (D + 127) / 128 : D / 32, chunks = RB / 16;
-    uint32_t sc[NB];                                         // scales on their way: lanes 0-15 keys', 16-31 values'
-    // codes of step i into its stage, its scales into registers
-    auto fetch = [&](int i, int stage, int page) {
-      const int key = key0 + i * TILE;
-      const bool page_ok = page >= 0 && page < a.num_pages;
-      const uint32_t st = mine_u + stage * S::STAGE;
-      const int rem = (int)((uint32_t)(key + (pl.whole_steps ? 0 : my)) % pl.page_size);
-      int64_t row = page_ok ? ((int64_t)page * a.page_size + rem) * a.Hk + kh : 0;
-      uint32_t mask;
-      if (pl.whole_steps) {
-        const int n = page_ok ? min(KEYS, end - key) : 0;
-        mask = (1u << n) - 1;
-        const int64_t base = row * RB;
+    // This lane's rows: keys g and 8 + g for the scores' operand; keys 2 c, 2 c + 1, 8 + 2 c and 9 + 2 c for the values' and for what
+    // is known of a score.
+    struct Step {
+      uint32_t live;                                         // a bit for each key that is seen
+      int64_t slot;                                          // of the first key (of key lane % 16)
+    };
+    auto step_of = [&](int i, int page) {
+      Step t;
+      const int key = key0 + i * TILE + (pl.whole_steps ? 0 : lane & 15);
+      const bool ok = page >= 0 && page < a.num_pages;
+      t.slot = ok ? (int64_t)page * a.page_size + (uint32_t)key % pl.page_size : 0;
+      t.live = pl.whole_steps ? (ok ? (1u << min(KEYS, end - key)) - 1 : 0) : __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
+      return t;
+    };
+    // A step's codes and scales on their way into stage `st`.  Where all of its keys are seen and lie behind one another and D
+    // fills the places, without a test for each copy: addresses and tests were half of the kernel's instructions.
+    const bool full = pl.whole_steps && D == DP;
+    constexpr int ROWS = 32 / S::CHUNKS;                     // rows that the warp copies at once
+    const int my_row = lane / S::CHUNKS, my_chunk = lane % S::CHUNKS, my = lane & 15;
+    const uint32_t my_src = (uint32_t)my_row * head_row + my_chunk * 16, my_dst = my_row * S::PITCH + my_chunk * 16;
+    uint32_t held[2];                                        // MXFP4: scale bytes of key (value) lane % 16 until they are put down
+    auto fetch = [&](const Step& t, int st) {
+      const uint32_t dst = ring_u + st * S::STAGE, dst_s = dst + 2 * KEYS * S::PITCH + (lane >> 4) * KEYS * S::SCALE + my * S::SCALE;
+      const uint8_t* scales = static_cast<const uint8_t*>(lane < 16 ? a.scales[0] : a.scales[1]) + kh * nb * SZ;
+      const bool seen = t.live >> my & 1;
+      if (full && t.live == 0xFFFFu) {
+        const int64_t base = t.slot * head_row + kh * RB;
+        const uint8_t* k = a.cache[0] + base;
+        const uint8_t* v = a.cache[1] + base;
 #pragma unroll
-        for (int x = 0; x < KEYS * S::CHUNKS / 32; ++x) {
-          const int idx = lane + 32 * x, r = idx / S::CHUNKS, ch = idx % S::CHUNKS;
-          const bool any = r < n && ch < chunks;
-          const int64_t src = any ? base + (int64_t)r * a.Hk * RB + ch * 16 : 0;
-          copy16(st + place<FORMAT, DP, false>(r, ch), a.cache[0] + src, any);
-          copy16(st + S::CODES + place<FORMAT, DP, true>(r, ch), a.cache[1] + src, any);
+        for (int x = 0; x < S::COPIES; ++x) {
+          const uint32_t from = my_src + x * ROWS * head_row;
+          copy16(dst + my_dst + x * ROWS * S::PITCH, k + from);
+          copy16(dst + KEYS * S::PITCH + my_dst + x * ROWS * S::PITCH, v + from);
         }
-        row += (int64_t)my * a.Hk;
+        scales += (t.slot + my) * head_scale;
       } else {
-        mask = __ballot_sync(0xFFFFFFFFu, page_ok) & 0xFFFFu;
-        const int64_t base = row * RB;
 #pragma unroll
-        for (int x = 0; x < KEYS * S::CHUNKS / 32; ++x) {
-          const int idx = lane + 32 * x, r = idx / S::CHUNKS, ch = idx % S::CHUNKS;
-          const int64_t from = __shfl_sync(0xFFFFFFFFu, base, r);
-          const bool any = (mask >> r & 1) && ch < chunks;
-          const int64_t src = any ? from + ch * 16 : 0;
-          copy16(st + place<FORMAT, DP, false>(r, ch), a.cache[0] + src, any);
-          copy16(st + S::CODES + place<FORMAT, DP, true>(r, ch), a.cache[1] + src, any);
+        for (int x = 0; x < S::COPIES; ++x) {
+          const int r = my_row + x * ROWS;
+          const int64_t slot = pl.whole_steps ? t.slot + r : __shfl_sync(0xFFFFFFFFu, t.slot, r);
+          const bool any = (t.live >> r & 1) && my_chunk * 16 < RB;
+          const int64_t from = any ? slot * head_row + kh * RB + my_chunk * 16 : 0;
+          copy16(dst + my_dst + x * ROWS * S::PITCH, a.cache[0] + from, any);
+          copy16(dst + KEYS * S::PITCH + my_dst + x * ROWS * S::PITCH, a.cache[1] + from, any);
+        }
+        scales += seen ? (pl.whole_steps ? t.slot + my : t.slot) * head_scale : 0;
+      }
+      if (S::FP8) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) copy4(dst_s + 4 * k, k < nb ? scales + 4 * k : scales, seen && k < nb);
+      } else {
+        held[0] = held[1] = 0;
+        if (seen && pl.wide_scales) {
+          if (DP == 64) held[0] = __ldg(reinterpret_cast<const uint16_t*>(scales));
+          else held[0] = __ldg(reinterpret_cast<const uint32_t*>(scales));
+          if (DP == 256) held[1] = __ldg(reinterpret_cast<const uint32_t*>(scales) + 1);
+        } else if (seen) {
+#pragma unroll
+          for (int k = 0; k < DP / 32; ++k)
+            if (k < nb) held[k / 4] |= (uint32_t)__ldg(scales + k) << (8 * (k & 3));
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      const bool ok = mask >> my & 1;
-      const void* src = lane < 16 ? a.scales[0] : a.scales[1];
-      if (S::FP8) {
-#pragma unroll
-        for (int k = 0; k < NB; ++k) sc[k] = ok && k < nb ? __float_as_uint(__ldg(static_cast<const float*>(src) + row * nb + k)) : 0;
-      } else {
-        const uint8_t* p = static_cast<const uint8_t*>(src) + row * nb;
-        if (pl.wide_scales) {
-          uint64_t w = 0;
-          if (ok) w = NB == 2 ? __ldg(reinterpret_cast<const uint16_t*>(p)) : NB == 4 ? __ldg(reinterpret_cast<const uint32_t*>(p)) : __ldg(reinterpret_cast<const unsigned long long*>(p));
-#pragma unroll
-          for (int k = 0; k < NB; ++k) sc[k] = (uint32_t)(w >> (8 * k)) & 255u;
-        } else {
-#pragma unroll
-          for (int k = 0; k < NB; ++k) sc[k] = ok && k < nb ? __ldg(p + k) : 0;
-        }
-      }
-      if (lane == 0) live[stage] = mask;
     };
-    // the scales that the last `fetch` asked for
-    auto put_scales = [&](int stage) {
-      uint32_t* dst = reinterpret_cast<uint32_t*>(mine + stage * S::STAGE + 2 * S::CODES + (lane < 16 ? 0 : S::SCALES));
+    auto put_scales = [&](int st) {
+      if (S::FP8) return;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(ring + st * S::STAGE + 2 * KEYS * S::PITCH + (lane >> 4) * KEYS * S::SCALE + my * S::SCALE);
 #pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        // MXFP4 keys: 2^(byte - 127); byte 0 is f32's subnormal 2^-127, byte 255 infinity.  Values: the byte.
-        const uint32_t v = S::FP8 || lane >= 16 ? sc[k] : sc[k] ? sc[k] << 23 : 0x00400000u;
-        dst[k * KEYS + my] = v;
-      }
+      for (int k = 0; k < S::SCALE / 4; ++k) dst[k] = held[k];
     };
-    int page;
-    uint32_t held[STAGES - 1][NB];
+    uint32_t lives[STAGES];                                  // of the steps under way, the next one first
+    int page_next;
     {
       int pages[STAGES];
 #pragma unroll
       for (int i = 0; i < STAGES; ++i) pages[i] = page_of(i);
+      uint32_t early[STAGES][2];
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i) {
-        fetch(i, i, pages[i]);
-#pragma unroll
-        for (int k = 0; k < NB; ++k) held[i][k] = sc[k];
+        const Step t = step_of(i, pages[i]);
+        lives[i] = t.live;
+        fetch(t, i);
+        early[i][0] = held[0], early[i][1] = held[1];
       }
-      page = pages[STAGES - 1];
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) {
+        held[0] = early[i][0], held[1] = early[i][1];
+        put_scales(i);
+      }
+      page_next = pages[STAGES - 1];
     }
 
     // ---- q: this lane's elements of rows g and g + 8, as the MMAs' A operands
     uint32_t q[STEPS][2 * R];
     float qf[R];                                             // what a score of the row is multiplied by
     {
-      auto place_of = [&](int s) {                           // the first of a step's two pairs
-        return S::FP8 ? (c + 4 * (s >> 2)) * 16 + (s & 3) * 4 : (s >> 1) * 32 + c * 8 + (s & 1) * 4;
+      auto place_of = [&](int z) {                           // the first of a step's two pairs
+        constexpr int PER_PLACE = S::KW * S::CODES / 4;      // steps of one place
+        return S::key_place(c, z / PER_PLACE) / 4 * S::CODES + z % PER_PLACE * 4;
       };
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -374,19 +409,15 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(con
           for (int e = 0; e < 2; ++e) q[s][e * R + r] = pack_half(value(raw[s][e], 0) * f, value(raw[s][e], 1) * f);
       }
     }
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-#pragma unroll
-      for (int k = 0; k < NB; ++k) sc[k] = held[i][k];
-      put_scales(i);
-    }
 
     // o[n][r]: elements d (rows of the MMA) of heads 8 r + 2 c and 8 r + 2 c + 1; m and l are those of heads g + 8 r
     float o[DT][R][4] = {}, m[R], l[R] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) m[r] = -INFINITY;
-    int ref[NB];                                             // exponent of the largest scale of values so far
-    float up0[NB], up1[NB];                                  // FP8: 2^(6 - (ref - 127)), in two factors that both exist
+    // FP8: the exponent of the largest scale of values so far, for each block, the same in the whole warp; MXFP4: that of
+    // this lane's block.  up: FP8, 2^(6 - (ref - 127)), in two factors that both exist.
+    int ref[NB], kref = -1000;                               // kref: MXFP4, the largest exponent of the keys' scales so far
+    float up0[NB], up1[NB];
 #pragma unroll
     for (int k = 0; k < NB; ++k) ref[k] = -1000, up0[k] = up1[k] = 1.0f;
 
@@ -394,57 +425,105 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(con
     for (int i = 0; i < steps; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();
-      // the next step to fetch, into the stage that was read last
-      const int next = page_of(i + STAGES);
-      fetch(i + STAGES - 1, st_new, page);
-      page = next;
-      const uint8_t* kc = mine + st * S::STAGE;
-      const uint8_t* vc = kc + S::CODES;
-      const float* ks = reinterpret_cast<const float*>(kc + 2 * S::CODES);
-      const uint32_t* vs = reinterpret_cast<const uint32_t*>(kc + 2 * S::CODES + S::SCALES);
-      const uint32_t mask = live[st];
+      // the step to fetch next, into the stage that was read last
+      const uint32_t live = lives[0];
+#pragma unroll
+      for (int x = 0; x + 2 < STAGES; ++x) lives[x] = lives[x + 1];
+      {
+        const Step t = step_of(i + STAGES - 1, page_next);
+        page_next = page_of(i + STAGES);
+        lives[STAGES - 2] = t.live;
+        fetch(t, st_new);
+      }
+      const uint8_t* keys = ring + st * S::STAGE;
+      const uint8_t* values = keys + KEYS * S::PITCH;
+      const uint8_t* key_scales = values + KEYS * S::PITCH;
+      const uint8_t* value_scales = key_scales + KEYS * S::SCALE;
+      uint32_t ksc[S::FP8 ? 4 : 2][S::FP8 ? NB : S::KX], vsc[4][NB];
+      if (S::FP8) {
+#pragma unroll
+        for (int y = 0; y < 4; y += 2) {                     // keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c
+          uint32_t w[2 * NB];
+          read_words(key_scales + (4 * y + 2 * c) * S::SCALE, w);
+#pragma unroll
+          for (int k = 0; k < 2 * NB; ++k) ksc[y + k / NB][k % NB] = w[k];
+          read_words(value_scales + (4 * y + 2 * c) * S::SCALE, w);
+#pragma unroll
+          for (int k = 0; k < 2 * NB; ++k) vsc[y + k / NB][k % NB] = w[k];
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int x = 0; x < S::KX; ++x) ksc[y][x] = key_scales[(8 * y + g) * S::SCALE + S::key_place(c, x) / 16];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) vsc[y][0] = value_scales[(y / 2 * 8 + 2 * c + y % 2) * S::SCALE + S::value_place(g, 0) / 16];
+      }
       // ---- scores of rows g (and g + 8) with keys 8 t + 2 c and 8 t + 2 c + 1
       float s[2][2 * R];
+      if (!S::FP8) {
+        int most = -1000;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int x = 0; x < S::KX; ++x)
+            if (ksc[y][x] != 255) most = max(most, (int)ksc[y][x]);
+        // codes are up to 6: 2^(8 + 4) times that is still an fp16
+        if (__any_sync(0xFFFFFFFFu, most > kref + 4)) kref = __reduce_max_sync(0xFFFFFFFFu, most);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        uint32_t kw[S::KX][S::KW];
+#pragma unroll
+        for (int x = 0; x < S::KX; ++x) read_words(keys + (8 * t + g) * S::PITCH + S::key_place(c, x), kw[x]);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
           float acc[4] = {};
           if (S::FP8) {
 #pragma unroll
-            for (int x = 2 * k; x < 2 * k + 2 && x < DP / 64; ++x) {
-              const uint4 w = *reinterpret_cast<const uint4*>(kc + place<FORMAT, DP, false>(8 * t + g, c + 4 * x));
-              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+            for (int x = 2 * k; x < 2 * k + 2 && x < S::KX; ++x)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const int z = 4 * x + y;
-                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, half2_of_e4m3(ws[y] & 0xFFFFu), half2_of_e4m3(ws[y] >> 16));
+              for (int y = 0; y < S::KW; ++y) {
+                const int z = S::KW * x + y;
+                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, half2_of_e4m3(kw[x][y] & 0xFFFFu), half2_of_e4m3(kw[x][y] >> 16));
+              }
+          } else {
+#pragma unroll
+            for (int x = 0; x < S::KX; ++x) {
+              const uint32_t f = half_pow2(ksc[t][x] == 255 ? 16 : (int)ksc[t][x] - kref + 8) * 0x10001u;
+#pragma unroll
+              for (int y = 0; y < 2 * S::KW; ++y) {
+                const int z = 2 * S::KW * x + y;
+                const uint32_t w = kw[x][y / 2] >> (16 * (y & 1));
+                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, mul_half2(half2_of_e2m1(w & 255u), f), mul_half2(half2_of_e2m1(w >> 8 & 255u), f));
               }
             }
-          } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(kc + place<FORMAT, DP, false>(8 * t + g, k) + 4 * c);
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const int z = 2 * k + y;
-              mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, half2_of_e2m1(w >> (16 * y) & 255u), half2_of_e2m1(w >> (16 * y + 8) & 255u));
-            }
           }
-          const float2 f = *reinterpret_cast<const float2*>(ks + k * KEYS + 8 * t + 2 * c);
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            s[t][2 * r] = k ? __fmaf_rn(acc[2 * r], f.x, s[t][2 * r]) : __fmul_rn(acc[2 * r], f.x);
-            s[t][2 * r + 1] = k ? __fmaf_rn(acc[2 * r + 1], f.y, s[t][2 * r + 1]) : __fmul_rn(acc[2 * r + 1], f.y);
+          for (int e = 0; e < 2 * R; ++e) {
+            const float v = acc[e];
+            if (S::FP8) {
+              const float f = __uint_as_float(ksc[2 * t + (e & 1)][k]);
+              s[t][e] = k ? __fmaf_rn(v, f, s[t][e]) : __fmul_rn(v, f);
+            } else {
+              s[t][e] = v;
+            }
           }
         }
 #pragma unroll
         for (int e = 0; e < 2 * R; ++e) s[t][e] = __fmul_rn(s[t][e], qf[e >> 1]);
+        if (!S::FP8) {
+          const int up = max(kref, 0) - 135;                 // 2^(kref - 127 - 8)
+#pragma unroll
+          for (int e = 0; e < 2 * R; ++e) s[t][e] = s[t][e] * pow2(up / 2) * pow2(up - up / 2);
+        }
       }
-      if (mask != 0xFFFFu) {
+      if (live != 0xFFFFu) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2 * R; ++e)
-            if (!(mask >> (8 * t + 2 * c + (e & 1)) & 1)) s[t][e] = -INFINITY;
+            if (!(live >> (8 * t + 2 * c + (e & 1)) & 1)) s[t][e] = -INFINITY;
       }
       // ---- the running maximum: held up to a factor of 2^8
       bool grow = false;
@@ -476,20 +555,28 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(con
           l[r] += s[t][2 * r] + s[t][2 * r + 1];
         }
       }
-      // ---- values, block by block: O^T += V^T P^T, weight = p * scale / 2^ref * 2^6 (below 2^8 * 2 * 2^6)
-      const int rv[4] = {2 * c, 2 * c + 1, 8 + 2 * c, 9 + 2 * c};                  // this lane's keys
+      // ---- values: O^T += V^T P^T
+      uint32_t vw[4][S::VX][S::VW];
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < S::VX; ++x) read_words(values + (y / 2 * 8 + 2 * c + y % 2) * S::PITCH + S::value_place(g, x), vw[y][x]);
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        const uint2 w0 = *reinterpret_cast<const uint2*>(vs + k * KEYS + 2 * c), w1 = *reinterpret_cast<const uint2*>(vs + k * KEYS + 8 + 2 * c);
-        const uint32_t sw[4] = {w0.x, w0.y, w1.x, w1.y};
         int most = -1000;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int e = S::FP8 ? (int)(sw[x] >> 23 & 255u) : (int)sw[x];
+          const int e = S::FP8 ? (int)(vsc[x][k] >> 23 & 255u) : (int)vsc[x][0];
           if (e != 255) most = max(most, e);                 // (infinities and NaN go through as they are)
         }
         if (__any_sync(0xFFFFFFFFu, most > ref[k])) {
-          most = __reduce_max_sync(0xFFFFFFFFu, most);
+          // MXFP4: the four lanes that share the rows g of the MMAs have the same block and the same ref
+          if (S::FP8) {
+            most = __reduce_max_sync(0xFFFFFFFFu, most);
+          } else {
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = max(max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2)), ref[k]);
+          }
           const float down = ref[k] < 0 ? 1.0f : pow2(ref[k] - most);
 #pragma unroll
           for (int n = k * PER; n < (k + 1) * PER; ++n)
@@ -498,107 +585,108 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(DP, TWO)) kv_attend_kernel(con
 #pragma unroll
               for (int y = 0; y < 4; ++y) o[n][r][y] *= down;
           ref[k] = most;
-          const int up = 133 - most;
+          const int up = 133 - max(most, 0);
           up0[k] = pow2(up / 2), up1[k] = pow2(up - up / 2);
         }
-        float f[4];
+        // weights as fp16.  FP8: p * scale / 2^ref * 2^6 (below 2^8 * 2 * 2^6).  MXFP4: p * 2^7, and the codes are multiplied
+        // by scale / 2^ref * 2^8.
+        uint32_t p[R][2], f01 = 0, f23 = 0;
+        if (S::FP8) {
+          float f[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          f[x] = S::FP8 ? __uint_as_float(sw[x]) * up0[k] * up1[k] : sw[x] == 255 ? INFINITY : pow2((int)sw[x] - ref[k] + 6);
-        uint32_t p[R][2];
+          for (int x = 0; x < 4; ++x) f[x] = __uint_as_float(vsc[x][k]) * up0[k] * up1[k];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+          for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) p[r][t] = pack_half(s[t][2 * r] * f[2 * t], s[t][2 * r + 1] * f[2 * t + 1]);
+            for (int t = 0; t < 2; ++t) p[r][t] = pack_half(s[t][2 * r] * f[2 * t], s[t][2 * r + 1] * f[2 * t + 1]);
+        } else {
+          uint32_t f[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) f[x] = half_pow2(vsc[x][0] == 255 ? 16 : (int)vsc[x][0] - ref[0] + 8);
+          f01 = f[0] | f[1] << 16, f23 = f[2] | f[3] << 16;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) p[r][t] = pack_half(s[t][2 * r] * 128.0f, s[t][2 * r + 1] * 128.0f);
+        }
         // a tile of 16 elements: rows g and g + 8 of the MMA are two neighbours of this lane's, keys in pairs
         auto step = [&](int n, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
           for (int r = 0; r < R; ++r) mma(o[n][r], a0, a1, a2, a3, p[r][0], p[r][1]);
         };
         if (S::FP8) {
-          // block k's codes of lane g: elements 128 k + 2 PER g .. of the four rows
-          uint32_t w[4][4];
+          const int x = DP == 256 ? k : 0;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            if (DP == 64) {
-              const uint2 v = *reinterpret_cast<const uint2*>(vc + place<FORMAT, DP, true>(rv[y], g >> 1) + (g & 1) * 8);
-              w[y][0] = v.x, w[y][1] = v.y, w[y][2] = w[y][3] = 0;
-            } else {
-              const uint4 v = *reinterpret_cast<const uint4*>(vc + place<FORMAT, DP, true>(rv[y], 8 * k + g));
-              w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
-            }
-          }
-#pragma unroll
-          for (int z = 0; z < PER / 2; ++z) {
-            const uint32_t x0 = __byte_perm(w[0][z], w[1][z], 0x5140), x1 = __byte_perm(w[0][z], w[1][z], 0x7362);
-            const uint32_t y0 = __byte_perm(w[2][z], w[3][z], 0x5140), y1 = __byte_perm(w[2][z], w[3][z], 0x7362);
+          for (int z = 0; z < S::VW; ++z) {
+            const uint32_t x0 = __byte_perm(vw[0][x][z], vw[1][x][z], 0x5140), x1 = __byte_perm(vw[0][x][z], vw[1][x][z], 0x7362);
+            const uint32_t y0 = __byte_perm(vw[2][x][z], vw[3][x][z], 0x5140), y1 = __byte_perm(vw[2][x][z], vw[3][x][z], 0x7362);
             step(k * PER + 2 * z, half2_of_e4m3(x0 & 0xFFFFu), half2_of_e4m3(x0 >> 16), half2_of_e4m3(y0 & 0xFFFFu), half2_of_e4m3(y0 >> 16));
             step(k * PER + 2 * z + 1, half2_of_e4m3(x1 & 0xFFFFu), half2_of_e4m3(x1 >> 16), half2_of_e4m3(y1 & 0xFFFFu), half2_of_e4m3(y1 >> 16));
           }
         } else {
-          // block k: elements 32 k + 4 g .. + 3 of the four rows
-          uint32_t w[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) w[y] = *reinterpret_cast<const uint16_t*>(vc + place<FORMAT, DP, true>(rv[y], k) + 2 * g);
-          // pairs of rows: their nibbles side by side in a byte
-          const uint32_t x0 = (w[0] & 0x0F0Fu) | (w[1] & 0x0F0Fu) << 4, x1 = (w[0] >> 4 & 0x0F0Fu) | (w[1] & 0xF0F0u);
-          const uint32_t y0 = (w[2] & 0x0F0Fu) | (w[3] & 0x0F0Fu) << 4, y1 = (w[2] >> 4 & 0x0F0Fu) | (w[3] & 0xF0F0u);
-          step(2 * k, half2_of_e2m1(x0 & 255u), half2_of_e2m1(x1 & 255u), half2_of_e2m1(y0 & 255u), half2_of_e2m1(y1 & 255u));
-          step(2 * k + 1, half2_of_e2m1(x0 >> 8), half2_of_e2m1(x1 >> 8), half2_of_e2m1(y0 >> 8), half2_of_e2m1(y1 >> 8));
+          for (int z = 0; z < S::VW; ++z) {
+            // pairs of rows: their nibbles side by side in a byte, elements 0, 2, 4, 6 of the word and 1, 3, 5, 7
+            const uint32_t w0 = vw[0][0][z], w1 = vw[1][0][z], w2 = vw[2][0][z], w3 = vw[3][0][z];
+            const uint32_t x0 = (w0 & 0x0F0F0F0Fu) | (w1 << 4 & 0xF0F0F0F0u), x1 = (w0 >> 4 & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u);
+            const uint32_t y0 = (w2 & 0x0F0F0F0Fu) | (w3 << 4 & 0xF0F0F0F0u), y1 = (w2 >> 4 & 0x0F0F0F0Fu) | (w3 & 0xF0F0F0F0u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              step(4 * z + e, mul_half2(half2_of_e2m1(x0 >> 8 * e & 255u), f01), mul_half2(half2_of_e2m1(x1 >> 8 * e & 255u), f01),
+                   mul_half2(half2_of_e2m1(y0 >> 8 * e & 255u), f23), mul_half2(half2_of_e2m1(y1 >> 8 * e & 255u), f23));
+          }
         }
       }
-      // the scales asked for above; their stage is read next in STAGES - 1 steps
-      put_scales(st_new);
+      put_scales(st_new);                                    // asked for above; their stage is read in STAGES - 1 steps
       st_new = st;
       if (++st == STAGES) st = 0;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-
-    // ---- join the warps
     __syncwarp();
-    float* sums = reinterpret_cast<float*>(mine);            // [row][DP + 4], over the warp's own stages
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-      if (c == 0) join_ml[warp * 16 + g + 8 * r] = make_float2(m[r], l[r]);
-#pragma unroll
-      for (int n = 0; n < DT; ++n) {
-        const int up = max(ref[n / PER], 0) - 133;           // 2^(ref - 127 - 6)
-        const float f0 = pow2(up / 2), f1 = pow2(up - up / 2);
-        const int d = (n / PER) * 16 * PER + g * 2 * PER + 2 * (n % PER);
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          *reinterpret_cast<float2*>(sums + (8 * r + 2 * c + y) * (DP + 4) + d) = make_float2(o[n][r][y] * f0 * f1, o[n][r][2 + y] * f0 * f1);
-      }
-    }
-    __syncthreads();
+
+    // ---- join the warps, 8 heads at a time
     const bool whole = tile0 == 0 && tile1 == per - EXTRA;
     // a CTA's first segment may be the rest of a (sequence, head), its last one the beginning of one
     const int64_t slot = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
     if (!whole && tile1 == per - EXTRA) ending = {b * a.Hq + h0, rows, deal.owner(start + EXTRA)};
-    for (int row = 0; row < rows; ++row) {
-      float2 ml[WARPS];
-      float t = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) ml[w] = join_ml[w * 16 + row], t = fmaxf(t, ml[w].x);
-      const float sh = t == -INFINITY ? 0.0f : t;
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+      if (c == 0) join_ml[warp * 8 + g] = make_float2(m[r], l[r]);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) ml[w].x = exp2_approx(ml[w].x - sh), sum = __fmaf_rn(ml[w].y, ml[w].x, sum);
-      const int64_t i = b * a.Hq + h0 + row;
-      for (int d = threadIdx.x; d < D; d += NT) {
-        float v = 0.0f;
+      for (int n = 0; n < DT; ++n) {
+        const int up = max(ref[n / PER], 0) - (S::FP8 ? 133 : 142);                // 2^(ref - 127 - 6), MXFP4: - 7 - 8
+        const float f0 = pow2(up / 2), f1 = pow2(up - up / 2);
+        const int d = (n / PER) * 16 * PER + g * 2 * PER + 2 * (n % PER);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) v = __fmaf_rn(reinterpret_cast<const float*>(smem + w * S::WARP)[row * (DP + 4) + d], ml[w].x, v);
-        if (whole) static_cast<T*>(a.out)[i * D + d] = narrow<T>(sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
-        else parts.o[(slot * pl.rows + row) * D + d] = v;
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<float2*>(sums + (2 * c + y) * (DP + JOIN) + d) = make_float2(o[n][r][y] * f0 * f1, o[n][r][2 + y] * f0 * f1);
       }
-      if (threadIdx.x == 0) {
-        if (!whole) parts.ml[slot * pl.rows + row] = make_float2(t, sum);
-        else if (a.lse) a.lse[i] = sum > 0.0f ? (t + log2f(sum)) * 0.6931471805599453f : sum == 0.0f ? -INFINITY : sum;
+      __syncthreads();
+      for (int row = 0; row < min(8, rows - 8 * r); ++row) {
+        float2 ml[WARPS];
+        float t = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) ml[w] = join_ml[w * 8 + row], t = fmaxf(t, ml[w].x);
+        const float sh = t == -INFINITY ? 0.0f : t;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) ml[w].x = exp2_approx(ml[w].x - sh), sum = __fmaf_rn(ml[w].y, ml[w].x, sum);
+        const int64_t i = b * a.Hq + h0 + 8 * r + row, at_slot = slot * pl.rows + 8 * r + row;
+        for (int d = threadIdx.x; d < D; d += NT) {
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) v = __fmaf_rn(reinterpret_cast<const float*>(smem + w * RING)[row * (DP + JOIN) + d], ml[w].x, v);
+          if (whole) static_cast<T*>(a.out)[i * D + d] = narrow<T>(sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
+          else parts.o[at_slot * D + d] = v;
+        }
+        if (threadIdx.x == 0) {
+          if (!whole) parts.ml[at_slot] = make_float2(t, sum);
+          else if (a.lse) a.lse[i] = sum > 0.0f ? (t + log2f(sum)) * 0.6931471805599453f : sum == 0.0f ? -INFINITY : sum;
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
   if (threadIdx.x == 0) parts.endings[blockIdx.x] = ending;
   // sequences that have nothing
@@ -654,12 +742,12 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
   }
 }
 
-Plan plan_of(int Hq, int Hk, int D) {
+Plan plan_of(int format, int Hq, int Hk, int D) {
   Plan p{};
   const int group = Hq / Hk;
   p.groups = (group + 15) / 16;
   p.rows = std::min(group, 16);
-  p.ctas = ctas_per_sm(padded(D), p.rows > 8) * sm_count();
+  p.ctas = ctas_per_sm(format, padded(D), p.rows > 8) * sm_count();
   return p;
 }
 
@@ -676,15 +764,16 @@ template <typename Kernel> cudaError_t allow_shared(Kernel kernel, int bytes, st
 
 template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvAttendArgs& a, Plan pl, cudaStream_t stream) {
   using S = Shape<FORMAT, DP>;
+  constexpr int SMEM = WARPS * (S::STAGES * S::STAGE + 8 * 8);
   auto kernel = kv_attend_kernel<T, FORMAT, DP, TWO>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_shared(kernel, S::SMEM, done);
-  if (e != cudaSuccess) return e;
+  const cudaError_t set = allow_shared(kernel, SMEM, done);
+  if (set != cudaSuccess) return set;
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales[0]) | reinterpret_cast<uintptr_t>(a.scales[1]);
-  pl.wide_scales = FORMAT == EMU_KV_MXFP4 && a.D == DP && at % S::BLOCKS == 0;
+  pl.wide_scales = FORMAT == EMU_KV_MXFP4 && a.D == DP && at % std::min(4, DP / 32) == 0;
   pl.page_size = (uint32_t)std::min<int64_t>(a.page_size, 1ll << 31);
   pl.whole_steps = a.page_size % KEYS == 0;
-  kernel<<<pl.ctas, NT, S::SMEM, stream>>>(a, pl);
+  kernel<<<pl.ctas, NT, SMEM, stream>>>(a, pl);
   // launched early, so that its CTAs wait where the attention's finish
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.ctas, std::min(pl.rows, 4));
@@ -695,12 +784,12 @@ template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvA
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T>, a, pl, DP);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T>, a, pl, DP);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 template <typename T, int FORMAT> cudaError_t launch_sized(const KvAttendArgs& a, cudaStream_t stream) {
-  const Plan pl = plan_of(a.Hq, a.Hk, a.D);
+  const Plan pl = plan_of(FORMAT, a.Hq, a.Hk, a.D);
   const bool two = pl.rows > 8;
   if (a.D <= 64) return two ? launch<T, FORMAT, 64, true>(a, pl, stream) : launch<T, FORMAT, 64, false>(a, pl, stream);
   if (a.D <= 128) return two ? launch<T, FORMAT, 128, true>(a, pl, stream) : launch<T, FORMAT, 128, false>(a, pl, stream);
@@ -710,7 +799,9 @@ template <typename T, int FORMAT> cudaError_t launch_sized(const KvAttendArgs& a
 }  // namespace
 
 size_t kv_attend_workspace(int64_t, int Hq, int Hk, int D) {
-  const Plan p = plan_of(Hq, Hk, D);
+  // (both formats' of the head size: the larger one)
+  Plan p = plan_of(EMU_KV_MXFP4, Hq, Hk, D);
+  p.ctas = std::max(p.ctas, plan_of(EMU_KV_FP8, Hq, Hk, D).ctas);
   return parts_of(nullptr, p.ctas, p.rows, D).bytes;
 }
 
