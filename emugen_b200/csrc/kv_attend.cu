@@ -56,14 +56,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two codes -> two fp16 (the low byte's first)
-__device__ __forceinline__ uint32_t half2_of_e4m3(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// A word's codes -> fp16 pairs, the low byte's first.
+__device__ __forceinline__ void halves_of_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
-__device__ __forceinline__ uint32_t half2_of_e2m1(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)two, __NV_E2M1);
-  return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ void halves_of_e2m1(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -127,7 +126,7 @@ __device__ __forceinline__ int64_t tiles_of(const KvAttendArgs& a, int64_t b) {
 }
 // What a (sequence, head) counts for when the work is dealt out: its tiles and EXTRA places before them, for what
 // starting and joining it costs.
-constexpr int EXTRA = 2;
+constexpr int EXTRA = 4;
 __device__ __forceinline__ int64_t places_of(const KvAttendArgs& a, int64_t b) {
   const int64_t n = tiles_of(a, b);
   return n ? n + EXTRA : 0;
@@ -171,26 +170,26 @@ struct Deal {
 // The workspace: what each CTA ends, and the sums of its first and its last (sequence, head) where they are parts.
 struct Ending;
 struct Parts {
-  Ending* endings;             // [CTA]
+  Ending* endings;             // [sequence][head]
   float2* ml;                  // [slot][rows]: maximum (of log2 scores), sum
   float* o;                    // [slot][rows][D]
   size_t bytes;
 };
-__host__ __device__ inline Parts parts_of(void* workspace, int64_t ctas, int rows, int D) {
+__host__ __device__ inline Parts parts_of(void* workspace, int64_t items, int64_t ctas, int rows, int D) {
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  const size_t ml = (size_t)(ctas * 16 + 255) / 256 * 256, o = ml + (2 * ctas * rows * sizeof(float2) + 255) / 256 * 256;
+  const size_t ml = (size_t)(items * 8 + 255) / 256 * 256, o = ml + (2 * ctas * rows * sizeof(float2) + 255) / 256 * 256;
   return {reinterpret_cast<Ending*>(base), reinterpret_cast<float2*>(base + ml), reinterpret_cast<float*>(base + o), o + 2 * ctas * rows * D * sizeof(float)};
 }
 struct Plan {
   int ctas, groups, rows;      // CTAs, items of up to 16 query heads to a key head, rows of an item
+  bool wide_q;                 // four elements of q may be read at once
   bool wide_scales;            // MXFP4: a row's scale bytes may be read at once
   bool whole_steps;            // a step's 16 keys lie in one page
   uint32_t page_size;          // up to 2^31 (more than any length)
 };
-// What a CTA leaves for the join: where its run ends a (sequence, head) that another CTA began.
+// What the CTA that ends a (sequence, head) leaves for the join: the first and the last CTA of it (the same: nothing to join).
 struct Ending {
-  int64_t out;                 // the first row of the outputs
-  int rows, first;             // rows (0: nothing to join), the CTA that began it
+  int first, last;
 };
 
 // As many as registers (and shared memory) allow.
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
   float* sums = reinterpret_cast<float*>(ring);              // [8 rows][DP + 4]
   float2* join_ml = reinterpret_cast<float2*>(smem + WARPS * RING);                // [warp][8]
   const int D = a.D, HV = a.Hk * pl.groups, group = a.Hq / a.Hk;
-  const Parts parts = parts_of(a.workspace, pl.ctas, pl.rows, D);
+  const Parts parts = parts_of(a.workspace, a.B * HV, pl.ctas, pl.rows, D);
 
   asm volatile("griddepcontrol.launch_dependents;");        // the join's CTAs may come when there is room
   // this CTA's run of places
@@ -243,7 +242,6 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
   int64_t at = deal.begin(blockIdx.x);                       // `at` in the list of all places
   const int64_t hi = deal.begin(blockIdx.x + 1);
   if (at < hi) b = found[0], first = found[1];
-  Ending ending{0, 0, 0};
 
   while (at < hi) {
     const int64_t per = places_of(a, b);
@@ -260,6 +258,34 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
     const int kh = hv / pl.groups, h0 = kh * group + (hv % pl.groups) * 16, rows = min(16, group - (hv % pl.groups) * 16);
     const int len = (int)min((int64_t)a.lens[b], a.table_cols * a.page_size);
     const int32_t* table = a.table + b * a.table_stride;
+
+    // ---- this lane's elements of q's rows g and g + 8 as they are, asked for before the cache's
+    uint32_t raw[R][STEPS][2];
+    {
+      auto place_of = [&](int z) {                           // the first of a step's two pairs
+        constexpr int PER_PLACE = S::KW * S::CODES / 4;      // steps of one place
+        return S::key_place(c, z / PER_PLACE) / 4 * S::CODES + z % PER_PLACE * 4;
+      };
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int row = g + 8 * r;
+        const T* src = static_cast<const T*>(a.q) + b * a.q_stride[0] + (int64_t)(h0 + row) * a.q_stride[1];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          raw[r][s][0] = raw[r][s][1] = 0;
+          if (row < rows && place_of(s) < D) {               // (D is a multiple of 16)
+            if (pl.wide_q) {
+              const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + place_of(s)));
+              raw[r][s][0] = w.x, raw[r][s][1] = w.y;
+            } else {
+              const uint16_t* p = reinterpret_cast<const uint16_t*>(src) + place_of(s);
+              raw[r][s][0] = (uint32_t)p[0] | (uint32_t)p[1] << 16;
+              raw[r][s][1] = (uint32_t)p[2] | (uint32_t)p[3] << 16;
+            }
+          }
+        }
+      }
+    }
 
     // ---- steps of 16 keys; the warps take them in turn
     const int key0 = (int)(tile0 * TILE) + warp * KEYS, end = (int)min((int64_t)len, tile1 * TILE);
@@ -366,48 +392,31 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       page_next = pages[STAGES - 1];
     }
 
-    // ---- q: this lane's elements of rows g and g + 8, as the MMAs' A operands
+    // ---- q as the MMAs' A operands: fp16, multiplied by a power of two
     uint32_t q[STEPS][2 * R];
     float qf[R];                                             // what a score of the row is multiplied by
-    {
-      auto place_of = [&](int z) {                           // the first of a step's two pairs
-        constexpr int PER_PLACE = S::KW * S::CODES / 4;      // steps of one place
-        return S::key_place(c, z / PER_PLACE) / 4 * S::CODES + z % PER_PLACE * 4;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      auto value = [&](uint32_t w, int i) {
+        const uint16_t u = (uint16_t)(i ? w >> 16 : w);
+        return widen<T>(*reinterpret_cast<const T*>(&u));
       };
+      float top = 0.0f;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int row = g + 8 * r;
-        const T* src = static_cast<const T*>(a.q) + b * a.q_stride[0] + (int64_t)(h0 + row) * a.q_stride[1];
-        float top = 0.0f;
-        uint32_t raw[STEPS][2];                              // pairs as they were read
+      for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+        for (int e = 0; e < 2; ++e) top = fmaxf(top, fmaxf(fabsf(value(raw[r][s][e], 0)), fabsf(value(raw[r][s][e], 1))));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      int e2 = top > 0.0f && top < INFINITY ? (int)(__float_as_uint(top) >> 23) - 127 : 14;
+      e2 = max(e2, -113);
+      const float f = pow2(14 - e2);
+      qf[r] = a.scale * 1.4426950408889634f * pow2(max(e2 - 14, -126));
+      if (e2 - 14 < -126) qf[r] *= pow2(e2 - 14 + 126);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool in = row < rows && place_of(s) < D;   // (D is a multiple of 16)
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(src) + place_of(s) + 2 * e;
-            raw[s][e] = in ? (uint32_t)p[0] | (uint32_t)p[1] << 16 : 0;
-          }
-        auto value = [&](uint32_t w, int i) {
-          const uint16_t u = (uint16_t)(i ? w >> 16 : w);
-          return widen<T>(*reinterpret_cast<const T*>(&u));
-        };
+      for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) top = fmaxf(top, fmaxf(fabsf(value(raw[s][e], 0)), fabsf(value(raw[s][e], 1))));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        int e2 = top > 0.0f && top < INFINITY ? (int)(__float_as_uint(top) >> 23) - 127 : 14;
-        e2 = max(e2, -113);
-        const float f = pow2(14 - e2);
-        qf[r] = a.scale * 1.4426950408889634f * pow2(max(e2 - 14, -126));
-        if (e2 - 14 < -126) qf[r] *= pow2(e2 - 14 + 126);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) q[s][e * R + r] = pack_half(value(raw[s][e], 0) * f, value(raw[s][e], 1) * f);
-      }
+        for (int e = 0; e < 2; ++e) q[s][e * R + r] = pack_half(value(raw[r][s][e], 0) * f, value(raw[r][s][e], 1) * f);
     }
 
     // o[n][r]: elements d (rows of the MMA) of heads 8 r + 2 c and 8 r + 2 c + 1; m and l are those of heads g + 8 r
@@ -485,17 +494,21 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
 #pragma unroll
               for (int y = 0; y < S::KW; ++y) {
                 const int z = S::KW * x + y;
-                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, half2_of_e4m3(kw[x][y] & 0xFFFFu), half2_of_e4m3(kw[x][y] >> 16));
+                uint32_t b0, b1;
+                halves_of_e4m3(kw[x][y], b0, b1);
+                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, b0, b1);
               }
           } else {
 #pragma unroll
             for (int x = 0; x < S::KX; ++x) {
               const uint32_t f = half_pow2(ksc[t][x] == 255 ? 16 : (int)ksc[t][x] - kref + 8) * 0x10001u;
 #pragma unroll
-              for (int y = 0; y < 2 * S::KW; ++y) {
-                const int z = 2 * S::KW * x + y;
-                const uint32_t w = kw[x][y / 2] >> (16 * (y & 1));
-                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, mul_half2(half2_of_e2m1(w & 255u), f), mul_half2(half2_of_e2m1(w >> 8 & 255u), f));
+              for (int y = 0; y < S::KW; ++y) {
+                const int z = 2 * (S::KW * x + y);
+                uint32_t h[4];
+                halves_of_e2m1(kw[x][y], h);
+                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, mul_half2(h[0], f), mul_half2(h[1], f));
+                mma(acc, q[z + 1][0], TWO ? q[z + 1][1] : 0, q[z + 1][R], TWO ? q[z + 1][2 * R - 1] : 0, mul_half2(h[2], f), mul_half2(h[3], f));
               }
             }
           }
@@ -620,8 +633,11 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
           for (int z = 0; z < S::VW; ++z) {
             const uint32_t x0 = __byte_perm(vw[0][x][z], vw[1][x][z], 0x5140), x1 = __byte_perm(vw[0][x][z], vw[1][x][z], 0x7362);
             const uint32_t y0 = __byte_perm(vw[2][x][z], vw[3][x][z], 0x5140), y1 = __byte_perm(vw[2][x][z], vw[3][x][z], 0x7362);
-            step(k * PER + 2 * z, half2_of_e4m3(x0 & 0xFFFFu), half2_of_e4m3(x0 >> 16), half2_of_e4m3(y0 & 0xFFFFu), half2_of_e4m3(y0 >> 16));
-            step(k * PER + 2 * z + 1, half2_of_e4m3(x1 & 0xFFFFu), half2_of_e4m3(x1 >> 16), half2_of_e4m3(y1 & 0xFFFFu), half2_of_e4m3(y1 >> 16));
+            uint32_t h[4];
+            halves_of_e4m3(x0, h[0], h[1]), halves_of_e4m3(y0, h[2], h[3]);
+            step(k * PER + 2 * z, h[0], h[1], h[2], h[3]);
+            halves_of_e4m3(x1, h[0], h[1]), halves_of_e4m3(y1, h[2], h[3]);
+            step(k * PER + 2 * z + 1, h[0], h[1], h[2], h[3]);
           }
         } else {
 #pragma unroll
@@ -630,10 +646,11 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
             const uint32_t w0 = vw[0][0][z], w1 = vw[1][0][z], w2 = vw[2][0][z], w3 = vw[3][0][z];
             const uint32_t x0 = (w0 & 0x0F0F0F0Fu) | (w1 << 4 & 0xF0F0F0F0u), x1 = (w0 >> 4 & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u);
             const uint32_t y0 = (w2 & 0x0F0F0F0Fu) | (w3 << 4 & 0xF0F0F0F0u), y1 = (w2 >> 4 & 0x0F0F0F0Fu) | (w3 & 0xF0F0F0F0u);
+            uint32_t hx0[4], hx1[4], hy0[4], hy1[4];
+            halves_of_e2m1(x0, hx0), halves_of_e2m1(x1, hx1), halves_of_e2m1(y0, hy0), halves_of_e2m1(y1, hy1);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              step(4 * z + e, mul_half2(half2_of_e2m1(x0 >> 8 * e & 255u), f01), mul_half2(half2_of_e2m1(x1 >> 8 * e & 255u), f01),
-                   mul_half2(half2_of_e2m1(y0 >> 8 * e & 255u), f23), mul_half2(half2_of_e2m1(y1 >> 8 * e & 255u), f23));
+              step(4 * z + e, mul_half2(hx0[e], f01), mul_half2(hx1[e], f01), mul_half2(hy0[e], f23), mul_half2(hy1[e], f23));
           }
         }
       }
@@ -648,7 +665,7 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
     const bool whole = tile0 == 0 && tile1 == per - EXTRA;
     // a CTA's first segment may be the rest of a (sequence, head), its last one the beginning of one
     const int64_t slot = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
-    if (!whole && tile1 == per - EXTRA) ending = {b * a.Hq + h0, rows, deal.owner(start + EXTRA)};
+    if (tile1 == per - EXTRA && threadIdx.x == 0) parts.endings[b * HV + hv] = {whole ? (int)blockIdx.x : deal.owner(start + EXTRA), (int)blockIdx.x};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
@@ -688,53 +705,87 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       __syncthreads();
     }
   }
-  if (threadIdx.x == 0) parts.endings[blockIdx.x] = ending;
   // sequences that have nothing
   for (int64_t i = blockIdx.x; i < a.B; i += gridDim.x)
     if (tiles_of(a, i) == 0) {
+      for (int x = threadIdx.x; x < HV; x += NT) parts.endings[i * HV + x] = {0, 0};
       for (int64_t x = threadIdx.x; x < (int64_t)a.Hq * D; x += NT) static_cast<T*>(a.out)[i * a.Hq * D + x] = narrow<T>(0.0f);
       if (a.lse)
         for (int h = threadIdx.x; h < a.Hq; h += NT) a.lse[i * a.Hq + h] = -INFINITY;
     }
 }
 
-// Joins the sums of each (sequence, head) that lies in several CTAs, in the order of its tiles: CTA (i, y) the rows y, y +
-// gridDim.y, .. of the one that the run of the attention's CTA i ends.  Threads [part][element]; then a sum over the parts' shares.
-constexpr int JOIN_NT = 512;
+// Joins the sums of each (sequence, head) that lies in several CTAs, in the order of its tiles.  A CTA to a row of an item (where
+// there are many, to every gridDim.x-th item): the parts' factors first, then threads [part][element], then a sum over
+// the parts' shares.
+constexpr int JOIN_NT = 512, JOIN_PARTS = 1024, FEW = 8;
 template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ Plan pl, int lanes) {
-  __shared__ float so[JOIN_NT], sl[JOIN_NT], stop[JOIN_NT / 32];
+  __shared__ float so[JOIN_NT], factor[JOIN_PARTS], part_sum[JOIN_NT / 32], part_top[JOIN_NT / 32];
+  const int HV = a.Hk * pl.groups, group = a.Hq / a.Hk, row = blockIdx.y, warp = threadIdx.x >> 5;
+  const Parts parts = parts_of(a.workspace, a.B * HV, pl.ctas, pl.rows, a.D);
   asm volatile("griddepcontrol.wait;" ::: "memory");         // the attention's results are there
-  const Parts parts = parts_of(a.workspace, pl.ctas, pl.rows, a.D);
-  const Ending e = parts.endings[blockIdx.x];
-  const int n = (int)blockIdx.x - e.first + 1;
-  const int d = threadIdx.x % lanes, part = threadIdx.x / lanes, step = JOIN_NT / lanes;
-  for (int row = blockIdx.y; row < e.rows; row += gridDim.y) {
-    auto slot = [&](int i) { return (2 * (int64_t)(e.first + i) + (i == 0 ? 1 : 0)) * pl.rows + row; };
+  for (int64_t item = blockIdx.x; item < a.B * HV; item += gridDim.x) {
+    const Ending e = parts.endings[item];
+    const int n = e.last - e.first + 1;
+    const int64_t b = item / HV;
+    const int hv = (int)(item - b * HV);
+    if (n < 2) continue;
+    const int d = threadIdx.x % lanes, shares = JOIN_NT / lanes;
+    if (n <= FEW) {                                          // as many rows at once as there are threads for
+      const int r = row + threadIdx.x / lanes, hq = hv % pl.groups * 16 + r;
+      if (row % shares || r >= pl.rows || hq >= group || d >= a.D) continue;
+      auto slot = [&](int i) { return (2 * (int64_t)(e.first + i) + (i == 0 ? 1 : 0)) * pl.rows + r; };
+      float top = -INFINITY, sum = 0.0f, v = 0.0f;
+      for (int i = 0; i < n; ++i) top = fmaxf(top, parts.ml[slot(i)].x);
+      const float sh = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float2 ml = parts.ml[slot(i)];
+        const float f = exp2_approx(ml.x - sh);
+        sum = __fmaf_rn(ml.y, f, sum);
+        v = __fmaf_rn(parts.o[slot(i) * a.D + d], f, v);
+      }
+      const int64_t i = b * a.Hq + hv / pl.groups * group + hq;
+      static_cast<T*>(a.out)[i * a.D + d] = narrow<T>(sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
+      if (d == 0 && a.lse) a.lse[i] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : sum == 0.0f ? -INFINITY : sum;
+      continue;
+    }
+    const int hq = hv % pl.groups * 16 + row;
+    if (hq >= group) continue;
+    // a CTA's first (sequence, head) is in its even slot; this one's first part is the last of its CTA
+    const int64_t slot0 = (2 * (int64_t)e.first) * pl.rows + row, step = 2 * pl.rows;
+    auto slot = [&](int i) { return slot0 + i * step + (i == 0 ? pl.rows : 0); };
     float top = -INFINITY;
     for (int i = threadIdx.x; i < n; i += JOIN_NT) top = fmaxf(top, parts.ml[slot(i)].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if ((threadIdx.x & 31) == 0) stop[threadIdx.x >> 5] = top;
+    if ((threadIdx.x & 31) == 0) part_top[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < JOIN_NT / 32; ++w) top = fmaxf(top, stop[w]);
+    for (int w = 0; w < JOIN_NT / 32; ++w) top = fmaxf(top, part_top[w]);
     const float sh = top == -INFINITY ? 0.0f : top;
-    float v = 0.0f, sum = 0.0f;
-#pragma unroll 8
-    for (int i = part; i < n; i += step) {
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < n; i += JOIN_NT) {
       const float2 ml = parts.ml[slot(i)];
-      const float x = d < a.D ? parts.o[slot(i) * a.D + d] : 0.0f;
-      const float f = exp2_approx(ml.x - sh);
-      sum = __fmaf_rn(ml.y, f, sum);
-      v = __fmaf_rn(x, f, v);
+      factor[i] = exp2_approx(ml.x - sh);
+      sum = __fmaf_rn(ml.y, factor[i], sum);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xFFFFFFFFu, sum, o));
+    if ((threadIdx.x & 31) == 0) part_sum[warp] = sum;
+    __syncthreads();
+    float v = 0.0f;
+    if (d < a.D) {
+#pragma unroll 8
+      for (int i = threadIdx.x / lanes; i < n; i += shares) v = __fmaf_rn(parts.o[slot(i) * a.D + d], factor[i], v);
     }
     so[threadIdx.x] = v;
-    if (d == 0) sl[part] = sum;
     __syncthreads();
     if (threadIdx.x < a.D) {
       v = 0.0f, sum = 0.0f;
-      for (int x = 0; x < step; ++x) v = __fadd_rn(v, so[x * lanes + threadIdx.x]), sum = __fadd_rn(sum, sl[x]);
-      const int64_t i = e.out + row;
+      for (int x = 0; x < shares; ++x) v = __fadd_rn(v, so[x * lanes + threadIdx.x]);
+      for (int w = 0; w < JOIN_NT / 32; ++w) sum = __fadd_rn(sum, part_sum[w]);
+      const int64_t i = b * a.Hq + hv / pl.groups * group + hq;
       static_cast<T*>(a.out)[i * a.D + threadIdx.x] = narrow<T>(sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
       if (threadIdx.x == 0 && a.lse) a.lse[i] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : sum == 0.0f ? -INFINITY : sum;
     }
@@ -747,7 +798,7 @@ Plan plan_of(int format, int Hq, int Hk, int D) {
   const int group = Hq / Hk;
   p.groups = (group + 15) / 16;
   p.rows = std::min(group, 16);
-  p.ctas = ctas_per_sm(format, padded(D), p.rows > 8) * sm_count();
+  p.ctas = std::min(JOIN_PARTS, ctas_per_sm(format, padded(D), p.rows > 8) * sm_count());
   return p;
 }
 
@@ -771,12 +822,13 @@ template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvA
   if (set != cudaSuccess) return set;
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales[0]) | reinterpret_cast<uintptr_t>(a.scales[1]);
   pl.wide_scales = FORMAT == EMU_KV_MXFP4 && a.D == DP && at % std::min(4, DP / 32) == 0;
+  pl.wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride[0] * 2) | (uintptr_t)(a.q_stride[1] * 2)) & 7) == 0;
   pl.page_size = (uint32_t)std::min<int64_t>(a.page_size, 1ll << 31);
   pl.whole_steps = a.page_size % KEYS == 0;
   kernel<<<pl.ctas, NT, SMEM, stream>>>(a, pl);
   // launched early, so that its CTAs wait where the attention's finish
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.ctas, std::min(pl.rows, 4));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(a.B * a.Hk * pl.groups, std::max(1, 4096 / pl.rows)), pl.rows);
   cfg.blockDim = dim3(JOIN_NT);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
@@ -798,11 +850,11 @@ template <typename T, int FORMAT> cudaError_t launch_sized(const KvAttendArgs& a
 
 }  // namespace
 
-size_t kv_attend_workspace(int64_t, int Hq, int Hk, int D) {
+size_t kv_attend_workspace(int64_t B, int Hq, int Hk, int D) {
   // (both formats' of the head size: the larger one)
   Plan p = plan_of(EMU_KV_MXFP4, Hq, Hk, D);
   p.ctas = std::max(p.ctas, plan_of(EMU_KV_FP8, Hq, Hk, D).ctas);
-  return parts_of(nullptr, p.ctas, p.rows, D).bytes;
+  return parts_of(nullptr, B * Hk * p.groups, p.ctas, p.rows, D).bytes;
 }
 
 cudaError_t launch_kv_attend(const KvAttendArgs& a, cudaStream_t stream) {
