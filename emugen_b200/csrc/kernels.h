@@ -137,7 +137,7 @@ struct KvReadArgs {
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream);
 
 // Norms of queries and keys with the position rotation (norm_rope.cu).  Index 0: queries, 1: keys.
-constexpr int NORM_ROPE_CTAS = 4;   // most CTAs for each SM that write a share of the weights' gradients
+constexpr int NORM_ROPE_CTAS = 2;   // CTAs that an SM holds
 struct NormRopeArgs {
   const void* x[2];
   int64_t token_stride[2], head_stride[2];
@@ -155,7 +155,8 @@ struct NormRopeArgs {
   int64_t dy_token_stride[2], dy_head_stride[2];
   void* dw[2];
   float* partial;               // norm_rope_workspace bytes
-  int chunks[2], heads_per_unit;   // set by the launcher
+  int split, heads_per_unit[2];   // from here on set by the launcher
+  bool vec;
 };
 size_t norm_rope_workspace(int64_t D);
 cudaError_t launch_norm_rope(NormRopeArgs a, bool back, cudaStream_t stream);
