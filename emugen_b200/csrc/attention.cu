@@ -25,7 +25,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int THREADS = 384;                                // warps 10 and 11 fill up the third warpgroup
+constexpr int THREADS = 384;                                // the third warpgroup's rest fills it up
 // 128 threads x 40 + 256 x 232 = 64512 = 384 x 168, what the CTA is launched with
 constexpr int REG_LOW = 40, REG_HIGH = 232;
 
@@ -271,7 +271,301 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     redo = mine && ok && worst != 0.0f && l > 0.0f;
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
       const int src = __ffs(rows) - 1;
-      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src));
+      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), 0, a.D);
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(*tmem_slot, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------ few tiles of rows
+// Where there are fewer pairs of tiles than SMs, a CTA owns one tile of rows and its two warpgroups take the tiles of keys in
+// turn, so that a tile of rows takes half the time.  Tensor memory holds S (and P) of three tiles of keys beside O: a tile's
+// products run ahead of and behind its softmax.
+//
+//   warps 0-3, 4-7   softmax of every other tile of keys, a thread to a row; at the end half of its row's output each
+//   warps 8, 10      MMA issuers, of S and of O += P V: an issuer is held up while its MMAs run, and the other's waits pass
+//                    meanwhile (one for both: 650 of 1690 clocks a tile without an MMA).  Warp 8 owns the tensor memory.
+//   warp 9           TMA: Q once, then K and V tiles through two rings
+template <int DP> struct Few {
+  static constexpr int TILE = 128 * DP * 2;                 // 128 rows of DP elements, as DP / 64 boxes of 128 x 128 bytes
+  static constexpr int SLOTS = DP == 128 ? 3 : 5;           // of K, and of V
+  static constexpr int BARS = 1 + 4 * SLOTS + 3 + 3 + 3 + 1 + 2 + 1 + 2;
+  static constexpr int SMEM = 1024 + (1 + 2 * SLOTS) * TILE + BARS * 8 + 16 + 3 * 128 * 4;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+constexpr uint32_t FEW_O = 384;                             // tensor memory columns: S (and P) of three tiles, O
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
+                                                              const __grid_constant__ Tiling tl) {
+  using C = Few<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  const Unit u = unit_of(a, tl, a.cu_q, a.Tq, 1);
+  if (!u.any) return;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const Rows qr = u.rows;
+  const Rows kr = u.b < a.B ? rows_of(a.cu_k, u.b, a.Tk) : Rows{0, 0};
+  const int64_t nq = qr.count(), nk = kr.count();
+  // keys that the unit's last token sees
+  const int64_t last = min(u.t0 + tl.tokens, qr.end) - 1 - qr.begin;
+  const int64_t most = a.causal ? max((int64_t)0, min(nk, last + 1 + nk - nq)) : nk;
+  const int tiles = (int)((most + 127) / 128);
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* ring_k = smem + C::TILE;
+  uint8_t* ring_v = ring_k + C::SLOTS * C::TILE;
+  float* ref = reinterpret_cast<float*>(ring_v + C::SLOTS * C::TILE);             // [row]: the maximum that the weights are held to
+  float* sums = ref + 128;                                   // [warpgroup][row], at the end
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sums + 256);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* k_empty = k_full + C::SLOTS;
+  uint64_t* v_full = k_empty + C::SLOTS;
+  uint64_t* v_empty = v_full + C::SLOTS;
+  uint64_t* s_full = v_empty + C::SLOTS;                     // [place]
+  uint64_t* p_full = s_full + 3;                             // [place]
+  uint64_t* p_free = p_full + 3;                             // [place]
+  uint64_t* pv_done = p_free + 3;
+  uint64_t* ref_full = pv_done + 1;                          // [warpgroup]: it has written `ref` of its tile
+  uint64_t* o_full = ref_full + 2;
+  uint64_t* drained = o_full + 1;                            // [issuer]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&map_q), ptx::prefetch_tmap(&map_k), ptx::prefetch_tmap(&map_v);
+    ptx::mbar_init(q_full, 1), ptx::mbar_init(pv_done, 1), ptx::mbar_init(o_full, 1);
+    for (int i = 0; i < C::SLOTS; ++i)
+      ptx::mbar_init(&k_full[i], 1), ptx::mbar_init(&k_empty[i], 1), ptx::mbar_init(&v_full[i], 1), ptx::mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < 3; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&p_full[i], 128), ptx::mbar_init(&p_free[i], 1);
+    for (int i = 0; i < 2; ++i) ptx::mbar_init(&ref_full[i], 128), ptx::mbar_init(&drained[i], 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  // no load may be in flight across the register split: the TMEM address is read after it
+  if (warp >= 8) {
+    ptx::setmaxnreg_dec<REG_LOW>();
+    if (warp == 9 && lane == 0 && tiles) {
+      const int head = u.kh * tl.group + u.chunk * tl.heads;
+      ptx::mbar_arrive_expect_tx(q_full, (DP / 64) * tl.heads * tl.tokens * 128);
+      for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(smem + x * 16384, &map_q, q_full, x * 64, head, (int)u.t0);
+      Ring<C::SLOTS> k, v;
+      auto load = [&](const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty, Ring<C::SLOTS>& r, int j) {
+        if (j >= C::SLOTS && !wait_or_record(&empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_FWD_SLOT)) return false;
+        ptx::mbar_arrive_expect_tx(&full[r.at], C::TILE);
+        for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring + r.at * C::TILE + x * 16384, map, &full[r.at], x * 64, u.kh, (int)(kr.begin + (int64_t)j * 128));
+        r.next();
+        return true;
+      };
+      // in the order of their use: K_0, K_1, K_2, V_0, K_3, V_1, ..
+      bool ok = true;
+      for (int j = 0; j < min(3, tiles) && ok; ++j) ok = load(&map_k, ring_k, k_full, k_empty, k, j);
+      for (int j = 0; j < tiles && ok; ++j) {
+        ok = load(&map_v, ring_v, v_full, v_empty, v, j);
+        if (ok && j + 3 < tiles) ok = load(&map_k, ring_k, k_full, k_empty, k, j + 3);
+      }
+      if (!ok) {                                             // time for the copies in flight to land before the CTA exits
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) {}
+      }
+    } else if ((warp == 8 || warp == 10) && tiles) {
+      const uint32_t tmem = *tmem_slot;
+      constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+      Ring<C::SLOTS> slot;
+      Ring<3> place;
+      bool ok = true;
+      if (warp == 8) {                                       // S = Q K^T
+        const uint32_t id = ptx::idesc_16_f32(128, 128, BF, false);
+        const int ks = tl.d16 / 16;
+        // descriptors of the first slot; a slot or a step of the sums further on is an addition to them
+        const uint64_t q_desc = ptx::smem_desc_sw128(ptx::smem_u32(smem)), k_desc = ptx::smem_desc_sw128(ptx::smem_u32(ring_k));
+        ok = warp_wait_or_record(q_full, 0, tl.wait_limit, WAIT_FWD_Q);
+        for (int j = 0; j < tiles && ok; ++j, slot.next(), place.next()) {
+          if (!warp_wait_or_record(&k_full[slot.at], slot.parity, tl.wait_limit, WAIT_FWD_K)) { ok = false; break; }
+          // the weights of tile j - 3, in the same place, have been used
+          if (j >= 3 && !warp_wait_or_record(&p_free[place.at], place.parity ^ 1, tl.wait_limit, WAIT_FWD_P)) { ok = false; break; }
+          ptx::tc_fence_after();
+          if (ptx::elect_one()) {
+            const uint64_t kd = k_desc + (uint32_t)(slot.at * (C::TILE >> 4));
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+              constexpr int BOX = 16384 >> 4, STEP = 32 >> 4;
+              if (s < ks) ptx::mma_f16(tmem + place.at * 128, q_desc + (s / 4) * BOX + (s % 4) * STEP, kd + (s / 4) * BOX + (s % 4) * STEP, id, s > 0);
+            }
+            if (!(j == 0 && tl.hold_first_ready)) ptx::mma_commit(&s_full[place.at]);
+            ptx::mma_commit(&k_empty[slot.at]);
+          }
+          __syncwarp();
+        }
+      } else {                                               // O += P V
+        const uint32_t id = ptx::idesc_16_f32(128, tl.d16, BF, true);
+        const uint64_t v_desc = ptx::smem_desc_mn_sw128(ptx::smem_u32(ring_v), 16384);
+        for (int j = 0; j < tiles && ok; ++j, slot.next(), place.next()) {
+          if (!warp_wait_or_record(&v_full[slot.at], slot.parity, tl.wait_limit, WAIT_FWD_V)) { ok = false; break; }
+          if (!warp_wait_or_record(&p_full[place.at], place.parity, tl.wait_limit, WAIT_FWD_P)) { ok = false; break; }
+          ptx::tc_fence_after();
+          if (ptx::elect_one()) {
+            const uint64_t vd = v_desc + (uint32_t)(slot.at * (C::TILE >> 4));
+#pragma unroll
+            for (int s = 0; s < 8; ++s) ptx::mma_f16_ta(tmem + FEW_O, tmem + place.at * 128 + s * 8, vd + s * 128, id, j > 0 || s > 0);
+            ptx::mma_commit(&p_free[place.at]);
+            ptx::mma_commit(&v_empty[slot.at]);
+            ptx::mma_commit(pv_done);
+            if (j + 1 == tiles) ptx::mma_commit(o_full);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok) {                                             // the MMAs in flight are waited for
+        uint64_t* bar = &drained[warp == 10];
+        if (ptx::elect_one()) ptx::mma_commit(bar);
+        __syncwarp();
+        warp_wait_or_record(bar, 0, DRAIN_LIMIT, WAIT_DRAIN);
+      }
+    }
+  } else {
+    ptx::setmaxnreg_inc<REG_HIGH>();
+    const uint32_t tmem = *tmem_slot;
+    // softmax of row r, tiles w, w + 2, ..
+    const int w = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int64_t t = u.t0 + r / tl.heads;
+    const int gh = u.chunk * tl.heads + r % tl.heads, h = u.kh * tl.group + gh;
+    const bool mine = r < tl.heads * tl.tokens && gh < tl.group && t < qr.end;
+    // this row sees the first n keys
+    const int64_t n = !mine ? 0 : a.causal ? max((int64_t)0, min(nk, t - qr.begin + 1 + nk - nq)) : nk;
+    // all rows of the tile see the first ones
+    const int64_t first = a.causal ? u.t0 - qr.begin + 1 + nk - nq : nk;
+    const float c = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = w; j < tiles; j += 2) {
+      const int place = j % 3;
+      const uint32_t s_at = lanes + place * 128;
+      if (!warp_wait_or_record(&s_full[place], (j / 3) & 1, tl.wait_limit, WAIT_FWD_S)) { ok = false; break; }
+      ptx::tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_ld_regs(s_at + 32 * x, s[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) ptx::tmem_wait_regs(s[x]);
+      if ((int64_t)(j + 1) * 128 > first || (int64_t)(j + 1) * 128 > nk) {      // the same for the whole tile
+        const int lim = (int)max((int64_t)0, min((int64_t)128, n - (int64_t)j * 128));
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (x * 32 + e >= lim) s[x][e] = 0xFF800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
+      // The weights are held to the maximum up to a factor of 2^8: P stays below 2^8, l and O in range, and most
+      // tiles need no correction of O.  The other warpgroup has left what its tile, the one before, was held to.
+      if (j > 0 && !warp_wait_or_record(&ref_full[w ^ 1], ((j - 1) >> 1) & 1, tl.wait_limit, WAIT_FWD_S)) { ok = false; break; }
+      float now = j > 0 ? ref[r] : -INFINITY;
+      const float tm = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), now);
+      if (__any_sync(0xFFFFFFFFu, (tm - now) * c > 8.0f)) {
+        if (j > 0) {
+          // Tile j - 1's product has to be there; this tile's waits for its weights.  (S of this tile came behind the product
+          // of tile j - 3: the barrier is at tile j - 2's round or further, so both rounds are waited for in turn.)
+          if (j > 1 && !warp_wait_or_record(pv_done, j & 1, tl.wait_limit, WAIT_FWD_O)) { ok = false; break; }
+          if (!warp_wait_or_record(pv_done, (j - 1) & 1, tl.wait_limit, WAIT_FWD_O)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const float f = tm == -INFINITY ? 1.0f : exp2f((now - tm) * c);
+#pragma unroll
+          for (int x = 0; x < DP; x += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_regs(lanes + FEW_O + x, o);
+            ptx::tmem_wait_regs(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            ptx::tmem_st_regs(lanes + FEW_O + x, o);
+          }
+        }
+        now = tm;
+      }
+      ref[r] = now;
+      ptx::mbar_arrive(&ref_full[w]);
+      if (__any_sync(0xFFFFFFFFu, now != m)) {               // this warpgroup's sum, from its own tile before
+        l *= now == -INFINITY ? 1.0f : exp2f((m - now) * c);
+        m = now;
+      }
+      const float shift = m == -INFINITY ? 0.0f : -m * c;
+      const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t p[32];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t z = ptx::fma2(ptx::join2(s[2 * x + y][e], s[2 * x + y][e + 1]), c2, sh2);
+            const float p0 = exp2_approx(ptx::lo2(z)), p1 = exp2_approx(ptx::hi2(z));
+            sum[y] = ptx::add2(sum[y], ptx::join2(__float_as_uint(p0), __float_as_uint(p1)));
+            p[y * 16 + e / 2] = pack2<T>(p0, p1);
+          }
+        ptx::tmem_st_regs(s_at + 32 * x, p);
+      }
+      const uint64_t all = ptx::add2(sum[0], sum[1]);
+      l += ptx::lo2(all) + ptx::hi2(all);
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(&p_full[place]);
+    }
+    // both warpgroups' sums, held to the last tile's maximum
+    if (ok && tiles) ok = warp_wait_or_record(o_full, 0, tl.wait_limit, WAIT_FWD_O);
+    ptx::tc_fence_after();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float last_m = tiles ? ref[r] : -INFINITY;
+    sums[w * 128 + r] = m == last_m ? l : l * exp2f((m - last_m) * c);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    m = last_m, l = sums[r] + sums[128 + r];
+    const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
+    float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
+    constexpr int HALF = DP / 2;
+#pragma unroll
+    for (int x = 0; x < HALF; x += 32) {
+      uint32_t o[32];
+      if (tiles) {
+        ptx::tmem_ld_regs(lanes + FEW_O + w * HALF + x, o);
+        ptx::tmem_wait_regs(o);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        const int d = w * HALF + x + e;
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // a row without keys gives zeros, whatever its place held
+          const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
+          if (d < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
+          v[k] = pack2<T>(v0, v1);
+        }
+        if (mine && ok && d < a.D) *reinterpret_cast<uint4*>(out + d) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
+    // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
+    // from the keys that they see alone (this thread's half).  (Where the sum is NaN, the scores are, and the row is NaN by right.)
+    const bool redo = mine && ok && worst != 0.0f && l > 0.0f;
+    for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
+      const int src = __ffs(rows) - 1;
+      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), w * HALF, min(a.D, (w + 1) * HALF));
     }
   }
   ptx::tc_fence_before();
@@ -290,14 +584,21 @@ template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t
   if (!make_rows_map(&mq, a.q, a.Tq, a.Hq, a.D, a.q_stride, a.dtype, tl.heads, tl.tokens) ||
       !make_rows_map(&mk, a.k, a.Tk, a.Hk, a.D, a.k_stride, a.dtype, 1, 128) || !make_rows_map(&mv, a.v, a.Tk, a.Hk, a.D, a.v_stride, a.dtype, 1, 128))
     return cudaErrorUnknown;
-  auto kernel = attention_kernel<T, DP>;
-  static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_shared(kernel, Fwd<DP>::SMEM, done);
-  if (e != cudaSuccess) return e;
-  const int64_t grid = units(a.Tq, a.B, 2 * tl.tokens) * tl.chunks * a.Hk;
+  // One tile to a CTA while the pairs of tiles would not fill the SMs, or not twice with several sequences, whose lengths may
+  // differ: 32 heads on 8 of 128, causal, us: 512 tokens 12.3 against 16.4, 1024 22.8 against 24.7, 1536 37 against 31.5,
+  // 4096 137 against 132; 9 sequences of 2051 queries and 20011 keys, 20 heads on 4 of 80: 59 against 90.
+  const int64_t heads = (int64_t)tl.chunks * a.Hk, pairs = units(a.Tq, a.B, 2 * tl.tokens) * heads, sms = sm_count();
+  const bool few = pairs <= (a.B > 1 ? sms + sms / 2 : sms);
+  const int64_t grid = few ? units(a.Tq, a.B, tl.tokens) * heads : pairs;
   if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  kernel<<<(unsigned)grid, THREADS, Fwd<DP>::SMEM, stream>>>(mq, mk, mv, a, tl);
-  return cudaGetLastError();
+  static std::atomic<uint64_t> done[2] = {{0}, {0}};
+  auto start = [&](auto kernel, int bytes, std::atomic<uint64_t>& set) {
+    const cudaError_t e = allow_shared(kernel, bytes, set);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)grid, THREADS, bytes, stream>>>(mq, mk, mv, a, tl);
+    return cudaGetLastError();
+  };
+  return few ? start(attention_few_kernel<T, DP>, Few<DP>::SMEM, done[1]) : start(attention_kernel<T, DP>, Fwd<DP>::SMEM, done[0]);
 }
 
 }  // namespace

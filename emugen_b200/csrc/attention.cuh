@@ -99,8 +99,8 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t)
   return s;
 }
 
-// o_t of one head.
-template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h) {
+// Elements [d0, d1) of o_t of one head.
+template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h, int d0, int d1) {
   const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
   const int kh = h / (a.Hq / a.Hk);
   const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];
@@ -122,7 +122,7 @@ template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs
     m = top;
     if (settled(o, a.D)) break;
   }
-  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, 0, a.D, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
+  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, d0, d1, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
 }
 
 // A query's shift -lse log2 e and its delta, at [t * Hq + h].
