@@ -21,14 +21,20 @@ from .fp8 import _DTYPE, _on, _raw_stream
 
 
 def _plain(name: str, *tensors) -> None:
-    """Refuse inputs with a forward-mode tangent."""
+    """Refuse inputs with a forward-mode tangent (there are none outside of a dual level)."""
+    if forward_ad._current_level < 0:
+        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -53,7 +59,7 @@ def _norm_rope(q, k, qw, kw, cos, sin, positions, eps, interleaved):
     dev = q.device
     q, k = _rows(q), _rows(k)
     with _on(dev.index):
-        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
+        yq, yk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
         args = _norm_rope_args(q, k, qw, kw, cos, sin, positions, eps, interleaved)
         status = _lib.load().emu_qk_norm_rope(ctypes.byref(args), yq.data_ptr(), yk.data_ptr(), _raw_stream(dev.index))
     if status:
@@ -106,24 +112,26 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 
     The backward pass makes q's and k's gradients whenever it runs.  For one that a CUDA graph is to capture,
     see fp8.linear_fp8."""
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise RuntimeError(f"q and k must be [tokens, heads, head_size] of the same tokens and head size, got {list(q.shape)} and {list(k.shape)}")
-    if q.dtype != k.dtype or q.dtype not in _DTYPE:
-        raise RuntimeError(f"q and k must share one of float16, bfloat16, float32, got {q.dtype} and {k.dtype}")
-    T, Hq, D = q.shape
-    if Hq < 1 or k.shape[1] < 1:
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2]:
+        raise RuntimeError(f"q and k must be [tokens, heads, head_size] of the same tokens and head size, got {list(qs)} and {list(ks)}")
+    if dtype != k.dtype or dtype not in _DTYPE:
+        raise RuntimeError(f"q and k must share one of float16, bfloat16, float32, got {dtype} and {k.dtype}")
+    T, Hq, D = qs
+    if Hq < 1 or ks[1] < 1:
         raise RuntimeError("q and k must have heads")
     if D < 8 or D > 256 or D % 8:
         raise RuntimeError(f"head_size must be a multiple of 8 up to 256, got {D}")
     for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != q.dtype or tuple(w.shape) != (D,)):
-            raise RuntimeError(f"{n} must be {q.dtype} [{D}], got {w.dtype} {list(w.shape)}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape:
+        if w is not None and (w.dtype != dtype or w.shape != (D,)):
+            raise RuntimeError(f"{n} must be {dtype} [{D}], got {w.dtype} {list(w.shape)}")
+    table = cos.shape
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(table) != 2 or table != sin.shape:
         raise RuntimeError("cos and sin must be float32 [positions, half]")
-    half = cos.shape[1]
+    half = table[1]
     if 2 * half > D or not interleaved and half % 8:
         raise RuntimeError(f"half (cos.shape[1]) must be at most head_size / 2, a multiple of 8 unless interleaved, got {half}")
-    if positions.dtype != torch.int64 or tuple(positions.shape) != (T,):
+    if positions.dtype != torch.int64 or positions.shape != (T,):
         raise RuntimeError(f"positions must be int64 [{T}], got {positions.dtype} {list(positions.shape)}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
@@ -131,9 +139,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     if cos.requires_grad or sin.requires_grad:
         raise RuntimeError("qk_norm_rope has no gradient for cos and sin")
     at = q.get_device()
-    if at < 0 or any(t is not None and t.get_device() != at for t in (k, q_weight, k_weight, cos, sin, positions)):
+    if (at < 0 or k.get_device() != at or cos.get_device() != at or sin.get_device() != at or positions.get_device() != at
+            or q_weight is not None and q_weight.get_device() != at or k_weight is not None and k_weight.get_device() != at):
         raise RuntimeError("q, k, the weights, cos, sin and positions must be on the same CUDA device")
-    qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    qw = None if q_weight is None else q_weight.contiguous()
+    kw = None if k_weight is None else k_weight.contiguous()
     cos, sin, positions = cos.contiguous(), sin.contiguous(), positions.contiguous()
     if _wants_grad(q, k, qw, kw):
         return _NormRope.apply(q, k, qw, kw, cos, sin, positions, float(eps), bool(interleaved))
@@ -227,18 +237,19 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     rounded to the inputs' dtype for the products.  The same result every run.  With return_lse also f32 [query heads,
     query tokens]: the logarithm of the sum of exp(score), -inf where no key is seen (not differentiable).
     Reverse mode only.  For a backward pass that a CUDA graph is to capture, see fp8.linear_fp8."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or qs[2] != ks[2]:
         raise RuntimeError("q must be [query tokens, heads, head_size], k and v [key tokens, heads, head_size], got "
-                           f"{list(q.shape)}, {list(k.shape)} and {list(v.shape)}")
-    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError(f"q, k and v must share one of float16, bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
-    D = q.shape[2]
+                           f"{list(qs)}, {list(ks)} and {list(v.shape)}")
+    if dtype != k.dtype or dtype != v.dtype or dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q, k and v must share one of float16, bfloat16, got {dtype}, {k.dtype} and {v.dtype}")
+    D = qs[2]
     if D < 8 or D > 128 or D % 8:
         raise RuntimeError(f"head_size must be a multiple of 8 up to 128, got {D}")
-    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise RuntimeError(f"query heads ({q.shape[1]}) must be a positive multiple of key heads ({k.shape[1]})")
+    if ks[1] < 1 or qs[1] < 1 or qs[1] % ks[1]:
+        raise RuntimeError(f"query heads ({qs[1]}) must be a positive multiple of key heads ({ks[1]})")
     if cu_k is None:
-        if q.shape[0] != k.shape[0]:
+        if qs[0] != ks[0]:
             raise RuntimeError("cu_k is needed where q and k have different numbers of tokens")
         cu_k = cu_q
     for n, c in (("cu_q", cu_q), ("cu_k", cu_k)):
@@ -249,7 +260,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         raise ValueError("scale must be positive and finite")
     _plain("packed_attention", q, k, v)
     at = q.get_device()
-    if at < 0 or any(t.get_device() != at for t in (k, v, cu_q, cu_k)):
+    if at < 0 or k.get_device() != at or v.get_device() != at or cu_q.get_device() != at or cu_k.get_device() != at:
         raise RuntimeError("q, k, v, cu_q and cu_k must be on the same CUDA device")
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     q, k, v = _aligned(q), _aligned(k), _aligned(v)

@@ -200,17 +200,21 @@ def attend_kv_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     dev = k_cache.device
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] < 1 or q.shape[1] % heads:
-        raise RuntimeError(f"q must be [sequences, a multiple of {heads}, {D}], got {list(q.shape)}")
-    B, Hq = q.shape[0], q.shape[1]
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
-        raise RuntimeError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {list(block_table.shape)}")
-    if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != B:
+    qs = q.shape
+    if len(qs) != 3 or qs[2] != D or qs[1] < 1 or qs[1] % heads:
+        raise RuntimeError(f"q must be [sequences, a multiple of {heads}, {D}], got {list(qs)}")
+    if D > 256:
+        raise RuntimeError(f"head_size must be at most 256, got {D}")
+    B, Hq = qs[0], qs[1]
+    table = block_table.shape
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != B:
+        raise RuntimeError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {list(table)}")
+    if lens.dtype != torch.int32 or lens.shape != (B,):
         raise RuntimeError(f"lens must be int32 [{B}], got {lens.dtype} {list(lens.shape)}")
     at = dev.index
     if q.get_device() != at or block_table.get_device() != at or lens.get_device() != at:
         raise RuntimeError("q, block_table and lens must be on the cache's device")
-    cols = block_table.shape[1]
+    cols = table[1]
     if q.stride(2) != 1:
         q = q.contiguous()
     if block_table.stride(1) != 1 and cols > 1 or block_table.stride(0) < cols and B > 1:
