@@ -173,11 +173,11 @@ def load() -> ctypes.CDLL:
         L.emu_qk_norm_rope_backward.restype = i32
         L.emu_qk_norm_rope_backward.argtypes = [norm_rope, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, size, vp]
         L.emu_attention.restype = i32
-        L.emu_attention.argtypes = [attention, vp, vp, vp]
+        L.emu_attention.argtypes = [attention, vp, vp, vp, vp]
         L.emu_attention_backward_workspace_size.restype = size
         L.emu_attention_backward_workspace_size.argtypes = [attention]
         L.emu_attention_backward.restype = i32
-        L.emu_attention_backward.argtypes = [attention, vp, vp, vp, i64, i64, vp, vp, vp, vp, size, vp]
+        L.emu_attention_backward.argtypes = [attention, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, size, vp]
         L.emu_kv_attend_workspace_size.restype = size
         L.emu_kv_attend_workspace_size.argtypes = [i64, i32, i32, i32]
         L.emu_kv_attend.restype = i32

@@ -175,23 +175,24 @@ def _attention_args(q, k, v, cu_q, cu_k, causal: bool, scale: float):
                                  q.shape[2], _DTYPE[q.dtype], int(causal), scale)
 
 
-def _forward(q, k, v, cu_q, cu_k, causal, scale, want_lse):
+def _forward(q, k, v, cu_q, cu_k, causal, scale, want_lse, want_low=False):
     dev = q.device
     with _on(dev.index):
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev) if want_lse else None
+        low = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_low else None
         args = _attention_args(q, k, v, cu_q, cu_k, causal, scale)
-        status = _lib.load().emu_attention(ctypes.byref(args), out.data_ptr(), _ptr(lse), _raw_stream(dev.index))
+        status = _lib.load().emu_attention(ctypes.byref(args), out.data_ptr(), _ptr(low), _ptr(lse), _raw_stream(dev.index))
     if status:
         _lib._check(status)
-    return out, lse
+    return out, low, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
-        out, lse = _forward(q, k, v, cu_q, cu_k, causal, scale, True)
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, out, lse)
+        out, low, lse = _forward(q, k, v, cu_q, cu_k, causal, scale, True, True)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, out, low, lse)
         ctx.rest = causal, scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -200,7 +201,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, _):
-        q, k, v, cu_q, cu_k, out, lse = ctx.saved_tensors
+        q, k, v, cu_q, cu_k, out, low, lse = ctx.saved_tensors
         if do is None:
             return None, None, None, None, None, None, None
         dev = q.device
@@ -212,7 +213,7 @@ class _Attention(torch.autograd.Function):
             args = _attention_args(q, k, v, cu_q, cu_k, *ctx.rest)
             need = L.emu_attention_backward_workspace_size(ctypes.byref(args))
             work = torch.empty(need, dtype=torch.uint8, device=dev)
-            status = L.emu_attention_backward(ctypes.byref(args), out.data_ptr(), lse.data_ptr(), do.data_ptr(), *_strides(do),
+            status = L.emu_attention_backward(ctypes.byref(args), out.data_ptr(), low.data_ptr(), lse.data_ptr(), do.data_ptr(), *_strides(do),
                                               _ptr(dq), _ptr(dk), _ptr(dv), work.data_ptr(), need, _raw_stream(dev.index))
         if status:
             _lib._check(status)
@@ -267,7 +268,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if _wants_grad(q, k, v):
         out, lse = _Attention.apply(q, k, v, cu_q, cu_k, bool(causal), scale)
     else:
-        out, lse = _forward(q, k, v, cu_q, cu_k, bool(causal), scale, return_lse)
+        out, _, lse = _forward(q, k, v, cu_q, cu_k, bool(causal), scale, return_lse)
     return (out, lse) if return_lse else out
 
 

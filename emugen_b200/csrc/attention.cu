@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     ptx::tc_fence_after();
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
     T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
+    T* low = static_cast<T*>(a.low) + (t * a.Hq + h) * a.D;  // where it is wanted
     float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
 #pragma unroll
     for (int x = 0; x < DP; x += 32) {
@@ -263,6 +264,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
           w[k] = pack2<T>(v0, v1);
         }
         if (mine && ok && x + e < a.D) *reinterpret_cast<uint4*>(out + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (a.low && mine && ok && x + e < a.D) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k]) * f) : 0.0f, n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k + 1]) * f) : 0.0f);
+          *reinterpret_cast<uint4*>(low + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
     if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
     m = last_m, l = sums[r] + sums[128 + r];
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
     T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
+    T* low = static_cast<T*>(a.low) + (t * a.Hq + h) * a.D;  // where it is wanted
     float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
     constexpr int HALF = DP / 2;
 #pragma unroll
@@ -557,6 +564,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
           v[k] = pack2<T>(v0, v1);
         }
         if (mine && ok && d < a.D) *reinterpret_cast<uint4*>(out + d) = make_uint4(v[0], v[1], v[2], v[3]);
+        if (a.low && mine && ok && d < a.D) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = pack2<T>(n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k]) * f) : 0.0f, n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k + 1]) * f) : 0.0f);
+          *reinterpret_cast<uint4*>(low + d) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
       }
     }
     if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;

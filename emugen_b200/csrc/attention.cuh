@@ -46,6 +46,12 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
 
+// What rounding to T takes from v; 0 where v is infinite or NaN, or becomes it.
+template <typename T> __device__ __forceinline__ float rounded_off(float v) {
+  const float r = __fsub_rn(v, widen<T>(narrow<T>(v)));
+  return fabsf(r) < INFINITY ? r : 0.0f;
+}
+
 // One row at a time, a warp to a row: lane l holds elements l, l + 32, l + 64 and l + 96 of it.  Nothing that the mask
 // hides is read, so that infinities and NaN there reach no result.
 struct Lanes {
@@ -122,7 +128,13 @@ template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs
     m = top;
     if (settled(o, a.D)) break;
   }
-  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, d0, d1, o, l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l);
+  const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, d0, d1, o, f);
+  if (a.low) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = rounded_off<T>(__fmul_rn(o.v[i], f));
+    store_row(static_cast<T*>(a.low) + (t * a.Hq + h) * a.D, d0, d1, o, 1.0f);
+  }
 }
 
 // A query's shift -lse log2 e and its delta, at [t * Hq + h].

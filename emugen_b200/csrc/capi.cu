@@ -729,14 +729,14 @@ static emu::AttnArgs attention_args(const emu_attention_args* p) {
   return a;
 }
 
-emu_status emu_attention(const emu_attention_args* p, void* out, float* lse, void* stream) {
+emu_status emu_attention(const emu_attention_args* p, void* out, void* out_low, float* lse, void* stream) {
   const emu_status st = check_attention(p);
   if (st != EMU_OK) return st;
   if (p->total_q == 0) return ok();
   if (!out) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
-  if (!aligned(out, 16) || !aligned(lse, 4)) return fail(EMU_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned, lse 4-byte");
+  if (!aligned(out, 16) || !aligned(out_low, 16) || !aligned(lse, 4)) return fail(EMU_ERR_INVALID_ARGUMENT, "out and out_low must be 16-byte aligned, lse 4-byte");
   emu::AttnArgs a = attention_args(p);
-  a.out = out, a.lse = lse;
+  a.out = out, a.low = out_low, a.lse = lse;
   return cuda_status(emu::launch_attention(a, static_cast<cudaStream_t>(stream)), "emu_attention launch");
 }
 
@@ -745,8 +745,8 @@ size_t emu_attention_backward_workspace_size(const emu_attention_args* p) {
   return emu::attention_backward_workspace(p->total_q, p->total_k, p->heads_q, p->heads_k);
 }
 
-emu_status emu_attention_backward(const emu_attention_args* p, const void* out, const float* lse, const void* dout,
-                                  int64_t dout_token_stride, int64_t dout_head_stride, void* dq, void* dk, void* dv,
+emu_status emu_attention_backward(const emu_attention_args* p, const void* out, const void* out_low, const float* lse,
+                                  const void* dout, int64_t dout_token_stride, int64_t dout_head_stride, void* dq, void* dk, void* dv,
                                   void* workspace, size_t workspace_bytes, void* stream) {
   const emu_status st = check_attention(p);
   if (st != EMU_OK) return st;
@@ -759,15 +759,15 @@ emu_status emu_attention_backward(const emu_attention_args* p, const void* out, 
     return cuda_status(e, "emu_attention_backward memset");
   }
   if (!out || !lse || !dout || !workspace) return fail(EMU_ERR_INVALID_ARGUMENT, "pointers must not be NULL");
-  if (!aligned(out, 16) || !aligned(dout, 16) || !aligned(lse, 4) || !aligned(workspace, 256))
-    return fail(EMU_ERR_INVALID_ARGUMENT, "out and dout must be 16-byte aligned, lse 4-byte, workspace 256-byte");
+  if (!aligned(out, 16) || !aligned(out_low, 16) || !aligned(dout, 16) || !aligned(lse, 4) || !aligned(workspace, 256))
+    return fail(EMU_ERR_INVALID_ARGUMENT, "out, out_low and dout must be 16-byte aligned, lse 4-byte, workspace 256-byte");
   if (dout_token_stride < 8 || dout_token_stride % 8 != 0 || dout_head_stride < 8 || dout_head_stride % 8 != 0 ||
       dout_token_stride >= (1ll << 38) || dout_head_stride >= (1ll << 38))
     return fail(EMU_ERR_INVALID_ARGUMENT, "strides must be positive multiples of 8 elements");
   const size_t need = emu_attention_backward_workspace_size(p);
   if (workspace_bytes < need) return fail(EMU_ERR_INVALID_ARGUMENT, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
   emu::AttnArgs a = attention_args(p);
-  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
+  a.out = const_cast<void*>(out), a.low = const_cast<void*>(out_low), a.lse = const_cast<float*>(lse);
   a.dout = dout, a.dout_stride[0] = dout_token_stride, a.dout_stride[1] = dout_head_stride;
   a.dq = dq, a.dk = dk, a.dv = dv, a.workspace = workspace;
   return cuda_status(emu::launch_attention_backward(a, static_cast<cudaStream_t>(stream)), "emu_attention_backward launch");

@@ -173,6 +173,7 @@ struct AttnArgs {
   const int32_t* cu_k;
   float scale;
   void* out;                    // [Tq][Hq][D]
+  void* low;                    // [Tq][Hq][D]: what rounding took from out; may be null
   float* lse;                   // [Hq][Tq]
   const void* dout;             // backward pass from here on
   int64_t dout_stride[2];

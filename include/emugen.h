@@ -496,7 +496,8 @@ EMU_API emu_status emu_qk_norm_rope_backward(const emu_norm_rope_args* args, con
  * result, whatever they hold.  Scores, sums and the softmax's statistics in f32; p is rounded to the inputs' dtype for its
  * product.  lse f32 [heads_q][total_q] (may be NULL): log of the sum of exp(score), -infinity for a query without keys.
  * dtype fp16 / bf16; head_size a multiple of 8 up to 128; tensors 16-byte aligned, strides multiples of 8 elements; out is
- * contiguous [total_q][heads_q][head_size].  scale positive.  The same result every run.
+ * contiguous [total_q][heads_q][head_size].  out_low, the same (may be NULL): what its rounding took away, for the backward
+ * pass, whose differences of small numbers would show it.  scale positive.  The same result every run.
  */
 typedef struct {
   const void* q;
@@ -509,16 +510,16 @@ typedef struct {
   int32_t heads_q, heads_k, head_size, dtype, causal;
   float scale;
 } emu_attention_args;
-EMU_API emu_status emu_attention(const emu_attention_args* args, void* out, float* lse, void* stream);
+EMU_API emu_status emu_attention(const emu_attention_args* args, void* out, void* out_low, float* lse, void* stream);
 /*
  * Its gradients from dout: dq [total_q][heads_q][head_size], dk and dv [total_k][heads_k][head_size], contiguous, each may be
- * NULL (not wanted).  out and lse are emu_attention's.  ds = p (dout . v - dout . out) is rounded to the inputs' dtype for
+ * NULL (not wanted).  out, out_low (may be NULL) and lse are emu_attention's.  ds = p (dout . v - dout . out) is rounded to the inputs' dtype for
  * its products (fp16: scaled by a power of two that keeps it in range).  No atomic additions: the same result every run.
  * workspace: emu_attention_backward_workspace_size(args) bytes on the device, 256-byte aligned.
  */
 EMU_API size_t emu_attention_backward_workspace_size(const emu_attention_args* args);
-EMU_API emu_status emu_attention_backward(const emu_attention_args* args, const void* out, const float* lse,
-                                          const void* dout, int64_t dout_token_stride, int64_t dout_head_stride, void* dq,
+EMU_API emu_status emu_attention_backward(const emu_attention_args* args, const void* out, const void* out_low,
+                                          const float* lse, const void* dout, int64_t dout_token_stride, int64_t dout_head_stride, void* dq,
                                           void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
 /*

@@ -3,7 +3,8 @@
 With u = half a step of the tensors' 16-bit type and f = 2^-23 for each f32 operation of a chain:
   scores      |error| <= f (D + 4) scale sum |q_d k_d|                  (a D-term sum, the scale, log2 e)
   p           relative: twice the row's largest score error (numerator and sum) + u (its rounding) + f * 64
-  ds          p (dp - delta) relative as p, + u; dp and delta as sums of D terms, delta of the rounded output too
+  ds          p (dp - delta) relative as p, + u; dp and delta as sums of D terms, delta of the output before its rounding (with a rest of it that was
+              rounded in its turn: u^2, or half a subnormal step)
 Sums over n terms add f n times the sum of magnitudes.  16-bit results: u relative, and half a subnormal step."""
 import math
 
@@ -83,7 +84,7 @@ def attention(q, k, v, cu_q, cu_k, causal, scale, do=None, p_step=None, v_low=No
             dv_t[j0:j1, g] += (p * (b_err + u + F * (nq + 64)) + LOWEST * seen).t() @ w.abs()
             dp = w @ c0.t()
             delta = (w * o).sum(1, keepdim=True)
-            dp_err = F * (D + 4) * (w.abs() @ c0.abs().t()) + F * (D + 4) * (w * o).abs().sum(1, keepdim=True) + (w.abs() * o_t).sum(1, keepdim=True)
+            dp_err = F * (D + 4) * (w.abs() @ c0.abs().t()) + F * (D + 4) * (w * o).abs().sum(1, keepdim=True) + (w.abs() * (o_t - u * o.abs() + u * u * o.abs())).sum(1, keepdim=True)
             ds = p * (dp - delta)
             # (fp16: held to 2^-24 of a bound on |dp - delta| times 2^-15)
             bound = 2 * w.norm(dim=1).amax() * c0.norm(dim=1).amax()

@@ -316,3 +316,124 @@ def test_registered_operator():
     assert torch.equal(torch.ops.emugen.packed_attention(q, k, v, c, None, False), want)
     fn = torch.compile(lambda *a: torch.ops.emugen.packed_attention(*a, None, False), fullgraph=True, backend="aot_eager")
     assert torch.equal(fn(q, k, v, c), want)
+
+
+# Calls with so many (sequence, key head) pairs of tiles that a CTA takes two of them: the tests above take one.
+WIDE = dict(Hq=128, Hk=64)
+
+
+@pytest.mark.parametrize("lens", [([300], [300]), ([0, 3, 0, 130], [2, 0, 0, 7]), ([127, 1, 129], [127, 1, 129]), ([64, 200], [190, 3]),
+                                  ([9], [1000]), ([257, 30], [256, 30]), ([70] * 5, [70, 69, 71, 0, 140])], ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 40), (torch.float16, 104)])
+def test_two_tiles_to_a_cta(lens, causal, dtype, D):
+    _check(*lens, **WIDE, D=D, dtype=dtype, causal=causal, seed=len(lens[0]), back=D == 40)
+
+
+@pytest.mark.parametrize("peak,scale", [(30.0, None), (1.0, 1.5), (1.0, 1e-4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_two_tiles_peaked_and_flat(dtype, peak, scale):
+    _check([520], [520], 80, 80, 64, dtype, True, seed=9, peak=peak, scale=scale, back=False)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_two_tiles_hidden_places(bad, D):
+    nq, nk, Hq, Hk = [150, 10, 140], [150, 4, 140], 64, 64
+    q, k, v, _ = _make(nq, nk, Hq, Hk, D, torch.bfloat16, 3, extra=20)
+    cq, ck = _cu(nq), _cu(nk)
+    want = O.attention(q, k, v, cq, ck, True, D ** -0.5)
+    q, k, v = (t.clone() for t in (q, k, v))
+    q[cq[1]:cq[1] + 6] = bad
+    q[cq[-1]:] = bad
+    for t in (k, v):
+        t[ck[-1] - 1:] = bad                           # the last query alone sees the last key
+    out = attention.packed_attention(q, k, v, _tensor(cq), _tensor(ck))
+    O.check(out[:cq[-1] - 1], tuple(w[:cq[-1] - 1] for w in want["out"]), "out")
+    assert (out[cq[-1]:] == 0).all() and (out[cq[1]:cq[1] + 6] == 0).all() and out[cq[-1] - 1].isnan().all()
+
+
+def test_two_tiles_layouts_and_replay():
+    """Slices of a fused projection and heads before tokens, on another stream and replayed: the same bits."""
+    T, Hq, Hk, D = 300, 128, 64, 64
+    q, k, v, _ = _make([T], [T], Hq, Hk, D, torch.bfloat16, 11)
+    c = _tensor([0, 101, T])
+    want = attention.packed_attention(q, k, v, c)
+    fused = torch.cat([q, k, v], 1)
+    parts = fused[:, :Hq], fused[:, Hq:Hq + Hk], fused[:, Hq + Hk:]
+    assert torch.equal(attention.packed_attention(*parts, c), want)
+    assert torch.equal(attention.packed_attention(*(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)), c), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attention.packed_attention(*parts, c)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("Hq,Hk,T", [(130, 1, 40), (200, 1, 400), (258, 2, 33)])
+def test_groups_of_more_than_a_tile(Hq, Hk, T):
+    """More query heads to a key head than a tile has rows."""
+    _check([T - 7, 7], [T - 7, 7], Hq, Hk, 64, torch.bfloat16, True, seed=T, back=T < 100)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_delta_from_the_output_before_its_rounding(dtype):
+    """Two keys of equal weight whose values have much in common: p is exact, the output's rounding is far above the
+    differences dp - delta, and dq has to come out to its own roundings all the same."""
+    n, D = 64, 128
+    g = torch.Generator().manual_seed(6)
+    q = torch.zeros(2 * n, 2, D, dtype=dtype, device="cuda")
+    k = torch.randn(2 * n, 2, D, generator=g).to(dtype).cuda()
+    v = (100 + torch.randn(2 * n, 2, D, generator=g)).to(dtype).cuda()
+    do = torch.randn(2 * n, 2, D, generator=g).to(dtype).cuda()
+    cu = list(range(0, 2 * n + 1, 2))
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = attention.packed_attention(*x, _tensor(cu), causal=False)
+    want = O.attention(q, k, v, cu, cu, False, D ** -0.5, do, p_step=0)
+    O.check(out, want["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, x, do)):
+        O.check(got, want[name], name)
+
+
+@pytest.mark.parametrize("heads,what", [(4, "forward"), (128, "forward"), (4, "gradients")])
+def test_timed_out_wait_is_reported_and_the_context_survives(heads, what):
+    """A tile of scores that is never announced: the kernel gives up and returns, the next query of the device's status
+    tells, and the next call is right."""
+    from emugen_b200 import _lib
+
+    L = _lib.load()
+    q, k, v, do = _make([200], [200], heads, heads, 64, torch.bfloat16, 17)
+    c = _tensor([0, 200])
+    x = [t.requires_grad_() for t in (q, k, v)]
+
+    def run():
+        out = attention.packed_attention(*x, c)
+        return out, torch.autograd.grad(out, x, do)
+
+    want = run()
+    torch.cuda.synchronize()
+    _lib.device_status()
+    out = attention.packed_attention(*x, c)
+    torch.cuda.synchronize()
+    prev = _lib.set_wait_limit(1 << 20)
+    L.emu_test_hold_first_ready(1)
+    try:
+        if what == "forward":
+            with torch.no_grad():
+                attention.packed_attention(q, k, v, c)
+        else:
+            torch.autograd.grad(out, x, do)
+        with pytest.raises(_lib.EmuError) as err:
+            _lib.device_status()
+        assert err.value.status == _lib.EMU_ERR_TIMEOUT and "wait ran out" in str(err.value)
+        _lib.device_status()
+    finally:
+        L.emu_test_hold_first_ready(0)
+        _lib.set_wait_limit(prev)
+    got = run()
+    _lib.device_status()
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))

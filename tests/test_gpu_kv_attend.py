@@ -259,3 +259,20 @@ def test_registered_operator():
 
     q, cache, table, lens = _make([50, 20], 4, 2, 64, 16, "fp8", torch.bfloat16, 12)
     assert torch.equal(torch.ops.emugen.attend_kv_cache(q, *cache, table, lens), kvcache.attend_kv_cache(q, *cache, table, lens))
+
+
+def test_refusals_of_arguments():
+    cache = kvcache.make_kv_cache(2, 4, 2, 64)
+    q = torch.zeros(3, 4, 64, dtype=torch.float16, device="cuda")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for args, msg in [((q.float(), *cache, table, lens), "float16 or bfloat16"), ((q[:, :3], *cache, table, lens), "multiple of 2"),
+                      ((q[..., :32], *cache, table, lens), "must be"), ((q, *cache, table.long(), lens), "block_table"), ((q, *cache, table[:2], lens), "block_table"),
+                      ((q, *cache, table, lens.long()), "lens"), ((q, *cache, table, lens[:2]), "lens"), ((q.cpu(), *cache, table, lens), "device"),
+                      ((q, *cache, table, lens.cpu()), "device")]:
+        with pytest.raises(RuntimeError, match=msg):
+            kvcache.attend_kv_cache(*args)
+    big = kvcache.make_kv_cache(2, 4, 1, 272)
+    with pytest.raises(RuntimeError, match="at most 256"):
+        kvcache.attend_kv_cache(torch.zeros(3, 4, 272, dtype=torch.float16, device="cuda"), *big, table, lens)
+    with pytest.raises(RuntimeError, match="scale"):
+        kvcache.attend_kv_cache(q, *cache, table, lens, scale=0.0)
