@@ -186,6 +186,7 @@ struct Plan {
   bool wide_scales;            // MXFP4: a row's scale bytes may be read at once
   bool whole_steps;            // a step's 16 keys lie in one page
   uint32_t page_size;          // up to 2^31 (more than any length)
+  uint32_t tile_columns, tile_off;                           // pages in a tile of keys, and what is left
 };
 // What the CTA that ends a (sequence, head) leaves for the join: the first and the last CTA of it (the same: nothing to join).
 struct Ending {
@@ -294,10 +295,20 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
     constexpr int SZ = S::FP8 ? 4 : 1;                       // bytes of a scale
     // from slot to slot, in bytes (16 slots stay below 2^32)
     const uint32_t head_row = (uint32_t)(a.Hk * RB), head_scale = (uint32_t)(a.Hk * nb * SZ);
-    // The page of step i's keys (of its key lane % 16 where a step may lie in several); -1 past the end.
-    auto page_of = [&](int i) {
-      const int key = key0 + i * TILE + (pl.whole_steps ? 0 : lane & 15);
-      return i < steps && key < end ? __ldg(table + (uint32_t)key / pl.page_size) : -1;
+    // The step whose page is looked up next: its key (of a step in several pages its key lane % 16) counted back from the end,
+    // and its place in the table and in the page, which move on by additions alone (divisions were a tenth of the
+    // kernel's instructions).
+    const int key_first = key0 + (pl.whole_steps ? 0 : lane & 15);
+    struct Look {
+      int left, column, page;
+      uint32_t off;
+    } look{end - key_first, (int)((uint32_t)key_first / pl.page_size), 0, (uint32_t)key_first % pl.page_size};
+    auto look_up = [&]() {
+      Look r = look;
+      r.page = look.left > 0 ? __ldg(table + look.column) : -1;
+      look.left -= TILE, look.column += pl.tile_columns, look.off += pl.tile_off;
+      if (look.off >= pl.page_size) look.off -= pl.page_size, ++look.column;
+      return r;
     };
     // This lane's rows: keys g and 8 + g for the scores' operand; keys 2 c, 2 c + 1, 8 + 2 c and 9 + 2 c for the values' and for what
     // is known of a score.
@@ -305,12 +316,11 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       uint32_t live;                                         // a bit for each key that is seen
       int64_t slot;                                          // of the first key (of key lane % 16)
     };
-    auto step_of = [&](int i, int page) {
+    auto step_of = [&](const Look& k) {
       Step t;
-      const int key = key0 + i * TILE + (pl.whole_steps ? 0 : lane & 15);
-      const bool ok = page >= 0 && page < a.num_pages;
-      t.slot = ok ? (int64_t)page * a.page_size + (uint32_t)key % pl.page_size : 0;
-      t.live = pl.whole_steps ? (ok ? (1u << min(KEYS, end - key)) - 1 : 0) : __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
+      const bool ok = k.page >= 0 && k.page < a.num_pages;
+      t.slot = ok ? (int64_t)k.page * a.page_size + k.off : 0;
+      t.live = pl.whole_steps ? (ok ? (1u << min(KEYS, k.left)) - 1 : 0) : __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
       return t;
     };
     // A step's codes and scales on their way into stage `st`.  Where all of its keys are seen and lie behind one another and D
@@ -371,15 +381,15 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       for (int k = 0; k < S::SCALE / 4; ++k) dst[k] = held[k];
     };
     uint32_t lives[STAGES];                                  // of the steps under way, the next one first
-    int page_next;
+    Look next;
     {
-      int pages[STAGES];
+      Look pages[STAGES];
 #pragma unroll
-      for (int i = 0; i < STAGES; ++i) pages[i] = page_of(i);
+      for (int i = 0; i < STAGES; ++i) pages[i] = look_up();
       uint32_t early[STAGES][2];
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i) {
-        const Step t = step_of(i, pages[i]);
+        const Step t = step_of(pages[i]);
         lives[i] = t.live;
         fetch(t, i);
         early[i][0] = held[0], early[i][1] = held[1];
@@ -389,7 +399,7 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
         held[0] = early[i][0], held[1] = early[i][1];
         put_scales(i);
       }
-      page_next = pages[STAGES - 1];
+      next = pages[STAGES - 1];
     }
 
     // ---- q as the MMAs' A operands: fp16, multiplied by a power of two
@@ -439,8 +449,8 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
 #pragma unroll
       for (int x = 0; x + 2 < STAGES; ++x) lives[x] = lives[x + 1];
       {
-        const Step t = step_of(i + STAGES - 1, page_next);
-        page_next = page_of(i + STAGES);
+        const Step t = step_of(next);
+        next = look_up();
         lives[STAGES - 2] = t.live;
         fetch(t, st_new);
       }
@@ -824,6 +834,7 @@ template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvA
   pl.wide_scales = FORMAT == EMU_KV_MXFP4 && a.D == DP && at % std::min(4, DP / 32) == 0;
   pl.wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride[0] * 2) | (uintptr_t)(a.q_stride[1] * 2)) & 7) == 0;
   pl.page_size = (uint32_t)std::min<int64_t>(a.page_size, 1ll << 31);
+  pl.tile_columns = TILE / pl.page_size, pl.tile_off = TILE % pl.page_size;
   pl.whole_steps = a.page_size % KEYS == 0;
   kernel<<<pl.ctas, NT, SMEM, stream>>>(a, pl);
   // launched early, so that its CTAs wait where the attention's finish
