@@ -90,18 +90,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
         for (int x = 0; x < DP / 64; ++x)
           ptx::tma_load_3d(smem + i * C::TILE + x * 16384, &map_q, q_full, x * 64, head, (int)(u.t0 + i * tl.tokens));
       Ring<C::SLOTS> r;
-      bool ok = true;
       int i = 0;
       for (; i < 2 * tiles; ++i, r.next()) {
-        if (i >= C::SLOTS && !wait_or_record(&kv_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_FWD_SLOT)) { ok = false; break; }
+        if (i >= C::SLOTS && !wait_or_record(&kv_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_FWD_SLOT)) break;
         ptx::mbar_arrive_expect_tx(&kv_full[r.at], C::TILE);
         for (int x = 0; x < DP / 64; ++x)
           ptx::tma_load_3d(ring + r.at * C::TILE + x * 16384, i & 1 ? &map_v : &map_k, &kv_full[r.at], x * 64, u.kh, (int)(kr.begin + (i >> 1) * 128));
       }
-      if (!ok) {                                             // every copy has landed before the CTA exits
-        wait_or_record(q_full, 0, DRAIN_LIMIT, WAIT_DRAIN);
-        for (int j = max(0, i - C::SLOTS); j < i; ++j) wait_or_record(&kv_full[j % C::SLOTS], (j / C::SLOTS) & 1, DRAIN_LIMIT, WAIT_DRAIN);
-      }
+      drain<1>(q_full, 1), drain<C::SLOTS>(kv_full, i);
     } else if (warp == 8 && tiles) {
       const uint32_t tmem = *tmem_slot;
       constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
@@ -366,24 +362,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
       ptx::mbar_arrive_expect_tx(q_full, (DP / 64) * tl.heads * tl.tokens * 128);
       for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(smem + x * 16384, &map_q, q_full, x * 64, head, (int)u.t0);
       Ring<C::SLOTS> k, v;
-      auto load = [&](const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty, Ring<C::SLOTS>& r, int j) {
+      int keys = 0, values = 0;                              // tiles asked for
+      auto load = [&](const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty, Ring<C::SLOTS>& r, int& j) {
         if (j >= C::SLOTS && !wait_or_record(&empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_FWD_SLOT)) return false;
         ptx::mbar_arrive_expect_tx(&full[r.at], C::TILE);
         for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring + r.at * C::TILE + x * 16384, map, &full[r.at], x * 64, u.kh, (int)(kr.begin + (int64_t)j * 128));
-        r.next();
+        r.next(), ++j;
         return true;
       };
       // in the order of their use: K_0, K_1, K_2, V_0, K_3, V_1, ..
       bool ok = true;
-      for (int j = 0; j < min(3, tiles) && ok; ++j) ok = load(&map_k, ring_k, k_full, k_empty, k, j);
-      for (int j = 0; j < tiles && ok; ++j) {
-        ok = load(&map_v, ring_v, v_full, v_empty, v, j);
-        if (ok && j + 3 < tiles) ok = load(&map_k, ring_k, k_full, k_empty, k, j + 3);
+      while (keys < min(3, tiles) && ok) ok = load(&map_k, ring_k, k_full, k_empty, k, keys);
+      while (values < tiles && ok) {
+        ok = load(&map_v, ring_v, v_full, v_empty, v, values);
+        if (ok && keys < tiles) ok = load(&map_k, ring_k, k_full, k_empty, k, keys);
       }
-      if (!ok) {                                             // time for the copies in flight to land before the CTA exits
-        const long long t0 = clock64();
-        while (clock64() - t0 < 200000) {}
-      }
+      drain<1>(q_full, 1), drain<C::SLOTS>(k_full, keys), drain<C::SLOTS>(v_full, values);
     } else if ((warp == 8 || warp == 10) && tiles) {
       const uint32_t tmem = *tmem_slot;
       constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;

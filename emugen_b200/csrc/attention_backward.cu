@@ -199,22 +199,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
       }
       const uint32_t bytes = (DP / 64) * tl.heads * tl.tokens * 128;
       Ring<C::SLOTS> r;
-      bool ok = true;
-      int i = 0, tile = 0, chunk = 0;
+      int i = 0, queries = 0, tile = 0, chunk = 0;            // queries, i: tiles of Q and of dO asked for
       for (; i < steps; ++i, r.next()) {
         const int head = u.kh * tl.group + chunk * tl.heads, row = (int)(qr.begin + first + (int64_t)tile * tl.tokens);
-        if (i >= C::SLOTS && !wait_or_record(&q_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) { ok = false; break; }
+        if (i >= C::SLOTS && !wait_or_record(&q_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) break;
         ptx::mbar_arrive_expect_tx(&q_full[r.at], bytes);
         for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring_q + r.at * C::TILE + x * 16384, &map_q, &q_full[r.at], x * 64, head, row);
-        if (i >= C::SLOTS && !wait_or_record(&g_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) { ok = false; break; }
+        ++queries;
+        if (i >= C::SLOTS && !wait_or_record(&g_empty[r.at], r.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) break;
         ptx::mbar_arrive_expect_tx(&g_full[r.at], bytes);
         for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring_g + r.at * C::TILE + x * 16384, &map_g, &g_full[r.at], x * 64, head, row);
         if (++tile == tiles) tile = 0, ++chunk;
       }
-      if (!ok) {                                             // time for the copies in flight to land before the CTA exits
-        const long long t0 = clock64();
-        while (clock64() - t0 < 200000) {}
-      }
+      drain<1>(kv_full, 1), drain<C::SLOTS>(q_full, queries), drain<C::SLOTS>(g_full, i);
     } else if (warp == 10 && steps) {
       const float2* src = work_of(a.workspace).stats;
       Ring<C::STATS> r;
@@ -526,20 +523,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
       }
       Ring<C::K_SLOTS> k;
       Ring<C::V_SLOTS> v;
-      bool ok = true;
-      for (int j = 0; j < tiles; ++j, k.next(), v.next()) {
+      int keys = 0, j = 0;                                   // tiles of K and of V asked for
+      for (; j < tiles; ++j, k.next(), v.next()) {
         const int row = (int)(kr.begin + (int64_t)j * 128);
-        if (j >= C::K_SLOTS && !wait_or_record(&k_empty[k.at], k.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) { ok = false; break; }
+        if (j >= C::K_SLOTS && !wait_or_record(&k_empty[k.at], k.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) break;
         ptx::mbar_arrive_expect_tx(&k_full[k.at], C::TILE);
         for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring_k + k.at * C::TILE + x * 16384, &map_k, &k_full[k.at], x * 64, u.kh, row);
-        if (j >= C::V_SLOTS && !wait_or_record(&v_empty[v.at], v.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) { ok = false; break; }
+        ++keys;
+        if (j >= C::V_SLOTS && !wait_or_record(&v_empty[v.at], v.parity ^ 1, tl.wait_limit, WAIT_BACK_SLOT)) break;
         ptx::mbar_arrive_expect_tx(&v_full[v.at], C::TILE);
         for (int x = 0; x < DP / 64; ++x) ptx::tma_load_3d(ring_v + v.at * C::TILE + x * 16384, &map_v, &v_full[v.at], x * 64, u.kh, row);
       }
-      if (!ok) {                                             // time for the copies in flight to land before the CTA exits
-        const long long t0 = clock64();
-        while (clock64() - t0 < 200000) {}
-      }
+      drain<1>(fixed, 1), drain<C::K_SLOTS>(k_full, keys), drain<C::V_SLOTS>(v_full, j);
     } else if (warp == 8 && tiles) {
       const uint32_t tmem = *tmem_slot;
       constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;

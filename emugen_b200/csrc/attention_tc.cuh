@@ -45,6 +45,12 @@ template <int N> struct Ring {
   }
 };
 
+// The copies into a ring of N slots, filled in turn by `issued` loads, have all landed: a CTA does not exit before (after a failed
+// wait nothing else may have waited for them).
+template <int N> __device__ __forceinline__ void drain(uint64_t* full, int issued) {
+  for (int j = max(0, issued - N); j < issued; ++j) wait_or_record(&full[j % N], (j / N) & 1, DRAIN_LIMIT, WAIT_DRAIN);
+}
+
 // How rows of queries are put into tiles of up to 128: `tokens` consecutive tokens, `heads` query heads of each, row
 // token * heads + head.  All heads of a group as a rule; groups of more than 128 in `chunks`.
 struct Tiling {
