@@ -239,33 +239,31 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     if (ok && tiles) ok = warp_wait_or_record(&o_full[i], 0, tl.wait_limit, WAIT_FWD_O);
     ptx::tc_fence_after();
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
-    T* low = static_cast<T*>(a.low) + (t * a.Hq + h) * a.D;  // where it is wanted
     float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
+    RowsOut<DP / 8> rows_out{smem + i * C::TILE + (warp & 3) * 32 * DP * 2};         // (Q's place: its products are done)
+    for (int pass = 0; pass < (a.low ? 2 : 1); ++pass) {     // the output, and what its rounding took away
 #pragma unroll
-    for (int x = 0; x < DP; x += 32) {
-      uint32_t o[32];
-      if (tiles) {
-        ptx::tmem_ld_regs(o_at + x, o);
-        ptx::tmem_wait_regs(o);
-      }
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // a row without keys gives zeros, whatever its place held
-          const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-          if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-          w[k] = pack2<T>(v0, v1);
+      for (int x = 0; x < DP; x += 32) {
+        uint32_t o[32];
+        if (tiles) {
+          ptx::tmem_ld_regs(o_at + x, o);
+          ptx::tmem_wait_regs(o);
         }
-        if (mine && ok && x + e < a.D) *reinterpret_cast<uint4*>(out + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (a.low && mine && ok && x + e < a.D) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k]) * f) : 0.0f, n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k + 1]) * f) : 0.0f);
-          *reinterpret_cast<uint4*>(low + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // a row without keys gives zeros, whatever its place held
+            float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
+            if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
+            if (pass) v0 = rounded_off<T>(v0), v1 = rounded_off<T>(v1);
+            w[k] = pack2<T>(v0, v1);
+          }
+          rows_out.put((x + e) / 8, w);
         }
       }
+      rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D, mine && ok, a.D / 8);
     }
     if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
@@ -535,35 +533,32 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
     asm volatile("bar.sync 1, 256;" ::: "memory");
     m = last_m, l = sums[r] + sums[128 + r];
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    T* out = static_cast<T*>(a.out) + (t * a.Hq + h) * a.D;
-    T* low = static_cast<T*>(a.low) + (t * a.Hq + h) * a.D;  // where it is wanted
     float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
     constexpr int HALF = DP / 2;
+    RowsOut<HALF / 8> rows_out{smem + (w * 128 + (warp & 3) * 32) * HALF * 2};       // (Q's place: its products are done)
+    for (int pass = 0; pass < (a.low ? 2 : 1); ++pass) {     // the output, and what its rounding took away
 #pragma unroll
-    for (int x = 0; x < HALF; x += 32) {
-      uint32_t o[32];
-      if (tiles) {
-        ptx::tmem_ld_regs(lanes + FEW_O + w * HALF + x, o);
-        ptx::tmem_wait_regs(o);
-      }
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        const int d = w * HALF + x + e;
-        uint32_t v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // a row without keys gives zeros, whatever its place held
-          const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-          if (d < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-          v[k] = pack2<T>(v0, v1);
+      for (int x = 0; x < HALF; x += 32) {
+        uint32_t o[32];
+        if (tiles) {
+          ptx::tmem_ld_regs(lanes + FEW_O + w * HALF + x, o);
+          ptx::tmem_wait_regs(o);
         }
-        if (mine && ok && d < a.D) *reinterpret_cast<uint4*>(out + d) = make_uint4(v[0], v[1], v[2], v[3]);
-        if (a.low && mine && ok && d < a.D) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = pack2<T>(n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k]) * f) : 0.0f, n > 0 ? rounded_off<T>(__uint_as_float(o[e + 2 * k + 1]) * f) : 0.0f);
-          *reinterpret_cast<uint4*>(low + d) = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // a row without keys gives zeros, whatever its place held
+            float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
+            if (w * HALF + x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
+            if (pass) v0 = rounded_off<T>(v0), v1 = rounded_off<T>(v1);
+            v[k] = pack2<T>(v0, v1);
+          }
+          rows_out.put((x + e) / 8, v);
         }
       }
+      rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D + w * HALF, mine && ok, (a.D - w * HALF) / 8);
     }
     if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     const bool keys = half == 1;
     void* base = keys ? a.dk : a.dv;
     const bool mine = ok && base && t < kr.end;
-    T* out = static_cast<T*>(base) + (t * a.Hk + u.kh) * a.D;
+    RowsOut<DP / 8> rows_out{smem + half * C::TILE + (warp & 3) * 32 * DP * 2};      // (the places of K and V: their products are done)
     const float f = keys ? a.scale / ds_factor<T>(w) : exp2f(-P_LOG2<T>);
     float worst = 0.0f;
 #pragma unroll
@@ -434,9 +434,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
           if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
           v[k] = pack2<T>(v0, v1);
         }
-        if (mine && x + e < a.D) *reinterpret_cast<uint4*>(out + x + e) = make_uint4(v[0], v[1], v[2], v[3]);
+        rows_out.put((x + e) / 8, v);
       }
     }
+    rows_out.store(static_cast<T*>(base) + (t * a.Hk + u.kh) * a.D, mine, a.D / 8);
     // A query that does not see the key was multiplied by 0, which infinities and NaN turn into NaN: such rows are made
     // again from the queries that see them alone.
     const bool redo = mine && worst != 0.0f;
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
     if (ok && tiles) ok = warp_wait_or_record(done, 0, tl.wait_limit, WAIT_BACK_DONE);
     ptx::tc_fence_after();
     constexpr int HALF = DP / 2;
-    T* out = static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D;
+    RowsOut<HALF / 8> rows_out{smem + (half * 128 + (warp & 3) * 32) * HALF * 2};    // (Q's place: its products are done)
     const float f = a.scale / factor;
     float worst = 0.0f;
 #pragma unroll
@@ -684,9 +685,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
           if (d < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
           v[k] = pack2<T>(v0, v1);
         }
-        if (mine && ok && d < a.D) *reinterpret_cast<uint4*>(out + d) = make_uint4(v[0], v[1], v[2], v[3]);
+        rows_out.put((x + e) / 8, v);
       }
     }
+    rows_out.store(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D + half * HALF, mine && ok, (a.D - half * HALF) / 8);
     // a hidden key that is infinite or NaN: the row again, from the keys that it sees alone (this thread's half of it)
     const bool redo = mine && ok && worst != 0.0f;
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {

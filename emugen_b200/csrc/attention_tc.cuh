@@ -118,6 +118,28 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A warp's 32 rows, one to a lane, on their way out through 32 x CHUNKS x 16 bytes of shared memory: stored by the lanes that have
+// them, each 16-byte piece would be a memory line of its own, and the stores were an eighth of the forward pass.
+template <int CHUNKS> struct RowsOut {
+  uint8_t* at;
+  static __device__ __forceinline__ int place(int row, int k) { return (row * CHUNKS + (k ^ (CHUNKS == 4 ? row >> 1 & 3 : row & 7))) * 16; }
+  __device__ __forceinline__ void put(int k, const uint32_t (&v)[4]) { *reinterpret_cast<uint4*>(at + place(threadIdx.x & 31, k)) = make_uint4(v[0], v[1], v[2], v[3]); }
+  // To `to` of each lane that has `any`, the first `count` pieces.  (The whole warp.)
+  __device__ __forceinline__ void store(void* to, bool any, int count) {
+    const int lane = threadIdx.x & 31, k = lane % CHUNKS;
+    const uint32_t rows = __ballot_sync(0xFFFFFFFFu, any);   // (the warp's writes above come before the reads below)
+    __syncwarp();
+#pragma unroll 4
+    for (int i = 0; i < 32; i += 32 / CHUNKS) {
+      const int row = i + lane / CHUNKS;
+      uint8_t* p = reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(to), row));
+      const uint4 v = *reinterpret_cast<const uint4*>(at + place(row, k));
+      if ((rows >> row & 1) && k < count) *reinterpret_cast<uint4*>(p + 16 * k) = v;
+    }
+    __syncwarp();
+  }
+};
+
 // ------------------------------------------------------------------------------ host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
