@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     if (ok && tiles) ok = warp_wait_or_record(&o_full[i], 0, tl.wait_limit, WAIT_FWD_O);
     ptx::tc_fence_after();
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
+    const uint64_t f2 = ptx::join2(__float_as_uint(f), __float_as_uint(f));
+    uint64_t worst = 0;                                      // NaN where an output is NaN or infinite
     RowsOut<DP / 8> rows_out{smem + i * C::TILE + (warp & 3) * 32 * DP * 2};         // (Q's place: its products are done)
     for (int pass = 0; pass < (a.low ? 2 : 1); ++pass) {     // the output, and what its rounding took away
 #pragma unroll
@@ -250,25 +251,20 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
           ptx::tmem_wait_regs(o);
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // a row without keys gives zeros, whatever its place held
-            float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-            if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-            if (pass) v0 = rounded_off<T>(v0), v1 = rounded_off<T>(v1);
-            w[k] = pack2<T>(v0, v1);
+        for (int e = 0; e < 32; e += 8)
+          if (x + e < a.D) {
+            uint32_t v[4];
+            round8<T>(o + e, f2, pass, worst, v);
+            if (n <= 0) v[0] = v[1] = v[2] = v[3] = 0;                 // whatever its place held
+            rows_out.put((x + e) / 8, v);
           }
-          rows_out.put((x + e) / 8, w);
-        }
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D, mine && ok, a.D / 8);
     }
     if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone.  (Where the sum is NaN, the scores are, and the row is NaN by right.)
-    redo = mine && ok && worst != 0.0f && l > 0.0f;
+    redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
       const int src = __ffs(rows) - 1;
       row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), 0, a.D);
@@ -533,7 +529,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
     asm volatile("bar.sync 1, 256;" ::: "memory");
     m = last_m, l = sums[r] + sums[128 + r];
     const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    float worst = 0.0f;                                      // 0, or NaN where an output is NaN or infinite
+    const uint64_t f2 = ptx::join2(__float_as_uint(f), __float_as_uint(f));
+    uint64_t worst = 0;                                      // NaN where an output is NaN or infinite
     constexpr int HALF = DP / 2;
     RowsOut<HALF / 8> rows_out{smem + (w * 128 + (warp & 3) * 32) * HALF * 2};       // (Q's place: its products are done)
     for (int pass = 0; pass < (a.low ? 2 : 1); ++pass) {     // the output, and what its rounding took away
@@ -545,25 +542,20 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
           ptx::tmem_wait_regs(o);
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // a row without keys gives zeros, whatever its place held
-            float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-            if (w * HALF + x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-            if (pass) v0 = rounded_off<T>(v0), v1 = rounded_off<T>(v1);
-            v[k] = pack2<T>(v0, v1);
+        for (int e = 0; e < 32; e += 8)
+          if (w * HALF + x + e < a.D) {
+            uint32_t v[4];
+            round8<T>(o + e, f2, pass, worst, v);
+            if (n <= 0) v[0] = v[1] = v[2] = v[3] = 0;                 // whatever its place held
+            rows_out.put((x + e) / 8, v);
           }
-          rows_out.put((x + e) / 8, v);
-        }
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D + w * HALF, mine && ok, (a.D - w * HALF) / 8);
     }
     if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone (this thread's half).  (Where the sum is NaN, the scores are, and the row is NaN by right.)
-    const bool redo = mine && ok && worst != 0.0f && l > 0.0f;
+    const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
       const int src = __ffs(rows) - 1;
       row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), w * HALF, min(a.D, (w + 1) * HALF));

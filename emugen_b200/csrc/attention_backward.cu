@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     const bool mine = ok && base && t < kr.end;
     RowsOut<DP / 8> rows_out{smem + half * C::TILE + (warp & 3) * 32 * DP * 2};      // (the places of K and V: their products are done)
     const float f = keys ? a.scale / ds_factor<T>(w) : exp2f(-P_LOG2<T>);
-    float worst = 0.0f;
+    const uint64_t out2 = ptx::join2(__float_as_uint(f), __float_as_uint(f));
+    uint64_t worst = 0;                                      // NaN where a gradient is NaN or infinite
 #pragma unroll
     for (int x = 0; x < DP; x += 32) {
       uint32_t o[32];
@@ -426,21 +427,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
         ptx::tmem_wait_regs(o);
       }
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        uint32_t v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float v0 = steps ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = steps ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-          if (x + e < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-          v[k] = pack2<T>(v0, v1);
+      for (int e = 0; e < 32; e += 8)
+        if (x + e < a.D) {
+          uint32_t v[4];
+          round8<T>(o + e, out2, false, worst, v);
+          if (!steps) v[0] = v[1] = v[2] = v[3] = 0;         // whatever its place held
+          rows_out.put((x + e) / 8, v);
         }
-        rows_out.put((x + e) / 8, v);
-      }
     }
     rows_out.store(static_cast<T*>(base) + (t * a.Hk + u.kh) * a.D, mine, a.D / 8);
     // A query that does not see the key was multiplied by 0, which infinities and NaN turn into NaN: such rows are made
     // again from the queries that see them alone.
-    const bool redo = mine && worst != 0.0f;
+    const bool redo = mine && steps && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
       const int64_t row = __shfl_sync(0xFFFFFFFFu, t, __ffs(rows) - 1);
       if (keys) row_dkv<T, true>(a, w.stats, u.b, row, u.kh);
@@ -667,7 +665,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
     constexpr int HALF = DP / 2;
     RowsOut<HALF / 8> rows_out{smem + (half * 128 + (warp & 3) * 32) * HALF * 2};    // (Q's place: its products are done)
     const float f = a.scale / factor;
-    float worst = 0.0f;
+    const uint64_t out2 = ptx::join2(__float_as_uint(f), __float_as_uint(f));
+    uint64_t worst = 0;                                      // NaN where a gradient is NaN or infinite
 #pragma unroll
     for (int x = 0; x < HALF; x += 32) {
       uint32_t o[32];
@@ -676,21 +675,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
         ptx::tmem_wait_regs(o);
       }
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        const int d = half * HALF + x + e;
-        uint32_t v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float v0 = n > 0 ? __uint_as_float(o[e + 2 * k]) * f : 0.0f, v1 = n > 0 ? __uint_as_float(o[e + 2 * k + 1]) * f : 0.0f;
-          if (d < a.D) worst = __fmaf_rn(v0, 0.0f, __fmaf_rn(v1, 0.0f, worst));
-          v[k] = pack2<T>(v0, v1);
+      for (int e = 0; e < 32; e += 8)
+        if (half * HALF + x + e < a.D) {
+          uint32_t v[4];
+          round8<T>(o + e, out2, false, worst, v);
+          if (n <= 0) v[0] = v[1] = v[2] = v[3] = 0;         // whatever its place held
+          rows_out.put((x + e) / 8, v);
         }
-        rows_out.put((x + e) / 8, v);
-      }
     }
     rows_out.store(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D + half * HALF, mine && ok, (a.D - half * HALF) / 8);
     // a hidden key that is infinite or NaN: the row again, from the keys that it sees alone (this thread's half of it)
-    const bool redo = mine && ok && worst != 0.0f;
+    const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
     for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
       const int src = __ffs(rows) - 1;
       row_dq<T>(a, w.stats, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), half * HALF, min(a.D, (half + 1) * HALF));

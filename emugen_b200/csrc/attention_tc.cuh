@@ -118,6 +118,27 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Eight sums times f (twice, f2) in 16 bits, or with `rest` what that rounding takes away.  worst: NaN once one of them is infinite
+// or NaN (a rest of an infinite value is).
+template <typename T> __device__ __forceinline__ uint64_t widen2(uint32_t w);
+template <> __device__ __forceinline__ uint64_t widen2<__nv_bfloat16>(uint32_t w) { return ptx::join2(w << 16, w & 0xFFFF0000u); }
+template <> __device__ __forceinline__ uint64_t widen2<__half>(uint32_t w) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return ptx::join2(__float_as_uint(v.x), __float_as_uint(v.y));
+}
+template <typename T> __device__ __forceinline__ void round8(const uint32_t* o, uint64_t f2, bool rest, uint64_t& worst, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint64_t v = ptx::mul2(ptx::join2(o[2 * k], o[2 * k + 1]), f2);
+    w[k] = pack2<T>(ptx::lo2(v), ptx::hi2(v));
+    if (rest) {
+      v = ptx::fma2(widen2<T>(w[k]), ptx::join2(0xBF800000u, 0xBF800000u), v);
+      w[k] = pack2<T>(ptx::lo2(v), ptx::hi2(v));
+    }
+    worst = ptx::fma2(v, 0, worst);
+  }
+}
+
 // A warp's 32 rows, one to a lane, on their way out through 32 x CHUNKS x 16 bytes of shared memory: stored by the lanes that have
 // them, each 16-byte piece would be a memory line of its own, and the stores were an eighth of the forward pass.
 template <int CHUNKS> struct RowsOut {
