@@ -95,6 +95,12 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// An 8 x 8 matrix of fp16 pairs, row lane / 4 and columns 2 (lane % 4) and the next, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 // 2^e as fp16 bits: subnormal below -14, 0 below -24, infinity above 15
 __device__ __forceinline__ uint32_t half_pow2(int e) { return e > 15 ? 0x7C00u : e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u; }
 
@@ -182,6 +188,7 @@ __host__ __device__ inline Parts parts_of(void* workspace, int64_t items, int64_
 }
 struct Plan {
   int ctas, groups, rows;      // CTAs, items of up to 16 query heads to a key head, rows of an item
+  int side_bits, sets;         // sets of 2^side_bits CTAs that take the same keys of neighbouring heads
   bool wide_q;                 // four elements of q may be read at once
   bool wide_scales;            // MXFP4: a row's scale bytes may be read at once
   bool whole_steps;            // a step's 16 keys lie in one page
@@ -212,6 +219,7 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
   float* sums = reinterpret_cast<float*>(ring);              // [8 rows][DP + 4]
   float2* join_ml = reinterpret_cast<float2*>(smem + WARPS * RING);                // [warp][8]
   const int D = a.D, HV = a.Hk * pl.groups, group = a.Hq / a.Hk;
+  const int set = blockIdx.x >> pl.side_bits, side = blockIdx.x & ((1 << pl.side_bits) - 1), HS = HV >> pl.side_bits;            // (sequence, set of heads)s of a sequence
   const Parts parts = parts_of(a.workspace, a.B * HV, pl.ctas, pl.rows, D);
 
   asm volatile("griddepcontrol.launch_dependents;");        // the join's CTAs may come when there is room
@@ -220,17 +228,17 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
   {
     int64_t base = 0;
     if (a.B <= NT) {
-      const int64_t n = threadIdx.x < a.B ? places_of(a, threadIdx.x) * HV : 0;
+      const int64_t n = threadIdx.x < a.B ? places_of(a, threadIdx.x) * HS : 0;
       const int64_t before = block_scan(n, tmp, total);
-      const int64_t lo = Deal(total, pl.ctas).begin(blockIdx.x);
+      const int64_t lo = Deal(total, pl.sets).begin(set);
       if (before <= lo && lo < before + n) found[0] = threadIdx.x, found[1] = before;
     } else {
       int64_t sum = 0;
       for (int64_t i = threadIdx.x; i < a.B; i += NT) sum += places_of(a, i);
-      block_scan(sum * HV, tmp, total);
-      const int64_t lo = Deal(total, pl.ctas).begin(blockIdx.x);
+      block_scan(sum * HS, tmp, total);
+      const int64_t lo = Deal(total, pl.sets).begin(set);
       for (int64_t b0 = 0; b0 < a.B && base <= lo; b0 += NT) {
-        const int64_t n = b0 + threadIdx.x < a.B ? places_of(a, b0 + threadIdx.x) * HV : 0;
+        const int64_t n = b0 + threadIdx.x < a.B ? places_of(a, b0 + threadIdx.x) * HS : 0;
         int64_t all;
         const int64_t before = base + block_scan(n, tmp, all);
         if (before <= lo && lo < before + n) found[0] = b0 + threadIdx.x, found[1] = before;
@@ -239,24 +247,25 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
     }
     __syncthreads();
   }
-  const Deal deal(total, pl.ctas);
-  int64_t at = deal.begin(blockIdx.x);                       // `at` in the list of all places
-  const int64_t hi = deal.begin(blockIdx.x + 1);
+  const Deal deal(total, pl.sets);
+  int64_t at = deal.begin(set);                              // `at` in the list of all places
+  const int64_t hi = set < pl.sets ? deal.begin(set + 1) : at;
   if (at < hi) b = found[0], first = found[1];
 
   while (at < hi) {
     const int64_t per = places_of(a, b);
-    if (per == 0 || at >= first + per * HV) {
-      first += per * HV;
+    if (per == 0 || at >= first + per * HS) {
+      first += per * HS;
       ++b;
       continue;
     }
-    const int hv = at - first <= 0xFFFFFFFF ? (int)((uint32_t)(at - first) / (uint32_t)per) : (int)((at - first) / per);
-    const int64_t start = first + hv * per, stop = start + per;                    // this (sequence, head)'s places
+    const int hs = at - first <= 0xFFFFFFFF ? (int)((uint32_t)(at - first) / (uint32_t)per) : (int)((at - first) / per);
+    const int64_t start = first + hs * per, stop = start + per;                    // this (sequence, set of heads)'s places
     const int64_t tile0 = max((int64_t)0, at - start - EXTRA), tile1 = min(hi, stop) - start - EXTRA;
     at = min(hi, stop);
     if (tile1 <= tile0) continue;
-    const int kh = hv / pl.groups, h0 = kh * group + (hv % pl.groups) * 16, rows = min(16, group - (hv % pl.groups) * 16);
+    const int kh = (hs / pl.groups << pl.side_bits) + side, part = hs % pl.groups, hv = kh * pl.groups + part;
+    const int h0 = kh * group + part * 16, rows = min(16, group - part * 16);
     const int len = (int)min((int64_t)a.lens[b], a.table_cols * a.page_size);
     const int32_t* table = a.table + b * a.table_stride;
 
@@ -423,22 +432,26 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       const float f = pow2(14 - e2);
       qf[r] = a.scale * 1.4426950408889634f * pow2(max(e2 - 14, -126));
       if (e2 - 14 < -126) qf[r] *= pow2(e2 - 14 + 126);
+      qf[r] = fmaxf(qf[r], 1.4e-45f);                        // -inf times it stays -inf
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int e = 0; e < 2; ++e) q[s][e * R + r] = pack_half(value(raw[r][s][e], 0) * f, value(raw[r][s][e], 1) * f);
     }
 
-    // o[n][r]: elements d (rows of the MMA) of heads 8 r + 2 c and 8 r + 2 c + 1; m and l are those of heads g + 8 r
-    float o[DT][R][4] = {}, m[R], l[R] = {};
+    // o[n][r]: elements d (rows of the MMA) of heads 8 r + 2 c and 8 r + 2 c + 1, as are m, l and what a score is multiplied by (up_s: MXFP4 with
+    // 2^(kref - 127 - 8))
+    float o[DT][R][4] = {}, m[R][2], l[R][2] = {}, up_q[R][2], up_s[R][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = -INFINITY;
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) m[r][y] = -INFINITY, up_s[r][y] = up_q[r][y] = __shfl_sync(0xFFFFFFFFu, qf[r], 8 * c + 4 * y);
     // FP8: the exponent of the largest scale of values so far, for each block, the same in the whole warp; MXFP4: that of
-    // this lane's block.  up: FP8, 2^(6 - (ref - 127)), in two factors that both exist.
+    // this lane's block.  up: FP8, 2^(6 - (ref - 127)), in two factors that both exist; limit: the smallest scale past ref.
     int ref[NB], kref = -1000;                               // kref: MXFP4, the largest exponent of the keys' scales so far
-    float up0[NB], up1[NB];
+    float up0[NB], up1[NB], limit[NB];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) ref[k] = -1000, up0[k] = up1[k] = 1.0f;
+    for (int k = 0; k < NB; ++k) ref[k] = -1000, up0[k] = up1[k] = 1.0f, limit[k] = 0.0f;
 
     int st = 0, st_new = STAGES - 1;                         // the stage that is read, and the one that is filled
     for (int i = 0; i < steps; ++i) {
@@ -458,28 +471,28 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
       const uint8_t* values = keys + KEYS * S::PITCH;
       const uint8_t* key_scales = values + KEYS * S::PITCH;
       const uint8_t* value_scales = key_scales + KEYS * S::SCALE;
-      uint32_t ksc[S::FP8 ? 4 : 2][S::FP8 ? NB : S::KX], vsc[4][NB];
-      if (S::FP8) {
+      uint32_t ksc[2][S::FP8 ? NB : S::KX], vsc[S::FP8 ? 2 : 4][NB];
 #pragma unroll
-        for (int y = 0; y < 4; y += 2) {                     // keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c
-          uint32_t w[2 * NB];
-          read_words(key_scales + (4 * y + 2 * c) * S::SCALE, w);
+      for (int y = 0; y < 2; ++y) {                          // keys g and 8 + g
+        if (S::FP8) {
+          uint32_t w[NB];
+          read_words(key_scales + (8 * y + g) * S::SCALE, w);
 #pragma unroll
-          for (int k = 0; k < 2 * NB; ++k) ksc[y + k / NB][k % NB] = w[k];
-          read_words(value_scales + (4 * y + 2 * c) * S::SCALE, w);
+          for (int k = 0; k < NB; ++k) ksc[y][k] = w[k];
+          read_words(value_scales + (8 * y + g) * S::SCALE, w);
 #pragma unroll
-          for (int k = 0; k < 2 * NB; ++k) vsc[y + k / NB][k % NB] = w[k];
-        }
-      } else {
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
+          for (int k = 0; k < NB; ++k) vsc[y][k] = w[k];
+        } else {
 #pragma unroll
           for (int x = 0; x < S::KX; ++x) ksc[y][x] = key_scales[(8 * y + g) * S::SCALE + S::key_place(c, x) / 16];
+        }
+      }
+      if (!S::FP8) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) vsc[y][0] = value_scales[(y / 2 * 8 + 2 * c + y % 2) * S::SCALE + S::value_place(g, 0) / 16];
       }
-      // ---- scores of rows g (and g + 8) with keys 8 t + 2 c and 8 t + 2 c + 1
-      float s[2][2 * R];
+      // ---- scores, S^T = K Q^T: keys g and 8 + g with heads 8 r + 2 c and 8 r + 2 c + 1
+      float s[R][4];
       if (!S::FP8) {
         int most = -1000;
 #pragma unroll
@@ -488,96 +501,115 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
           for (int x = 0; x < S::KX; ++x)
             if (ksc[y][x] != 255) most = max(most, (int)ksc[y][x]);
         // codes are up to 6: 2^(8 + 4) times that is still an fp16
-        if (__any_sync(0xFFFFFFFFu, most > kref + 4)) kref = __reduce_max_sync(0xFFFFFFFFu, most);
+        if (__any_sync(0xFFFFFFFFu, most > kref + 4)) {
+          kref = __reduce_max_sync(0xFFFFFFFFu, most);
+          const int up = max(kref, 0) - 135;
+          // (held inside f32: past it scores are infinite, far below it all the same)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) up_s[r][y] = fmaxf(fminf(up_q[r][y] * pow2(up / 2) * pow2(up - up / 2), 3.4028235e38f), 1.4e-45f);
+        }
       }
+      uint32_t kw[2][S::KX][S::KW];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t kw[S::KX][S::KW];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < S::KX; ++x) read_words(keys + (8 * t + g) * S::PITCH + S::key_place(c, x), kw[x]);
+        for (int x = 0; x < S::KX; ++x) read_words(keys + (8 * t + g) * S::PITCH + S::key_place(c, x), kw[t][x]);
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          float acc[4] = {};
-          if (S::FP8) {
+      for (int k = 0; k < NB; ++k) {
+        constexpr int CHAINS = 2 / R;                        // MMAs one after the other wait for one another's sums
+        float acc[R][CHAINS][4] = {};
+        if (S::FP8) {
 #pragma unroll
-            for (int x = 2 * k; x < 2 * k + 2 && x < S::KX; ++x)
+          for (int x = 2 * k; x < 2 * k + 2 && x < S::KX; ++x)
 #pragma unroll
-              for (int y = 0; y < S::KW; ++y) {
-                const int z = S::KW * x + y;
-                uint32_t b0, b1;
-                halves_of_e4m3(kw[x][y], b0, b1);
-                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, b0, b1);
-              }
-          } else {
+            for (int y = 0; y < S::KW; ++y) {
+              const int z = S::KW * x + y;
+              uint32_t h[4];
+              halves_of_e4m3(kw[0][x][y], h[0], h[2]);
+              halves_of_e4m3(kw[1][x][y], h[1], h[3]);
 #pragma unroll
-            for (int x = 0; x < S::KX; ++x) {
-              const uint32_t f = half_pow2(ksc[t][x] == 255 ? 16 : (int)ksc[t][x] - kref + 8) * 0x10001u;
+              for (int r = 0; r < R; ++r) mma(acc[r][z % CHAINS], h[0], h[1], h[2], h[3], q[z][r], q[z][R + r]);
+            }
+        } else {
 #pragma unroll
-              for (int y = 0; y < S::KW; ++y) {
-                const int z = 2 * (S::KW * x + y);
-                uint32_t h[4];
-                halves_of_e2m1(kw[x][y], h);
-                mma(acc, q[z][0], TWO ? q[z][1] : 0, q[z][R], TWO ? q[z][2 * R - 1] : 0, mul_half2(h[0], f), mul_half2(h[1], f));
-                mma(acc, q[z + 1][0], TWO ? q[z + 1][1] : 0, q[z + 1][R], TWO ? q[z + 1][2 * R - 1] : 0, mul_half2(h[2], f), mul_half2(h[3], f));
+          for (int x = 0; x < S::KX; ++x) {
+            uint32_t f[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) f[t] = half_pow2(ksc[t][x] == 255 ? 16 : (int)ksc[t][x] - kref + 8) * 0x10001u;
+#pragma unroll
+            for (int y = 0; y < S::KW; ++y) {
+              const int z = 2 * (S::KW * x + y);
+              uint32_t h0[4], h1[4];
+              halves_of_e2m1(kw[0][x][y], h0);
+              halves_of_e2m1(kw[1][x][y], h1);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h0[e] = mul_half2(h0[e], f[0]), h1[e] = mul_half2(h1[e], f[1]);
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                mma(acc[r][0], h0[0], h1[0], h0[1], h1[1], q[z][r], q[z][R + r]);
+                mma(acc[r][CHAINS - 1], h0[2], h1[2], h0[3], h1[3], q[z + 1][r], q[z + 1][R + r]);
               }
             }
           }
+        }
 #pragma unroll
-          for (int e = 0; e < 2 * R; ++e) {
-            const float v = acc[e];
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = CHAINS == 2 ? __fadd_rn(acc[r][0][e], acc[r][CHAINS - 1][e]) : acc[r][0][e];
             if (S::FP8) {
-              const float f = __uint_as_float(ksc[2 * t + (e & 1)][k]);
-              s[t][e] = k ? __fmaf_rn(v, f, s[t][e]) : __fmul_rn(v, f);
+              const float f = __uint_as_float(ksc[e >> 1][k]);
+              s[r][e] = k ? __fmaf_rn(v, f, s[r][e]) : __fmul_rn(v, f);
             } else {
-              s[t][e] = v;
+              s[r][e] = v;
             }
           }
-        }
-#pragma unroll
-        for (int e = 0; e < 2 * R; ++e) s[t][e] = __fmul_rn(s[t][e], qf[e >> 1]);
-        if (!S::FP8) {
-          const int up = max(kref, 0) - 135;                 // 2^(kref - 127 - 8)
-#pragma unroll
-          for (int e = 0; e < 2 * R; ++e) s[t][e] = s[t][e] * pow2(up / 2) * pow2(up - up / 2);
-        }
       }
       if (live != 0xFFFFu) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
+          if (!(live >> (8 * t + g) & 1)) {
 #pragma unroll
-          for (int e = 0; e < 2 * R; ++e)
-            if (!(live >> (8 * t + 2 * c + (e & 1)) & 1)) s[t][e] = -INFINITY;
+            for (int r = 0; r < R; ++r) s[r][2 * t] = s[r][2 * t + 1] = -INFINITY;
+          }
       }
       // ---- the running maximum: held up to a factor of 2^8
       bool grow = false;
-      float top[R];
+      float top[R][2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        grow = grow || top[r] - m[r] > 8.0f;
-      }
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          top[r][y] = __fmul_rn(fmaxf(s[r][y], s[r][2 + y]), up_s[r][y]);
+          grow = grow || top[r][y] - m[r][y] > 8.0f;
+        }
       if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
-          top[r] = fmaxf(m[r], fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2)));
-          const float f = top[r] == -INFINITY ? 1.0f : exp2_approx(m[r] - top[r]);
-          m[r] = top[r];
-          l[r] *= f;
-          const float fx = __shfl_sync(0xFFFFFFFFu, f, 8 * c), fy = __shfl_sync(0xFFFFFFFFu, f, 8 * c + 4);   // heads 2 c, 2 c + 1
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int n = 0; n < DT; ++n) o[n][r][0] *= fx, o[n][r][1] *= fy, o[n][r][2] *= fx, o[n][r][3] *= fy;
-        }
+          for (int y = 0; y < 2; ++y) {
+            float t = top[r][y];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, x));
+            t = fmaxf(m[r][y], t);
+            const float f = t == -INFINITY ? 1.0f : exp2_approx(m[r][y] - t);
+            m[r][y] = t;
+            l[r][y] *= f;
+#pragma unroll
+            for (int n = 0; n < DT; ++n) o[n][r][y] *= f, o[n][r][2 + y] *= f;
+          }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float sh = m[r] == -INFINITY ? 0.0f : m[r];
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          s[t][2 * r] = exp2_approx(s[t][2 * r] - sh), s[t][2 * r + 1] = exp2_approx(s[t][2 * r + 1] - sh);
-          l[r] += s[t][2 * r] + s[t][2 * r + 1];
+        for (int y = 0; y < 2; ++y) {
+          const float sh = m[r][y] == -INFINITY ? 0.0f : -m[r][y];
+#pragma unroll
+          for (int e = y; e < 4; e += 2) s[r][e] = exp2_approx(__fmaf_rn(s[r][e], up_s[r][y], sh));
+          l[r][y] += s[r][y] + s[r][2 + y];
         }
-      }
       // ---- values: O^T += V^T P^T
       uint32_t vw[4][S::VX][S::VW];
 #pragma unroll
@@ -587,16 +619,25 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         int most = -1000;
+        bool past;
+        if (S::FP8) {
+          past = fmaxf(fabsf(__uint_as_float(vsc[0][k])), fabsf(__uint_as_float(vsc[1][k]))) >= limit[k];
+        } else {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int e = S::FP8 ? (int)(vsc[x][k] >> 23 & 255u) : (int)vsc[x][0];
-          if (e != 255) most = max(most, e);                 // (infinities and NaN go through as they are)
+          for (int x = 0; x < 4; ++x)
+            if (vsc[x][0] != 255) most = max(most, (int)vsc[x][0]);
+          past = most > ref[k];
         }
-        if (__any_sync(0xFFFFFFFFu, most > ref[k])) {
-          // MXFP4: the four lanes that share the rows g of the MMAs have the same block and the same ref
-          if (S::FP8) {
-            most = __reduce_max_sync(0xFFFFFFFFu, most);
+        if (__any_sync(0xFFFFFFFFu, past)) {
+          if (S::FP8) {                                      // (infinities and NaN go through as they are)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int e = (int)(vsc[x][k] >> 23 & 255u);
+              if (e != 255) most = max(most, e);
+            }
+            most = max(__reduce_max_sync(0xFFFFFFFFu, most), ref[k]);
           } else {
+            // the four lanes that share the rows g of the MMAs have the same block and the same ref
             most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
             most = max(max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2)), ref[k]);
           }
@@ -610,28 +651,26 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
           ref[k] = most;
           const int up = 133 - max(most, 0);
           up0[k] = pow2(up / 2), up1[k] = pow2(up - up / 2);
+          limit[k] = __uint_as_float((uint32_t)(max(most, 0) + 1) << 23);
         }
         // weights as fp16.  FP8: p * scale / 2^ref * 2^6 (below 2^8 * 2 * 2^6).  MXFP4: p * 2^7, and the codes are multiplied
         // by scale / 2^ref * 2^8.
         uint32_t p[R][2], f01 = 0, f23 = 0;
+        float f[2] = {128.0f, 128.0f};
         if (S::FP8) {
-          float f[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) f[x] = __uint_as_float(vsc[x][k]) * up0[k] * up1[k];
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) p[r][t] = pack_half(s[t][2 * r] * f[2 * t], s[t][2 * r + 1] * f[2 * t + 1]);
+          for (int t = 0; t < 2; ++t) f[t] = __uint_as_float(vsc[t][k]) * up0[k] * up1[k];
         } else {
-          uint32_t f[4];
+          uint32_t h[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) f[x] = half_pow2(vsc[x][0] == 255 ? 16 : (int)vsc[x][0] - ref[0] + 8);
-          f01 = f[0] | f[1] << 16, f23 = f[2] | f[3] << 16;
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) p[r][t] = pack_half(s[t][2 * r] * 128.0f, s[t][2 * r + 1] * 128.0f);
+          for (int x = 0; x < 4; ++x) h[x] = half_pow2(vsc[x][0] == 255 ? 16 : (int)vsc[x][0] - ref[0] + 8);
+          f01 = h[0] | h[1] << 16, f23 = h[2] | h[3] << 16;
         }
+        // from a key's heads to a head's keys
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) p[r][t] = transposed(pack_half(s[r][2 * t] * f[t], s[r][2 * t + 1] * f[t]));
         // a tile of 16 elements: rows g and g + 8 of the MMA are two neighbours of this lane's, keys in pairs
         auto step = [&](int n, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
@@ -675,12 +714,15 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
     const bool whole = tile0 == 0 && tile1 == per - EXTRA;
     // a CTA's first segment may be the rest of a (sequence, head), its last one the beginning of one
     const int64_t slot = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
-    if (tile1 == per - EXTRA && threadIdx.x == 0) parts.endings[b * HV + hv] = {whole ? (int)blockIdx.x : deal.owner(start + EXTRA), (int)blockIdx.x};
+    if (tile1 == per - EXTRA && threadIdx.x == 0) parts.endings[b * HV + hv] = {whole ? (int)blockIdx.x : (deal.owner(start + EXTRA) << pl.side_bits) + side, (int)blockIdx.x};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-      if (c == 0) join_ml[warp * 8 + g] = make_float2(m[r], l[r]);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r][y] += __shfl_xor_sync(0xFFFFFFFFu, l[r][y], x);
+        if (g == 0) join_ml[warp * 8 + 2 * c + y] = make_float2(m[r][y], l[r][y]);
+      }
 #pragma unroll
       for (int n = 0; n < DT; ++n) {
         const int up = max(ref[n / PER], 0) - (S::FP8 ? 133 : 142);                // 2^(ref - 127 - 6), MXFP4: - 7 - 8
@@ -736,7 +778,7 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
   asm volatile("griddepcontrol.wait;" ::: "memory");         // the attention's results are there
   for (int64_t item = blockIdx.x; item < a.B * HV; item += gridDim.x) {
     const Ending e = parts.endings[item];
-    const int n = e.last - e.first + 1;
+    const int n = ((e.last - e.first) >> pl.side_bits) + 1;
     const int64_t b = item / HV;
     const int hv = (int)(item - b * HV);
     if (n < 2) continue;
@@ -744,7 +786,7 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
     if (n <= FEW) {                                          // as many rows at once as there are threads for
       const int r = row + threadIdx.x / lanes, hq = hv % pl.groups * 16 + r;
       if (row % shares || r >= pl.rows || hq >= group || d >= a.D) continue;
-      auto slot = [&](int i) { return (2 * (int64_t)(e.first + i) + (i == 0 ? 1 : 0)) * pl.rows + r; };
+      auto slot = [&](int i) { return (2 * (int64_t)(e.first + (i << pl.side_bits)) + (i == 0 ? 1 : 0)) * pl.rows + r; };
       float top = -INFINITY, sum = 0.0f, v = 0.0f;
       for (int i = 0; i < n; ++i) top = fmaxf(top, parts.ml[slot(i)].x);
       const float sh = top == -INFINITY ? 0.0f : top;
@@ -763,7 +805,7 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
     const int hq = hv % pl.groups * 16 + row;
     if (hq >= group) continue;
     // a CTA's first (sequence, head) is in its even slot; this one's first part is the last of its CTA
-    const int64_t slot0 = (2 * (int64_t)e.first) * pl.rows + row, step = 2 * pl.rows;
+    const int64_t slot0 = (2 * (int64_t)e.first) * pl.rows + row, step = 2 * pl.rows << pl.side_bits;
     auto slot = [&](int i) { return slot0 + i * step + (i == 0 ? pl.rows : 0); };
     float top = -INFINITY;
     for (int i = threadIdx.x; i < n; i += JOIN_NT) top = fmaxf(top, parts.ml[slot(i)].x);
@@ -809,6 +851,11 @@ Plan plan_of(int format, int Hq, int Hk, int D) {
   p.groups = (group + 15) / 16;
   p.rows = std::min(group, 16);
   p.ctas = std::min(JOIN_PARTS, ctas_per_sm(format, padded(D), p.rows > 8) * sm_count());
+  const int row = format == EMU_KV_FP8 ? D : D / 2;
+  // Neighbouring heads side by side where a slot's row is long: CTAs that read its pieces at about the same time find the memory's
+  // rows open (64 sequences, 262144 slots of 8 heads of 128 bytes: 128 -> 117 us; sets of 8 118).
+  while (p.side_bits < 2 && Hk % (2 << p.side_bits) == 0 && Hk * row >= 512) ++p.side_bits;
+  p.sets = p.ctas >> p.side_bits;
   return p;
 }
 
