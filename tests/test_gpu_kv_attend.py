@@ -96,6 +96,14 @@ def test_long_and_many(fmt, lens):
 
 
 @pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("Hq,Hk", [(8, 4), (96, 4), (12, 12), (18, 6), (32, 8), (10, 10)])
+@pytest.mark.parametrize("lens", [[3000, 0, 70, 1], [64] * 90], ids=["ragged", "many"])
+def test_neighbouring_heads_side_by_side(fmt, Hq, Hk, lens):
+    """Slots with long rows, whose heads go to CTAs in sets of 2 or 4; some sets' runs end inside sequences."""
+    _check(lens, Hq, Hk, 256, 16, fmt, torch.bfloat16, seed=Hq)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
 @pytest.mark.parametrize("spread,scale", [(4.0, None), (0.1, 3.0), (1.0, 1e-3)])
 def test_scales_far_apart_and_peaked_scores(fmt, spread, scale):
     _check([700, 33], 8, 2, 64, 16, fmt, torch.float16 if spread < 2 else torch.bfloat16, seed=4, spread=spread, scale=scale)
