@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(NT, ctas_per_sm(FORMAT, DP, TWO)) kv_attend_ke
 // there are many, to every gridDim.x-th item): the parts' factors first, then threads [part][element], then a sum over
 // the parts' shares.
 constexpr int JOIN_NT = 512, JOIN_PARTS = 1024, FEW = 8;
-template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ Plan pl, int lanes) {
+template <typename T, bool MANY> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ Plan pl, int lanes) {
   __shared__ float so[JOIN_NT], factor[JOIN_PARTS], part_sum[JOIN_NT / 32], part_top[JOIN_NT / 32];
   const int HV = a.Hk * pl.groups, group = a.Hq / a.Hk, row = blockIdx.y, warp = threadIdx.x >> 5;
   const Parts parts = parts_of(a.workspace, a.B * HV, pl.ctas, pl.rows, a.D);
@@ -816,6 +816,15 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
     // a CTA's first (sequence, head) is in its even slot; this one's first part is the last of its CTA
     const int64_t slot0 = (2 * (int64_t)e.first) * pl.rows + row, step = 2 * pl.rows << pl.side_bits;
     auto slot = [&](int i) { return slot0 + i * step + (i == 0 ? pl.rows : 0); };
+    // MANY: the first parts' shares are asked for before the factors are known
+    const int share = threadIdx.x / lanes;
+    constexpr int EARLY = MANY ? 24 : 0;
+    float early[MANY ? EARLY : 1];
+#pragma unroll
+    for (int x = 0; x < EARLY; ++x) {
+      const int i = share + x * shares;
+      early[x] = i < n && d < a.D ? parts.o[slot(i) * a.D + d] : 0.0f;
+    }
     float top = -INFINITY;
     for (int i = threadIdx.x; i < n; i += JOIN_NT) top = fmaxf(top, parts.ml[slot(i)].x);
 #pragma unroll
@@ -837,8 +846,11 @@ template <typename T> __global__ void __launch_bounds__(JOIN_NT) kv_attend_join_
     __syncthreads();
     float v = 0.0f;
     if (d < a.D) {
+#pragma unroll
+      for (int x = 0; x < EARLY; ++x)
+        if (share + x * shares < n) v = __fmaf_rn(early[x], factor[share + x * shares], v);
 #pragma unroll 8
-      for (int i = threadIdx.x / lanes; i < n; i += shares) v = __fmaf_rn(parts.o[slot(i) * a.D + d], factor[i], v);
+      for (int i = share + EARLY * shares; i < n; i += shares) v = __fmaf_rn(parts.o[slot(i) * a.D + d], factor[i], v);
     }
     so[threadIdx.x] = v;
     __syncthreads();
@@ -903,7 +915,10 @@ template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvA
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T>, a, pl, DP);
+  // MANY where most (sequence, head)s lie in more than FEW CTAs (400001 keys on one head 47 -> 43 us); its registers leave room for
+  // fewer CTAs, which costs where there are many (262144 keys 113 -> 122 us).
+  const bool many = pl.ctas > FEW * a.B * a.Hk * pl.groups;
+  const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, true>, a, pl, DP) : cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, false>, a, pl, DP);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
