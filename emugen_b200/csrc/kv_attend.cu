@@ -19,10 +19,10 @@
 // of one or several (sequence, head)s.  Where a run is not all of a (sequence, head), its sums go to the workspace, and a
 // second kernel joins them in the tiles' order.  Neighbouring heads go to neighbouring CTAs where a slot's row is long.
 //
-// Measured, both kernels: 64 sequences, 262144 slots of 8 heads of 128 in FP8, 32 query heads: 117 us for 553 MB (4.7 TB/s, 72%
+// Measured, both kernels: 64 sequences, 262144 slots of 8 heads of 128 in FP8, 32 query heads: 113 .. 120 us for 555 MB (4.7 TB/s, 72%
 // of a copy's rate; the first kernel 105 us at 5.3 TB/s: memory waits, issue slots 48% busy).  4 sequences, 400001 slots on one
-// head: 46 us (104 MB): 14 steps to a warp, so that starting and joining count.  4 bits, 33 sequences, 100003 slots of 4
-// heads of 64: 33 us (27 MB), 10 steps to a warp.
+// head, 16 query heads: 43 us (106 MB): 21 steps to a warp, so that starting and joining count.  4 bits, 33 sequences, 100003
+// slots of 4 heads of 64: 33 us (27 MB), 10 steps to a warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>

@@ -513,14 +513,16 @@ typedef struct {
 EMU_API emu_status emu_attention(const emu_attention_args* args, void* out, void* out_low, float* lse, void* stream);
 /*
  * Its gradients from dout: dq [total_q][heads_q][head_size], dk and dv [total_k][heads_k][head_size], contiguous, each may be
- * NULL (not wanted).  out, out_low (may be NULL) and lse are emu_attention's.  ds = p (dout . v - dout . out) is rounded to the inputs' dtype for
- * its products (fp16: scaled by a power of two that keeps it in range).  No atomic additions: the same result every run.
+ * NULL (not wanted).  out, out_low (may be NULL) and lse are emu_attention's.  ds = p (dout . v - dout . (out + out_low)) is
+ * rounded to the inputs' dtype for its products (fp16: scaled by a power of two that keeps it in range).  No atomic
+ * additions: the same result every run.
  * workspace: emu_attention_backward_workspace_size(args) bytes on the device, 256-byte aligned.
  */
 EMU_API size_t emu_attention_backward_workspace_size(const emu_attention_args* args);
 EMU_API emu_status emu_attention_backward(const emu_attention_args* args, const void* out, const void* out_low,
-                                          const float* lse, const void* dout, int64_t dout_token_stride, int64_t dout_head_stride, void* dq,
-                                          void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+                                          const float* lse, const void* dout, int64_t dout_token_stride,
+                                          int64_t dout_head_stride, void* dq, void* dk, void* dv, void* workspace,
+                                          size_t workspace_bytes, void* stream);
 
 /*
  * Attention of one new token for each sequence over a quantised cache (emu_kv_write's layout, num_pages * page_size slots):
