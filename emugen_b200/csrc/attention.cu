@@ -11,7 +11,8 @@
 //   warp 9           TMA: Q once, then K and V tiles through a ring
 //
 // Bound by the tensor cores, and on long inputs by power: 16384 causal tokens, 32 heads on 8 of 128, bf16: 2.0 ms, 1.10 PFLOP/s (79%
-// of a sustained library product's rate; the SM clock falls to 1.4 .. 1.7 GHz).  8192 tokens in 3 sequences 230 us.  S is
+// of a sustained library product's rate; the SM clock falls to 1.4 .. 1.7 GHz).  8192 tokens in 3 sequences, with
+// the rest for a backward pass, 249 us.  S is
 // not rounded, l and O are held in f32; the weights are rounded to the inputs' type (a 2^-9 or 2^-12 of them), which is
 // what the second product takes.
 #include <cuda.h>

@@ -437,3 +437,20 @@ def test_timed_out_wait_is_reported_and_the_context_survives(heads, what):
     got = run()
     _lib.device_status()
     assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last sequences as on their own."""
+    T, Hq, Hk, D, n = 135000, 128, 8, 128, 100
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, do = (torch.randn(T, Hq, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    k, v = (torch.randn(T, Hk, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    assert q.numel() > 2 ** 31
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = attention.packed_attention(*x, _tensor(list(range(0, T + 1, n))))
+    grads = torch.autograd.grad(out, x, do)
+    tail = [t[-2 * n:].detach() for t in x]
+    want = O.attention(*tail, [0, n, 2 * n], [0, n, 2 * n], True, D ** -0.5, do[-2 * n:])
+    O.check(out[-2 * n:], want["out"], "out")
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        O.check(t[-2 * n:], want[name], name)

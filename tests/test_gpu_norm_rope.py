@@ -182,3 +182,21 @@ def test_without_eps(dtype, T, D):
         r = O.norm_rope(t[live], w, cos, sin, pos[live], 0.0, False, g[live])
         assert (y[~live] == 0).all() and (dx[~live] == 0).all()
         O.check(y[live], r[0:2]), O.check(dx[live], r[2:4]), O.check(dw, r[4:6])
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last tokens as on their own."""
+    T, H, D = 70000, 128, 256
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, gq = (torch.randn(T, H, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    k, gk = (torch.randn(T, 1, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    assert q.numel() > 2 ** 31
+    w = torch.ones(D, device="cuda", dtype=torch.bfloat16)
+    cos, sin = _table(500, 128)
+    pos = torch.arange(T, device="cuda") % 500
+    x = [t.requires_grad_() for t in (q, k)]
+    y = attention.qk_norm_rope(*x, w, w, cos, sin, pos)
+    grads = torch.autograd.grad(y, x, (gq, gk))
+    for a, b, t, u in zip(y, grads, x, (gq, gk)):
+        r = O.norm_rope(t[-50:].detach(), w, cos, sin, pos[-50:], 1e-6, False, u[-50:])
+        O.check(a[-50:], r[0:2]), O.check(b[-50:], r[2:4])
