@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
 template <int DP> struct Few {
   static constexpr int TILE = 128 * DP * 2;                 // 128 rows of DP elements, as DP / 64 boxes of 128 x 128 bytes
   static constexpr int SLOTS = DP == 128 ? 3 : 5;           // of K, and of V
-  static constexpr int BARS = 1 + 4 * SLOTS + 3 + 3 + 3 + 1 + 2 + 1 + 2;
+  static constexpr int BARS = 1 + 4 * SLOTS + 3 + 3 + 3 + 2 + 1 + 2;
   static constexpr int SMEM = 1024 + (1 + 2 * SLOTS) * TILE + BARS * 8 + 16 + 3 * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
@@ -331,16 +331,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
   uint64_t* v_empty = v_full + C::SLOTS;
   uint64_t* s_full = v_empty + C::SLOTS;                     // [place]
   uint64_t* p_full = s_full + 3;                             // [place]
-  uint64_t* p_free = p_full + 3;                             // [place]
-  uint64_t* pv_done = p_free + 3;
-  uint64_t* ref_full = pv_done + 1;                          // [warpgroup]: it has written `ref` of its tile
+  uint64_t* p_free = p_full + 3;                             // [place]: its weights' product, and so all before it, is in O
+  uint64_t* ref_full = p_free + 3;                           // [warpgroup]: it has written `ref` of its tile
   uint64_t* o_full = ref_full + 2;
   uint64_t* drained = o_full + 1;                            // [issuer]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&map_q), ptx::prefetch_tmap(&map_k), ptx::prefetch_tmap(&map_v);
-    ptx::mbar_init(q_full, 1), ptx::mbar_init(pv_done, 1), ptx::mbar_init(o_full, 1);
+    ptx::mbar_init(q_full, 1), ptx::mbar_init(o_full, 1);
     for (int i = 0; i < C::SLOTS; ++i)
       ptx::mbar_init(&k_full[i], 1), ptx::mbar_init(&k_empty[i], 1), ptx::mbar_init(&v_full[i], 1), ptx::mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 3; ++i) ptx::mbar_init(&s_full[i], 1), ptx::mbar_init(&p_full[i], 128), ptx::mbar_init(&p_free[i], 1);
@@ -420,7 +419,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
             for (int s = 0; s < 8; ++s) ptx::mma_f16_ta(tmem + FEW_O, tmem + place.at * 128 + s * 8, vd + s * 128, id, j > 0 || s > 0);
             ptx::mma_commit(&p_free[place.at]);
             ptx::mma_commit(&v_empty[slot.at]);
-            ptx::mma_commit(pv_done);
             if (j + 1 == tiles) ptx::mma_commit(o_full);
           }
           __syncwarp();
@@ -479,10 +477,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
       const float tm = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), now);
       if (__any_sync(0xFFFFFFFFu, (tm - now) * c > 8.0f)) {
         if (j > 0) {
-          // Tile j - 1's product has to be there; this tile's waits for its weights.  (S of this tile came behind the product
-          // of tile j - 3: the barrier is at tile j - 2's round or further, so both rounds are waited for in turn.)
-          if (j > 1 && !warp_wait_or_record(pv_done, j & 1, tl.wait_limit, WAIT_FWD_O)) { ok = false; break; }
-          if (!warp_wait_or_record(pv_done, (j - 1) & 1, tl.wait_limit, WAIT_FWD_O)) { ok = false; break; }
+          // Tile j - 1's product has to be there; this tile's waits for its weights.  A wait for a parity tells a round from the
+          // one before it alone, so the barrier may be at tile j - 1's round or the next, and it is: S of tile j - 1 waited for
+          // the round before, and the next one's end, tile j + 2's product, is behind this tile's, which needs this warp.
+          if (!warp_wait_or_record(&p_free[(j - 1) % 3], ((j - 1) / 3) & 1, tl.wait_limit, WAIT_FWD_O)) { ok = false; break; }
           ptx::tc_fence_after();
           const float f = tm == -INFINITY ? 1.0f : exp2f((now - tm) * c);
 #pragma unroll
