@@ -13,13 +13,14 @@
 // Bound by the tensor cores, and on long inputs by power: 16384 causal tokens, 32 heads on 8 of 128, bf16: 2.0 ms, 1.10 PFLOP/s (79%
 // of a sustained library product's rate; the SM clock falls to 1.4 .. 1.7 GHz).  8192 tokens in 3 sequences, with
 // the rest for a backward pass, 249 us.  S is
-// not rounded, l and O are held in f32; the weights are rounded to the inputs' type (a 2^-9 or 2^-12 of them), which is
+// not rounded, l and O are held in f32; the weights are rounded to the inputs' type (by up to 2^-8 or 2^-11 of them), which is
 // what the second product takes.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/emugen.h"
 #include "attention.cuh"
@@ -42,6 +43,11 @@ template <int DP> struct Fwd {
   static constexpr int SMEM = 1024 + 2 * TILE + SLOTS * TILE + BARS * 8 + 16;
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
+// fp16: P, and with it l and O, is held 2^7 times as large.  P is below 2^8 (the maximum is held up to that factor), so that it
+// stays below 2^15, and weights down to 2^-21 keep all their bits, those down to 2^-31 some; without it they were lost from 2^-14 and
+// gone below 2^-25, and 16384 keys 18 below a first one came out as zeros.  bf16 has f32's range.
+template <typename T> constexpr float P_LOG2 = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+
 // tensor memory columns: S (and P) of both tiles, O of both tiles
 constexpr uint32_t S_COL = 0, O_COL = 256;
 
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
 #pragma unroll
         for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
       const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      // The weights are held to the maximum up to a factor of 2^8: P stays below 2^8, l and O in range, and most
+      // The weights are held to the maximum up to a factor of 2^8: P, l and O stay in range, and most
       // tiles need no correction of O.
       const bool grow = (tm - m) * c > 8.0f;
       if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -218,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
           }
         }
       }
-      const float shift = m == -INFINITY ? 0.0f : -m * c;
+      const float shift = shift_of(m, c) + P_LOG2<T>;
       const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
       uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D, mine && ok, a.D / 8);
     }
-    if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
+    if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - (shift_of(m, c) + P_LOG2<T>)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone.  (Where the sum is NaN, the scores are, and the row is NaN by right.)
     redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
       for (int e = 0; e < 32; ++e)
 #pragma unroll
         for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
-      // The weights are held to the maximum up to a factor of 2^8: P stays below 2^8, l and O in range, and most
+      // The weights are held to the maximum up to a factor of 2^8: P, l and O stay in range, and most
       // tiles need no correction of O.  The other warpgroup has left what its tile, the one before, was held to.
       if (j > 0 && !warp_wait_or_record(&ref_full[w ^ 1], ((j - 1) >> 1) & 1, tl.wait_limit, WAIT_FWD_S)) { ok = false; break; }
       float now = j > 0 ? ref[r] : -INFINITY;
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
         l *= now == -INFINITY ? 1.0f : exp2f((m - now) * c);
         m = now;
       }
-      const float shift = m == -INFINITY ? 0.0f : -m * c;
+      const float shift = shift_of(m, c) + P_LOG2<T>;
       const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
       uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -556,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D + w * HALF, mine && ok, (a.D - w * HALF) / 8);
     }
-    if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - shift_of(m, c)) * 0.6931471805599453f : l;
+    if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - (shift_of(m, c) + P_LOG2<T>)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone (this thread's half).  (Where the sum is NaN, the scores are, and the row is NaN by right.)
     const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;

@@ -48,3 +48,37 @@ def test_even_tiles_and_then_a_higher_one(tile, D, causal, heads):
             bonus = torch.zeros(n)
             bonus[late] = rise
             _check(*_scored(n, bonus, D, dtype, tile, heads, heads // 2), causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("above", [10.0, 14.0, 16.0, 17.0, 18.0])
+@pytest.mark.parametrize("heads", [2, 160])            # one tile of rows to a CTA, and two
+def test_a_first_key_above_the_rest(dtype, above, heads):
+    """A key without a value has nearly all of the weight; the output is what the weights of the 16384 others, down to 2^-26,
+    leave of theirs."""
+    nq, nk, D = 64, 16385, 64
+    bonus = torch.zeros(nk)
+    bonus[0] = above
+    q, k, v = _scored(nk, bonus, D, dtype, int(above), heads, heads // 2)
+    q, v = q[:nq].contiguous(), (1 + 0.25 * v.float()).to(dtype)
+    v[0] = 0
+    out, lse = attention.packed_attention(q, k, v, _cu(nq), _cu(nk), causal=False, return_lse=True)
+    want = O.attention(q, k, v, [0, nq], [0, nk], False, D ** -0.5)
+    O.check(out, want["out"], "out")
+    O.check(lse, want["lse"], "lse")
+    _lib.device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", ["first", "recent", "both"])
+@pytest.mark.parametrize("heads", [2, 40])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_of_peaked_rows(dtype, shape, heads, causal):
+    """A first key 9 above the rest, and scores that rise by 1 every 32 keys, so that the recent ones are far above the old."""
+    n, D = 700, 64
+    bonus = torch.arange(n) / 32.0 if shape != "first" else torch.zeros(n)
+    if shape != "recent":
+        bonus[0] = bonus[-1] + 9
+    q, k, v = _scored(n, bonus, D, dtype, 3, heads, heads // 2)
+    do = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    _check(q, k, v, causal, do)
