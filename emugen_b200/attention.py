@@ -235,8 +235,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
 
     fp16 or bf16 tensors of one CUDA device, head_size a multiple of 8 up to 128; rows that do not start on 16-byte
     boundaries are copied first.  Scores, softmax and sums in f32; its weights, and in the backward pass the scores' gradients, are
-    rounded to the inputs' dtype for the products; a call that is differentiated also keeps what the output's rounding took
-    away (as large as the output).  The same result every run.  With return_lse also f32 [query heads,
+    rounded to the inputs' dtype for the products (in fp16 after a power of two that keeps small ones, taken from the row, sequence
+    and key head alone); a call that is differentiated also keeps what the output's rounding took away (as large as the output).
+    The same result every run.  With return_lse also f32 [query heads,
     query tokens]: the logarithm of the sum of exp(score), -inf where no key is seen (not differentiable).
     Reverse mode only.  For a backward pass that a CUDA graph is to capture, see fp8.linear_fp8."""
     qs, ks, dtype = q.shape, k.shape, q.dtype

@@ -26,26 +26,46 @@ constexpr int THREADS = 384;                                // warps 10, 11 (11 
 constexpr int REG_LOW = 40, REG_HIGH = 232;                 // 128 x 40 + 256 x 232 = 64512 = 384 x 168, the launch's
 
 // fp16: P is held 2^15 times as large, so that weights down to 2^-29 keep all their bits, and ds is multiplied by a power of
-// two that puts a bound of it at 2^14: |dp - delta| <= 2 |dO_i| |v_j|, as o_i is a mean of values.  bf16 needs neither.
+// two that puts a bound of it at 2^14: |dp - delta| <= 2 |dO_i| |v_j|, as o_i is a mean of values.  A row of dq has its own |dO_i|, with
+// the largest |v_j| of its sequence and key head; dk adds up over rows, and takes the largest |dO_i| of the sequence and key head (with
+// one factor for the whole call, a sequence 2^22 times larger left none of its neighbour's bits).  bf16 needs neither.
 template <typename T> constexpr float P_LOG2 = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
 struct Work {
-  uint32_t* top;               // bits of the largest |dO_i|^2 and |v_j|^2 (fp16)
   float2* stats;               // [Tq][Hq]: -lse log2 e, delta
+  float* norms;                // from here on fp16.  [Tq][Hq]: |dO_i|^2
+  uint32_t* top_g;             // [sequence][key head]: bits of the largest |dO_i|^2
+  uint32_t* top_v;             // the same of |v_j|^2
+  size_t bytes;
 };
-__host__ __device__ inline Work work_of(void* p) { return {static_cast<uint32_t*>(p), reinterpret_cast<float2*>(static_cast<uint8_t*>(p) + 256)}; }
+__host__ __device__ inline Work work_of(void* p, int64_t Tq, int64_t B, int Hq, int Hk, bool half) {
+  uint8_t* base = static_cast<uint8_t*>(p) + 256;
+  const size_t rows = (size_t)Tq * Hq, heads = (size_t)B * Hk;
+  Work w;
+  w.stats = reinterpret_cast<float2*>(base);
+  w.norms = reinterpret_cast<float*>(base + rows * 8);
+  w.top_g = reinterpret_cast<uint32_t*>(base + rows * 12);
+  w.top_v = w.top_g + heads;
+  w.bytes = 256 + (half ? rows * 12 + heads * 8 : rows * 8);
+  return w;
+}
+__host__ __device__ inline Work work_of(const AttnArgs& a) { return work_of(a.workspace, a.Tq, a.B, a.Hq, a.Hk, a.dtype == EMU_DTYPE_F16); }
 
-// The factor of ds.
-template <typename T> __device__ __forceinline__ float ds_factor(const Work& w) {
-  if (!std::is_same<T, __half>::value) return 1.0f;
-  const float b = 4.0f * __uint_as_float(__ldg(w.top)) * __uint_as_float(__ldg(w.top + 1));
+// The factor of ds where |dO_i|^2 <= g and |v_j|^2 <= v.
+__device__ __forceinline__ float ds_factor(float g, float v) {
+  const float b = 4.0f * g * v;
   return b > 0.0f && b < INFINITY ? exp2f(floorf((28.0f - log2f(b)) * 0.5f)) : 1.0f;
+}
+// The largest so far, of sequence b and key head kh; additions to it in any order give the same.
+__device__ __forceinline__ void keep_largest(uint32_t* top, float norm) {
+  const uint32_t bits = __float_as_uint(norm);               // (a positive number's bits grow with it)
+  if (bits > __ldcg(top)) atomicMax(top, bits);
 }
 
 // ------------------------------------------------------------------------------ statistics
 // delta of each (token, head), from the output before its rounding where its rest was kept: ds is what is left of
 // dp - delta, so that a sequence of 2 tokens had 0.0039 of its gradients' norm off without the rest, 0.0026 with it.  Beside
-// the shift of its scores; fp16: the largest norms.  16 lanes to a row, 8 elements each.
+// the shift of its scores; fp16: its norm, and the largest of its sequence and key head.  16 lanes to a row, 8 elements each.
 template <typename T> __device__ __forceinline__ void load8(const T* p, bool any, float (&v)[8]) {
   uint4 w = make_uint4(0, 0, 0, 0);
   if (any) w = __ldg(reinterpret_cast<const uint4*>(p));
@@ -60,7 +80,7 @@ __device__ __forceinline__ float sum16(float v) {
 }
 template <typename T> __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_constant__ AttnArgs a) {
   constexpr bool HALF = std::is_same<T, __half>::value;
-  const Work w = work_of(a.workspace);
+  const Work w = work_of(a);
   const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, nq = a.Tq * a.Hq;
   const int d = (threadIdx.x & 15) * 8;
   const bool in = row < nq;
@@ -76,19 +96,15 @@ template <typename T> __global__ void __launch_bounds__(256) attention_stats_ker
   if (HALF) norm = sum16(norm);
   const float lse = in ? a.lse[(int64_t)h * a.Tq + t] : -INFINITY;
   if (in && (threadIdx.x & 15) == 0) w.stats[row] = make_float2(lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, s);
-  if (lse == -INFINITY) norm = 0.0f;                         // sees no key (or is behind the last sequence)
-  if (HALF) {
-    if (!(norm < INFINITY)) norm = 0.0f;
-    __shared__ float best[16];
-    if ((threadIdx.x & 15) == 0) best[threadIdx.x / 16] = norm;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 16; ++i) norm = fmaxf(norm, best[i]);
-      if (norm > 0.0f) atomicMax(w.top, __float_as_uint(norm));     // a maximum: the same in any order
-    }
+  if (HALF && in && (threadIdx.x & 15) == 0) {
+    // (-infinity: sees no key, or is behind the last sequence)
+    if (lse == -INFINITY || !(norm < INFINITY)) norm = 0.0f;
+    w.norms[row] = norm;
+    const int64_t b = norm > 0.0f ? sequence_of(a.cu_q, a.B, t) : a.B;
+    if (b < a.B) keep_largest(w.top_g + b * a.Hk + h / (a.Hq / a.Hk), norm);
   }
 }
-// fp16: the values' largest norm, over those that some query sees.
+// fp16: the values' largest norm of each sequence and key head, over those that some query sees.
 __global__ void __launch_bounds__(256) attention_norms_kernel(const __grid_constant__ AttnArgs a) {
   const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
   const int d = (threadIdx.x & 15) * 8;
@@ -103,14 +119,7 @@ __global__ void __launch_bounds__(256) attention_norms_kernel(const __grid_const
     for (int i = 0; i < 8; ++i) norm = __fmaf_rn(v[i], v[i], norm);
   }
   norm = sum16(norm);
-  if (!(norm < INFINITY)) norm = 0.0f;
-  __shared__ float best[16];
-  if ((threadIdx.x & 15) == 0) best[threadIdx.x / 16] = norm;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) norm = fmaxf(norm, best[i]);
-    if (norm > 0.0f) atomicMax(work_of(a.workspace).top + 1, __float_as_uint(norm));
-  }
+  if ((threadIdx.x & 15) == 0 && norm > 0.0f && norm < INFINITY) keep_largest(work_of(a).top_v + b * a.Hk + (row - t * a.Hk), norm);
 }
 
 // ------------------------------------------------------------------------------ the keys' and values' gradients
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
       }
       drain<1>(kv_full, 1), drain<C::SLOTS>(q_full, queries), drain<C::SLOTS>(g_full, i);
     } else if (warp == 10 && steps) {
-      const float2* src = work_of(a.workspace).stats;
+      const float2* src = work_of(a).stats;
       Ring<C::STATS> r;
       int tile = 0, chunk = 0;
       for (int i = 0; i < steps; ++i, r.next()) {
@@ -311,8 +320,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     const int half = warp >> 2, key = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + KV_S + half * 64, dp_at = lanes + KV_DP + half * 64;
-    const Work w = work_of(a.workspace);
-    const float c = a.scale * 1.4426950408889634f, factor = ds_factor<T>(w) * exp2f(-P_LOG2<T>);
+    const Work w = work_of(a);
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    auto factor_of = [&] {
+      const int64_t top = u.b * a.Hk + u.kh;
+      return HALF && steps ? ds_factor(__uint_as_float(__ldg(w.top_g + top)), __uint_as_float(__ldg(w.top_v + top))) : 1.0f;
+    };
+    const float c = a.scale * 1.4426950408889634f, factor = factor_of() * exp2f(-P_LOG2<T>);
     const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c));
     const uint64_t f2 = ptx::join2(__float_as_uint(factor), __float_as_uint(factor));
     const uint64_t minus = ptx::join2(0xBF800000u, 0xBF800000u);
@@ -383,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
             uint64_t y0 = ptx::fma2(ptx::join2(__float_as_uint(dl.x), __float_as_uint(dl.y)), minus, ptx::join2(g[x][e], g[x][e + 1]));
             uint64_t y1 = ptx::fma2(ptx::join2(__float_as_uint(dl.z), __float_as_uint(dl.w)), minus, ptx::join2(g[x][e + 2], g[x][e + 3]));
             uint64_t p0 = ptx::join2(s[x][e], s[x][e + 1]), p1 = ptx::join2(s[x][e + 2], s[x][e + 3]);
-            if (std::is_same<T, __half>::value) p0 = ptx::mul2(p0, f2), p1 = ptx::mul2(p1, f2);
+            if (HALF) p0 = ptx::mul2(p0, f2), p1 = ptx::mul2(p1, f2);
             y0 = ptx::mul2(p0, y0), y1 = ptx::mul2(p1, y1);
             g[x][e] = (uint32_t)y0, g[x][e + 1] = (uint32_t)(y0 >> 32), g[x][e + 2] = (uint32_t)y1, g[x][e + 3] = (uint32_t)(y1 >> 32);
           }
@@ -419,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     void* base = keys ? a.dk : a.dv;
     const bool mine = ok && base && t < kr.end;
     RowsOut<DP / 8> rows_out{smem + half * C::TILE + (warp & 3) * 32 * DP * 2};      // (the places of K and V: their products are done)
-    const float f = keys ? a.scale / ds_factor<T>(w) : exp2f(-P_LOG2<T>);
+    const float f = keys ? a.scale / factor_of() : exp2f(-P_LOG2<T>);
     const uint64_t out2 = ptx::join2(__float_as_uint(f), __float_as_uint(f));
     uint64_t worst = 0;                                      // NaN where a gradient is NaN or infinite
 #pragma unroll
@@ -608,9 +622,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
     const bool mine = r < tl.heads * tl.tokens && gh < tl.group && t < qr.end;
     const int64_t n = !mine ? 0 : a.causal ? max((int64_t)0, min(nk, t - qr.begin + 1 + nk - nq)) : nk;
     const int64_t first = a.causal ? u.t0 - qr.begin + 1 + nk - nq : nk;     // keys that every row sees
-    const Work w = work_of(a.workspace);
+    const Work w = work_of(a);
     const float2 st = mine ? w.stats[t * a.Hq + h] : make_float2(0.0f, 0.0f);
-    const float c = a.scale * 1.4426950408889634f, factor = ds_factor<T>(w);
+    const bool scaled = std::is_same<T, __half>::value && mine && u.b < a.B;
+    const float factor = scaled ? ds_factor(w.norms[t * a.Hq + h], __uint_as_float(__ldg(w.top_v + u.b * a.Hk + u.kh))) : 1.0f;
+    const float c = a.scale * 1.4426950408889634f;
     const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(st.x), __float_as_uint(st.x));
     const uint64_t dl2 = ptx::join2(__float_as_uint(-st.y), __float_as_uint(-st.y)), f2 = ptx::join2(__float_as_uint(factor), __float_as_uint(factor));
     bool ok = true;
@@ -712,7 +728,7 @@ template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t
       !make_rows_map(&mk, a.k, a.Tk, a.Hk, a.D, a.k_stride, a.dtype, 1, 128) || !make_rows_map(&mv, a.v, a.Tk, a.Hk, a.D, a.v_stride, a.dtype, 1, 128))
     return cudaErrorUnknown;
   if (std::is_same<T, __half>::value) {
-    const cudaError_t e = cudaMemsetAsync(a.workspace, 0, 8, stream);
+    const cudaError_t e = cudaMemsetAsync(work_of(a).top_g, 0, (size_t)a.B * a.Hk * 8, stream);
     if (e != cudaSuccess) return e;
     if (a.Tk) attention_norms_kernel<<<(unsigned)((a.Tk * a.Hk + 15) / 16), 256, 0, stream>>>(a);
   }
@@ -740,7 +756,7 @@ template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t
 
 }  // namespace
 
-size_t attention_backward_workspace(int64_t Tq, int64_t, int Hq, int) { return 256 + (size_t)Tq * Hq * sizeof(float2); }
+size_t attention_backward_workspace(int64_t Tq, int64_t B, int Hq, int Hk, int dtype) { return work_of(nullptr, Tq, B, Hq, Hk, dtype == EMU_DTYPE_F16).bytes; }
 
 cudaError_t take_attention_backward_wait_error(int* code) { return take_error(code); }
 

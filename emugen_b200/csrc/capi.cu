@@ -741,8 +741,8 @@ emu_status emu_attention(const emu_attention_args* p, void* out, void* out_low, 
 }
 
 size_t emu_attention_backward_workspace_size(const emu_attention_args* p) {
-  if (!p || p->total_q < 0 || p->total_k < 0 || p->heads_q < 1 || p->heads_k < 1) return 0;
-  return emu::attention_backward_workspace(p->total_q, p->total_k, p->heads_q, p->heads_k);
+  if (!p || p->total_q < 0 || p->total_k < 0 || p->sequences < 0 || p->heads_q < 1 || p->heads_k < 1) return 0;
+  return emu::attention_backward_workspace(p->total_q, p->sequences, p->heads_q, p->heads_k, p->dtype);
 }
 
 emu_status emu_attention_backward(const emu_attention_args* p, const void* out, const void* out_low, const float* lse,

@@ -182,7 +182,7 @@ struct AttnArgs {
   void* dv;                     // contiguous; any of the three may be null
   void* workspace;
 };
-size_t attention_backward_workspace(int64_t Tq, int64_t Tk, int Hq, int Hk);
+size_t attention_backward_workspace(int64_t Tq, int64_t B, int Hq, int Hk, int dtype);
 cudaError_t launch_attention(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream);
 // as take_wait_error, for the waits of attention's kernels

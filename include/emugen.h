@@ -514,8 +514,8 @@ EMU_API emu_status emu_attention(const emu_attention_args* args, void* out, void
 /*
  * Its gradients from dout: dq [total_q][heads_q][head_size], dk and dv [total_k][heads_k][head_size], contiguous, each may be
  * NULL (not wanted).  out, out_low (may be NULL) and lse are emu_attention's.  ds = p (dout . v - dout . (out + out_low)) is
- * rounded to the inputs' dtype for its products (fp16: scaled by a power of two that keeps it in range).  No atomic
- * additions: the same result every run.
+ * rounded to the inputs' dtype for its products (fp16: scaled by a power of two that keeps it in range, in dq one for each row and head,
+ * in dk one for each sequence and key head).  No atomic additions: the same result every run.
  * workspace: emu_attention_backward_workspace_size(args) bytes on the device, 256-byte aligned.
  */
 EMU_API size_t emu_attention_backward_workspace_size(const emu_attention_args* args);
