@@ -19,6 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .attention import _plain, _wants_grad
 from .fp8 import _DTYPE, _on, _raw_stream
 
 
@@ -193,9 +194,13 @@ def attend_kv_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     own row first.  Positions on a page that does not exist are not seen, and a sequence that sees none gets zeros.
     scale: of the scores (default head_size ** -0.5).  With return_lse also f32 [sequences, query heads]: the logarithm of
     the sum of exp(score), -inf where nothing is seen.  head_size up to 256.  Scores, sums and the softmax in f32, the
-    weights of the values rounded to fp16; the same result every run.  Not differentiable."""
+    weights of the values rounded to fp16; the same result every run.  Not differentiable: a q that wants a gradient or has a
+    forward-mode tangent is refused (torch.no_grad() or q.detach() around generation)."""
     if v_cache is None or v_scale is None:
         raise RuntimeError("attend_kv_cache needs a cache of keys and values")
+    if _wants_grad(q, k_scale, v_scale):
+        raise RuntimeError("attend_kv_cache is not differentiable: call it under torch.no_grad() or with detached tensors")
+    _plain("attend_kv_cache", q, k_scale, v_scale)
     fmt, pages, page_size, heads, D = _geometry(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     if q.dtype not in (torch.float16, torch.bfloat16):

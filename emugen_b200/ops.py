@@ -158,7 +158,8 @@ def attend_kv_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                     scale: Optional[float] = None) -> torch.Tensor:
     """Attention of one new token for each sequence over its cached rows: [sequences, query heads, head_size]."""
-    return kvcache.attend_kv_cache(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, scale=scale)
+    with torch.no_grad():
+        return kvcache.attend_kv_cache(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, scale=scale)
 
 
 @attend_kv_cache.register_fake
