@@ -12,6 +12,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace emu {
@@ -91,6 +93,47 @@ __device__ __forceinline__ bool settled(const Lanes& r, int D) {
   return __all_sync(0xFFFFFFFFu, nan);
 }
 
+// The tokens, counted from t0, of [t0, t1) with an element [d0, d1) of heads [h0, h1) that is infinite or NaN: the first and the last (none:
+// INT_MAX, -1); with `stop` the search ends where the first one is known.  The whole warp; 16 lanes to a row, 8 elements each.  Rows
+// start on 16 bytes, d0 and d1 are multiples of 8, d1 - d0 <= 128.
+struct Span {
+  int first, last;
+};
+template <typename T> __device__ __forceinline__ Span not_finite(const T* p, int64_t token_stride, int64_t head_stride, int64_t t0, int64_t t1, int h0, int h1, int d0, int d1, bool stop = false) {
+  constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  const int lane = threadIdx.x & 31, d = d0 + (lane & 15) * 8, heads = h1 - h0;
+  const int tokens = heads > 0 ? (int)max((int64_t)0, t1 - t0) : 0;
+  int first = 0x7FFFFFFF, last = -1, t = 0, h = lane >> 4;
+  p += t0 * token_stride + h0 * head_stride + d;
+  auto next = [&] {
+    for (h += 2; h >= heads && t < tokens; h -= heads) ++t;
+  };
+  if (h >= heads) h = 0, t = 1;                              // (one head)
+  while (__any_sync(0xFFFFFFFFu, t < tokens)) {
+    constexpr int U = 8;                                     // rows under way
+    uint4 w[U];
+    int at[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0), at[i] = t;
+      if (t < tokens && d < d1) w[i] = __ldg(reinterpret_cast<const uint4*>(p + t * token_stride + h * head_stride));
+      next();
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t u = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+        bad = bad || (u & EXPONENT) == EXPONENT || (u >> 16 & EXPONENT) == EXPONENT;
+      }
+      if (bad) first = min(first, at[i]), last = max(last, at[i]);
+    }
+    if (stop && __any_sync(0xFFFFFFFFu, last >= 0)) break;
+  }
+  return {__reduce_min_sync(0xFFFFFFFFu, first), __reduce_max_sync(0xFFFFFFFFu, last)};
+}
+
 // The keys that query t of sequence b sees: the first `n` of the sequence's.
 struct Seen {
   Rows k;
@@ -103,6 +146,29 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t)
   s.n = s.k.count();
   if (a.causal) s.n = max((int64_t)0, min(s.n, t - q.begin + 1 + s.k.count() - q.count()));
   return s;
+}
+
+// Which of the lanes with `bad`, a row of sequence b that is not finite in elements [d0, d1), have to be made again: a row that sees the
+// first n keys met one that it does not see only if one of keys n .. end - 1, which were multiplied too, is not finite there.  What is
+// not finite by right stays as it is.  VALUES: of v, else k.  (bf16: of values past 2^118, weights of up to 2^8 can leave f32's range
+// where the row's result does not; so it is made again too where none that it sees is infinite or NaN.)  low: the row of what rounding
+// took from the output, or null: 0 where it is not finite, in rows that stay.  (The whole warp.)
+template <typename T, bool VALUES> __device__ __noinline__ uint32_t rows_made_again(const AttnArgs& a, bool bad, int64_t b, int n, int64_t end, int kh, int d0, int d1, T* low) {
+  const int64_t k0 = rows_of(a.cu_k, b, a.Tk).begin;
+  const int least = __reduce_min_sync(0xFFFFFFFFu, bad ? n : 0x7FFFFFFF);
+  const T* x = static_cast<const T*>(VALUES ? a.v : a.k);
+  const int64_t ts = VALUES ? a.v_stride[0] : a.k_stride[0], hs = VALUES ? a.v_stride[1] : a.k_stride[1];
+  const Span hidden = not_finite(x, ts, hs, k0 + least, min(k0 + end, a.Tk), kh, kh + 1, d0, d1);
+  bool made = hidden.last >= 0 && n - least <= hidden.last;
+  if (VALUES && std::is_same<T, __nv_bfloat16>::value) {
+    const int most = __reduce_max_sync(0xFFFFFFFFu, bad ? n : 0);
+    const Span seen = not_finite(x, ts, hs, k0, k0 + most, kh, kh + 1, d0, d1, true);
+    made = made || seen.first >= n;
+  }
+  if (VALUES && low && bad && !made)
+    for (int d = d0; d < d1; ++d)
+      if (!(fabsf(widen<T>(low[d])) < INFINITY)) low[d] = narrow<T>(0.0f);
+  return __ballot_sync(0xFFFFFFFFu, bad && made);
 }
 
 // Elements [d0, d1) of o_t of one head.

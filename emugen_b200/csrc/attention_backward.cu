@@ -148,6 +148,34 @@ __device__ __forceinline__ void zero_rest(uint8_t* tiles, int count, int boxes, 
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Which keys' rows of dK (`keys`) or dV with `bad`, that are not finite, have to be made again: those where one of the rows that were
+// multiplied but do not see the key is not finite: the tiles' first ones, up to the key's, tokens behind the sequence, heads behind the
+// group.  What is not finite by right stays as it is.  (The whole warp.  A function that finds its place again: what the kernel
+// would keep for it through its loop would not fit its registers.)
+template <typename T> __device__ __noinline__ uint32_t keys_made_again(const AttnArgs& a, const Tiling& tl, bool keys, int key, bool bad) {
+  Unit u;
+  u.kh = (int)(blockIdx.x % a.Hk);
+  find_unit(u, a.cu_k, a.B, a.Tk, 128, blockIdx.x / a.Hk);
+  const Rows qr = rows_of(a.cu_q, u.b, a.Tq);
+  const int64_t nq = qr.count(), hidden = u.rows.count() - nq, j0 = u.t0 - u.rows.begin;
+  const int64_t first = a.causal ? max((int64_t)0, j0 - hidden) / tl.tokens * tl.tokens : 0;
+  const int64_t end = min(qr.begin + first + (nq - first + tl.tokens - 1) / tl.tokens * tl.tokens, a.Tq);
+  const T* src = static_cast<const T*>(keys ? a.q : a.dout);
+  const int64_t ts = keys ? a.q_stride[0] : a.dout_stride[0], hs = keys ? a.q_stride[1] : a.dout_stride[1];
+  const int h0 = u.kh * tl.group, h1 = h0 + tl.group, h2 = min(h0 + tl.chunks * tl.heads, a.Hq);
+  // the first query that sees the key, of this lane's and of the last one's
+  const int64_t sees = a.causal ? max((int64_t)0, j0 + key - hidden) : 0;
+  const int64_t most = __shfl_sync(0xFFFFFFFFu, sees, 31 - __clz(__ballot_sync(0xFFFFFFFFu, bad)));
+  bool made = false;
+#pragma unroll 1
+  for (int part = 0; part < 3; ++part) {
+    const Span s = not_finite(src, ts, hs, part == 1 ? qr.end : qr.begin + first, part == 0 ? qr.begin + most : part == 1 ? end : qr.end,
+                              part == 2 ? h1 : h0, part == 0 ? h1 : h2, 0, a.D);
+    made = made || (s.last >= 0 && (part > 0 || first + s.first < sees));
+  }
+  return __ballot_sync(0xFFFFFFFFu, bad && made);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
@@ -455,8 +483,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     rows_out.store(static_cast<T*>(base) + (t * a.Hk + u.kh) * a.D, mine, a.D / 8);
     // A query that does not see the key was multiplied by 0, which infinities and NaN turn into NaN: such rows are made
     // again from the queries that see them alone.
-    const bool redo = mine && steps && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
-    for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
+    const bool bad = mine && steps && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
+    for (uint32_t rows = __any_sync(0xFFFFFFFFu, bad) ? keys_made_again<T>(a, tl, keys, key, bad) : 0; rows; rows &= rows - 1) {
       const int64_t row = __shfl_sync(0xFFFFFFFFu, t, __ffs(rows) - 1);
       if (keys) row_dkv<T, true>(a, w.stats, u.b, row, u.kh);
       else row_dkv<T, false>(a, w.stats, u.b, row, u.kh);
@@ -705,9 +733,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
     rows_out.store(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D + half * HALF, mine && ok, (a.D - half * HALF) / 8);
     // a hidden key that is infinite or NaN: the row again, from the keys that it sees alone (this thread's half of it)
     const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
-    for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, redo); rows; rows &= rows - 1) {
+    const int d0 = half * HALF, d1 = min(a.D, (half + 1) * HALF);
+    for (uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, false>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, d0, d1, static_cast<T*>(nullptr)) : 0; rows; rows &= rows - 1) {
       const int src = __ffs(rows) - 1;
-      row_dq<T>(a, w.stats, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), half * HALF, min(a.D, (half + 1) * HALF));
+      row_dq<T>(a, w.stats, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), d0, d1);
     }
   }
   ptx::tc_fence_before();
