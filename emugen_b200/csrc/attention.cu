@@ -46,7 +46,9 @@ template <int DP> struct Fwd {
 // fp16: P, and with it l and O, is held 2^7 times as large.  P is below 2^8 (the maximum is held up to that factor), so that it
 // stays below 2^15, and weights down to 2^-21 keep all their bits, those down to 2^-31 some; without it they were lost from 2^-14 and
 // gone below 2^-25, and 16384 keys 18 below a first one came out as zeros.  bf16 has f32's range.
-template <typename T> constexpr float P_LOG2 = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+template <typename T> __device__ __forceinline__ float held_shift(float m, float c) {
+  return std::is_same<T, __half>::value ? shift_of(m, c) + 7.0f : shift_of(m, c);
+}
 
 // tensor memory columns: S (and P) of both tiles, O of both tiles
 constexpr uint32_t S_COL = 0, O_COL = 256;
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
           }
         }
       }
-      const float shift = shift_of(m, c) + P_LOG2<T>;
+      const float shift = held_shift<T>(m, c);
       const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
       uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D, mine && ok, a.D / 8);
     }
-    if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - (shift_of(m, c) + P_LOG2<T>)) * 0.6931471805599453f : l;
+    if (mine && ok && a.lse) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - held_shift<T>(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone.  (Where the sum is NaN, the scores are, and the row is NaN by right.)
     redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
         l *= now == -INFINITY ? 1.0f : exp2f((m - now) * c);
         m = now;
       }
-      const float shift = shift_of(m, c) + P_LOG2<T>;
+      const float shift = held_shift<T>(m, c);
       const uint64_t c2 = ptx::join2(__float_as_uint(c), __float_as_uint(c)), sh2 = ptx::join2(__float_as_uint(shift), __float_as_uint(shift));
       uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
       }
       rows_out.store(static_cast<T*>(pass ? a.low : a.out) + (t * a.Hq + h) * a.D + w * HALF, mine && ok, (a.D - w * HALF) / 8);
     }
-    if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - (shift_of(m, c) + P_LOG2<T>)) * 0.6931471805599453f : l;
+    if (mine && ok && a.lse && w == 0) a.lse[(int64_t)h * a.Tq + t] = n == 0 || l == 0.0f ? -INFINITY : l > 0.0f ? (log2f(l) - held_shift<T>(m, c)) * 0.6931471805599453f : l;
     // A value that the mask hides was multiplied by 0, which infinities and NaN turn into NaN: such rows are made again
     // from the keys that they see alone (this thread's half).  (Where the sum is NaN, the scores are, and the row is NaN by right.)
     const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
