@@ -156,7 +156,7 @@ struct NormRopeArgs {
   void* dw[2];
   float* partial;               // norm_rope_workspace bytes
   int split, heads_per_unit[2];   // from here on set by the launcher
-  bool vec;
+  bool vec, vec_table;          // rows and weights, cosines and sines may be read 16 bytes at once
 };
 size_t norm_rope_workspace(int64_t D);
 cudaError_t launch_norm_rope(NormRopeArgs a, bool back, cudaStream_t stream);
