@@ -30,17 +30,6 @@ __device__ __forceinline__ Rows rows_of(const int32_t* cu, int64_t b, int64_t to
   r.end = min(max((int64_t)cu[b + 1], r.begin), total);
   return r;
 }
-// The sequence that holds row t, or B for a row behind the last one.
-__device__ __forceinline__ int64_t sequence_of(const int32_t* cu, int64_t B, int64_t t) {
-  int64_t lo = 0, hi = B;
-  while (lo < hi) {
-    const int64_t m = (lo + hi) / 2;
-    if ((int64_t)cu[m + 1] > t) hi = m;
-    else lo = m + 1;
-  }
-  return lo;
-}
-
 template <typename T> __device__ __forceinline__ float widen(T v);
 template <> __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }

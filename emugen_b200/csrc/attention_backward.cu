@@ -56,16 +56,21 @@ __device__ __forceinline__ float ds_factor(float g, float v) {
   const float b = 4.0f * g * v;
   return b > 0.0f && b < INFINITY ? exp2f(floorf((28.0f - log2f(b)) * 0.5f)) : 1.0f;
 }
-// The largest so far, of sequence b and key head kh; additions to it in any order give the same.
-__device__ __forceinline__ void keep_largest(uint32_t* top, float norm) {
-  const uint32_t bits = __float_as_uint(norm);               // (a positive number's bits grow with it)
-  if (bits > __ldcg(top)) atomicMax(top, bits);
+// The sequence that holds row t, or B for a row behind the last one.
+__device__ __forceinline__ int64_t sequence_of(const int32_t* cu, int64_t B, int64_t t) {
+  int64_t lo = 0, hi = B;
+  while (lo < hi) {
+    const int64_t m = (lo + hi) / 2;
+    if ((int64_t)cu[m + 1] > t) hi = m;
+    else lo = m + 1;
+  }
+  return lo;
 }
 
 // ------------------------------------------------------------------------------ statistics
 // delta of each (token, head), from the output before its rounding where its rest was kept: ds is what is left of
 // dp - delta, so that a sequence of 2 tokens had 0.0039 of its gradients' norm off without the rest, 0.0026 with it.  Beside
-// the shift of its scores; fp16: its norm, and the largest of its sequence and key head.  16 lanes to a row, 8 elements each.
+// the shift of its scores; fp16: its norm.  16 lanes to a row, 8 elements each.
 template <typename T> __device__ __forceinline__ void load8(const T* p, bool any, float (&v)[8]) {
   uint4 w = make_uint4(0, 0, 0, 0);
   if (any) w = __ldg(reinterpret_cast<const uint4*>(p));
@@ -95,31 +100,81 @@ template <typename T> __global__ void __launch_bounds__(256) attention_stats_ker
   s = sum16(__fadd_rn(s, rest));
   if (HALF) norm = sum16(norm);
   const float lse = in ? a.lse[(int64_t)h * a.Tq + t] : -INFINITY;
-  if (in && (threadIdx.x & 15) == 0) w.stats[row] = make_float2(lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, s);
-  if (HALF && in && (threadIdx.x & 15) == 0) {
+  if (in && (threadIdx.x & 15) == 0) {
+    w.stats[row] = make_float2(lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, s);
     // (-infinity: sees no key, or is behind the last sequence)
-    if (lse == -INFINITY || !(norm < INFINITY)) norm = 0.0f;
-    w.norms[row] = norm;
-    const int64_t b = norm > 0.0f ? sequence_of(a.cu_q, a.B, t) : a.B;
-    if (b < a.B) keep_largest(w.top_g + b * a.Hk + h / (a.Hq / a.Hk), norm);
+    if (HALF) w.norms[row] = lse == -INFINITY || !(norm < INFINITY) ? 0.0f : norm;
   }
 }
-// fp16: the values' largest norm of each sequence and key head, over those that some query sees.
-__global__ void __launch_bounds__(256) attention_norms_kernel(const __grid_constant__ AttnArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-  const int d = (threadIdx.x & 15) * 8;
-  float norm = 0.0f;
-  const bool in = row < a.Tk * a.Hk;
-  const int64_t t = in ? row / a.Hk : 0;
-  const int64_t b = in ? sequence_of(a.cu_k, a.B, t) : a.B;
-  if (b < a.B && rows_of(a.cu_q, b, a.Tq).count() > 0) {
-    float v[8];
-    load8(static_cast<const __half*>(a.v) + t * a.v_stride[0] + (row - t * a.Hk) * a.v_stride[1] + d, d < a.D, v);
+
+// fp16: the largest norms of each sequence and key head.  A warp has 32 tokens of a key head, a lane the largest of its token; one lane of
+// each of their sequences tells the memory.  (3001 tokens of 12 heads: 16 us with the statistics, 28 where each row told it by itself; with
+// rows of one head side by side in the statistics' blocks, to put them together there, 8192 tokens of 32 heads took 53 us for 32.)  In any
+// order the same.  b: B where the token has none.
+__device__ __forceinline__ void keep_largest(uint32_t* top, int Hk, int64_t B, int64_t b, float norm) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) norm = __fmaf_rn(v[i], v[i], norm);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t s = __shfl_down_sync(0xFFFFFFFFu, b, o);
+    const float n = __shfl_down_sync(0xFFFFFFFFu, norm, o);
+    if (lane + o < 32 && s == b) norm = fmaxf(norm, n);
   }
-  norm = sum16(norm);
-  if ((threadIdx.x & 15) == 0 && norm > 0.0f && norm < INFINITY) keep_largest(work_of(a).top_v + b * a.Hk + (row - t * a.Hk), norm);
+  // the first token of a sequence now has the largest of them
+  const int64_t before = __shfl_up_sync(0xFFFFFFFFu, b, 1);
+  if (b >= B || (lane > 0 && before == b)) return;
+  const uint32_t bits = __float_as_uint(norm);               // (a positive number's bits grow with it)
+  uint32_t* to = top + b * Hk;
+  if (bits > __ldcg(to)) atomicMax(to, bits);
+}
+// Warps of the queries' norms first, then those of the values, which are made here from those that some query sees.
+inline int64_t norm_warps(int64_t tokens, int heads) { return (tokens + 31) / 32 * heads; }
+__global__ void __launch_bounds__(256) attention_norms_kernel(const __grid_constant__ AttnArgs a, int64_t query_warps, int64_t warps) {
+  const Work w = work_of(a);
+  int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (i >= warps) return;
+  const bool values = i >= query_warps;
+  if (values) i -= query_warps;
+  const int kh = (int)(i % a.Hk), lane = threadIdx.x & 31;
+  const int64_t t0 = i / a.Hk * 32, t = t0 + lane;
+  float norm = 0.0f;
+  int64_t b = a.B;
+  if (!values) {
+    const int group = a.Hq / a.Hk;
+    if (t < a.Tq) {
+      const float* p = w.norms + t * a.Hq + kh * group;
+#pragma unroll 4
+      for (int g = 0; g < group; ++g) norm = fmaxf(norm, __ldg(p + g));
+      b = sequence_of(a.cu_q, a.B, t);
+    }
+    keep_largest(w.top_g + kh, a.Hk, a.B, b, norm);
+    return;
+  }
+  // a row to 16 lanes, 16 times two rows; the sums change places so that token t0 + l's is in lane l
+  const int d = (lane & 15) * 8;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 16; r0 += 8) {
+    uint4 v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int64_t at = t0 + 2 * (r0 + r) + (lane >> 4);
+      v[r] = make_uint4(0, 0, 0, 0);
+      if (at < a.Tk && d < a.D) v[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(a.v) + at * a.v_stride[0] + kh * a.v_stride[1] + d));
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const __half* e = reinterpret_cast<const __half*>(&v[r]);
+      float n = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n = __fmaf_rn(__half2float(e[k]), __half2float(e[k]), n);
+      n = sum16(n);
+      const float from = __shfl_sync(0xFFFFFFFFu, n, (lane & 1) * 16);
+      if (lane >> 1 == r0 + r) norm = from;
+    }
+  }
+  if (!(norm < INFINITY)) norm = 0.0f;
+  if (t < a.Tk) b = sequence_of(a.cu_k, a.B, t);
+  if (b < a.B && rows_of(a.cu_q, b, a.Tq).count() == 0) b = a.B;
+  keep_largest(w.top_v + kh, a.Hk, a.B, b, norm);
 }
 
 // ------------------------------------------------------------------------------ the keys' and values' gradients
@@ -756,12 +811,13 @@ template <typename T, int DP> cudaError_t launch(const AttnArgs& a, cudaStream_t
       !make_rows_map(&mg, a.dout, a.Tq, a.Hq, a.D, a.dout_stride, a.dtype, tl.heads, tl.tokens) ||
       !make_rows_map(&mk, a.k, a.Tk, a.Hk, a.D, a.k_stride, a.dtype, 1, 128) || !make_rows_map(&mv, a.v, a.Tk, a.Hk, a.D, a.v_stride, a.dtype, 1, 128))
     return cudaErrorUnknown;
+  attention_stats_kernel<T><<<(unsigned)((a.Tq * a.Hq + 15) / 16), 256, 0, stream>>>(a);
   if (std::is_same<T, __half>::value) {
     const cudaError_t e = cudaMemsetAsync(work_of(a).top_g, 0, (size_t)a.B * a.Hk * 8, stream);
     if (e != cudaSuccess) return e;
-    if (a.Tk) attention_norms_kernel<<<(unsigned)((a.Tk * a.Hk + 15) / 16), 256, 0, stream>>>(a);
+    const int64_t queries = norm_warps(a.Tq, a.Hk), warps = queries + norm_warps(a.Tk, a.Hk);
+    attention_norms_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(a, queries, warps);
   }
-  attention_stats_kernel<T><<<(unsigned)((a.Tq * a.Hq + 15) / 16), 256, 0, stream>>>(a);
   if ((a.dk || a.dv) && a.Tk) {
     auto kernel = attention_dkv_kernel<T, DP>;
     static std::atomic<uint64_t> set{0};
