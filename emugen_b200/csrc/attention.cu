@@ -280,10 +280,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     // from the keys that they see alone.  (Where the sum is NaN, the scores are, and the row is NaN by right.)
     redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
     T* low = a.low ? static_cast<T*>(a.low) + (t * a.Hq + h) * a.D : nullptr;
-    for (uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, true>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, 0, a.D, low) : 0; rows; rows &= rows - 1) {
-      const int src = __ffs(rows) - 1;
-      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), 0, a.D);
-    }
+    const uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, true>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, 0, a.D, low) : 0;
+    if (rows) make_again<T, AGAIN_OUT>(a, nullptr, rows, u.b, t, h, make_float2(held_shift<T>(m, c), f), 0, a.D);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -571,10 +569,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_few_kernel(const __grid_
     const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f) && l > 0.0f;
     const int d0 = w * HALF, d1 = min(a.D, (w + 1) * HALF);
     T* low = a.low ? static_cast<T*>(a.low) + (t * a.Hq + h) * a.D : nullptr;
-    for (uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, true>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, d0, d1, low) : 0; rows; rows &= rows - 1) {
-      const int src = __ffs(rows) - 1;
-      row_forward<T>(a, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), d0, d1);
-    }
+    const uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, true>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, d0, d1, low) : 0;
+    if (rows) make_again<T, AGAIN_OUT>(a, nullptr, rows, u.b, t, h, make_float2(held_shift<T>(m, c), f), d0, d1);
   }
   ptx::tc_fence_before();
   __syncthreads();

@@ -43,45 +43,6 @@ template <typename T> __device__ __forceinline__ float rounded_off(float v) {
   return fabsf(r) < INFINITY ? r : 0.0f;
 }
 
-// One row at a time, a warp to a row: lane l holds elements l, l + 32, l + 64 and l + 96 of it.  Nothing that the mask
-// hides is read, so that infinities and NaN there reach no result.
-struct Lanes {
-  float v[4];
-};
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-  return v;
-}
-template <typename T> __device__ __forceinline__ Lanes load_row(const T* p, int D) {
-  Lanes r;
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.v[i] = lane + 32 * i < D ? widen<T>(p[lane + 32 * i]) : 0.0f;
-  return r;
-}
-__device__ __forceinline__ float dot(const Lanes& a, const Lanes& b) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s = __fmaf_rn(a.v[i], b.v[i], s);
-  return warp_sum(s);
-}
-// Elements [d0, d1) of the row.
-template <typename T> __device__ __forceinline__ void store_row(T* p, int d0, int d1, const Lanes& r, float f) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i >= d0 && lane + 32 * i < d1) p[lane + 32 * i] = narrow<T>(__fmul_rn(r.v[i], f));
-}
-// Whether every element of the row is NaN: nothing that is added changes it any more.
-__device__ __forceinline__ bool settled(const Lanes& r, int D) {
-  const int lane = threadIdx.x & 31;
-  bool nan = true;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) nan = nan && (isnan(r.v[i]) || lane + 32 * i >= D);
-  return __all_sync(0xFFFFFFFFu, nan);
-}
-
 // The tokens, counted from t0, of [t0, t1) with an element [d0, d1) of heads [h0, h1) that is infinite or NaN: the first and the last (none:
 // INT_MAX, -1); with `stop` the search ends where the first one is known.  The whole warp; 16 lanes to a row, 8 elements each.  Rows
 // start on 16 bytes, d0 and d1 are multiples of 8, d1 - d0 <= 128.
@@ -123,20 +84,6 @@ template <typename T> __device__ __forceinline__ Span not_finite(const T* p, int
   return {__reduce_min_sync(0xFFFFFFFFu, first), __reduce_max_sync(0xFFFFFFFFu, last)};
 }
 
-// The keys that query t of sequence b sees: the first `n` of the sequence's.
-struct Seen {
-  Rows k;
-  int64_t n;
-};
-__device__ __forceinline__ Seen seen_by(const AttnArgs& a, int64_t b, int64_t t) {
-  const Rows q = rows_of(a.cu_q, b, a.Tq);
-  Seen s;
-  s.k = rows_of(a.cu_k, b, a.Tk);
-  s.n = s.k.count();
-  if (a.causal) s.n = max((int64_t)0, min(s.n, t - q.begin + 1 + s.k.count() - q.count()));
-  return s;
-}
-
 // Which of the lanes with `bad`, a row of sequence b that is not finite in elements [d0, d1), have to be made again: a row that sees the
 // first n keys met one that it does not see only if one of keys n .. end - 1, which were multiplied too, is not finite there.  What is
 // not finite by right stays as it is.  VALUES: of v, else k.  (bf16: of values past 2^118, weights of up to 2^8 can leave f32's range
@@ -160,89 +107,154 @@ template <typename T, bool VALUES> __device__ __noinline__ uint32_t rows_made_ag
   return __ballot_sync(0xFFFFFFFFu, bad && made);
 }
 
-// Elements [d0, d1) of o_t of one head.
-template <typename T> __device__ __forceinline__ void row_forward(const AttnArgs& a, int64_t b, int64_t t, int h, int d0, int d1) {
-  const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
-  const int kh = h / (a.Hq / a.Hk);
-  const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];
-  const T* v = static_cast<const T*>(a.v) + kh * a.v_stride[1];
-  Seen s{{0, 0}, 0};
-  if (b < a.B) s = seen_by(a, b, t);
-  const Lanes x = load_row(q, a.D);
-  Lanes o{};
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = s.k.begin; j < s.k.begin + s.n; ++j) {
-    const float z = __fmul_rn(dot(x, load_row(k + j * a.k_stride[0], a.D)), a.scale);
-    const float top = fmaxf(m, z);
-    const float shift = top == -INFINITY ? 0.0f : top;
-    const float old = expf(m - shift), p = expf(z - shift);
-    const Lanes y = load_row(v + j * a.v_stride[0], a.D);
-    l = __fmaf_rn(l, old, p);
+// Rows of the output or of the gradients made again from what they see alone, in f32 by one warp, 8 rows at a time: they share what is
+// read of the other side, and their sums over the head share the exchanges between lanes (one row after the other: 93 ms for one infinity
+// in the middle of dO of 4096 causal tokens, 32 heads on 8 of 128; so 7.5, 9.4 with two of the other side's rows at a time; without the
+// infinity 0.65).  Lane l holds elements 4 l .. 4 l + 3.
+//   OUT  o_i = sum_j w_ij v_j        w = exp2(c s + known.x) known.y         (known: the held shift, 1 / l)
+//   DQ   dq_i = scale sum_j w_ij k_j  w = exp2(c s + known.x) (dp - known.y)  (known: the query's statistics)
+//   DK   dk_j = scale sum_i w_ij q_i  the same, the statistics of query i;   DV   dv_j = sum_i w_ij dO_i,  w = exp2(c s + stats.x)
+enum Again { AGAIN_OUT, AGAIN_DQ, AGAIN_DK, AGAIN_DV };
+
+template <typename T> __device__ __forceinline__ uint2 load4(const T* p, bool any) { return any ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0); }
+template <typename T> __device__ __forceinline__ void widen4(const uint2& w, float (&v)[4]) {
+  const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(p, y.v[i], __fmul_rn(o.v[i], old));
-    m = top;
-    if (settled(o, a.D)) break;
-  }
-  const float f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-  store_row(static_cast<T*>(a.out) + (t * a.Hq + h) * a.D, d0, d1, o, f);
-  if (a.low) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = rounded_off<T>(__fmul_rn(o.v[i], f));
-    store_row(static_cast<T*>(a.low) + (t * a.Hq + h) * a.D, d0, d1, o, 1.0f);
-  }
+  for (int i = 0; i < 4; ++i) v[i] = widen<T>(e[i]);
 }
-
-// A query's shift -lse log2 e and its delta, at [t * Hq + h].
-__device__ __forceinline__ float2 stat_of(const float2* stats, const AttnArgs& a, int64_t t, int h) { return stats[t * a.Hq + h]; }
-
-// Elements [d0, d1) of dq_t of one head.
-template <typename T> __device__ __forceinline__ void row_dq(const AttnArgs& a, const float2* stats, int64_t b, int64_t t, int h, int d0, int d1) {
-  const T* q = static_cast<const T*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1];
-  const T* g = static_cast<const T*>(a.dout) + t * a.dout_stride[0] + h * a.dout_stride[1];
-  const int kh = h / (a.Hq / a.Hk);
-  const T* k = static_cast<const T*>(a.k) + kh * a.k_stride[1];
-  const T* v = static_cast<const T*>(a.v) + kh * a.v_stride[1];
-  Seen s{{0, 0}, 0};
-  if (b < a.B) s = seen_by(a, b, t);
-  const Lanes x = load_row(q, a.D), y = load_row(g, a.D);
-  const float2 st = stat_of(stats, a, t, h);
-  const float c = a.scale * 1.4426950408889634f;
-  Lanes o{};
-  for (int64_t j = s.k.begin; j < s.k.begin + s.n; ++j) {
-    const Lanes kj = load_row(k + j * a.k_stride[0], a.D);
-    const float p = exp2f(__fmaf_rn(dot(x, kj), c, st.x));
-    const float ds = __fmul_rn(p, dot(y, load_row(v + j * a.v_stride[0], a.D)) - st.y);
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+  uint2 w;
+  T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = __fmaf_rn(ds, kj.v[i], o.v[i]);
-    if (settled(o, a.D)) break;
-  }
-  store_row(static_cast<T*>(a.dq) + (t * a.Hq + h) * a.D, d0, d1, o, a.scale);
+  for (int i = 0; i < 4; ++i) e[i] = narrow<T>(v[i]);
+  *reinterpret_cast<uint2*>(p) = w;
 }
-
-// dk_t (KEYS) or dv_t of one key head, t a row of the keys.
-template <typename T, bool KEYS> __device__ __forceinline__ void row_dkv(const AttnArgs& a, const float2* stats, int64_t b, int64_t t, int kh) {
-  Lanes o{};
-  if (b < a.B) {
-    const Rows q = rows_of(a.cu_q, b, a.Tq), kr = rows_of(a.cu_k, b, a.Tk);
-    const Lanes kj = load_row(static_cast<const T*>(a.k) + t * a.k_stride[0] + kh * a.k_stride[1], a.D);
-    const Lanes vj = load_row(static_cast<const T*>(a.v) + t * a.v_stride[0] + kh * a.v_stride[1], a.D);
-    const int64_t first = a.causal ? max((int64_t)0, (t - kr.begin) - (kr.count() - q.count())) : 0;
-    const int group = a.Hq / a.Hk;
-    const float c = a.scale * 1.4426950408889634f;
-    bool done = false;
-    for (int h = kh * group; h < (kh + 1) * group && !done; ++h)
-      for (int64_t i = q.begin + first; i < q.end && !done; ++i) {
-        const Lanes x = load_row(static_cast<const T*>(a.q) + i * a.q_stride[0] + h * a.q_stride[1], a.D);
-        const Lanes g = load_row(static_cast<const T*>(a.dout) + i * a.dout_stride[0] + h * a.dout_stride[1], a.D);
-        const float2 st = stat_of(stats, a, i, h);
-        const float p = exp2f(__fmaf_rn(dot(x, kj), c, st.x));
-        const float w = KEYS ? __fmul_rn(p, dot(g, vj) - st.y) : p;
+// Sums over the warp of 8 numbers of each lane: lane l gets that of number l / 4.
+__device__ __forceinline__ float sum8(float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o.v[e] = __fmaf_rn(w, KEYS ? x.v[e] : g.v[e], o.v[e]);
-        done = settled(o, a.D);
+  for (int o = 16, n = 4; o >= 4; o >>= 1, n >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) {
+        const float keep = lane & o ? v[k + n] : v[k], give = lane & o ? v[k] : v[k + n];
+        v[k] = __fadd_rn(keep, __shfl_xor_sync(0xFFFFFFFFu, give, o));
       }
+  float s = __fadd_rn(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 2));
+  return __fadd_rn(s, __shfl_xor_sync(0xFFFFFFFFu, s, 1));
+}
+
+// rows: the lanes whose rows are meant; t, head: a lane's row (a query and its head, or a key and its head) in sequence b.
+// Elements [d0, d1), multiples of 8, are written.  (The whole warp.)
+template <typename T, Again WHAT>
+__device__ __noinline__ void make_again(const AttnArgs& a, const float2* stats, uint32_t rows, int64_t b, int64_t t, int head, float2 known, int d0, int d1) {
+  constexpr bool QUERIES = WHAT == AGAIN_OUT || WHAT == AGAIN_DQ, TWO = WHAT == AGAIN_DQ || WHAT == AGAIN_DK;
+  constexpr bool FIRST = TWO;                                // which of the other side's two rows is added up
+  constexpr int N = 8, U = 4;                                // rows at a time, rows of the other side at a time
+  const int lane = threadIdx.x & 31, e = lane * 4, group = a.Hq / a.Hk;
+  const bool live = e < a.D;
+  const Rows qr = rows_of(a.cu_q, b, a.Tq), kr = rows_of(a.cu_k, b, a.Tk);
+  const int64_t ahead = kr.count() - qr.count();
+  const float c = a.scale * 1.4426950408889634f;
+  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v), *g = static_cast<const T*>(a.dout);
+  while (rows) {
+    int src[N], own = 0, count = 0;
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      src[r] = rows ? __ffs(rows) - 1 : src[0];              // (places without a row do the first one's work)
+      count += rows != 0;
+      rows &= rows - 1;
+      if (lane >> 2 == r) own = src[r];
+    }
+    // of the row whose sums this lane gets
+    const int64_t t_own = __shfl_sync(0xFFFFFFFFu, t, own);
+    const float2 known_own = make_float2(__shfl_sync(0xFFFFFFFFu, known.x, own), __shfl_sync(0xFFFFFFFFu, known.y, own));
+    // a query sees keys up to `limit`, a key is seen by queries from `limit`
+    const int limit = QUERIES ? (int)(a.causal ? max((int64_t)0, min(kr.count(), t_own - qr.begin + 1 + ahead)) : kr.count())
+                              : (int)(a.causal ? max((int64_t)0, t_own - kr.begin - ahead) : 0);
+    const int from = QUERIES ? 0 : __reduce_min_sync(0xFFFFFFFFu, limit), to = QUERIES ? __reduce_max_sync(0xFFFFFFFFu, limit) : (int)qr.count();
+    float x[N][4], y[TWO ? N : 1][4], acc[N][4] = {};
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const int64_t tr = __shfl_sync(0xFFFFFFFFu, t, src[r]);
+      const int hr = __shfl_sync(0xFFFFFFFFu, head, src[r]);
+      widen4<T>(load4((QUERIES ? q + tr * a.q_stride[0] + hr * a.q_stride[1] : k + tr * a.k_stride[0] + hr * a.k_stride[1]) + e, live), x[r]);
+      if (TWO) widen4<T>(load4((QUERIES ? g + tr * a.dout_stride[0] + hr * a.dout_stride[1] : v + tr * a.v_stride[0] + hr * a.v_stride[1]) + e, live), y[TWO ? r : 0]);
+    }
+    const int kh = QUERIES ? __shfl_sync(0xFFFFFFFFu, head, src[0]) / group : __shfl_sync(0xFFFFFFFFu, head, src[0]);
+    bool done = false;
+    for (int h = QUERIES ? kh : kh * group; h < (QUERIES ? kh + 1 : (kh + 1) * group) && !done; ++h) {
+      const T* first = (QUERIES ? k + kr.begin * a.k_stride[0] + h * a.k_stride[1] : q + qr.begin * a.q_stride[0] + h * a.q_stride[1]) + e;
+      const T* second = (QUERIES ? v + kr.begin * a.v_stride[0] + h * a.v_stride[1] : g + qr.begin * a.dout_stride[0] + h * a.dout_stride[1]) + e;
+      const int64_t fs = QUERIES ? a.k_stride[0] : a.q_stride[0], ss = QUERIES ? a.v_stride[0] : a.dout_stride[0];
+      for (int i0 = from; i0 < to && !done; i0 += U) {
+        uint2 wf[U], ws[U];
+        float2 st[U];
+#pragma unroll
+        for (int z = 0; z < U; ++z) {
+          const bool in = i0 + z < to;
+          wf[z] = load4(first + (i0 + z) * fs, live && in), ws[z] = load4(second + (i0 + z) * ss, live && in);
+          st[z] = QUERIES ? known_own : in ? __ldg(stats + (qr.begin + i0 + z) * a.Hq + h) : make_float2(0.0f, 0.0f);
+        }
+        float weight[U];
+        uint32_t sees[U];
+#pragma unroll
+        for (int z = 0; z < U; ++z) {
+          float f[4], s[4], part[N];
+          widen4<T>(wf[z], f), widen4<T>(ws[z], s);
+#pragma unroll
+          for (int r = 0; r < N; ++r) part[r] = __fmaf_rn(x[r][3], f[3], __fmaf_rn(x[r][2], f[2], __fmaf_rn(x[r][1], f[1], __fmul_rn(x[r][0], f[0]))));
+          weight[z] = exp2f(__fmaf_rn(sum8(part), c, st[z].x));
+          if (TWO) {
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+              const float(&yr)[4] = y[TWO ? r : 0];
+              part[r] = __fmaf_rn(yr[3], s[3], __fmaf_rn(yr[2], s[2], __fmaf_rn(yr[1], s[1], __fmul_rn(yr[0], s[0]))));
+            }
+            weight[z] = __fmul_rn(weight[z], sum8(part) - st[z].y);
+          }
+          if (WHAT == AGAIN_OUT) weight[z] = __fmul_rn(weight[z], known_own.y);
+          sees[z] = __ballot_sync(0xFFFFFFFFu, i0 + z < to && (QUERIES ? i0 + z < limit : i0 + z >= limit));
+        }
+#pragma unroll
+        for (int z = 0; z < U; ++z) {
+          float u[4];
+          widen4<T>(FIRST ? wf[z] : ws[z], u);
+#pragma unroll
+          for (int r = 0; r < N; ++r) {
+            const float w = __shfl_sync(0xFFFFFFFFu, weight[z], 4 * r);
+            if (sees[z] >> (4 * r) & 1)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) acc[r][n] = __fmaf_rn(w, u[n], acc[r][n]);
+          }
+        }
+        if ((i0 - from) % 64 == 0) {                         // once every element is NaN, nothing changes it any more
+          bool nan = true;
+#pragma unroll
+          for (int r = 0; r < N; ++r)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) nan = nan && isnan(acc[r][n]);
+          done = __all_sync(0xFFFFFFFFu, nan || !live);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const int64_t tr = __shfl_sync(0xFFFFFFFFu, t, src[r]);
+      const int hr = __shfl_sync(0xFFFFFFFFu, head, src[r]);
+      if (r >= count || e < d0 || e >= d1) continue;
+      const int64_t at = (tr * (QUERIES ? a.Hq : a.Hk) + hr) * a.D + e;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (TWO) acc[r][n] = __fmul_rn(acc[r][n], a.scale);
+      store4(static_cast<T*>(WHAT == AGAIN_OUT ? a.out : WHAT == AGAIN_DQ ? a.dq : WHAT == AGAIN_DK ? a.dk : a.dv) + at, acc[r]);
+      if (WHAT == AGAIN_OUT && a.low) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[r][n] = rounded_off<T>(acc[r][n]);
+        store4(static_cast<T*>(a.low) + at, acc[r]);
+      }
+    }
   }
-  store_row(static_cast<T*>(KEYS ? a.dk : a.dv) + (t * a.Hk + kh) * a.D, 0, a.D, o, KEYS ? a.scale : 1.0f);
 }
 
 }  // namespace attn

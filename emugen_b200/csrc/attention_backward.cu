@@ -539,11 +539,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dkv_kernel(const __grid_
     // A query that does not see the key was multiplied by 0, which infinities and NaN turn into NaN: such rows are made
     // again from the queries that see them alone.
     const bool bad = mine && steps && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
-    for (uint32_t rows = __any_sync(0xFFFFFFFFu, bad) ? keys_made_again<T>(a, tl, keys, key, bad) : 0; rows; rows &= rows - 1) {
-      const int64_t row = __shfl_sync(0xFFFFFFFFu, t, __ffs(rows) - 1);
-      if (keys) row_dkv<T, true>(a, w.stats, u.b, row, u.kh);
-      else row_dkv<T, false>(a, w.stats, u.b, row, u.kh);
-    }
+    const uint32_t rows = __any_sync(0xFFFFFFFFu, bad) ? keys_made_again<T>(a, tl, keys, key, bad) : 0;
+    if (rows && keys) make_again<T, AGAIN_DK>(a, w.stats, rows, u.b, t, u.kh, make_float2(0.0f, 0.0f), 0, a.D);
+    else if (rows) make_again<T, AGAIN_DV>(a, w.stats, rows, u.b, t, u.kh, make_float2(0.0f, 0.0f), 0, a.D);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -789,10 +787,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_dq_kernel(const __grid_c
     // a hidden key that is infinite or NaN: the row again, from the keys that it sees alone (this thread's half of it)
     const bool redo = mine && ok && n > 0 && (ptx::lo2(worst) != 0.0f || ptx::hi2(worst) != 0.0f);
     const int d0 = half * HALF, d1 = min(a.D, (half + 1) * HALF);
-    for (uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, false>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, d0, d1, static_cast<T*>(nullptr)) : 0; rows; rows &= rows - 1) {
-      const int src = __ffs(rows) - 1;
-      row_dq<T>(a, w.stats, u.b, __shfl_sync(0xFFFFFFFFu, t, src), __shfl_sync(0xFFFFFFFFu, h, src), d0, d1);
-    }
+    const uint32_t rows = __any_sync(0xFFFFFFFFu, redo) ? rows_made_again<T, false>(a, redo, u.b, (int)n, (int64_t)tiles * 128, u.kh, d0, d1, static_cast<T*>(nullptr)) : 0;
+    if (rows) make_again<T, AGAIN_DQ>(a, w.stats, rows, u.b, t, h, st, d0, d1);
   }
   ptx::tc_fence_before();
   __syncthreads();
