@@ -22,7 +22,7 @@
 // Measured, both kernels: 64 sequences, 262144 slots of 8 heads of 128 in FP8, 32 query heads: 113 .. 120 us for 555 MB (4.7 TB/s, 72%
 // of a copy's rate; the first kernel 105 us at 5.3 TB/s: memory waits, issue slots 48% busy).  4 sequences, 400001 slots on one
 // head, 16 query heads: 43 us (106 MB): 21 steps to a warp, so that starting and joining count.  4 bits, 33 sequences, 100003
-// slots of 4 heads of 64: 33 us (27 MB), 10 steps to a warp.
+// slots of 4 heads of 64: 33 us (27 MB), 10 steps to a warp, each of which waits for the scale bytes that it asked for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>
@@ -137,7 +137,8 @@ __device__ __forceinline__ int64_t tiles_of(const KvAttendArgs& a, int64_t b) {
   return len > 0 && a.num_pages > 0 ? (len + TILE - 1) / TILE : 0;
 }
 // What a (sequence, head) counts for when the work is dealt out: its tiles and EXTRA places before them, for what
-// starting and joining it costs.
+// starting and joining it costs.  Calls with EXTRA 0, 2, 4, 8, us: 33 sequences, 100003 slots in 4 bits 50, 42, 40, 40; 64 sequences,
+// 16384 slots of 8 heads 38, 34, 32, 32; 262144 in 4 bits 138, 134, 130, 132; 400001 slots on one head 52, 52, 50, 48.
 constexpr int EXTRA = 4;
 __device__ __forceinline__ int64_t places_of(const KvAttendArgs& a, int64_t b) {
   const int64_t n = tiles_of(a, b);
@@ -874,7 +875,9 @@ Plan plan_of(int format, int Hq, int Hk, int D) {
   p.ctas = std::min(JOIN_PARTS, ctas_per_sm(format, padded(D), p.rows > 8) * sm_count());
   const int row = format == EMU_KV_FP8 ? D : D / 2;
   // Neighbouring heads side by side where a slot's row is long: CTAs that read its pieces at about the same time find the memory's
-  // rows open (64 sequences, 262144 slots of 8 heads of 128 bytes: 128 -> 117 us; sets of 8 118).
+  // rows open (64 sequences, 262144 slots of 8 heads of 128 bytes: 128 -> 117 us; sets of 8 118; of 64 bytes, 512 in all, 120 -> 89 us a
+  // call; 4 heads of 128 bytes 84 -> 81).  Shorter rows would gain too (524288 slots of 4 heads of 64 bytes 107 -> 87, of 2 of 128 83 ->
+  // 79); they have not been put so yet.
   while (p.side_bits < 2 && Hk % (2 << p.side_bits) == 0 && Hk * row >= 512) ++p.side_bits;
   p.sets = p.ctas >> p.side_bits;
   return p;
@@ -915,8 +918,9 @@ template <typename T, int FORMAT, int DP, bool TWO> cudaError_t launch(const KvA
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  // MANY where most (sequence, head)s lie in more than FEW CTAs (400001 keys on one head 47 -> 43 us); its registers leave room for
-  // fewer CTAs, which costs where there are many (262144 keys 113 -> 122 us).
+  // MANY where most (sequence, head)s lie in more than FEW CTAs (400001 keys on one head 47 -> 43 us; a call of one sequence of 8192 on 8 heads
+  // 26 -> 22, 8 sequences of 100000 on 2 heads 34 -> 32); its registers leave room for fewer CTAs, which costs where there are many
+  // (262144 keys 113 -> 122 us; calls of 16 sequences of 131072 on 4 heads 52 -> 58, 64 of 16384 on 8 32 -> 40).
   const bool many = pl.ctas > FEW * a.B * a.Hk * pl.groups;
   const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, true>, a, pl, DP) : cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, false>, a, pl, DP);
   if (e != cudaSuccess) return e;

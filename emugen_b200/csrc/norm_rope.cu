@@ -12,9 +12,9 @@
 // cosines and sines are read once for all of them.  A lane has two runs of 8 elements, which hold both elements of its 8
 // pairs (i .. i + 7 and i + half .. i + half + 7; interleaved, 16 neighbours): the turn needs no exchange between lanes, and
 // what is done once for a row (sum, root, addresses) is spread over 16 elements.
-// Measured: 16384 tokens of 32 + 8 heads of 128, bf16: 68 us (344 MB, 5.0 TB/s, 76% of a copy's rate; the loads of the next rows are
-// under way while a row is made, and the rest is their latency).  8191 tokens of 24 + 6 heads of 96, fp16, interleaved: 30 us,
-// gradients 53 + 4 (2 of 8 lanes have no elements at this head size).
+// Measured: 16384 tokens of 32 + 8 heads of 128, bf16: 68 us (344 MB, 5.0 TB/s, 76% of a copy's rate; a group's units are whole, so that
+// the longest path has 80 rows where an even share is 69).  8191 tokens of 24 + 6 heads of 96, fp16, interleaved: 30 us, gradients
+// 53 + 4 (36 rows for 26, and 2 of 8 lanes have no elements at this head size).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
